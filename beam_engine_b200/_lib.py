@@ -18,7 +18,7 @@ PP32 = C.POINTER(P32)
 
 (BE_OK, BE_EINVAL, BE_ENOMEM, BE_ECUDA, BE_ENOT_ALLOCATED, BE_ECAPACITY, BE_EDEVICE_RANGE,
  BE_EDEVICE_TIMEOUT, BE_ENOTSUP) = range(9)
-BE_F32, BE_F16, BE_BF16 = 0, 1, 2
+BE_F32, BE_F16, BE_BF16, BE_E4M3 = 0, 1, 2, 3
 BE_CAPS_SLOTS = 1
 
 
@@ -72,6 +72,24 @@ _SIGS = {
                                     C.c_int, C.c_int, f32, vp, i64, vp, vp, vp, vp, vp]),
     "be_attn_run_fixed_2s": (C.c_int, [vp, vp, C.c_int, vp, i64, vp, C.c_int, C.c_int, C.c_int,
                                     C.c_int, C.c_int, f32, vp, i64, vp, vp, vp, vp, vp, vp]),
+    # 8-bit pools, windowed attention
+    "be_rope_append_paged_kv": (C.c_int, [vp, vp, i64, i64, vp, vp, vp, vp, vp, C.c_int, vp, vp, vp,
+                                          C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp,
+                                          i64, vp]),
+    "be_rope_qkv_append8": (C.c_int, [vp, i64, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, vp, vp,
+                                      C.c_int, C.c_int, vp, vp, C.c_int, vp, i64, vp]),
+    "be_read_paged_kv8": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp,
+                                    C.c_int, vp]),
+    "be_fork_tail_copy8": (C.c_int, [vp, i64, vp, i64, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
+                                     vp, vp, vp, C.c_int, vp]),
+    "be_fork_tail_copy8_list": (C.c_int, [vp, i64, vp, i64, C.c_int, C.c_int, C.c_int, C.c_int,
+                                          C.c_int, vp, C.c_int, C.c_int, vp]),
+    "be_paged_plan": (C.c_int, [C.c_int, PP32, PP32, PP32, PP32, P32, C.c_int, C.c_int, C.c_int,
+                                C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp, i64,
+                                C.POINTER(AttnPlanInfo)]),
+    "be_paged_attn_run": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp, i64, vp, vp,
+                                    C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, f32, vp,
+                                    i64, vp, vp, vp, vp]),
     # host page manager
     "be_trie_create": (vp, [C.c_int, C.c_int]),
     "be_trie_destroy": (None, [vp]),

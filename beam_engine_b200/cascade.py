@@ -17,6 +17,12 @@ Decode plans (no causal group of more than one query) with head_dim 128 and
 page size 16 run as beam-tile plans (``be_tile_plan`` / ``be_attn_tiles_run``:
 one launch, each page read once per KV head, partial rows merged inside the
 kernel); ``BE_ATTN_TILES=0`` keeps the work-item kernels.
+
+``plan(..., kv_data_type=torch.float8_e4m3fn)`` plans for a cache in 8 bits (``run`` then takes
+its scales as ``kv_scale``), ``plan(..., window_left=w, num_sinks=s)`` lets the query at position
+p see the tokens t >= p - w and the first s tokens only; a query's tokens are those of its
+groups in level order, and the queries of a last-level group are its last tokens.  Both go
+through ``be_paged_plan`` / ``be_paged_attn_run`` (bf16 / fp16 queries, head_dim 64 or 128).
 """
 from __future__ import annotations
 
@@ -29,7 +35,8 @@ import torch
 
 from . import _lib
 from ._lib import AttnPlanInfo, TilePlanInfo, check, lib
-from .page_table import dtype_code, require_cuda, stream_ptr
+from .page_table import (check_pool8, dtype_code, is_8bit, require_cuda, require_same_device,
+                         stream_ptr)
 
 
 def _i32(x):
@@ -217,6 +224,24 @@ class _Plan:
         check(rc, "be_attn_run")
 
 
+    def run_paged(self, q, kv, kv_scale, num_qo_heads, num_kv_heads, head_dim, sm_scale, out,
+                  lse=None):
+        """A be_paged_plan plan (placed like a work-item plan)."""
+        if q.stride(-1) != 1 or q.stride(-2) != head_dim or q.stride(0) % 8 or q.data_ptr() % 16:
+            q = q.contiguous()
+        i = self.info
+        with torch.cuda.device(q.device):
+            rc = lib().be_paged_attn_run(
+                self.plan_dev, i.n_work_wide, i.n_work - i.n_work_wide, i.n_merge, i.n_parts,
+                i.page_size, q.data_ptr(), q.stride(0), kv.data_ptr(),
+                kv_scale.data_ptr() if kv_scale is not None else None, kv.shape[0], num_qo_heads,
+                num_kv_heads, head_dim, dtype_code(q.dtype),
+                _lib.BE_E4M3 if kv_scale is not None else dtype_code(kv.dtype), sm_scale,
+                out.data_ptr(), out.stride(0), lse.data_ptr() if lse is not None else None,
+                self.mid_o, self.mid_lse, stream_ptr(q.device))
+        check(rc, "be_paged_attn_run")
+
+
 _plan_cap = 4096     # int32 capacity of the next host plan buffer (grows on demand)
 
 
@@ -258,7 +283,10 @@ class MultiLevelCascadeAttentionWrapper:
              paged_kv_indices_arr: List[torch.Tensor], paged_kv_last_page_len: List[torch.Tensor],
              num_qo_heads: int, num_kv_heads: int, head_dim: int, page_size: int,
              causal: bool = False, pos_encoding_mode: str = "NONE", sm_scale: Optional[float] = None,
-             q_data_type=None, split_tokens: int = 0, **_):
+             q_data_type=None, split_tokens: int = 0, kv_data_type=None, window_left: int = -1,
+             num_sinks: int = 0, **_):
+        if num_sinks < 0:
+            raise ValueError(f"num_sinks {num_sinks} is negative")
         if pos_encoding_mode != "NONE":
             raise ValueError("only pos_encoding_mode='NONE' is supported")
         if len(qo_indptr_arr) != self.num_levels:
@@ -274,7 +302,11 @@ class MultiLevelCascadeAttentionWrapper:
         self._levels_args = (L, ptrs, ng, nq, page_size, num_qo_heads, num_kv_heads, causal,
                              split_tokens, head_dim, arrs)
         self.tiles = False
-        if split_tokens == 0 and tiles_eligible(head_dim, page_size, num_qo_heads, num_kv_heads):
+        self._window = (window_left if window_left >= 0 else -1, num_sinks)
+        self.paged = window_left >= 0 or (kv_data_type is not None and is_8bit(kv_data_type))
+        if self.paged:
+            self._plan_paged()
+        elif split_tokens == 0 and tiles_eligible(head_dim, page_size, num_qo_heads, num_kv_heads):
             g = num_qo_heads // num_kv_heads
             qo0 = arrs[0][0] if L else np.zeros(1, np.int32)
             rows = tile_rows_for(int(np.max(np.diff(qo0))) * g if len(qo0) > 1 else g)
@@ -287,7 +319,7 @@ class MultiLevelCascadeAttentionWrapper:
             if ps.build_tiles(tfn):
                 ps.place_tiles(num_kv_heads, head_dim)
                 self.tiles = True
-        if not self.tiles:
+        if not self.tiles and not self.paged:
             self._plan_items()
         self.num_queries = nq
         self.hq, self.hkv, self.d = num_qo_heads, num_kv_heads, head_dim
@@ -308,10 +340,61 @@ class MultiLevelCascadeAttentionWrapper:
         ps.tinfo = None
         self.tiles = False
 
+    def _plan_paged(self):
+        """The plan (be_paged_plan) of the last plan() call's levels for 8-bit caches and windows."""
+        (L, ptrs, ng, nq, page_size, hq, hkv, causal, _, head_dim, _) = self._levels_args
+        if head_dim not in (64, 128):
+            raise ValueError(f"head_dim {head_dim}: 8-bit caches and windows take 64 or 128")
+        ps = self._plan
+        window, sinks = self._window
+
+        def fn(buf, cap, info):
+            return lib().be_paged_plan(L, *ptrs, _lib.ptr32(ng), nq, page_size, hq, hkv,
+                                       1 if causal else 0, window, sinks, ps.num_sms, buf, cap,
+                                       info)
+        ps.build(fn)
+        ps.place(hq, head_dim)
+        ps.tinfo = None
+        self.tiles = False
+        self.paged = True
+
+    def _run_paged(self, q, kv, kv_scale, return_lse, out):
+        n, hq, d = self.num_queries, self.hq, self.d
+        page_size = self._plan.info.page_size
+        if q.shape != (n, hq, d):
+            raise ValueError(f"q must be {(n, hq, d)}, got {tuple(q.shape)}")
+        if kv.dim() != 5 or kv.shape[1:] != (2, page_size, self.hkv, d) or not kv.is_contiguous():
+            raise ValueError(f"paged_kv_cache must be contiguous [pages, 2, {page_size}, "
+                             f"{self.hkv}, {d}], got {tuple(kv.shape)}")
+        if is_8bit(kv.dtype):
+            check_pool8(kv, kv_scale)
+            require_same_device(kv, q, kv_scale, self._plan.ws)
+        elif kv_scale is not None or kv.dtype != q.dtype:
+            raise ValueError(f"a cache of {kv.dtype} takes queries of its type (got {q.dtype}) and "
+                             "no kv_scale")
+        else:
+            require_same_device(kv, q, self._plan.ws)
+        if out is None:
+            out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
+        elif (out.shape != (n, hq, d) or out.dtype != q.dtype or out.device != q.device
+              or out.stride(-1) != 1 or out.stride(-2) != d):
+            raise ValueError(f"out must be {q.dtype} {(n, hq, d)} on {q.device} with contiguous "
+                             "heads")
+        lse = torch.empty((n, hq), dtype=torch.float32, device=q.device) if return_lse else None
+        if n:
+            self._plan.run_paged(q, kv, kv_scale, hq, self.hkv, d, self.sm_scale, out, lse)
+        return (out, lse) if return_lse else out
+
     def run(self, q: torch.Tensor, paged_kv_cache: torch.Tensor, return_lse: bool = False,
-            out: Optional[torch.Tensor] = None):
+            out: Optional[torch.Tensor] = None, kv_scale: Optional[torch.Tensor] = None):
         if q.shape[0] != self.num_queries:
             raise ValueError(f"q has {q.shape[0]} rows, plan has {self.num_queries} queries")
+        if is_8bit(paged_kv_cache.dtype) and not self.paged:
+            self._plan_paged()               # 8-bit caches run on their own plan
+        if self.paged:
+            return self._run_paged(q, paged_kv_cache, kv_scale, return_lse, out)
+        if kv_scale is not None:
+            raise ValueError("kv_scale belongs to a float8_e4m3fn cache")
         if out is None:
             out = torch.empty((q.shape[0], self.hq, self.d), dtype=q.dtype, device=q.device)
         lse = torch.empty((q.shape[0], self.hq), dtype=torch.float32,
@@ -342,7 +425,8 @@ class BatchPrefillWithPagedKVCacheWrapper:
                          page_size, causal=causal, pos_encoding_mode=pos_encoding_mode,
                          sm_scale=sm_scale, **kw)
 
-    def run(self, q, paged_kv_cache, return_lse=False, out=None):
-        return self._inner.run(q, paged_kv_cache, return_lse=return_lse, out=out)
+    def run(self, q, paged_kv_cache, return_lse=False, out=None, kv_scale=None):
+        return self._inner.run(q, paged_kv_cache, return_lse=return_lse, out=out,
+                               kv_scale=kv_scale)
 
     forward = run

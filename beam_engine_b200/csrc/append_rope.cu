@@ -1,0 +1,594 @@
+// Append to a paged cache with the position rotation on the way, into 8-bit
+// (e4m3) pages with one scale per block or into pages of the rows' own type,
+// and the read-back of 8-bit pages as values.
+//
+// A block is one page x plane (K | V) x KV head.  Its scale is a power of two,
+//   e = the smallest integer in [-40, 40] with amax <= 448 * 2^e,
+// over the block's finite new values, and never below the scale the block had,
+// unless the call writes the page's slot 0, which begins the block anew.  With
+// powers of two the scale costs no precision (e4m3 keeps 4 significant bits at
+// every exponent, so up to one binary order less head room only moves where
+// the subnormals begin), multiplying by it is exact, and tokens re-rounded when a
+// later append raises the scale change only where they fall below the new
+// subnormal step.  [-40, 40] keeps 1 / s and ratios of scales far inside fp32.
+//
+// Work split: a scale depends on every row that the call puts into its page, so
+// one CTA owns a page.  Rows of a page are usually adjacent (a prompt) or alone
+// (a beam step); a CTA takes the runs of equal pages that start inside its span
+// of rows and looks for other runs of the same page anywhere in the call; the
+// CTA of the first such run does the page, so rows may come in any order.  Up to
+// ROPE_SCAN_ROWS rows a CTA compares every row's page itself.  Above that a
+// first launch resolves the pages and lists the run starts per 256 rows, and the
+// search reads only those lists (a 16th of the rows for a prompt with pages of 16).
+//
+// Bound: HBM (rows in, codes out) for prompts; latency for a beam step.
+#include "common.cuh"
+
+namespace be {
+
+constexpr int ROPE_SCAN_ROWS = 512;   // largest call whose CTAs scan all rows
+constexpr int ROPE_BLOCK = 256;       // rows per run-start list of the first launch
+constexpr int ROPE_MAX_PAGE = 256;    // slots of a page (shared row table)
+constexpr int ROPE_TAB = 16;          // rows whose cos / sin are in shared memory at once
+constexpr float kE4M3Max = 448.f;
+constexpr int kScaleExpMin = -40, kScaleExpMax = 40;
+
+struct RopeAppend {
+  const char* k;
+  const char* v;
+  int64_t k_stride, v_stride;       // elements between rows
+  char* q;                          // fused rows whose q heads are rotated in place, or null
+  int64_t q_stride;
+  int hq;
+  const int32_t* batch;             // null: write_page / write_pos name the slots directly
+  const int32_t* pos;               // positions in the sequence (slots come from them with batch)
+  const int32_t* rope_pos;          // positions of the rotation
+  const int32_t* kv_indices;
+  const int32_t* kv_indptr;
+  const int32_t* write_page;
+  const int32_t* write_pos;
+  const float* inv_freq;            // null: no rotation
+  char* cache;
+  float* scale;                     // [pages][2][hkv]; null: cache of the rows' type
+  int n, num_pages, ps, hkv, D, span;
+  int32_t* page_of;                 // workspace of the first launch: [n] pages,
+  int32_t* slot_of;                 // [n] slots,
+  int32_t* starts;                  // [ceil(n / 256)][256] run starts,
+  int32_t* n_starts;                // [ceil(n / 256)]
+};
+
+__device__ __forceinline__ void rope_slot(const RopeAppend& a, int i, int& page, int& slot) {
+  if (a.batch) {
+    const int pos = a.pos[i];
+    const int b = a.batch[i];
+    page = -1;
+    slot = 0;
+    if (pos >= 0) {
+      page = a.kv_indices[a.kv_indptr[b] + pos / a.ps];
+      slot = pos % a.ps;
+    }
+  } else {
+    page = a.write_page[i];
+    slot = a.write_pos[i];
+  }
+  if (page < 0 || page >= a.num_pages || slot < 0 || slot >= a.ps) page = -1;
+}
+
+// Smallest e in [-40, 40] with amax <= 448 * 2^e (448 = 1.75 * 2^8), read off the
+// exponent and mantissa bits; amax is finite and >= 0.
+__device__ __forceinline__ float block_scale(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+  e = min(max(e, kScaleExpMin), kScaleExpMax);   // amax = 0 and subnormals: -40
+  return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+
+__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// two e4m3 codes (low byte first) -> two halves, exactly
+__device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t two) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)two));
+  return r;
+}
+__device__ __forceinline__ void e4m3x4_to_f(uint32_t w, float* f) {
+  const uint32_t a = e4m3x2_to_h2(w & 0xffffu), b = e4m3x2_to_h2(w >> 16);
+  const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a));
+  const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&b));
+  f[0] = x.x; f[1] = x.y; f[2] = y.x; f[3] = y.y;
+}
+
+// First launch of a call with many rows: page and slot of every row, and per 256
+// rows the list of rows whose page differs from the row before.
+__global__ void __launch_bounds__(ROPE_BLOCK) rope_runs_kernel(const RopeAppend a) {
+  __shared__ int count;
+  pdl_wait();
+  pdl_trigger();   // the append launch waits for this grid before it reads the lists
+  if (threadIdx.x == 0) count = 0;
+  __syncthreads();
+  const int i = blockIdx.x * ROPE_BLOCK + threadIdx.x;
+  if (i < a.n) {
+    int page, slot, before = -1, s2;
+    rope_slot(a, i, page, slot);
+    if (i > 0) rope_slot(a, i - 1, before, s2);
+    a.page_of[i] = page;
+    a.slot_of[i] = slot;
+    if (page < 0) flag_range_error();
+    if (page >= 0 && (i == 0 || before != page))
+      a.starts[blockIdx.x * ROPE_BLOCK + atomicAdd(&count, 1)] = i;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) a.n_starts[blockIdx.x] = count;
+}
+
+// cos / sin of rows rows[0..m) into the table.  The angle is a product of two fp32
+// numbers in 64 bits, reduced to turns there: the rounding of an fp32 product
+// alone is 6e-3 rad at position 100 000.
+__device__ __forceinline__ void rope_table(const RopeAppend& a, const int* rows, int m, int half,
+                                           float2* tab) {
+  for (int i = threadIdx.x; i < m * half; i += blockDim.x) {
+    const int r = i / half, d = i - r * half;
+    const double turns = (double)a.rope_pos[rows[r]] * (double)a.inv_freq[d] * 0.15915494309189535;
+    const float t = (float)(turns - rint(turns));
+    float s, c;
+    sincospif(2.f * t, &s, &c);
+    tab[i] = make_float2(c, s);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, bool vec, float* f) {
+  if constexpr (sizeof(T) == 2) {
+    if (vec) {
+      const int4 raw = *reinterpret_cast<const int4*>(p);
+      const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = to_f(e[i]);
+      return;
+    }
+  } else if (vec) {
+    const float4 x = reinterpret_cast<const float4*>(p)[0], y = reinterpret_cast<const float4*>(p)[1];
+    f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w;
+    f[4] = y.x; f[5] = y.y; f[6] = y.z; f[7] = y.w;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = to_f(p[i]);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, bool vec, const float* f) {
+  if (vec) {
+    if constexpr (sizeof(T) == 2) {
+      int4 raw;
+      T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = from_f<T>(f[i]);
+      *reinterpret_cast<int4*>(p) = raw;
+    } else {
+      reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+      reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) p[i] = from_f<T>(f[i]);
+}
+
+// Eight dims of each half of one K or V row: dims [8 j, 8 j + 8) in lo, those + D/2
+// in hi, rotated by the row's table entry when `tab` is set.
+template <typename T>
+__device__ __forceinline__ void rope_load(const T* src, int j, int half, bool vec,
+                                          const float2* tab, float* lo, float* hi) {
+  load8<T>(src + 8 * j, vec, lo);
+  load8<T>(src + 8 * j + half, vec, hi);
+  if (!tab) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 cs = tab[8 * j + i];
+    const float x = lo[i], y = hi[i];
+    lo[i] = x * cs.x - y * cs.y;
+    hi[i] = y * cs.x + x * cs.y;
+  }
+}
+
+__device__ __forceinline__ float finite_abs(float x) {   // 0 for infinities and NaN
+  const float a = fabsf(x);
+  return a < INFINITY ? a : 0.f;
+}
+
+template <typename T, bool QUANT>
+__global__ void __launch_bounds__(256) rope_append_kernel8(const RopeAppend a) {
+  extern __shared__ float2 tab[];                  // [ROPE_TAB][D / 2]
+  __shared__ int row_of[ROPE_MAX_PAGE];            // slot -> row of the call (the last one), or -1
+  __shared__ int list[ROPE_MAX_PAGE];              // rows of the page in slot order
+  __shared__ int n_list, first;
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+  const int D = a.D, half = D / 2, lp = D / 16;    // lanes per row: 8 + 8 dims each
+  const bool listed = a.page_of != nullptr;
+  const int i0 = blockIdx.x * a.span, i1 = min(a.n, i0 + a.span);
+  const int tpw = 32 / lp;                         // rows per warp pass
+  const int j = lane % lp, sub = lane / lp;
+  const bool vec_k = ((((uintptr_t)a.k) | (a.k_stride * sizeof(T))) & 15) == 0;
+  const bool vec_v = ((((uintptr_t)a.v) | (a.v_stride * sizeof(T))) & 15) == 0;
+
+  // ---- q heads of the span's rows, rotated in place ----
+  if (a.q) {
+    const bool vec_q = ((((uintptr_t)a.q) | (a.q_stride * sizeof(T))) & 15) == 0;
+    for (int b0 = i0; b0 < i1; b0 += ROPE_TAB) {
+      const int m = min(ROPE_TAB, i1 - b0);
+      __syncthreads();
+      if (tid < m) list[tid] = b0 + tid;
+      __syncthreads();
+      rope_table(a, list, m, half, tab);
+      __syncthreads();
+      for (int u = tid / lp; u < m * a.hq; u += blockDim.x / lp) {
+        const int r = u / a.hq, h = u - r * a.hq;
+        T* dst = reinterpret_cast<T*>(a.q) + (b0 + r) * a.q_stride + (int64_t)h * D;
+        float lo[8], hi[8];
+        rope_load<T>(dst, j, half, vec_q, tab + r * half, lo, hi);
+        store8<T>(dst + 8 * j, vec_q, lo);
+        store8<T>(dst + 8 * j + half, vec_q, hi);
+      }
+    }
+  }
+
+  for (int i = i0; i < i1; ++i) {
+    // ---- does a run of rows of one page start here? ----
+    int page, slot, before = -1, s2;
+    if (listed) {
+      page = a.page_of[i];
+      before = i > 0 ? a.page_of[i - 1] : -1;
+    } else {
+      rope_slot(a, i, page, slot);
+      if (i > 0) rope_slot(a, i - 1, before, s2);
+      if (page < 0 && tid == 0) flag_range_error();
+    }
+    if (page < 0 || before == page) continue;     // uniform over the CTA
+    // ---- rows of the call that go into this page, and the first of them ----
+    __syncthreads();
+    for (int s = tid; s < a.ps; s += blockDim.x) row_of[s] = -1;
+    if (tid == 0) first = a.n;
+    __syncthreads();
+    if (listed) {
+      const int nb = (a.n + ROPE_BLOCK - 1) / ROPE_BLOCK;
+      for (int b = tid; b < nb; b += blockDim.x) {
+        const int m = a.n_starts[b];
+        for (int k = 0; k < m; ++k) {
+          int r = a.starts[b * ROPE_BLOCK + k];
+          if (a.page_of[r] != page) continue;
+          atomicMin(&first, r);
+          for (; r < a.n && a.page_of[r] == page; ++r) atomicMax(&row_of[a.slot_of[r]], r);
+        }
+      }
+    } else {
+      for (int r = tid; r < a.n; r += blockDim.x) {
+        int p, s;
+        rope_slot(a, r, p, s);
+        if (p != page) continue;
+        atomicMin(&first, r);
+        atomicMax(&row_of[s], r);
+      }
+    }
+    __syncthreads();
+    if (first != i) continue;                     // another CTA (or run) has the page
+    if (warp == 0) {                              // compact, in slot order
+      int m = 0;
+      for (int s0 = 0; s0 < a.ps; s0 += 32) {
+        const int s = s0 + lane;
+        const int r = s < a.ps ? row_of[s] : -1;
+        const unsigned has = __ballot_sync(0xffffffffu, r >= 0);
+        if (r >= 0) list[m + __popc(has & ((1u << lane) - 1))] = s;
+        m += __popc(has);
+      }
+      if (lane == 0) n_list = m;
+    }
+    __syncthreads();
+    const int m = n_list;
+    const bool fresh = row_of[0] >= 0;
+    const int64_t plane_rows = (int64_t)a.ps * a.hkv;
+    // two phases over the rows in batches of ROPE_TAB: the largest value, then the codes.
+    // A page of one batch keeps its table between them.
+    __shared__ float amax_s[2 * 64];              // per (plane, head): hkv <= 64
+    __shared__ int batch_rows[ROPE_TAB];
+    const int units = 2 * a.hkv;
+    for (int u = tid; u < units; u += blockDim.x) amax_s[u] = 0.f;
+    const int n_batch = (m + ROPE_TAB - 1) / ROPE_TAB;
+    for (int phase = QUANT ? 0 : 1; phase < 2; ++phase) {
+      for (int b = 0; b < n_batch; ++b) {
+        const int c0 = b * ROPE_TAB, cm = min(ROPE_TAB, m - c0);
+        if (phase == (QUANT ? 0 : 1) || n_batch > 1) {
+          __syncthreads();
+          if (tid < cm) batch_rows[tid] = row_of[list[c0 + tid]];
+          __syncthreads();
+          if (a.inv_freq) rope_table(a, batch_rows, cm, half, tab);
+          __syncthreads();
+        }
+        for (int u = warp; u < units; u += warps) {
+          const int plane = u >= a.hkv, h = plane ? u - a.hkv : u;
+          const bool rot = !plane && a.inv_freq;
+          const T* base = reinterpret_cast<const T*>(plane ? a.v : a.k) + (int64_t)h * D;
+          const int64_t stride = plane ? a.v_stride : a.k_stride;
+          const bool vec = plane ? vec_v : vec_k;
+          float best = 0.f, s = 1.f, inv = 1.f;
+          if (QUANT && phase == 1) {
+            s = amax_s[u];                        // by now the block's new scale
+            inv = 1.f / s;                        // exact: a power of two
+          }
+          for (int t0 = 0; t0 < cm; t0 += tpw) {
+            const int t = t0 + sub;
+            if (t >= cm) continue;
+            const int r = batch_rows[t];
+            float lo[8], hi[8];
+            rope_load<T>(base + r * stride, j, half, vec, rot ? tab + t * half : nullptr, lo, hi);
+            if (QUANT && phase == 0) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) best = fmaxf(best, fmaxf(finite_abs(lo[k]), finite_abs(hi[k])));
+              continue;
+            }
+            const int64_t row = ((int64_t)page * 2 + plane) * plane_rows + (int64_t)list[c0 + t] * a.hkv + h;
+            if constexpr (QUANT) {
+              char* dst = a.cache + row * D + 8 * j;
+              uint2 cl, ch;
+              cl.x = to_e4m3x2(lo[0] * inv, lo[1] * inv) | to_e4m3x2(lo[2] * inv, lo[3] * inv) << 16;
+              cl.y = to_e4m3x2(lo[4] * inv, lo[5] * inv) | to_e4m3x2(lo[6] * inv, lo[7] * inv) << 16;
+              ch.x = to_e4m3x2(hi[0] * inv, hi[1] * inv) | to_e4m3x2(hi[2] * inv, hi[3] * inv) << 16;
+              ch.y = to_e4m3x2(hi[4] * inv, hi[5] * inv) | to_e4m3x2(hi[6] * inv, hi[7] * inv) << 16;
+              *reinterpret_cast<uint2*>(dst) = cl;
+              *reinterpret_cast<uint2*>(dst + half) = ch;
+            } else {
+              T* dst = reinterpret_cast<T*>(a.cache) + row * D + 8 * j;
+              const bool vec_c = ((uintptr_t)a.cache & 15) == 0;
+              store8<T>(dst, vec_c, lo);
+              store8<T>(dst + half, vec_c, hi);
+            }
+          }
+          if (QUANT && phase == 0) {
+#pragma unroll
+            for (int off = 16; off; off >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, off));
+            if (lane == 0) amax_s[u] = fmaxf(amax_s[u], best);   // only this warp has unit u
+          }
+        }
+      }
+      if (QUANT && phase == 0) {
+        __syncthreads();
+        // the new scales; where one grew, the tokens that were there get its steps
+        for (int u = warp; u < units; u += warps) {
+          float* sp = a.scale + (int64_t)page * units + u;
+          const float old = fresh ? 0.f : *sp;
+          const float s = fmaxf(block_scale(amax_s[u]), old);
+          __syncwarp();
+          if (lane == 0) {
+            amax_s[u] = s;
+            *sp = s;
+          }
+          if (fresh || !(s > old)) continue;
+          const float ratio = old / s;            // a power of two, or 0 for a block never written
+          const int plane = u >= a.hkv, h = plane ? u - a.hkv : u;
+          const int words = D / 4;
+          for (int w = lane; w < a.ps * words; w += 32) {
+            const int sl = w / words;
+            if (row_of[sl] >= 0) continue;        // written below
+            uint32_t* p = reinterpret_cast<uint32_t*>(
+                a.cache + (((int64_t)page * 2 + plane) * plane_rows + (int64_t)sl * a.hkv + h) * D) +
+                (w - sl * words);
+            float f[4];
+            e4m3x4_to_f(*p, f);
+            *p = to_e4m3x2(f[0] * ratio, f[1] * ratio) | to_e4m3x2(f[2] * ratio, f[3] * ratio) << 16;
+          }
+        }
+        __syncthreads();
+      }
+    }
+  }
+}
+
+// Pages of an 8-bit cache as the values they stand for: out [n][2][ps][hkv][D].
+template <typename T>
+__global__ void __launch_bounds__(256) read_pages_kernel(const char* __restrict__ cache,
+                                                         const float* __restrict__ scale,
+                                                         const int32_t* __restrict__ pages, int n,
+                                                         int num_pages, int ps, int hkv, int D,
+                                                         T* __restrict__ out) {
+  pdl_wait();
+  const int per_row = D / 8;
+  const int64_t page_vecs = (int64_t)2 * ps * hkv * per_row;
+  const int64_t total = n * page_vecs;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t pg = i / page_vecs;
+    const int in = (int)(i - pg * page_vecs);      // < 2^31: pages are at most 256 slots
+    const int row = in / per_row, h = row % hkv, plane = row / (ps * hkv);
+    const int page = pages[pg];
+    float f[8];
+    if (page < 0 || page >= num_pages) {
+      if (in == 0) flag_range_error();
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] = 0.f;
+    } else {
+      const uint2 c = __ldg(reinterpret_cast<const uint2*>(cache + (page * page_vecs + in) * 8));
+      const float s = scale[((int64_t)page * 2 + plane) * hkv + h];
+      e4m3x4_to_f(c.x, f);
+      e4m3x4_to_f(c.y, f + 4);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] *= s;
+    }
+    store8<T>(out + i * 8, true, f);
+  }
+}
+
+static int rope_append_launch(RopeAppend& a, int dtype, int32_t* workspace, cudaStream_t st) {
+  // one row per CTA while that is what fills the GPU (a beam step), pages' worth of rows
+  // once there are many: the search for other runs is then shared by a CTA's rows
+  a.span = a.n <= ROPE_SCAN_ROWS ? 1 : 16;
+  if (a.n > ROPE_SCAN_ROWS) {
+    const int nb = (a.n + ROPE_BLOCK - 1) / ROPE_BLOCK;
+    a.page_of = workspace;
+    a.slot_of = a.page_of + a.n;
+    a.n_starts = a.slot_of + a.n;
+    a.starts = a.n_starts + nb;
+    BE_CUDA_CHECK(launch_pdl(rope_runs_kernel, dim3(nb), dim3(ROPE_BLOCK), 0, st, a));
+  }
+  const dim3 grid((a.n + a.span - 1) / a.span);
+  const size_t smem = (size_t)ROPE_TAB * (a.D / 2) * sizeof(float2);   // <= 16 KB
+#define BE_ROPE8(T)                                                                            \
+  do {                                                                                         \
+    if (a.scale)                                                                               \
+      BE_CUDA_CHECK(launch_pdl(rope_append_kernel8<T, true>, grid, dim3(256), smem, st, a));   \
+    else                                                                                       \
+      BE_CUDA_CHECK(launch_pdl(rope_append_kernel8<T, false>, grid, dim3(256), smem, st, a));  \
+  } while (0)
+  switch (dtype) {
+    case BE_BF16: BE_ROPE8(__nv_bfloat16); break;
+    case BE_F16: BE_ROPE8(__half); break;
+    default: BE_ROPE8(float);
+  }
+#undef BE_ROPE8
+  BE_LAUNCH_CHECK();
+  return BE_OK;
+}
+
+static int rope_append_check(const char* fn, const RopeAppend& a, int dtype, int cache_dtype,
+                             const int32_t* workspace, int64_t workspace_ints) {
+  const int D = a.D;
+  if (a.n < 0 || a.num_pages < 1 || a.ps < 1 || a.ps > ROPE_MAX_PAGE || a.hkv < 1 || a.hkv > 64 ||
+      dtype < BE_F32 || dtype > BE_BF16 || (cache_dtype != BE_E4M3 && cache_dtype != dtype)) {
+    set_error("%s: invalid shape or type (page size 1..%d, kv heads 1..64, cache e4m3 or of the rows' type)",
+              fn, ROPE_MAX_PAGE);
+    return BE_EINVAL;
+  }
+  if (D != 32 && D != 64 && D != 128 && D != 256) {
+    set_error("%s: head_dim %d is not 32, 64, 128 or 256", fn, D);
+    return BE_EINVAL;
+  }
+  if (a.n == 0) return BE_OK;
+  if (!a.k || !a.v || !a.cache || (cache_dtype == BE_E4M3) != (a.scale != nullptr) ||
+      (!a.batch && (!a.write_page || !a.write_pos)) ||
+      (a.batch && (!a.pos || !a.kv_indices || !a.kv_indptr)) || (a.inv_freq && !a.rope_pos)) {
+    set_error("%s: null pointer (an 8-bit cache needs kv_scale, another cache has none)", fn);
+    return BE_EINVAL;
+  }
+  if (cache_dtype == BE_E4M3 && (uintptr_t)a.cache % 8) {
+    set_error("%s: the cache must be 8-byte aligned", fn);
+    return BE_EINVAL;
+  }
+  if (a.n > ROPE_SCAN_ROWS && (!workspace || workspace_ints < 4ll * a.n + 512)) {
+    set_error("%s: %d rows need a workspace of %lld ints", fn, a.n, 4ll * a.n + 512);
+    return BE_ECAPACITY;
+  }
+  return BE_OK;
+}
+
+}  // namespace be
+
+using namespace be;
+
+extern "C" int be_rope_append_paged_kv(const void* append_key, const void* append_value,
+                                       int64_t key_row_stride, int64_t value_row_stride,
+                                       const int32_t* batch_indices, const int32_t* positions,
+                                       const int32_t* rope_positions, const int32_t* kv_indices,
+                                       const int32_t* kv_indptr, int nnz, const float* inv_freq,
+                                       void* paged_kv_cache, float* kv_scale, int num_pages,
+                                       int page_size, int num_kv_heads, int head_dim, int dtype,
+                                       int cache_dtype, int32_t* workspace,
+                                       int64_t workspace_ints, void* stream) {
+  RopeAppend a{};
+  a.k = (const char*)append_key;
+  a.v = (const char*)append_value;
+  a.k_stride = key_row_stride;
+  a.v_stride = value_row_stride;
+  a.batch = batch_indices;
+  a.pos = positions;
+  a.rope_pos = rope_positions ? rope_positions : positions;
+  a.kv_indices = kv_indices;
+  a.kv_indptr = kv_indptr;
+  a.inv_freq = inv_freq;
+  a.cache = (char*)paged_kv_cache;
+  a.scale = kv_scale;
+  a.n = nnz;
+  a.num_pages = num_pages;
+  a.ps = page_size;
+  a.hkv = num_kv_heads;
+  a.D = head_dim;
+  if (nnz > 0 && !batch_indices) {
+    set_error("be_rope_append_paged_kv: null pointer");
+    return BE_EINVAL;
+  }
+  const int rc = rope_append_check("be_rope_append_paged_kv", a, dtype, cache_dtype, workspace,
+                                   workspace_ints);
+  if (rc != BE_OK || nnz == 0) return rc;
+  return rope_append_launch(a, dtype, workspace, (cudaStream_t)stream);
+}
+
+extern "C" int be_rope_qkv_append8(void* qkv, int64_t row_stride, int n, int num_qo_heads,
+                                   int num_kv_heads, int head_dim, const int32_t* positions,
+                                   const float* inv_freq, void* paged_kv_cache, float* kv_scale,
+                                   int num_pages, int page_size, const int32_t* write_page,
+                                   const int32_t* write_pos, int dtype, int32_t* workspace,
+                                   int64_t workspace_ints, void* stream) {
+  if (num_qo_heads < 0 || !inv_freq || !positions) {
+    set_error("be_rope_qkv_append8: invalid shape or null pointer");
+    return BE_EINVAL;
+  }
+  const int elt = dtype_size(dtype);
+  RopeAppend a{};
+  a.q = (char*)qkv;
+  a.q_stride = a.k_stride = a.v_stride = row_stride;
+  a.hq = num_qo_heads;
+  a.k = (const char*)qkv + (int64_t)num_qo_heads * head_dim * elt;
+  a.v = a.k + (int64_t)num_kv_heads * head_dim * elt;
+  a.rope_pos = positions;
+  a.write_page = write_page;
+  a.write_pos = write_pos;
+  a.inv_freq = inv_freq;
+  a.cache = (char*)paged_kv_cache;
+  a.scale = kv_scale;
+  a.n = n;
+  a.num_pages = num_pages;
+  a.ps = page_size;
+  a.hkv = num_kv_heads;
+  a.D = head_dim;
+  if (n > 0 && !qkv) {
+    set_error("be_rope_qkv_append8: null pointer");
+    return BE_EINVAL;
+  }
+  const int rc = rope_append_check("be_rope_qkv_append8", a, dtype, BE_E4M3, workspace, workspace_ints);
+  if (rc != BE_OK || n == 0) return rc;
+  return rope_append_launch(a, dtype, workspace, (cudaStream_t)stream);
+}
+
+extern "C" int be_read_paged_kv8(const void* paged_kv_cache, const float* kv_scale,
+                                 const int32_t* pages, int n, int num_pages, int page_size,
+                                 int num_kv_heads, int head_dim, void* out, int out_dtype,
+                                 void* stream) {
+  if (n < 0 || num_pages < 1 || page_size < 1 || page_size > ROPE_MAX_PAGE || num_kv_heads < 1 ||
+      num_kv_heads > 64 || head_dim < 8 || head_dim > 256 || head_dim % 8 || out_dtype < BE_F32 ||
+      out_dtype > BE_BF16) {
+    set_error("be_read_paged_kv8: invalid shape or dtype");
+    return BE_EINVAL;
+  }
+  if (n == 0) return BE_OK;
+  if (!paged_kv_cache || !kv_scale || !pages || !out || (uintptr_t)paged_kv_cache % 8 ||
+      (uintptr_t)out % 16) {
+    set_error("be_read_paged_kv8: null or misaligned pointer");
+    return BE_EINVAL;
+  }
+  const int64_t vecs = (int64_t)n * 2 * page_size * num_kv_heads * (head_dim / 8);
+  const dim3 grid((unsigned)std::min<int64_t>((vecs + 255) / 256, 148 * 16));
+  cudaStream_t st = (cudaStream_t)stream;
+#define BE_READ8(T)                                                                            \
+  BE_CUDA_CHECK(launch_pdl(read_pages_kernel<T>, grid, dim3(256), 0, st,                       \
+                           (const char*)paged_kv_cache, kv_scale, pages, n, num_pages, page_size, \
+                           num_kv_heads, head_dim, (T*)out))
+  switch (out_dtype) {
+    case BE_BF16: BE_READ8(__nv_bfloat16); break;
+    case BE_F16: BE_READ8(__half); break;
+    default: BE_READ8(float);
+  }
+#undef BE_READ8
+  BE_LAUNCH_CHECK();
+  return BE_OK;
+}

@@ -9,6 +9,8 @@
 #include "attention_narrow.cu"
 #include "attention_tiles.cu"
 #include "attn_api.cu"
+#include "append_rope.cu"
+#include "attention_paged.cu"
 #include "attn_noalloc.cu"
 #include "model_ops.cu"
 #include "select_ops.cu"

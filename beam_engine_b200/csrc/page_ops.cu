@@ -113,11 +113,18 @@ __global__ void __launch_bounds__(256) append_rows_kernel(
 // In one page plane the first `len` tokens are one contiguous run of
 // len * hkv * head_dim elements, so each (copy, layer, plane) is a memcpy.
 // ---------------------------------------------------------------------------
+// Pools of 8-bit codes carry a scale per (page, plane, KV head): it goes with the tokens.
+__device__ __forceinline__ void copy_block_scales(float* scale, int src, int dst, int plane,
+                                                  int hkv) {
+  for (int h = threadIdx.x; h < hkv; h += blockDim.x)
+    scale[((int64_t)dst * 2 + plane) * hkv + h] = scale[((int64_t)src * 2 + plane) * hkv + h];
+}
+
 __global__ void __launch_bounds__(256) fork_kernel(
     char* __restrict__ pool, int64_t pool_layer_stride_b, int num_layers, int num_pages,
     int64_t plane_bytes, const int32_t* __restrict__ src_pages,
     const int32_t* __restrict__ dst_pages, const int32_t* __restrict__ lens, int64_t tok_bytes,
-    int num_segs) {
+    int num_segs, float* __restrict__ scale, int64_t scale_layer_stride, int hkv) {
   // one CTA per (copy, layer, plane) segment at a time (grid-stride); every thread
   // loads all of its <= ROW_UNROLL vectors of the segment before storing them
   for (int seg = blockIdx.x; seg < num_segs; seg += gridDim.x) {
@@ -134,6 +141,7 @@ __global__ void __launch_bounds__(256) fork_kernel(
                                                    ((int64_t)s * 2 + plane) * plane_bytes);
     int4* d4 = reinterpret_cast<int4*>(pool + layer * pool_layer_stride_b +
                                        ((int64_t)d * 2 + plane) * plane_bytes);
+    if (scale) copy_block_scales(scale + layer * scale_layer_stride, s, d, plane, hkv);
     for (int c0 = 0; c0 < n16; c0 += 256 * ROW_UNROLL) {
       int4 buf[ROW_UNROLL];
 #pragma unroll
@@ -218,6 +226,33 @@ extern "C" int be_append_paged_kv(const void* append_key, const void* append_val
   return BE_OK;
 }
 
+static int fork_tail_copy(const char* fn, void* paged_kv_cache, int64_t pool_layer_stride,
+                          float* kv_scale, int64_t scale_layer_stride, int num_layers,
+                          int num_pages, int page_size, int num_kv_heads, int head_dim, int elt,
+                          const int32_t* src_pages, const int32_t* dst_pages, const int32_t* lens,
+                          int num_copies, void* stream) {
+  const int64_t tok_bytes = (int64_t)num_kv_heads * head_dim * elt;
+  if (tok_bytes % 16 || ((uintptr_t)paged_kv_cache % 16) || (pool_layer_stride * elt) % 16) {
+    set_error("%s: pool rows must be 16-byte aligned (kv_heads*head_dim*elt %% 16)", fn);
+    return BE_EINVAL;
+  }
+  const int64_t segs = (int64_t)num_copies * num_layers * 2;
+  if (segs >= (1ll << 31)) {
+    set_error("%s: too many copies x layers (%lld segments)", fn, (long long)segs);
+    return BE_EINVAL;
+  }
+  if (((int64_t)page_size * tok_bytes) >> 4 >= (1ll << 31)) {
+    set_error("%s: page too large", fn);
+    return BE_EINVAL;
+  }
+  const int grid = (int)(segs < 148 * 8 ? segs : 148 * 8);
+  fork_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(
+      (char*)paged_kv_cache, pool_layer_stride * elt, num_layers, num_pages, page_size * tok_bytes,
+      src_pages, dst_pages, lens, tok_bytes, (int)segs, kv_scale, scale_layer_stride, num_kv_heads);
+  BE_LAUNCH_CHECK();
+  return BE_OK;
+}
+
 extern "C" int be_fork_tail_copy(void* paged_kv_cache, int64_t pool_layer_stride, int num_layers,
                                  int num_pages, int page_size, int num_kv_heads, int head_dim,
                                  int dtype, const int32_t* src_pages, const int32_t* dst_pages,
@@ -228,27 +263,28 @@ extern "C" int be_fork_tail_copy(void* paged_kv_cache, int64_t pool_layer_stride
     return BE_EINVAL;
   }
   if (num_copies == 0) return BE_OK;
-  const int elt = dtype_size(dtype);
-  const int64_t tok_bytes = (int64_t)num_kv_heads * head_dim * elt;
-  if (tok_bytes % 16 || ((uintptr_t)paged_kv_cache % 16) || (pool_layer_stride * elt) % 16) {
-    set_error("be_fork_tail_copy: pool rows must be 16-byte aligned (kv_heads*head_dim*elt %% 16)");
+  return fork_tail_copy("be_fork_tail_copy", paged_kv_cache, pool_layer_stride, nullptr, 0,
+                        num_layers, num_pages, page_size, num_kv_heads, head_dim, dtype_size(dtype),
+                        src_pages, dst_pages, lens, num_copies, stream);
+}
+
+extern "C" int be_fork_tail_copy8(void* paged_kv_cache, int64_t pool_layer_stride, float* kv_scale,
+                                  int64_t scale_layer_stride, int num_layers, int num_pages,
+                                  int page_size, int num_kv_heads, int head_dim,
+                                  const int32_t* src_pages, const int32_t* dst_pages,
+                                  const int32_t* lens, int num_copies, void* stream) {
+  if (num_copies < 0 || num_layers < 1 || page_size < 1 || num_kv_heads < 1 || head_dim < 1) {
+    set_error("be_fork_tail_copy8: invalid shape");
     return BE_EINVAL;
   }
-  const int64_t segs = (int64_t)num_copies * num_layers * 2;
-  if (segs >= (1ll << 31)) {
-    set_error("be_fork_tail_copy: too many copies x layers (%lld segments)", (long long)segs);
+  if (num_copies == 0) return BE_OK;
+  if (!paged_kv_cache || !kv_scale || !src_pages || !dst_pages || !lens) {
+    set_error("be_fork_tail_copy8: null pointer");
     return BE_EINVAL;
   }
-  if (((int64_t)page_size * tok_bytes) >> 4 >= (1ll << 31)) {
-    set_error("be_fork_tail_copy: page too large");
-    return BE_EINVAL;
-  }
-  const int grid = (int)(segs < 148 * 8 ? segs : 148 * 8);
-  fork_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(
-      (char*)paged_kv_cache, pool_layer_stride * elt, num_layers, num_pages, page_size * tok_bytes,
-      src_pages, dst_pages, lens, tok_bytes, (int)segs);
-  BE_LAUNCH_CHECK();
-  return BE_OK;
+  return fork_tail_copy("be_fork_tail_copy8", paged_kv_cache, pool_layer_stride, kv_scale,
+                        scale_layer_stride, num_layers, num_pages, page_size, num_kv_heads,
+                        head_dim, 1, src_pages, dst_pages, lens, num_copies, stream);
 }
 
 extern "C" int be_device_status(int* out, void* stream) {
@@ -275,7 +311,8 @@ namespace be {
 
 __global__ void __launch_bounds__(256) fork_list_kernel(
     char* __restrict__ pool, int64_t pool_layer_stride_b, int num_layers, int num_pages,
-    int page_size, int64_t tok_bytes, const int32_t* __restrict__ list, int cap) {
+    int page_size, int64_t tok_bytes, const int32_t* __restrict__ list, int cap,
+    float* __restrict__ scale, int64_t scale_layer_stride, int hkv) {
   const int count = min(max(list[0], 0), cap);
   const int32_t* src_pages = list + 1;
   const int32_t* dst_pages = list + 1 + cap;
@@ -296,12 +333,31 @@ __global__ void __launch_bounds__(256) fork_list_kernel(
         pool + layer * pool_layer_stride_b + ((int64_t)s * 2 + plane) * plane_bytes);
     int4* d4 = reinterpret_cast<int4*>(pool + layer * pool_layer_stride_b +
                                        ((int64_t)d * 2 + plane) * plane_bytes);
+    if (scale) copy_block_scales(scale + layer * scale_layer_stride, s, d, plane, hkv);
     const int n16 = (int)((len * tok_bytes) >> 4);
     for (int c = threadIdx.x; c < n16; c += blockDim.x) d4[c] = __ldg(s4 + c);
   }
 }
 
 }  // namespace be
+
+static int fork_tail_copy_list(const char* fn, void* paged_kv_cache, int64_t pool_layer_stride,
+                               float* kv_scale, int64_t scale_layer_stride, int num_layers,
+                               int num_pages, int page_size, int num_kv_heads, int head_dim, int elt,
+                               const int32_t* copy_list, int cap, int num_sms, void* stream) {
+  using namespace be;
+  const int64_t tok_bytes = (int64_t)num_kv_heads * head_dim * elt;
+  if (tok_bytes % 16 || ((uintptr_t)paged_kv_cache % 16) || (pool_layer_stride * elt) % 16) {
+    set_error("%s: pool rows must be 16-byte aligned", fn);
+    return BE_EINVAL;
+  }
+  const int grid = 4 * (num_sms > 0 ? num_sms : 148);
+  fork_list_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(
+      (char*)paged_kv_cache, pool_layer_stride * elt, num_layers, num_pages, page_size, tok_bytes,
+      copy_list, cap, kv_scale, scale_layer_stride, num_kv_heads);
+  BE_LAUNCH_CHECK();
+  return BE_OK;
+}
 
 extern "C" int be_fork_tail_copy_list(void* paged_kv_cache, int64_t pool_layer_stride,
                                       int num_layers, int num_pages, int page_size,
@@ -314,16 +370,23 @@ extern "C" int be_fork_tail_copy_list(void* paged_kv_cache, int64_t pool_layer_s
     set_error("be_fork_tail_copy_list: invalid arguments");
     return BE_EINVAL;
   }
-  const int elt = dtype_size(dtype);
-  const int64_t tok_bytes = (int64_t)num_kv_heads * head_dim * elt;
-  if (tok_bytes % 16 || ((uintptr_t)paged_kv_cache % 16) || (pool_layer_stride * elt) % 16) {
-    set_error("be_fork_tail_copy_list: pool rows must be 16-byte aligned");
+  return fork_tail_copy_list("be_fork_tail_copy_list", paged_kv_cache, pool_layer_stride, nullptr,
+                             0, num_layers, num_pages, page_size, num_kv_heads, head_dim,
+                             dtype_size(dtype), copy_list, cap, num_sms, stream);
+}
+
+extern "C" int be_fork_tail_copy8_list(void* paged_kv_cache, int64_t pool_layer_stride,
+                                       float* kv_scale, int64_t scale_layer_stride,
+                                       int num_layers, int num_pages, int page_size,
+                                       int num_kv_heads, int head_dim, const int32_t* copy_list,
+                                       int cap, int num_sms, void* stream) {
+  using namespace be;
+  if (!paged_kv_cache || !kv_scale || !copy_list || cap < 0 || num_layers < 1 || page_size < 1 ||
+      num_kv_heads < 1 || head_dim < 1) {
+    set_error("be_fork_tail_copy8_list: invalid arguments");
     return BE_EINVAL;
   }
-  const int grid = 4 * (num_sms > 0 ? num_sms : 148);
-  fork_list_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(
-      (char*)paged_kv_cache, pool_layer_stride * elt, num_layers, num_pages, page_size, tok_bytes,
-      copy_list, cap);
-  BE_LAUNCH_CHECK();
-  return BE_OK;
+  return fork_tail_copy_list("be_fork_tail_copy8_list", paged_kv_cache, pool_layer_stride, kv_scale,
+                             scale_layer_stride, num_layers, num_pages, page_size, num_kv_heads,
+                             head_dim, 1, copy_list, cap, num_sms, stream);
 }

@@ -36,6 +36,11 @@ def dtype_code(dt):
     return _DT[dt]
 
 
+def is_8bit(dt):
+    """Whether a pool of this dtype holds 8-bit codes with a scale per block."""
+    return dt == torch.float8_e4m3fn
+
+
 def stream_ptr(device):
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
@@ -44,6 +49,64 @@ def require_cuda(*tensors):
     for t in tensors:
         if not t.is_cuda:
             raise RuntimeError("beam_engine_b200 kernels need CUDA tensors (no CPU fallback)")
+
+
+def require_same_device(first, *tensors):
+    require_cuda(first, *tensors)
+    for t in tensors:
+        if t.device != first.device:
+            raise ValueError(f"tensors on {first.device} and {t.device}")
+
+
+def check_pool8(pool, scale):
+    """A paged cache [pages, 2, page_size, kv_heads, head_dim] of codes with its scales."""
+    if scale is None:
+        raise ValueError("a float8_e4m3fn cache needs kv_scale [pages, 2, kv_heads]")
+    if (scale.dtype != torch.float32 or not scale.is_contiguous()
+            or scale.shape != (pool.shape[0], 2, pool.shape[3])):
+        raise ValueError("kv_scale must be contiguous float32 [pages, 2, kv_heads] "
+                         f"({(pool.shape[0], 2, pool.shape[3])}), got {scale.dtype} "
+                         f"{tuple(scale.shape)}")
+
+
+def append_rows(key, value, batch_indices, positions, pool, scale, kv_indices, kv_indptr,
+                inv_freq=None, rope_positions=None):
+    """be_rope_append_paged_kv on one layer's pool: ``scale`` None for a pool of the rows' type."""
+    P, _, ps, H, D = pool.shape
+    n = key.shape[0]
+    if key.shape != (n, H, D) or value.shape != (n, H, D):
+        raise ValueError(f"rows must be [n, {H}, {D}], got {tuple(key.shape)} and "
+                         f"{tuple(value.shape)}")
+    if key.dtype != value.dtype:
+        raise ValueError(f"keys are {key.dtype}, values {value.dtype}")
+    if key.stride(-1) != 1 or key.stride(-2) != D:
+        key = key.contiguous()
+    if value.stride(-1) != 1 or value.stride(-2) != D:
+        value = value.contiguous()
+    for name, t, m in (("batch_indices", batch_indices, n), ("positions", positions, n),
+                       ("rope_positions", rope_positions, n)):
+        if t is not None and t.shape != (m,):
+            raise ValueError(f"{name} must have {m} entries, got {tuple(t.shape)}")
+    ints = [t if t is None or (t.dtype == torch.int32 and t.is_contiguous())
+            else t.to(torch.int32).contiguous()
+            for t in (batch_indices, positions, kv_indices, kv_indptr, rope_positions)]
+    if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.shape != (D // 2,)
+                                 or not inv_freq.is_contiguous()):
+        raise ValueError(f"rope_inv_freq must be contiguous float32 [{D // 2}]")
+    dev = pool.device
+    require_same_device(pool, key, value, *[t for t in (*ints, inv_freq, scale) if t is not None])
+    ws = torch.empty(4 * n + 512, dtype=torch.int32, device=dev) if n > 512 else None
+    with torch.cuda.device(dev):
+        rc = lib().be_rope_append_paged_kv(
+            key.data_ptr(), value.data_ptr(), key.stride(0), value.stride(0), ints[0].data_ptr(),
+            ints[1].data_ptr(), ints[4].data_ptr() if ints[4] is not None else None,
+            ints[2].data_ptr(), ints[3].data_ptr(), n,
+            inv_freq.data_ptr() if inv_freq is not None else None, pool.data_ptr(),
+            scale.data_ptr() if scale is not None else None, P, ps, H, D, dtype_code(key.dtype),
+            _lib.BE_E4M3 if scale is not None else dtype_code(pool.dtype),
+            ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
+            stream_ptr(dev))
+    check(rc, "append_paged_kv_cache")
 
 
 class PageTable:
@@ -66,6 +129,11 @@ class PageTable:
         self.kv_cache = torch.zeros((layer_num, max_num_pages, 2, page_size, head_num, head_dim),
                                     dtype=store_dtype, device=self.device)
         self.kv_cache_at_layer: List[torch.Tensor] = [self.kv_cache[i] for i in range(layer_num)]
+        # 8-bit pools: a scale per (layer, page, K | V, head); 0 marks a block never written
+        self.kv_scale = None
+        if is_8bit(store_dtype):
+            self.kv_scale = torch.zeros((layer_num, max_num_pages, 2, head_num),
+                                        dtype=torch.float32, device=self.device)
         self._pages_buf = np.zeros(0, np.int32)
         logger.info("Initialized PageTable: %d layers, %d pages of size %d", layer_num,
                     max_num_pages, page_size)
@@ -127,6 +195,15 @@ class PageTable:
                 return x
             return torch.as_tensor(np.asarray(x, np.int32)).to(dev, non_blocking=True)
         s, d, n = as_dev(src), as_dev(dst), as_dev(lens)
+        if self.kv_scale is not None:
+            with torch.cuda.device(dev):
+                rc = lib().be_fork_tail_copy8(
+                    self.kv_cache.data_ptr(), self._layer_stride(), self.kv_scale.data_ptr(),
+                    self.kv_scale.stride(0), self.layer_num, self.max_num_pages, self.page_size,
+                    self.head_num, self.head_dim, s.data_ptr(), d.data_ptr(), n.data_ptr(),
+                    len(src), stream_ptr(dev))
+            check(rc, "copy_blocks")
+            return
         rc = lib().be_fork_tail_copy(self.kv_cache.data_ptr(), self._layer_stride(), self.layer_num,
                                      self.max_num_pages, self.page_size, self.head_num,
                                      self.head_dim, dtype_code(self.store_dtype), s.data_ptr(),
@@ -174,6 +251,11 @@ class PageTable:
     def _append(self, layer, keys, values, batch_indices, positions, kv_indices, kv_indptr,
                 num_layers=1):
         require_cuda(keys, values, self.kv_cache)
+        if self.kv_scale is not None:
+            for i in range(layer, layer + num_layers):
+                append_rows(keys, values, batch_indices, positions, self.kv_cache_at_layer[i],
+                            self.kv_scale[i], kv_indices, kv_indptr)
+            return
         if keys.dtype != self.store_dtype or values.dtype != self.store_dtype:
             keys = keys.to(self.store_dtype)
             values = values.to(self.store_dtype)
@@ -194,7 +276,19 @@ class PageTable:
                                       stream_ptr(self.kv_cache.device))
         check(rc, "append_paged_kv")
 
-    # -- flat slot views (page_table.py:211-241), zero copy -----------------
+    def read_pages(self, layer: int, pages, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """Pages of one layer as values [n, 2, page_size, heads, head_dim]: the codes of an 8-bit
+        pool times their scales, a copy of the pages otherwise."""
+        from .page import read_paged_kv_cache
+        if not isinstance(pages, torch.Tensor):
+            pages = torch.as_tensor(np.asarray(pages, np.int32))
+        pages = pages.to(self.kv_cache.device)
+        if self.kv_scale is None:
+            return self.kv_cache_at_layer[layer][pages.long()].to(dtype)
+        return read_paged_kv_cache(self.kv_cache_at_layer[layer], pages, self.kv_scale[layer],
+                                   dtype)
+
+    # -- flat slot views (page_table.py:211-241), zero copy (codes of an 8-bit pool) ---
     def get_k_buffer(self, layer: int) -> torch.Tensor:
         return self.kv_cache_at_layer[layer][:, 0]
 

@@ -32,7 +32,8 @@ typedef enum {
   BE_ENOTSUP = 8           /* plan shape this path does not serve (the caller takes another) */
 } be_status;
 
-typedef enum { BE_F32 = 0, BE_F16 = 1, BE_BF16 = 2 } be_dtype;
+typedef enum { BE_F32 = 0, BE_F16 = 1, BE_BF16 = 2,
+               BE_E4M3 = 3 /* caches only: 8-bit codes with a scale per block */ } be_dtype;
 
 const char* be_last_error(void);
 int be_version(void);
@@ -86,6 +87,55 @@ int be_fork_tail_copy_list(void* paged_kv_cache, int64_t pool_layer_stride, int 
                            int num_pages, int page_size, int num_kv_heads, int head_dim,
                            int dtype, const int32_t* copy_list, int cap, int num_sms,
                            void* stream);
+
+/* ------------------------------------------------------------------------
+ * 8-bit pools: e4m3 codes [num_pages, 2, page_size, num_kv_heads, head_dim]
+ * and kv_scale float32 [num_pages, 2, num_kv_heads]: the values of a block
+ * (page, plane, KV head) are code * scale.  The scales that the appends write
+ * are powers of two: 2^e with e the smallest integer in [-40, 40] for which
+ * the block's largest finite value is at most 448 * 2^e, and never below the
+ * scale the block had, unless the call writes the page's slot 0: that begins
+ * the block anew (what its other slots held is void).  Where a scale grows, the
+ * other slots' codes are rounded to it.  Rounding is to nearest, ties to even;
+ * infinities and values past 448 * 2^40 become the largest code, NaN stays NaN.
+ * The reference keeps its pool in the model's type (page_table.py:62-72).
+ * ---------------------------------------------------------------------- */
+
+/* be_append_paged_kv for one layer with the position rotation (HF rotate_half,
+ * modeling_llama.py:113-157; angles in 64 bits) applied to the keys on the way
+ * when inv_freq ([head_dim / 2] float32) is not NULL, by rope_positions (NULL:
+ * `positions`).  cache_dtype BE_E4M3 (kv_scale required) or `dtype`
+ * (kv_scale NULL).  Rows may come in any order; of two rows for one slot the later
+ * one in the call is kept.  Calls with more than 512 rows need a device workspace
+ * of 4 * nnz + 512 ints (free to reuse once the call's work is done).
+ * head_dim 32, 64, 128 or 256, page_size <= 256, num_kv_heads <= 64.          */
+int be_rope_append_paged_kv(const void* append_key, const void* append_value,
+                            int64_t key_row_stride, int64_t value_row_stride,
+                            const int32_t* batch_indices, const int32_t* positions,
+                            const int32_t* rope_positions, const int32_t* kv_indices,
+                            const int32_t* kv_indptr, int nnz, const float* inv_freq,
+                            void* paged_kv_cache, float* kv_scale, int num_pages, int page_size,
+                            int num_kv_heads, int head_dim, int dtype, int cache_dtype,
+                            int32_t* workspace, int64_t workspace_ints, void* stream);
+
+/* Pages of an 8-bit pool as values: out [n][2][page_size][num_kv_heads][head_dim]
+ * in out_dtype.  A page id out of range is flagged and reads as zeros.        */
+int be_read_paged_kv8(const void* paged_kv_cache, const float* kv_scale, const int32_t* pages,
+                      int n, int num_pages, int page_size, int num_kv_heads, int head_dim,
+                      void* out, int out_dtype, void* stream);
+
+/* be_fork_tail_copy / be_fork_tail_copy_list for 8-bit pools: the codes of
+ * tokens [0, len) and the blocks' scales (scale_layer_stride floats between
+ * layers; PageTable.copy_block, page_table.py:96-106).                        */
+int be_fork_tail_copy8(void* paged_kv_cache, int64_t pool_layer_stride, float* kv_scale,
+                       int64_t scale_layer_stride, int num_layers, int num_pages, int page_size,
+                       int num_kv_heads, int head_dim, const int32_t* src_pages,
+                       const int32_t* dst_pages, const int32_t* lens, int num_copies,
+                       void* stream);
+int be_fork_tail_copy8_list(void* paged_kv_cache, int64_t pool_layer_stride, float* kv_scale,
+                            int64_t scale_layer_stride, int num_layers, int num_pages,
+                            int page_size, int num_kv_heads, int head_dim,
+                            const int32_t* copy_list, int cap, int num_sms, void* stream);
 
 /* ------------------------------------------------------------------------
  * Paged attention plans.  A plan is a flat int32 buffer built on the host by
@@ -336,6 +386,57 @@ int be_attn_tiles_run(const int32_t* plan_dev, int max_pieces, int max_tiles, in
                       int cluster, int plan_early, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Paged attention over 8-bit or 16-bit pools with a sliding window and sinks:
+ * MultiLevelCascadeAttentionWrapper / BatchPrefillWithPagedKVCacheWrapper
+ * .plan / .run (modeling_llama.py:733-755, :775-798, :362) for what those take as
+ * kv_data_type and window_left.  A sequence is the tokens of a query's groups
+ * in level order, and the queries of a last-level group are its last tokens:
+ * query i of qlen at position p = tokens - qlen + i sees
+ *   t <= p (last level, causal_last != 0) and, when window_left >= 0,
+ *   t >= p - window_left or t < num_sinks.
+ * A query that sees nothing gets out = 0, lse = -inf.
+ * Plan buffer: header (be_attn_plan_info, BE_PLAN_HEADER_INTS ints), items
+ * (wide ones first), page list, merge lists.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  int32_t q_begin, q_len;   /* consecutive queries                                  */
+  int32_t kv_off;           /* the group's pages in the page list                   */
+  int32_t v_begin, v_end;   /* tokens v of the tile's index: t = v + (v >= n0 ? shift : 0) */
+  int32_t n0, shift;
+  int32_t pos0, pos_step;   /* query i is at token pos0 + i * pos_step of the group   */
+  int32_t sink_end;         /* tokens [0, sink_end) stay visible                     */
+  int32_t window;           /* -1: none                                             */
+  int32_t flags;            /* BE_ITEM_CAUSAL                                        */
+  int32_t part_base;        /* partial row of query 0, or -1: write the output       */
+  int32_t pad[3];
+} be_paged_item;
+#define BE_ITEM_CAUSAL 1
+
+/* Arguments as be_cascade_plan; window_left -1: no window.  At most 16 query
+ * heads per KV head.  On BE_ECAPACITY info->total_ints holds the size needed. */
+int be_paged_plan(int num_levels, const int32_t* const* qo_indptr, const int32_t* const* kv_indptr,
+                  const int32_t* const* kv_indices, const int32_t* const* last_page_len,
+                  const int32_t* num_groups, int num_queries, int page_size, int num_qo_heads,
+                  int num_kv_heads, int causal_last, int window_left, int num_sinks, int num_sms,
+                  int32_t* plan, int64_t plan_capacity, be_attn_plan_info* info);
+
+/* Runs a be_paged_plan plan in device memory (header included) for one layer.
+ * The launch shape depends on the max_* capacities only and the kernels read the plan's counts
+ * from its header, so a recorded launch serves every plan with at most
+ * max_wide wide and max_narrow narrow items, max_merge merged queries and
+ * max_parts partial rows.  dtype (q, out): BE_BF16 or BE_F16; cache_dtype BE_E4M3
+ * (kv_scale required) or dtype; head_dim 64 or 128.  q [n][num_qo_heads][head_dim]
+ * with q_row_stride elements between queries.  mid_o / mid_lse: float32 scratch of
+ * max_parts * num_qo_heads * head_dim and max_parts * num_qo_heads (calls that share
+ * them must not overlap on the GPU).                                          */
+int be_paged_attn_run(const int32_t* plan_dev, int max_wide, int max_narrow, int max_merge,
+                      int max_parts, int page_size, const void* q, int64_t q_row_stride,
+                      const void* paged_kv_cache, const float* kv_scale, int num_pages,
+                      int num_qo_heads, int num_kv_heads, int head_dim, int dtype,
+                      int cache_dtype, float sm_scale, void* out, int64_t out_row_stride,
+                      float* lse, float* mid_o, float* mid_lse, void* stream);
+
+/* ------------------------------------------------------------------------
  * Decoder-layer kernels of the model runner (the reference runs these as
  * separate PyTorch ops inside src/beam_engine/models/modeling_llama.py).
  * ---------------------------------------------------------------------- */
@@ -358,6 +459,15 @@ int be_rope_qkv_append(void* qkv, int64_t row_stride, int n, int num_qo_heads, i
                        void* paged_kv_cache, int num_pages, int page_size,
                        const int32_t* write_page, const int32_t* write_pos, int rope_k_in_place,
                        int dtype, void* stream);
+
+/* be_rope_qkv_append into an 8-bit pool (its rules and limits as
+ * be_rope_append_paged_kv): q rotated in place, rotated k and v rounded into
+ * page write_page[i] slot write_pos[i]; the QKV row's k and v stay as they were. */
+int be_rope_qkv_append8(void* qkv, int64_t row_stride, int n, int num_qo_heads, int num_kv_heads,
+                        int head_dim, const int32_t* positions, const float* inv_freq,
+                        void* paged_kv_cache, float* kv_scale, int num_pages, int page_size,
+                        const int32_t* write_page, const int32_t* write_pos, int dtype,
+                        int32_t* workspace, int64_t workspace_ints, void* stream);
 
 /* LlamaMLP activation (modeling_llama.py:160-173): out = silu(gate) * up on a
  * fused [n][2*ffn] gate|up projection.                                       */
