@@ -87,11 +87,11 @@ __global__ void __launch_bounds__(128) paged_narrow_kernel(const PagedParams p) 
   pdl_wait();
   const be_attn_plan_info* hdr = reinterpret_cast<const be_attn_plan_info*>(p.plan);
   const int n_wide = hdr->n_work_wide;
-  if ((int)blockIdx.x >= hdr->n_work - n_wide) return;
+  const int item = blockIdx.x / p.hkv, kvh = blockIdx.x - item * p.hkv;
+  if (item >= hdr->n_work - n_wide) return;
   const be_paged_item w =
-      reinterpret_cast<const be_paged_item*>(p.plan + hdr->off_work)[n_wide + blockIdx.x];
+      reinterpret_cast<const be_paged_item*>(p.plan + hdr->off_work)[n_wide + item];
   const int32_t* kvlist = p.plan + hdr->off_kvlist + w.kv_off;
-  const int kvh = blockIdx.y;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
   const int g = p.g, rows = w.q_len * g;
   const bool causal = (w.flags & BE_ITEM_CAUSAL) != 0;
@@ -445,11 +445,24 @@ __global__ void __launch_bounds__(128) paged_narrow_kernel(const PagedParams p) 
   }
 }
 
+template <typename T, typename CT, int D>
+static int paged_wide_launch(const PagedParams& p, int max_wide, cudaStream_t st);
+
 template <typename T>
-static int paged_launch(const PagedParams& p, bool q8, int D, int max_narrow, int max_merge,
-                        cudaStream_t st) {
+static int paged_launch(const PagedParams& p, bool q8, int D, int max_wide, int max_narrow,
+                        int max_merge, cudaStream_t st) {
+  if (max_wide > 0) {
+    int rc;
+    if (q8)
+      rc = D == 128 ? paged_wide_launch<T, E4M3, 128>(p, max_wide, st)
+                    : paged_wide_launch<T, E4M3, 64>(p, max_wide, st);
+    else
+      rc = D == 128 ? paged_wide_launch<T, T, 128>(p, max_wide, st)
+                    : paged_wide_launch<T, T, 64>(p, max_wide, st);
+    if (rc != BE_OK) return rc;
+  }
   if (max_narrow > 0) {
-    const dim3 grid(max_narrow, p.hkv);
+    const dim3 grid((unsigned)max_narrow * p.hkv);   // heads of an item next to each other
     auto go = [&](auto kernel) -> int {
       BE_CUDA_CHECK(launch_pdl(kernel, grid, dim3(128), 0, st, p));
       return BE_OK;
@@ -484,7 +497,8 @@ extern "C" int be_paged_attn_run(const int32_t* plan_dev, int max_wide, int max_
                                  float sm_scale, void* out, int64_t out_row_stride, float* lse,
                                  float* mid_o, float* mid_lse, void* stream) {
   if (max_wide < 0 || max_narrow < 0 || max_merge < 0 || max_parts < 0 || page_size < 1 ||
-      num_pages < 1 || num_kv_heads < 1 || num_kv_heads > 65535 || num_qo_heads < 1 ||
+      num_pages < 1 || num_kv_heads < 1 || num_kv_heads > 1024 || num_qo_heads < 1 ||
+      std::max(max_wide, max_narrow) > (1 << 20) ||
       num_qo_heads % num_kv_heads) {
     set_error("be_paged_attn_run: invalid shape");
     return BE_EINVAL;
@@ -497,8 +511,8 @@ extern "C" int be_paged_attn_run(const int32_t* plan_dev, int max_wide, int max_
     set_error("be_paged_attn_run: head_dim %d is not 64 or 128", head_dim);
     return BE_EINVAL;
   }
-  if (num_qo_heads / num_kv_heads > 16) {
-    set_error("be_paged_attn_run: %d query heads per KV head (at most 16)",
+  if (num_qo_heads / num_kv_heads > 128) {
+    set_error("be_paged_attn_run: %d query heads per KV head (at most 128)",
               num_qo_heads / num_kv_heads);
     return BE_EINVAL;
   }
@@ -532,6 +546,6 @@ extern "C" int be_paged_attn_run(const int32_t* plan_dev, int max_wide, int max_
   p.mid_lse = mid_lse;
   const bool q8 = cache_dtype == BE_E4M3;
   return dtype == BE_BF16
-             ? paged_launch<__nv_bfloat16>(p, q8, head_dim, max_narrow, max_merge, (cudaStream_t)stream)
-             : paged_launch<__half>(p, q8, head_dim, max_narrow, max_merge, (cudaStream_t)stream);
+             ? paged_launch<__nv_bfloat16>(p, q8, head_dim, max_wide, max_narrow, max_merge, (cudaStream_t)stream)
+             : paged_launch<__half>(p, q8, head_dim, max_wide, max_narrow, max_merge, (cudaStream_t)stream);
 }

@@ -1,0 +1,663 @@
+// Paged attention for wide tiles (17 to 256 query-head rows) over 8-bit or 16-bit caches,
+// with a causal limit, a window and sinks, on the 5th-generation tensor cores.
+//
+// One CTA = one item of be_paged_plan x one KV head: two row tiles of 128 (row r of the
+// item is query r / g, head r % g, so a KV head's tokens are loaded once for its g
+// query heads) against tiles of 128 tokens, in one pass with a running maximum:
+//   * loader warps (4): tokens' rows from global memory into the canonical 128-byte
+//     swizzle; 8-bit codes are scaled on the way (code * 2^e is exact in bf16, and
+//     in fp16 wherever fp16 holds the value), 16-bit rows go by cp.async; tokens are
+//     addressed one by one, so any page size and the joint of sinks and window cost nothing;
+//   * one warp issues S = Q K^T (128 x 128 x D) into TMEM and O += P V (128 x D x 128) with
+//     P read from TMEM, alternating between the row tiles so that one tile's softmax
+//     runs under the other's products;
+//   * softmax warps (4 per row tile, a thread per row): maximum, exponentials, P written
+//     over S in TMEM; O is rescaled only when a row's maximum grows by more than 2^8.
+// TMEM: S/P of tile 0 | S/P of tile 1 | O of tile 0 | O of tile 1 = 256 + 2 D columns (512 allocated).
+// A tile's S of step i + 1 overwrites its P of step i: both products come from one thread, and
+// the tensor core runs them in the order of issue.
+//
+// Values that are not finite: 0 * NaN is NaN in the product, so in token tiles that some row
+// sees in part the loader replaces them by 0 and the rows that see them mark
+// the dims in shared memory (+inf, -inf, or both for NaN), applied to O at the end.
+//
+// Every wait is bounded (2 s); one that runs out sets the device status and the abort flag, and all
+// roles leave their loops.
+#include <atomic>
+#include <climits>
+
+#include "common.cuh"
+
+namespace be {
+
+constexpr int PW_TOK = 128;                    // tokens per step
+constexpr int PW_THREADS = 13 * 32;            // 8 softmax warps, 4 loader warps, 1 issuer
+constexpr int PW_HALF = PW_TOK * 128;          // 64 dims of 128 rows
+constexpr int PW_STAGES = 2;
+
+template <int D>
+struct PwSmem {
+  static constexpr int TILE = (D / 64) * PW_HALF;      // one 128 x D operand tile
+  static constexpr int Q = 0, K = 2 * TILE, V = K + PW_STAGES * TILE, ODD = V + PW_STAGES * TILE;
+  static constexpr int BAR = ODD + 256 * (D / 32) * 8;  // two bit masks of D dims per row
+  static constexpr int BYTES = BAR + 256 + 1024;
+};
+
+// D[tmem] (+)= A[tmem] * B[smem], kind::f16
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t b,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+      "%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// two fp32 operations in one instruction (sm_100)
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_unpack(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// bits [0, n) of the 32 that start at bit 32 * word
+__device__ __forceinline__ uint32_t low_bits(int n, int word) {
+  const int k = min(max(n - 32 * word, 0), 32);
+  return k == 32 ? ~0u : (1u << k) - 1u;
+}
+
+// element x of a 16-bit pair: set to zero if not finite
+template <typename T>
+__device__ __forceinline__ uint32_t zero_not_finite(uint32_t w) {
+  const uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  if ((w & e) == e) w &= 0xffff0000u;
+  if ((w & (e << 16)) == (e << 16)) w &= 0x0000ffffu;
+  return w;
+}
+
+// Bounded wait of a whole warp: every lane sees the phase, and all agree on the outcome.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  const bool ok = !*abort_flag && mbar_wait(bar, parity);
+  return __all_sync(0xffffffffu, ok);
+}
+
+template <typename T, typename CT, int D>
+__global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedParams p) {
+  constexpr bool Q8 = std::is_same<CT, E4M3>::value;
+  using SM = PwSmem<D>;
+  constexpr int NH = D / 64;
+  constexpr int ROWB = D * CacheElt<CT>::bytes;
+  constexpr int CH = ROWB / 16;                 // 16-byte chunks per (token, head) row: 4, 8 or 16
+  constexpr int TPI = 32 / CH;                  // tokens per warp and load instruction
+  constexpr int ITS = 32 / TPI;                 // instructions for a warp's 32 tokens
+  extern __shared__ char smem_raw[];
+  char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                       ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SM::BAR);
+  uint64_t* k_full = bars;                      // [2], 4 loader warps
+  uint64_t* v_full = bars + 2;                  // [2]
+  uint64_t* k_empty = bars + 4;                 // [2], commit
+  uint64_t* v_empty = bars + 6;                 // [2]
+  uint64_t* s_full = bars + 8;                  // [row tile], commit
+  uint64_t* p_full = bars + 10;                 // [row tile], 4 softmax warps
+  uint64_t* o_done = bars + 12;                 // [row tile], commit
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bars + 14);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 15);
+  volatile int* odd = reinterpret_cast<volatile int*>(bars + 16);   // [2] per V stage: step + 1
+  // which tokens of a step exist, a word per loader warp; 4 steps deep, since the loaders are at
+  // most 2 steps past the softmax
+  uint32_t* exists = reinterpret_cast<uint32_t*>(bars + 18);        // [4][4]
+  uint64_t* drain = bars + 26;
+  uint32_t* odd_mask = reinterpret_cast<uint32_t*>(smem + SM::ODD);  // [256][2][D / 32]
+
+  pdl_wait();
+  const be_attn_plan_info* hdr = reinterpret_cast<const be_attn_plan_info*>(p.plan);
+  const int item = blockIdx.x / p.hkv, kvh = blockIdx.x - item * p.hkv;
+  if (item >= hdr->n_work_wide) return;
+  const be_paged_item w = reinterpret_cast<const be_paged_item*>(p.plan + hdr->off_work)[item];
+  const int32_t* kvlist = p.plan + hdr->off_kvlist + w.kv_off;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = p.g, rows = w.q_len * g;
+  const bool two = rows > 128;
+  const int steps = (w.v_end - w.v_begin + PW_TOK - 1) / PW_TOK;
+  const bool causal = (w.flags & BE_ITEM_CAUSAL) != 0, window = w.window >= 0;
+  const int pos_hi = w.pos0 + w.pos_step * (w.q_len - 1);
+  // whether every row sees every token of the step at v0 (page ids apart)
+  auto full_step = [&](int v0) {
+    const int t_lo = v0 + (v0 >= w.n0 ? w.shift : 0);
+    const int v1 = v0 + PW_TOK - 1, t_hi = v1 + (v1 >= w.n0 ? w.shift : 0);
+    return v1 < w.v_end && (!causal || t_hi <= w.pos0) &&
+           (!window || t_lo >= pos_hi - w.window || t_hi < w.sink_end);
+  };
+
+  if (tid == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&k_full[s], 4);
+      mbar_init(&v_full[s], 4);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_empty[s], 1);
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 4);
+      mbar_init(&o_done[s], 1);
+      odd[s] = 0;
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32((const void*)tmem_slot)), "n"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (warp < 8) {   // Q rows into shared memory, zeros past the item's rows
+    constexpr int QC = D / 8;
+    for (int idx = tid; idx < 256 * QC; idx += 256) {
+      const int r = idx / QC, c = idx % QC;
+      int4 val = make_int4(0, 0, 0, 0);
+      if (r < rows)
+        val = *reinterpret_cast<const int4*>(reinterpret_cast<const T*>(p.q) +
+                                             (w.q_begin + r / g) * p.q_row_stride +
+                                             (int64_t)(kvh * g + r % g) * D + c * 8);
+      *reinterpret_cast<int4*>(smem + SM::Q + (r >> 7) * SM::TILE + (c >> 3) * PW_HALF +
+                               (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) = val;
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 12) {
+    // ---------------- issuer ----------------
+    if (lane == 0) {
+      const uint32_t id_s = umma_idesc<T>(128, PW_TOK, 0), id_o = umma_idesc<T>(128, D, 1);
+      auto issue_s = [&](int tile, int stage) {
+        const uint32_t a0 = smem_u32(smem + SM::Q + tile * SM::TILE);
+        const uint32_t b0 = smem_u32(smem + SM::K + stage * SM::TILE);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * PW_HALF + (kk & 3) * 32;
+          umma_f16(tmem + tile * 128, umma_desc(a0 + off, 16, 1024), umma_desc(b0 + off, 16, 1024),
+                   id_s, kk > 0);
+        }
+        umma_commit(&s_full[tile]);
+      };
+      auto issue_o = [&](int tile, int stage, bool first) {
+        const uint32_t b0 = smem_u32(smem + SM::V + stage * SM::TILE);
+#pragma unroll
+        for (int ks = 0; ks < PW_TOK / 16; ++ks)
+          umma_f16_ts(tmem + 256 + tile * D, tmem + tile * 128 + ks * 8,
+                      umma_desc(b0 + ks * 2048, PW_HALF, 1024), id_o, !(first && ks == 0));
+        umma_commit(&o_done[tile]);
+      };
+      bool ok = mbar_wait(&k_full[0], 0);
+      if (ok) {
+        tc_fence_after();
+        issue_s(0, 0);
+        if (two) issue_s(1, 0);
+        umma_commit(&k_empty[0]);
+      }
+      for (int i = 0; ok && i < steps; ++i) {
+        const int st = i & 1, nx = (i + 1) & 1;
+        for (int tile = 0; tile < (two ? 2 : 1); ++tile) {
+          ok = ok && !*abort_flag && mbar_wait(&p_full[tile], i & 1);
+          if (tile == 0) ok = ok && mbar_wait(&v_full[st], (i >> 1) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          issue_o(tile, st, i == 0);
+          if (i + 1 < steps) {
+            if (tile == 0) {
+              ok = mbar_wait(&k_full[nx], ((i + 1) >> 1) & 1);
+              if (!ok) break;
+              tc_fence_after();
+            }
+            issue_s(tile, nx);
+          }
+        }
+        if (ok) {
+          umma_commit(&v_empty[st]);
+          if (i + 1 < steps) umma_commit(&k_empty[nx]);
+        }
+      }
+      if (!ok) {        // leave with no product in flight
+        *abort_flag = 1;
+        umma_commit(drain);
+        mbar_wait(drain, 0);
+      }
+    }
+  } else if (warp >= 8) {
+    // ---------------- loaders ----------------
+    const int lw = warp - 8;
+    const int64_t row_step = (int64_t)p.hkv * ROWB, plane_step = row_step * p.ps;
+    const char* base = p.pool + (int64_t)kvh * ROWB;
+    const int c = lane % CH, sub = lane / CH;
+    // a warp has 32 consecutive tokens of the step; lane L locates the L-th
+    auto token_of = [&](int it) { return lw * 32 + it * TPI + sub; };
+    const int ps_shift = (p.ps & (p.ps - 1)) == 0 ? __ffs(p.ps) - 1 : -1;
+    auto token_t = [&](int v) { return v + (v >= w.n0 ? w.shift : 0); };
+    auto page_of = [&](int v0) -> int {          // page id of this lane's token, -1 past the range
+      const int v = v0 + lw * 32 + lane;
+      if (v >= w.v_end) return -1;
+      const int t = token_t(v);
+      return kvlist[ps_shift >= 0 ? t >> ps_shift : t / p.ps];
+    };
+    auto locate = [&](int v0, int page, float& sk, float& sv) -> int64_t {
+      const int v = v0 + lw * 32 + lane;
+      sk = sv = 0.f;
+      if (page < 0 || page >= p.num_pages) {
+        if (v < w.v_end) flag_range_error();
+        return -1;
+      }
+      if constexpr (Q8) {
+        const float* s = p.scale + (int64_t)page * 2 * p.hkv + kvh;
+        sk = s[0];
+        sv = s[p.hkv];
+      }
+      const int t = token_t(v);
+      return (int64_t)page * 2 * plane_step +
+             (int64_t)(ps_shift >= 0 ? t & (p.ps - 1) : t % p.ps) * row_step;
+    };
+    auto dst_of = [&](char* tile, int tok, int chunk) {   // 16-byte chunk of 8 dims
+      return tile + (chunk >> 3) * PW_HALF + tok * 128 + (((chunk & 7) ^ (tok & 7)) << 4);
+    };
+    auto publish = [&](int i, int64_t at) {
+      const uint32_t has = __ballot_sync(0xffffffffu, at >= 0);
+      if (lane == 0) exists[(i & 3) * 4 + lw] = has;
+    };
+    auto signal = [&](uint64_t* bar) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    bool ok = true;
+    if constexpr (Q8) {
+      int4 ka[ITS], va[ITS];
+      auto load = [&](int4* buf, int64_t at, int64_t plane) {
+#pragma unroll
+        for (int it = 0; it < ITS; ++it) {
+          const int64_t o = __shfl_sync(0xffffffffu, at, it * TPI + sub);
+          buf[it] = o >= 0 ? __ldg(reinterpret_cast<const int4*>(base + o + plane + c * 16))
+                           : make_int4(0, 0, 0, 0);
+        }
+      };
+      auto store = [&](char* tile, const int4* buf, float scale, bool check) -> bool {
+        bool bad = false;
+#pragma unroll
+        for (int it = 0; it < ITS; ++it) {
+          const float s = __shfl_sync(0xffffffffu, scale, it * TPI + sub);
+          const uint64_t s2 = f2_pack(s, s);
+          const uint32_t wd[4] = {(uint32_t)buf[it].x, (uint32_t)buf[it].y, (uint32_t)buf[it].z,
+                                  (uint32_t)buf[it].w};
+          uint32_t o[8];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            float f[4];
+            e4m3x4_to_f(wd[x], f);
+            f2_unpack(f2_mul(f2_pack(f[0], f[1]), s2), f[0], f[1]);
+            f2_unpack(f2_mul(f2_pack(f[2], f[3]), s2), f[2], f[3]);
+            o[2 * x] = pack2<T>(f[0], f[1]);
+            o[2 * x + 1] = pack2<T>(f[2], f[3]);
+          }
+          if (check) {
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+              const uint32_t z = zero_not_finite<T>(o[x]);
+              bad |= z != o[x];
+              o[x] = z;
+            }
+          }
+          const int tok = token_of(it);
+          // the second half of the row's chunks stores its odd piece first: no bank twice
+          const int sw = c >= CH / 2 ? 1 : 0;
+          *reinterpret_cast<int4*>(dst_of(tile, tok, 2 * c + sw)) =
+              sw ? make_int4(o[4], o[5], o[6], o[7]) : make_int4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<int4*>(dst_of(tile, tok, 2 * c + 1 - sw)) =
+              sw ? make_int4(o[0], o[1], o[2], o[3]) : make_int4(o[4], o[5], o[6], o[7]);
+        }
+        return bad;
+      };
+      float sk, sv;
+      int64_t at = locate(w.v_begin, page_of(w.v_begin), sk, sv);
+      load(ka, at, 0);
+      int page_next = page_of(w.v_begin + PW_TOK);
+      for (int i = 0; i < steps; ++i) {
+        const int st = i & 1, v0 = w.v_begin + i * PW_TOK;
+        const bool check = !full_step(v0);
+        load(va, at, plane_step);
+        if (i >= 2) ok = warp_wait(&k_empty[st], ((i >> 1) - 1) & 1, abort_flag);
+        if (!ok) break;
+        store(smem + SM::K + st * SM::TILE, ka, sk, false);
+        publish(i, at);
+        signal(&k_full[st]);
+        const float sv_now = sv;
+        if (i + 1 < steps) {
+          at = locate(v0 + PW_TOK, page_next, sk, sv);
+          load(ka, at, 0);
+          page_next = page_of(v0 + 2 * PW_TOK);
+        }
+        if (i >= 2) ok = warp_wait(&v_empty[st], ((i >> 1) - 1) & 1, abort_flag);
+        if (!ok) break;
+        if (store(smem + SM::V + st * SM::TILE, va, sv_now, check)) odd[st] = i + 1;
+        signal(&v_full[st]);
+      }
+    } else {
+      auto copy = [&](char* tile, int64_t at, int64_t plane) {
+#pragma unroll
+        for (int it = 0; it < ITS; ++it) {
+          const int64_t o = __shfl_sync(0xffffffffu, at, it * TPI + sub);
+          cp_async16(smem_u32(dst_of(tile, token_of(it), c)),
+                     o >= 0 ? base + o + plane + c * 16 : p.pool, o >= 0);
+        }
+        cp_commit();
+      };
+      auto finish_v = [&](int i) {    // V of step i has landed: look at it where rows see it in part
+        const int st = i & 1;
+        if (!full_step(w.v_begin + i * PW_TOK)) {
+          bool bad = false;
+#pragma unroll
+          for (int it = 0; it < ITS; ++it) {
+            int4* a = reinterpret_cast<int4*>(dst_of(smem + SM::V + st * SM::TILE, token_of(it), c));
+            const int4 x = *a;
+            const int4 z = make_int4(zero_not_finite<T>(x.x), zero_not_finite<T>(x.y),
+                                     zero_not_finite<T>(x.z), zero_not_finite<T>(x.w));
+            if (z.x != x.x || z.y != x.y || z.z != x.z || z.w != x.w) {
+              bad = true;
+              *a = z;
+            }
+          }
+          if (bad) odd[st] = i + 1;
+        }
+        signal(&v_full[st]);
+      };
+      float sk, sv;
+      int page_next = page_of(w.v_begin);
+      for (int i = 0; i < steps; ++i) {
+        const int st = i & 1, v0 = w.v_begin + i * PW_TOK;
+        const int64_t at = locate(v0, page_next, sk, sv);
+        page_next = page_of(v0 + PW_TOK);
+        if (i >= 2) ok = warp_wait(&k_empty[st], ((i >> 1) - 1) & 1, abort_flag);
+        if (!ok) break;
+        copy(smem + SM::K + st * SM::TILE, at, 0);
+        publish(i, at);
+        if (i > 0) {
+          cp_wait<1>();
+          finish_v(i - 1);
+        }
+        if (i >= 2) ok = warp_wait(&v_empty[st], ((i >> 1) - 1) & 1, abort_flag);
+        if (!ok) break;
+        copy(smem + SM::V + st * SM::TILE, at, plane_step);
+        cp_wait<1>();
+        signal(&k_full[st]);
+      }
+      cp_wait<0>();
+      if (ok) finish_v(steps - 1);
+    }
+    if (!ok) *abort_flag = 1;
+  } else {
+    // ---------------- softmax: one row per thread ----------------
+    const int tile = warp >> 2, row = tid;                 // rows 0..255 of the item
+    if (tile == 0 || two) {
+      const uint32_t quad = (uint32_t)((warp & 3) * 32) << 16;
+      const uint32_t t_s = tmem + tile * 128 + quad, t_o = tmem + 256 + tile * D + quad;
+      const int pos = w.pos0 + w.pos_step * (row / g);
+      const float scale = p.scale_log2;
+      // what the row sees, in v: v <= vc and (v < vs or v >= vw).  With a gap the tokens before n0
+      // are the sinks; without one t is v.
+      const int vc = !causal ? INT_MAX - 1 : w.shift == 0 ? pos : pos >= w.n0 + w.shift
+                                                    ? pos - w.shift : min(pos, w.n0 - 1);
+      const int vs = w.shift == 0 ? w.sink_end : w.n0;
+      const int vw = window ? pos - w.window - w.shift : INT_MIN;
+      float m = kNoMax, l = 0.f;
+      bool ok = true, marked = false;
+      for (int i = 0; i < steps; ++i) {
+        const int v0 = w.v_begin + i * PW_TOK;
+        ok = warp_wait(&s_full[tile], i & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const uint4 ex4 = *reinterpret_cast<const uint4*>(exists + (i & 3) * 4);
+        // a negative scale turns the maximum around: such calls take the masked path throughout
+        const bool full = full_step(v0) && scale >= 0.f && (ex4.x & ex4.y & ex4.z & ex4.w) == ~0u;
+        uint32_t see[4] = {ex4.x, ex4.y, ex4.z, ex4.w};
+        if (!full) {
+          const int kc = (vc >= v0 + PW_TOK ? PW_TOK : vc - v0 + 1), ks = min(vs - v0, PW_TOK);
+          const int kw = vw <= v0 ? 0 : min(vw - v0, PW_TOK);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            see[j] &= low_bits(kc, j) & (low_bits(ks, j) | ~low_bits(kw, j));
+        }
+        uint32_t x[64];
+        float mx;
+        if (full) {
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c0 = 0; c0 < PW_TOK; c0 += 64) {
+            tmem_ld32_nw(t_s + c0, x);
+            tmem_ld32_nw(t_s + c0 + 32, x + 32);
+            tmem_wait();
+#pragma unroll
+            for (int k = 0; k < 64; k += 8)
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                m4[j] = fmaxf(fmaxf(m4[j], __uint_as_float(x[k + j])), __uint_as_float(x[k + 4 + j]));
+          }
+          mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * scale;
+        } else {
+          mx = -INFINITY;
+#pragma unroll 1
+          for (int j = 0; j < 4; ++j) {
+            tmem_ld32_nw(t_s + 32 * j, x);
+            tmem_wait();
+            const uint32_t bits = j == 0 ? see[0] : j == 1 ? see[1] : j == 2 ? see[2] : see[3];
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              mx = fmaxf(mx, (bits >> k) & 1 ? __uint_as_float(x[k]) * scale : -INFINITY);
+          }
+        }
+        if (__any_sync(0xffffffffu, mx > m + kLazyMax)) {
+          const float to = fmaxf(m, mx), f = ex2(m - to);
+          m = to;
+          l *= f;
+          if (i > 0) {        // O of the steps before: complete, then rescaled
+            ok = warp_wait(&o_done[tile], (i - 1) & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c0 = 0; c0 < D; c0 += 32) {
+              tmem_ld32_nw(t_o + c0, x);
+              tmem_wait();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * f);
+              tmem_st32(t_o + c0, x);
+            }
+            tmem_wait_st();
+          }
+        }
+        if (full) {
+          const uint64_t s2 = f2_pack(scale, scale), m2 = f2_pack(-m, -m);
+          uint64_t sum[2] = {0, 0};
+#pragma unroll
+          for (int c0 = 0; c0 < PW_TOK; c0 += 64) {
+            tmem_ld32_nw(t_s + c0, x);
+            tmem_ld32_nw(t_s + c0 + 32, x + 32);
+            tmem_wait();
+#pragma unroll
+            for (int h = 0; h < 64; h += 32) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int k = h; k < h + 32; k += 2) {
+                float a, b;
+                f2_unpack(f2_fma(f2_pack(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), s2, m2), a, b);
+                a = ex2(a);
+                b = ex2(b);
+                sum[(k >> 1) & 1] = f2_add(sum[(k >> 1) & 1], f2_pack(a, b));
+                pk[(k - h) >> 1] = pack2<T>(a, b);
+              }
+              tmem_st16(t_s + (c0 + h) / 2, pk);
+            }
+          }
+          float a, b;
+          f2_unpack(f2_add(sum[0], sum[1]), a, b);
+          l += a + b;
+        } else {
+#pragma unroll 1
+          for (int j = 0; j < 4; ++j) {
+            tmem_ld32_nw(t_s + 32 * j, x);
+            tmem_wait();
+            const uint32_t bits = j == 0 ? see[0] : j == 1 ? see[1] : j == 2 ? see[2] : see[3];
+            uint32_t pk[16];
+#pragma unroll
+            for (int k = 0; k < 32; k += 2) {
+              float a = ex2(fmaf(__uint_as_float(x[k]), scale, -m));
+              float b = ex2(fmaf(__uint_as_float(x[k + 1]), scale, -m));
+              a = (bits >> k) & 1 ? a : 0.f;
+              b = (bits >> k) & 2 ? b : 0.f;
+              l += a + b;
+              pk[k >> 1] = pack2<T>(a, b);
+            }
+            tmem_st16(t_s + 16 * j, pk);
+          }
+        }
+        tmem_wait_st();
+        if (!full_step(v0)) {
+          // values that are not finite, taken out of V: mark the dims of the rows that see them
+          // (before P is handed over: V's stage and its flag stay until P V of this step is done)
+          ok = warp_wait(&v_full[i & 1], (i >> 1) & 1, abort_flag);
+          if (!ok) break;
+          if (odd[i & 1] == i + 1) {
+            uint32_t* mask = odd_mask + row * (2 * (D / 32));
+            if (!marked)
+              for (int k = 0; k < 2 * (D / 32); ++k) mask[k] = 0;
+            marked = true;
+            for (int k = 0; row < rows && k < min(PW_TOK, w.v_end - v0); ++k) {
+              const int v = v0 + k, t = v + (v >= w.n0 ? w.shift : 0);
+              const int page = kvlist[t / p.ps];
+              if (page < 0 || page >= p.num_pages || (causal && t > pos) ||
+                  (window && t < pos - w.window && t >= w.sink_end))
+                continue;
+              const int64_t r = ((int64_t)page * 2 + 1) * p.ps + t % p.ps;
+              const char* src = p.pool + (r * p.hkv + kvh) * ROWB;
+              float s = 1.f;
+              if constexpr (Q8) s = p.scale[((int64_t)page * 2 + 1) * p.hkv + kvh];
+              for (int d = 0; d < D; ++d) {
+                float val;
+                if constexpr (Q8) {
+                  const uint32_t h2 = e4m3x2_to_h2(*reinterpret_cast<const uint8_t*>(src + d));
+                  val = to_f(from_f<T>(__low2float(*reinterpret_cast<const __half2*>(&h2)) * s));
+                } else {
+                  val = to_f(reinterpret_cast<const T*>(src)[d]);
+                }
+                if (!(val < INFINITY)) mask[d >> 5] |= 1u << (d & 31);
+                if (!(val > -INFINITY)) mask[D / 32 + (d >> 5)] |= 1u << (d & 31);
+              }
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[tile]);
+      }
+      // ---- epilogue ----
+      if (ok) ok = warp_wait(&o_done[tile], (steps - 1) & 1, abort_flag);
+      if (ok) {
+        tc_fence_after();
+        const float inv = l != 0.f ? 1.f / l : 0.f;
+        const int qi = row / g, head = kvh * g + row % g;
+        const int64_t dst_q = w.part_base < 0 ? w.q_begin + qi : w.part_base + qi;
+#pragma unroll
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t u[32];
+          tmem_ld32_nw(t_o + c0, u);
+          tmem_wait();
+          if (row >= rows) continue;
+          float f[32];
+#pragma unroll
+          for (int k = 0; k < 32; ++k) f[k] = l != 0.f ? __uint_as_float(u[k]) * inv : 0.f;
+          if (marked) {
+            const uint32_t up = odd_mask[row * (2 * (D / 32)) + (c0 >> 5)];
+            const uint32_t dn = odd_mask[row * (2 * (D / 32)) + D / 32 + (c0 >> 5)];
+            if (up | dn)
+#pragma unroll
+              for (int k = 0; k < 32; ++k) {
+                if ((up >> k) & 1) f[k] += INFINITY;
+                if ((dn >> k) & 1) f[k] -= INFINITY;
+              }
+          }
+          if (w.part_base < 0) {
+            T* dst = reinterpret_cast<T*>(p.out) + dst_q * p.out_row_stride + (int64_t)head * D + c0;
+#pragma unroll
+            for (int k = 0; k < 32; k += 4)
+              *reinterpret_cast<uint2*>(dst + k) =
+                  make_uint2(pack2<T>(f[k], f[k + 1]), pack2<T>(f[k + 2], f[k + 3]));
+          } else {
+            float* dst = p.mid_o + (dst_q * p.hq + head) * D + c0;
+#pragma unroll
+            for (int k = 0; k < 32; k += 4)
+              *reinterpret_cast<float4*>(dst + k) = make_float4(f[k], f[k + 1], f[k + 2], f[k + 3]);
+          }
+        }
+        if (row < rows) {
+          const float lse = l > 0.f ? (m + log2f(l)) * kLn2 : l == 0.f ? -INFINITY : l;
+          if (w.part_base >= 0)     // NaN as +inf: see the narrow kernel
+            p.mid_lse[dst_q * p.hq + head] = l >= 0.f ? lse : INFINITY;
+          else if (p.lse)
+            p.lse[dst_q * p.hq + head] = lse;
+        }
+      } else {
+        *abort_flag = 1;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
+  }
+}
+
+template <typename T, typename CT, int D>
+static int paged_wide_launch(const PagedParams& p, int max_wide, cudaStream_t st) {
+  auto kernel = paged_wide_kernel<T, CT, D>;
+  static std::atomic<uint64_t> ready{0};     // per device: the shared-memory limit is set
+  int dev = 0;
+  BE_CUDA_CHECK(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(ready.load() & bit)) {
+    BE_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       PwSmem<D>::BYTES));
+    ready.fetch_or(bit);
+  }
+  BE_CUDA_CHECK(launch_pdl(kernel, dim3((unsigned)max_wide * p.hkv), dim3(PW_THREADS),
+                           PwSmem<D>::BYTES, st, p));
+  return BE_OK;
+}
+
+}  // namespace be

@@ -9,7 +9,7 @@
 // and a window costs no partly filled steps and no second item.
 //
 // Narrow tiles hold up to 16 query-head rows (one query's heads, or a few), wide
-// tiles up to BE_PAGED_WIDE_ROWS.  Long ranges are split so that the items fill
+// tiles up to 256.  Long ranges are split so that the items fill
 // the GPU; rows in several items are partial and merged by log-sum-exp.
 #include <algorithm>
 #include <climits>
@@ -38,6 +38,57 @@ struct Tile {           // a run's queries [q0, q0 + ql) and the tokens they see
   bool wide;
 };
 
+// Steps of 128 tokens per wide item.  One CTA (item x KV head) occupies an SM, so what counts is
+// when the last SM is done if CTAs go longest first to whichever SM is free: that is tried for
+// whole tiles and for cuts at fractions of the average load, with 2 steps' time for a CTA's start
+// and end, one more for writing partial rows and 3 for their merge.
+int wide_chunk(const std::vector<Tile>& tiles, int64_t total_steps, int sms, int hkv) {
+  int longest = 0;
+  int64_t n = 0;
+  for (const Tile& t : tiles)
+    if (t.wide) {
+      longest = std::max(longest, (t.n + 127) / 128);
+      ++n;
+    }
+  if (n == 0 || n * hkv > 8 * (int64_t)sms) return 1 << 20;   // many CTAs: even as they are
+  const int64_t load = std::max<int64_t>(1, total_steps * hkv / sms);
+  int best_chunk = 1 << 20;
+  int64_t best = INT64_MAX;
+  std::vector<int> cost;
+  std::vector<int64_t> busy;
+  for (const double f : {0.0, 1.0, 0.5, 0.34, 0.25, 0.125}) {
+    const int chunk = f == 0.0 ? 1 << 20 : (int)std::max<int64_t>(1, (int64_t)(load * f + 0.999));
+    if (f != 0.0 && chunk >= longest) continue;
+    cost.clear();
+    bool split = false;
+    for (const Tile& t : tiles) {
+      if (!t.wide) continue;
+      const int steps = (t.n + 127) / 128, ns = (steps + chunk - 1) / chunk;
+      const int len = (steps + ns - 1) / ns;
+      split = split || ns > 1;
+      for (int s = 0; s < steps; s += len)
+        for (int h = 0; h < hkv; ++h) cost.push_back(std::min(len, steps - s) + 2 + (ns > 1));
+    }
+    if (cost.size() > 65536) continue;
+    std::sort(cost.begin(), cost.end(), [](int a, int b) { return a > b; });
+    busy.assign(sms, 0);
+    auto later = [](int64_t a, int64_t b) { return a > b; };      // min-heap
+    int64_t end = 0;
+    for (const int c : cost) {
+      std::pop_heap(busy.begin(), busy.end(), later);
+      busy.back() += c;
+      end = std::max(end, busy.back());
+      std::push_heap(busy.begin(), busy.end(), later);
+    }
+    end += split ? 3 : 0;
+    if (end < best) {
+      best = end;
+      best_chunk = chunk;
+    }
+  }
+  return best_chunk;
+}
+
 }  // namespace
 }  // namespace be
 
@@ -55,8 +106,8 @@ extern "C" int be_paged_plan(int num_levels, const int32_t* const* qo_indptr,
     return BE_EINVAL;
   }
   const int g = num_qo_heads / num_kv_heads;
-  if (g > 16) {
-    set_error("be_paged_plan: %d query heads per KV head (at most 16)", g);
+  if (g > 128) {
+    set_error("be_paged_plan: %d query heads per KV head (at most 128)", g);
     return BE_EINVAL;
   }
   // tokens of every query over all levels, and the start of each level's part
@@ -144,16 +195,20 @@ extern "C" int be_paged_plan(int num_levels, const int32_t* const* qo_indptr,
   }
   // tiles
   std::vector<Tile> tiles;
-  int64_t narrow_tokens = 0;
+  int64_t narrow_tokens = 0, wide_steps = 0;
   for (size_t r = 0; r < runs.size(); ++r) {
     const Run& R = runs[r];
-    const int tq = std::max(1, 16 / g);
+    // up to 16 rows the narrow kernel reads each token once for all of them; more rows are
+    // the tensor cores' (256 per tile, the tiles of a run of even size)
+    const bool wide = R.q_len * g > 16;
+    const int most = wide ? 256 / g : 16 / g;
+    const int nt = (R.q_len + most - 1) / most, tq = (R.q_len + nt - 1) / nt;
     for (int q0 = 0; q0 < R.q_len; q0 += tq) {
       Tile t;
       t.run = (int)r;
       t.q0 = q0;
       t.ql = std::min(tq, R.q_len - q0);
-      t.wide = false;
+      t.wide = wide;
       const int64_t pmin = R.pos0 + (int64_t)R.step * q0;
       const int64_t pmax = R.pos0 + (int64_t)R.step * (q0 + t.ql - 1);
       const int64_t hi = R.causal ? std::min<int64_t>(R.kv_len, pmax + 1) : R.kv_len;
@@ -170,7 +225,8 @@ extern "C" int be_paged_plan(int num_levels, const int32_t* const* qo_indptr,
         t.n = (int)(s + std::max<int64_t>(0, hi - lo));
       }
       if (t.n <= 0) continue;
-      narrow_tokens += t.n;
+      if (wide) wide_steps += (t.n + 127) / 128;
+      else narrow_tokens += t.n;
       tiles.push_back(t);
     }
   }
@@ -179,6 +235,7 @@ extern "C" int be_paged_plan(int num_levels, const int32_t* const* qo_indptr,
   const int64_t target = std::max<int64_t>(1, (int64_t)sms * 3 / num_kv_heads);
   const int64_t even = (narrow_tokens + target - 1) / std::max<int64_t>(1, target);
   const int chunk_n = (int)std::min<int64_t>(1 << 28, std::max<int64_t>(256, (even + 63) / 64 * 64));
+  const int chunk_w = wide_chunk(tiles, wide_steps, sms, num_kv_heads) * 128;
   struct Item {
     int tile, v0, v1, part;
   };
@@ -186,8 +243,9 @@ extern "C" int be_paged_plan(int num_levels, const int32_t* const* qo_indptr,
   std::vector<int32_t> cover(num_queries, 0);
   for (size_t i = 0; i < tiles.size(); ++i) {
     const Tile& t = tiles[i];
-    const int nsplit = (t.n + chunk_n - 1) / chunk_n;
-    const int len = ((t.n + nsplit - 1) / nsplit + 15) / 16 * 16;
+    const int chunk = t.wide ? chunk_w : chunk_n, unit = t.wide ? 128 : 16;
+    const int nsplit = (t.n + chunk - 1) / chunk;
+    const int len = ((t.n + nsplit - 1) / nsplit + unit - 1) / unit * unit;
     for (int v = 0; v < t.n; v += len) {
       items.push_back({(int)i, v, std::min(t.n, v + len), -1});
       for (int q = 0; q < t.ql; ++q) cover[runs[t.run].q_begin + t.q0 + q]++;

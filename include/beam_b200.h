@@ -412,7 +412,7 @@ typedef struct {
 } be_paged_item;
 #define BE_ITEM_CAUSAL 1
 
-/* Arguments as be_cascade_plan; window_left -1: no window.  At most 16 query
+/* Arguments as be_cascade_plan; window_left -1: no window.  At most 128 query
  * heads per KV head.  On BE_ECAPACITY info->total_ints holds the size needed. */
 int be_paged_plan(int num_levels, const int32_t* const* qo_indptr, const int32_t* const* kv_indptr,
                   const int32_t* const* kv_indices, const int32_t* const* last_page_len,

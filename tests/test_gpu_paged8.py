@@ -4,10 +4,13 @@
 Tolerances.  A code is the nearest of the block's values: at most half a step away, 2^-4 of the
 value (e4m3: 4 significant bits) or half the smallest step, s * 2^-10; rotated keys carry a few
 fp32 roundings besides.  Attention: the output is rounded once (eps / 2 of its type), the
-probabilities once (fp16 2^-11 over an 8-bit cache, eps / 2 of the cache's type otherwise; so
+probabilities once (fp16 2^-11 in narrow tiles over an 8-bit cache, eps / 2 of the query's type
+otherwise; so
 the output moves by at most that times A = sum p |v|), and scores in fp32 move each
 probability by a relative 2.4e-4 at the sizes here: D + 4 = 132 roundings of 2^-24 of sums whose terms
 come to sum |q k| sm_scale <= 30, 132 * 2^-24 * 30 = 2.36e-4 (the hardware exponential's 2^-22 besides).
+Below 2^-14 fp16 has steps of 2^-24: a probability there is off by up to 2^-25 of the row's
+largest, the output by 2^-25 B, B = sum |v| (a dim in which the heavy tokens have values near 0).
 (One token of weight near 1 whose probability and output round the same way takes the two half steps
 in full, so this term has to hold the scores' error alone.)"""
 import ctypes as C
@@ -314,14 +317,15 @@ def test_page_table_in_8_bits_copies_scales_with_tokens():
 # attention
 # ---------------------------------------------------------------------------
 def reference(q, pool, scale, ptr, pages, kv, qo, causal, window, sinks, sm):
-    """(out, lse, A) per query in 64 bits; A = sum p |v|.  Tokens a query does not see do not
+    """(out, lse, A, B) per query in 64 bits; A = sum p |v|, B = sum |v|.  Tokens a query does not see do not
     enter, whatever their cache slots hold."""
     val = pool.double() if scale is None else pool.double() * scale.double()[:, :, None, :, None]
     n, hq, d = q.shape
     hkv = pool.shape[3]
     g = hq // hkv
     out = torch.zeros((n, hq, d), dtype=torch.float64, device="cuda")
-    size, lse = torch.zeros_like(out), torch.full((n, hq), -math.inf, dtype=torch.float64, device="cuda")
+    size, whole = torch.zeros_like(out), torch.zeros_like(out)
+    lse = torch.full((n, hq), -math.inf, dtype=torch.float64, device="cuda")
     for r in range(len(kv)):
         m = qo[r + 1] - qo[r]
         if not m:
@@ -340,8 +344,9 @@ def reference(q, pool, scale, ptr, pages, kv, qo, causal, window, sinks, sm):
             pr = torch.exp(x - e[..., None])
             out[qo[r] + i] = torch.einsum("hgt,thd->hgd", pr, v).reshape(hq, d)
             size[qo[r] + i] = torch.einsum("hgt,thd->hgd", pr, v.abs()).reshape(hq, d)
+            whole[qo[r] + i] = v.abs().sum(0).repeat_interleave(g, 0)
             lse[qo[r] + i] = e.reshape(hq)
-    return out, lse, size
+    return out, lse, size, whole
 
 
 def make_pool(P, ps, hkv, d, dt, cache8, seed, spread=4, clean=True):
@@ -357,20 +362,22 @@ def make_pool(P, ps, hkv, d, dt, cache8, seed, spread=4, clean=True):
 
 
 def compare(out, lse, ref, dt, u):
-    o, e, a = ref
+    o, e, a, b = ref
     eps = torch.finfo(dt).eps / 2
     got = out.double()
     bad = torch.isnan(o)
     assert torch.equal(torch.isnan(got), bad)
-    tol = eps * o.abs() + (u + 2.4e-4) * a + 2.0 ** -24
+    tol = eps * o.abs() + (u + 2.4e-4) * a + 2.0 ** -24 + (2.0 ** -25 * b if u == 2.0 ** -11 else 0)
     assert ((got - o).abs()[~bad] <= tol[~bad]).all(), ((got - o).abs() / tol)[~bad].max()
     live = torch.isfinite(e)
     assert torch.equal(torch.isfinite(lse), live) and torch.equal(torch.isnan(lse), torch.isnan(e))
     assert ((lse.double() - e)[live].abs() <= 2e-5).all()
 
 
-def u_of(dt, cache8):
-    return 2.0 ** -11 if cache8 else torch.finfo(dt).eps / 2
+def u_of(dt, cache8, rows=1):
+    """Half a step of the type that P is rounded to: narrow tiles (16 rows) of an 8-bit cache use fp16,
+    wide ones the query's type."""
+    return 2.0 ** -11 if cache8 and rows <= 16 else torch.finfo(dt).eps / 2
 
 
 def single(dt, cache8, hq, hkv, d, ps, qlen, kv, causal, window, sinks, seed, qmul=1.5, poison=None,
@@ -396,7 +403,7 @@ def single(dt, cache8, hq, hkv, d, ps, qlen, kv, causal, window, sinks, seed, qm
     out, lse = w.run(q, pool, return_lse=True, kv_scale=scale)
     ref = reference(q, pool, scale, ptr, pages, kv, qo, causal, window, sinks,
                     d ** -0.5 if sm is None else sm)
-    compare(out, lse, ref, dt, u_of(dt, cache8))
+    compare(out, lse, ref, dt, u_of(dt, cache8, max(qlen) * (hq // hkv)))
     return w, q, pool, scale, out, lse
 
 
@@ -419,6 +426,41 @@ def test_paged_attention(dt, cache8, window, sinks, hq, hkv, d, ps, shape, clean
 @pytest.mark.parametrize("window,sinks", [(100, 4), (2000, 0), (10 ** 9, 0)])
 def test_long_contexts_are_split_and_merged(cache8, window, sinks):
     single(torch.bfloat16, cache8, 8, 2, 128, 16, [1, 2], [5003, 2500], True, window, sinks, 3)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cache8,window,sinks", [(True, -1, 0), (True, 300, 130), (False, 77, 5),
+                                                 (False, 10 ** 6, 0)])
+@pytest.mark.parametrize("hq,hkv,d,ps,qlen,kv", [
+    (8, 2, 128, 16, [300, 64], [1100, 64]), (4, 4, 64, 8, [257], [700]), (10, 2, 128, 16, [129], [129]),
+    (64, 1, 64, 16, [1, 5], [400, 333]), (128, 1, 128, 32, [3], [200]), (34, 2, 128, 16, [1], [3000])])
+def test_wide_tiles(dt, cache8, window, sinks, hq, hkv, d, ps, qlen, kv):
+    """More than 16 rows per KV head: prompts, chunks after a context, many heads per KV head."""
+    single(dt, cache8, hq, hkv, d, ps, qlen, kv, True, window, sinks, 7)
+    assert status() == 0
+
+
+def test_wide_tiles_split_over_tokens():
+    """One chunk after a long context: its tiles are cut and merged."""
+    w, *_ = single(torch.bfloat16, True, 8, 2, 128, 16, [40], [9000], True, -1, 0, 8)
+    assert w._inner._plan.info.n_parts > 40
+
+
+@pytest.mark.parametrize("qlen", [1, 40])
+def test_pages_that_do_not_exist_inside_a_tile(qlen):
+    """A bad page id in the middle of a sequence: its tokens drop out, the call is flagged."""
+    from beam_engine_b200.cascade import BatchPrefillWithPagedKVCacheWrapper
+    pool, scale = make_pool(40, 16, 2, 64, torch.bfloat16, True, 1)
+    q = torch.randn((qlen, 8, 64), device="cuda").bfloat16()
+    w = BatchPrefillWithPagedKVCacheWrapper(torch.empty(8 << 20, dtype=torch.uint8, device="cuda"))
+    pages = list(range(30))
+    w.plan([0, qlen], [0, 30], pages[:7] + [-3] + pages[8:20] + [40] + pages[21:], [16], 8, 2, 64, 16,
+           causal=False, kv_data_type=F8)
+    out, lse = w.run(q, pool, return_lse=True, kv_scale=scale)
+    keep = pages[:7] + pages[8:20] + pages[21:]
+    ref = reference(q, pool, scale, [0, 28], keep, [448], [0, qlen], False, -1, 0, 0.125)
+    compare(out, lse, ref, torch.bfloat16, 2.0 ** -11 if qlen == 1 else 2.0 ** -8)
+    assert status() == _lib.BE_EDEVICE_RANGE
 
 
 @pytest.mark.parametrize("window,sinks", [(-1, 0), (10, 2)])
@@ -480,12 +522,12 @@ def test_a_value_that_is_not_finite_reaches_only_the_queries_that_see_it(dt, cac
         w.plan([0, qlen], [0, n_p], pages, [(kv - 1) % ps + 1], 8, 2, 64, ps, causal=True,
                window_left=window, num_sinks=2, kv_data_type=F8 if cache8 else dt)
         out, lse = w.run(q, pool, return_lse=True, kv_scale=scale)
-        o, e, a = reference(q, pool, scale, [0, n_p], pages, [kv], [0, qlen], True, window, 2, 0.125)
+        o, e, a, _ = reference(q, pool, scale, [0, n_p], pages, [kv], [0, qlen], True, window, 2, 0.125)
         fin = torch.isfinite(o)
         assert torch.equal(torch.isnan(out), torch.isnan(o))
         assert torch.equal(out.double()[~fin & ~torch.isnan(o)], o[~fin & ~torch.isnan(o)])
         a = torch.where(torch.isfinite(a), a, torch.zeros_like(a))
-        tol = torch.finfo(dt).eps / 2 * o.abs() + (u_of(dt, cache8) + 2.4e-4) * a + 2.0 ** -24
+        tol = torch.finfo(dt).eps / 2 * o.abs() + (u_of(dt, cache8, qlen * 4) + 2.4e-4) * a + 2.0 ** -24
         assert ((out.double() - o).abs()[fin] <= tol[fin]).all()
         assert torch.equal(torch.isnan(lse), torch.isnan(e))
 
@@ -549,7 +591,7 @@ def test_cascade_levels(dt, cache8, window, sinks, beams, g):
     kv = [pre[i // beams] * ps + int(own[i]) for i in range(n)]
     ref = reference(q, pool, scale, np.concatenate([[0], np.cumsum([len(x) for x in lists])]).tolist(),
                     [p for x in lists for p in x], kv, list(range(n + 1)), True, window, sinks, d ** -0.5)
-    compare(out, lse, ref, dt, u_of(dt, cache8))
+    compare(out, lse, ref, dt, u_of(dt, cache8, beams * g))
 
 
 def test_a_cache_in_8_bits_is_planned_again_when_the_plan_did_not_know():
@@ -639,4 +681,4 @@ def test_append_then_attend_as_a_decode_loop_does(dt):
         out, lse = w.run(q, pool, return_lse=True, kv_scale=scale)
         values = read_paged_kv_cache(pool, i32(np.arange(P)), scale, torch.float32)
         ref = reference(q, values, None, [0, used], pages[:used], [at], [0, n], True, 40, 4, d ** -0.5)
-        compare(out, lse, ref, dt, 2.0 ** -11)
+        compare(out, lse, ref, dt, u_of(dt, True, n * 4))
