@@ -51,6 +51,29 @@ template <> struct CacheElt<E4M3> { static constexpr int bytes = 1; };
 constexpr float kLazyMax = 8.f;       // factors up to 2^8 before O is rescaled
 constexpr float kNoMax = -1e30f;      // running maximum of a row that has seen nothing
 
+// Loads that stay where they are written: a plain load of constant memory is moved down to its
+// first use, which puts its latency back into every step.
+__device__ __forceinline__ int4 ld_early16(const void* p) {
+  int4 v;
+  asm volatile("ld.global.nc.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ld_early8(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ int ld_early4(const int32_t* p) {
+  int v;
+  asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float ld_early4(const float* p) {
+  float v;
+  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
   return __byte_perm(a, b, sel);
 }
@@ -181,8 +204,7 @@ __global__ void __launch_bounds__(128) paged_narrow_kernel(const PagedParams p) 
       const int64_t o = __shfl_sync(0xffffffffu, at, n * 8 + r);
 #pragma unroll
       for (int k = 0; k < KP; ++k)
-        kraw[n][k] = o >= 0 ? __ldg(reinterpret_cast<const int4*>(base + o + k * 64 + c * 16))
-                            : make_int4(0, 0, 0, 0);
+        kraw[n][k] = o >= 0 ? ld_early16(base + o + k * 64 + c * 16) : make_int4(0, 0, 0, 0);
     }
   };
   auto load_v = [&](int64_t at) {
@@ -193,12 +215,11 @@ __global__ void __launch_bounds__(128) paged_narrow_kernel(const PagedParams p) 
 #pragma unroll
       for (int k = 0; k < VP; ++k) {
         if constexpr (VB == 16) {
-          const int4 x = o >= 0 ? __ldg(reinterpret_cast<const int4*>(src + k * 128 + r * 16))
-                                : make_int4(0, 0, 0, 0);
+          const int4 x = o >= 0 ? ld_early16(src + k * 128 + r * 16) : make_int4(0, 0, 0, 0);
           vraw[n][4 * k] = x.x; vraw[n][4 * k + 1] = x.y;
           vraw[n][4 * k + 2] = x.z; vraw[n][4 * k + 3] = x.w;
         } else {
-          const uint2 x = o >= 0 ? __ldg(reinterpret_cast<const uint2*>(src + r * 8)) : make_uint2(0, 0);
+          const uint2 x = o >= 0 ? ld_early8(src + r * 8) : make_uint2(0, 0);
           vraw[n][0] = x.x; vraw[n][1] = x.y;
         }
       }
@@ -309,7 +330,7 @@ __global__ void __launch_bounds__(128) paged_narrow_kernel(const PagedParams p) 
       }
     // ---- values that are not finite and not seen by every row: out of the product (0 * NaN is
     // NaN), added to the rows that see them ----
-    if (!full && rows > 1) {
+    if (!full) {
       bool odd = false;
 #pragma unroll
       for (int n = 0; n < 4; ++n)

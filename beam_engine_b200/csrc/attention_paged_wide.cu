@@ -3,22 +3,30 @@
 //
 // One CTA = one item of be_paged_plan x one KV head: two row tiles of 128 (row r of the
 // item is query r / g, head r % g, so a KV head's tokens are loaded once for its g
-// query heads) against tiles of 128 tokens, in one pass with a running maximum:
-//   * loader warps (4): tokens' rows from global memory into the canonical 128-byte
-//     swizzle; 8-bit codes are scaled on the way (code * 2^e is exact in bf16, and
-//     in fp16 wherever fp16 holds the value), 16-bit rows go by cp.async; tokens are
-//     addressed one by one, so any page size and the joint of sinks and window cost nothing;
+// query heads) against steps of 128 tokens, in one pass with a running maximum:
+//   * loader warps (7): tokens' rows from global memory into the canonical 128-byte
+//     swizzle, 16-bit rows by cp.async, 8-bit codes through registers; tokens are addressed one
+//     by one, so any page size and the joint of sinks and window cost nothing;
 //   * one warp issues S = Q K^T (128 x 128 x D) into TMEM and O += P V (128 x D x 128) with
 //     P read from TMEM, alternating between the row tiles so that one tile's softmax
-//     runs under the other's products;
-//   * softmax warps (4 per row tile, a thread per row): maximum, exponentials, P written
-//     over S in TMEM; O is rescaled only when a row's maximum grows by more than 2^8.
+//     runs under the other's products; P V starts on the first half of P;
+//   * softmax warps (4 per row tile, a thread per row): the maximum, then P written over S, 64 tokens
+//     at a time from TMEM in rolled loops (16 warps in three roles share the instruction cache: with a
+//     row's 128 scores in registers and every loop unrolled, fetching instructions took
+//     half of each step); O is rescaled only when a row's maximum grows by more than 2^8.
 // TMEM: S/P of tile 0 | S/P of tile 1 | O of tile 0 | O of tile 1 = 256 + 2 D columns (512 allocated).
 // A tile's S of step i + 1 overwrites its P of step i: both products come from one thread, and
 // the tensor core runs them in the order of issue.
 //
-// Values that are not finite: 0 * NaN is NaN in the product, so in token tiles that some row
-// sees in part the loader replaces them by 0 and the rows that see them mark
+// 8-bit caches: as in the narrow kernel the codes become halves by one exact conversion and
+// the scales stay out of the products.  x = s_K (q . c) and log2 s_V joins the exponent, so a group of
+// 8 tokens of one page costs one shared-memory read and three operations per row; scaling
+// the codes themselves on the way to shared memory was 3 times the loaders' work
+// (8 000 clocks a step against 4 600 for a 16-bit cache).  The planner aligns ranges to 8 tokens; pages
+// that are no multiple of 8 take scales token by token.
+//
+// Values that are not finite: 0 * NaN is NaN in the product, so in steps that some row
+// sees in part the loaders replace them by 0 and the rows that see them mark
 // the dims in shared memory (+inf, -inf, or both for NaN), applied to O at the end.
 //
 // Every wait is bounded (2 s); one that runs out sets the device status and the abort flag, and all
@@ -31,7 +39,8 @@
 namespace be {
 
 constexpr int PW_TOK = 128;                    // tokens per step
-constexpr int PW_THREADS = 13 * 32;            // 8 softmax warps, 4 loader warps, 1 issuer
+constexpr int PW_LOADERS = 7;
+constexpr int PW_THREADS = 16 * 32;            // 8 softmax warps, 7 loader warps, 1 issuer
 constexpr int PW_HALF = PW_TOK * 128;          // 64 dims of 128 rows
 constexpr int PW_STAGES = 2;
 
@@ -39,7 +48,9 @@ template <int D>
 struct PwSmem {
   static constexpr int TILE = (D / 64) * PW_HALF;      // one 128 x D operand tile
   static constexpr int Q = 0, K = 2 * TILE, V = K + PW_STAGES * TILE, ODD = V + PW_STAGES * TILE;
-  static constexpr int BAR = ODD + 256 * (D / 32) * 8;  // two bit masks of D dims per row
+  static constexpr int TAB = ODD + 256 * (D / 32) * 8;  // two bit masks of D dims per row
+  static constexpr int RS = TAB + 4 * PW_TOK * 16;      // scales of 4 steps' tokens
+  static constexpr int BAR = RS + 256 * 4;              // scales of the rows
   static constexpr int BYTES = BAR + 256 + 1024;
 };
 
@@ -91,6 +102,34 @@ __device__ __forceinline__ uint32_t low_bits(int n, int word) {
   return k == 32 ? ~0u : (1u << k) - 1u;
 }
 
+__device__ __forceinline__ void tmem_ld16_nw(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+      "%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+__device__ __forceinline__ void tmem_ld8_nw(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3])
+               : "memory");
+}
+// the 8 bits of tokens c0 .. c0 + 7 (c0 a multiple of 8)
+__device__ __forceinline__ uint32_t see_at(const uint32_t (&see)[4], int c0) {
+  const uint32_t w = c0 < 32 ? see[0] : c0 < 64 ? see[1] : c0 < 96 ? see[2] : see[3];
+  return (w >> (c0 & 31)) & 0xffu;
+}
+
 // element x of a 16-bit pair: set to zero if not finite
 template <typename T>
 __device__ __forceinline__ uint32_t zero_not_finite(uint32_t w) {
@@ -109,31 +148,34 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
 template <typename T, typename CT, int D>
 __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedParams p) {
   constexpr bool Q8 = std::is_same<CT, E4M3>::value;
+  using MT = typename std::conditional<Q8, __half, T>::type;   // type of the products
   using SM = PwSmem<D>;
-  constexpr int NH = D / 64;
   constexpr int ROWB = D * CacheElt<CT>::bytes;
   constexpr int CH = ROWB / 16;                 // 16-byte chunks per (token, head) row: 4, 8 or 16
   constexpr int TPI = 32 / CH;                  // tokens per warp and load instruction
-  constexpr int ITS = 32 / TPI;                 // instructions for a warp's 32 tokens
+  constexpr int UNITS = PW_TOK / TPI;           // such instructions per step, dealt to the warps
+  constexpr int ITS = (UNITS + PW_LOADERS - 1) / PW_LOADERS;
+  static_assert(ITS * TPI <= 32, "a lane locates one token");
   extern __shared__ char smem_raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                        ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SM::BAR);
-  uint64_t* k_full = bars;                      // [2], 4 loader warps
+  uint64_t* k_full = bars;                      // [2], the loader warps
   uint64_t* v_full = bars + 2;                  // [2]
   uint64_t* k_empty = bars + 4;                 // [2], commit
   uint64_t* v_empty = bars + 6;                 // [2]
   uint64_t* s_full = bars + 8;                  // [row tile], commit
-  uint64_t* p_full = bars + 10;                 // [row tile], 4 softmax warps
-  uint64_t* o_done = bars + 12;                 // [row tile], commit
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bars + 14);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 15);
-  volatile int* odd = reinterpret_cast<volatile int*>(bars + 16);   // [2] per V stage: step + 1
-  // which tokens of a step exist, a word per loader warp; 4 steps deep, since the loaders are at
-  // most 2 steps past the softmax
-  uint32_t* exists = reinterpret_cast<uint32_t*>(bars + 18);        // [4][4]
-  uint64_t* drain = bars + 26;
+  uint64_t* o_done = bars + 10;                 // [row tile], commit
+  uint64_t* p_full = bars + 12;                 // [row tile][half], 4 softmax warps
+  uint64_t* drain = bars + 16;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bars + 17);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 18);
+  volatile int* odd = reinterpret_cast<volatile int*>(bars + 19);   // [2] per V stage: step + 1
+  volatile int* gone = reinterpret_cast<volatile int*>(bars + 20);  // [4]: step + 1 that misses a page
   uint32_t* odd_mask = reinterpret_cast<uint32_t*>(smem + SM::ODD);  // [256][2][D / 32]
+  // per token of the last 4 steps (the loaders are at most 2 past the softmax): s_K, log2 s_V, 1 / s_V
+  float4* tab = reinterpret_cast<float4*>(smem + SM::TAB);
+  float* row_scale = reinterpret_cast<float*>(smem + SM::RS);
 
   pdl_wait();
   const be_attn_plan_info* hdr = reinterpret_cast<const be_attn_plan_info*>(p.plan);
@@ -157,14 +199,15 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
 
   if (tid == 0) {
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&k_full[s], 4);
-      mbar_init(&v_full[s], 4);
+      mbar_init(&k_full[s], PW_LOADERS);
+      mbar_init(&v_full[s], PW_LOADERS);
       mbar_init(&k_empty[s], 1);
       mbar_init(&v_empty[s], 1);
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 4);
       mbar_init(&o_done[s], 1);
-      odd[s] = 0;
+      mbar_init(&p_full[2 * s], 4);
+      mbar_init(&p_full[2 * s + 1], 4);
+      odd[s] = gone[s] = gone[2 + s] = 0;
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -178,15 +221,43 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
   }
   if (warp < 8) {   // Q rows into shared memory, zeros past the item's rows
     constexpr int QC = D / 8;
+    // the sign of sm_scale goes into Q, so that the largest score is the largest product
+    const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
     for (int idx = tid; idx < 256 * QC; idx += 256) {
       const int r = idx / QC, c = idx % QC;
-      int4 val = make_int4(0, 0, 0, 0);
-      if (r < rows)
-        val = *reinterpret_cast<const int4*>(reinterpret_cast<const T*>(p.q) +
-                                             (w.q_begin + r / g) * p.q_row_stride +
-                                             (int64_t)(kvh * g + r % g) * D + c * 8);
+      uint32_t x[4] = {0, 0, 0, 0};
+      if (r < rows) {
+        const int4 val = *reinterpret_cast<const int4*>(
+            reinterpret_cast<const T*>(p.q) + (w.q_begin + r / g) * p.q_row_stride +
+            (int64_t)(kvh * g + r % g) * D + c * 8);
+        x[0] = val.x ^ flip; x[1] = val.y ^ flip; x[2] = val.z ^ flip; x[3] = val.w ^ flip;
+      }
+      if constexpr (Q8) {
+        // bf16 rows into half range by a power of two, as in the narrow kernel
+        float back = 1.f;
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+          float f[8], mx = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x[i]));
+            f[2 * i] = y.x;
+            f[2 * i + 1] = y.y;
+            mx = fmaxf(mx, fmaxf(fabsf(y.x), fabsf(y.y)));
+          }
+#pragma unroll
+          for (int off = QC / 2; off; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+          int e = (int)(__float_as_uint(mx) >> 23) - 127;
+          e = mx < INFINITY ? min(max(e, -110), 110) : 0;
+          const float up = __uint_as_float((uint32_t)(8 - e + 127) << 23);
+          back = __uint_as_float((uint32_t)(e - 8 + 127) << 23);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = pack2<__half>(f[2 * i] * up, f[2 * i + 1] * up);
+        }
+        if (c == 0) row_scale[r] = back;
+      }
       *reinterpret_cast<int4*>(smem + SM::Q + (r >> 7) * SM::TILE + (c >> 3) * PW_HALF +
-                               (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) = val;
+                               (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) =
+          make_int4(x[0], x[1], x[2], x[3]);
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -195,232 +266,244 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 12) {
-    // ---------------- issuer ----------------
-    if (lane == 0) {
-      const uint32_t id_s = umma_idesc<T>(128, PW_TOK, 0), id_o = umma_idesc<T>(128, D, 1);
-      auto issue_s = [&](int tile, int stage) {
-        const uint32_t a0 = smem_u32(smem + SM::Q + tile * SM::TILE);
-        const uint32_t b0 = smem_u32(smem + SM::K + stage * SM::TILE);
+  if (warp >= 8) {
+    if (warp == 15) {
+      // ---------------- issuer ----------------
+      if (lane == 0) {
+        const uint32_t id_s = umma_idesc<MT>(128, PW_TOK, 0), id_o = umma_idesc<MT>(128, D, 1);
+        // descriptors once; per product only a constant is added (what one thread can issue
+        // bounds the rate: 65 clocks per 128 x 128 x 16, 100 with the descriptors made each time)
+        const uint64_t dq = umma_desc(smem_u32(smem + SM::Q), 16, 1024);
+        const uint64_t dk = umma_desc(smem_u32(smem + SM::K), 16, 1024);
+        const uint64_t dv = umma_desc(smem_u32(smem + SM::V), PW_HALF, 1024);
+        auto issue_s = [&](int tile, int stage) {
+          const uint64_t a = dq + tile * (SM::TILE >> 4), b = dk + stage * (SM::TILE >> 4);
+          const uint32_t d = tmem + tile * 128;
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * PW_HALF + (kk & 3) * 32;
-          umma_f16(tmem + tile * 128, umma_desc(a0 + off, 16, 1024), umma_desc(b0 + off, 16, 1024),
-                   id_s, kk > 0);
-        }
-        umma_commit(&s_full[tile]);
-      };
-      auto issue_o = [&](int tile, int stage, bool first) {
-        const uint32_t b0 = smem_u32(smem + SM::V + stage * SM::TILE);
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = ((kk >> 2) * PW_HALF + (kk & 3) * 32) >> 4;
+            umma_f16(d, a + off, b + off, id_s, kk > 0);
+          }
+          umma_commit(&s_full[tile]);
+        };
+        auto issue_o = [&](int tile, int stage, int half, bool first) {   // 64 tokens
+          const uint64_t b = dv + stage * (SM::TILE >> 4) + half * (4 * 2048 >> 4);
+          const uint32_t d = tmem + 256 + tile * D, a = tmem + tile * 128 + half * 32;
 #pragma unroll
-        for (int ks = 0; ks < PW_TOK / 16; ++ks)
-          umma_f16_ts(tmem + 256 + tile * D, tmem + tile * 128 + ks * 8,
-                      umma_desc(b0 + ks * 2048, PW_HALF, 1024), id_o, !(first && ks == 0));
-        umma_commit(&o_done[tile]);
-      };
-      bool ok = mbar_wait(&k_full[0], 0);
-      if (ok) {
-        tc_fence_after();
-        issue_s(0, 0);
-        if (two) issue_s(1, 0);
-        umma_commit(&k_empty[0]);
-      }
-      for (int i = 0; ok && i < steps; ++i) {
-        const int st = i & 1, nx = (i + 1) & 1;
-        for (int tile = 0; tile < (two ? 2 : 1); ++tile) {
-          ok = ok && !*abort_flag && mbar_wait(&p_full[tile], i & 1);
-          if (tile == 0) ok = ok && mbar_wait(&v_full[st], (i >> 1) & 1);
-          if (!ok) break;
+          for (int ks = 0; ks < 4; ++ks)
+            umma_f16_ts(d, a + ks * 8, b + ks * (2048 >> 4), id_o, !(first && half == 0 && ks == 0));
+        };
+        bool ok = mbar_wait(&k_full[0], 0);
+        if (ok) {
           tc_fence_after();
-          issue_o(tile, st, i == 0);
-          if (i + 1 < steps) {
-            if (tile == 0) {
-              ok = mbar_wait(&k_full[nx], ((i + 1) >> 1) & 1);
+          issue_s(0, 0);
+          if (two) issue_s(1, 0);
+          umma_commit(&k_empty[0]);
+        }
+        for (int i = 0; ok && i < steps; ++i) {
+          const int st = i & 1, nx = (i + 1) & 1;
+          for (int tile = 0; tile < (two ? 2 : 1); ++tile) {
+            if (tile == 0) ok = ok && mbar_wait(&v_full[st], (i >> 1) & 1);
+            for (int half = 0; half < 2; ++half) {
+              ok = ok && !*abort_flag && mbar_wait(&p_full[2 * tile + half], i & 1);
               if (!ok) break;
               tc_fence_after();
+              issue_o(tile, st, half, i == 0);
             }
-            issue_s(tile, nx);
-          }
-        }
-        if (ok) {
-          umma_commit(&v_empty[st]);
-          if (i + 1 < steps) umma_commit(&k_empty[nx]);
-        }
-      }
-      if (!ok) {        // leave with no product in flight
-        *abort_flag = 1;
-        umma_commit(drain);
-        mbar_wait(drain, 0);
-      }
-    }
-  } else if (warp >= 8) {
-    // ---------------- loaders ----------------
-    const int lw = warp - 8;
-    const int64_t row_step = (int64_t)p.hkv * ROWB, plane_step = row_step * p.ps;
-    const char* base = p.pool + (int64_t)kvh * ROWB;
-    const int c = lane % CH, sub = lane / CH;
-    // a warp has 32 consecutive tokens of the step; lane L locates the L-th
-    auto token_of = [&](int it) { return lw * 32 + it * TPI + sub; };
-    const int ps_shift = (p.ps & (p.ps - 1)) == 0 ? __ffs(p.ps) - 1 : -1;
-    auto token_t = [&](int v) { return v + (v >= w.n0 ? w.shift : 0); };
-    auto page_of = [&](int v0) -> int {          // page id of this lane's token, -1 past the range
-      const int v = v0 + lw * 32 + lane;
-      if (v >= w.v_end) return -1;
-      const int t = token_t(v);
-      return kvlist[ps_shift >= 0 ? t >> ps_shift : t / p.ps];
-    };
-    auto locate = [&](int v0, int page, float& sk, float& sv) -> int64_t {
-      const int v = v0 + lw * 32 + lane;
-      sk = sv = 0.f;
-      if (page < 0 || page >= p.num_pages) {
-        if (v < w.v_end) flag_range_error();
-        return -1;
-      }
-      if constexpr (Q8) {
-        const float* s = p.scale + (int64_t)page * 2 * p.hkv + kvh;
-        sk = s[0];
-        sv = s[p.hkv];
-      }
-      const int t = token_t(v);
-      return (int64_t)page * 2 * plane_step +
-             (int64_t)(ps_shift >= 0 ? t & (p.ps - 1) : t % p.ps) * row_step;
-    };
-    auto dst_of = [&](char* tile, int tok, int chunk) {   // 16-byte chunk of 8 dims
-      return tile + (chunk >> 3) * PW_HALF + tok * 128 + (((chunk & 7) ^ (tok & 7)) << 4);
-    };
-    auto publish = [&](int i, int64_t at) {
-      const uint32_t has = __ballot_sync(0xffffffffu, at >= 0);
-      if (lane == 0) exists[(i & 3) * 4 + lw] = has;
-    };
-    auto signal = [&](uint64_t* bar) {
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar);
-    };
-    bool ok = true;
-    if constexpr (Q8) {
-      int4 ka[ITS], va[ITS];
-      auto load = [&](int4* buf, int64_t at, int64_t plane) {
-#pragma unroll
-        for (int it = 0; it < ITS; ++it) {
-          const int64_t o = __shfl_sync(0xffffffffu, at, it * TPI + sub);
-          buf[it] = o >= 0 ? __ldg(reinterpret_cast<const int4*>(base + o + plane + c * 16))
-                           : make_int4(0, 0, 0, 0);
-        }
-      };
-      auto store = [&](char* tile, const int4* buf, float scale, bool check) -> bool {
-        bool bad = false;
-#pragma unroll
-        for (int it = 0; it < ITS; ++it) {
-          const float s = __shfl_sync(0xffffffffu, scale, it * TPI + sub);
-          const uint64_t s2 = f2_pack(s, s);
-          const uint32_t wd[4] = {(uint32_t)buf[it].x, (uint32_t)buf[it].y, (uint32_t)buf[it].z,
-                                  (uint32_t)buf[it].w};
-          uint32_t o[8];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            float f[4];
-            e4m3x4_to_f(wd[x], f);
-            f2_unpack(f2_mul(f2_pack(f[0], f[1]), s2), f[0], f[1]);
-            f2_unpack(f2_mul(f2_pack(f[2], f[3]), s2), f[2], f[3]);
-            o[2 * x] = pack2<T>(f[0], f[1]);
-            o[2 * x + 1] = pack2<T>(f[2], f[3]);
-          }
-          if (check) {
-#pragma unroll
-            for (int x = 0; x < 8; ++x) {
-              const uint32_t z = zero_not_finite<T>(o[x]);
-              bad |= z != o[x];
-              o[x] = z;
+            if (!ok) break;
+            umma_commit(&o_done[tile]);
+            if (i + 1 < steps) {
+              if (tile == 0) {
+                ok = mbar_wait(&k_full[nx], ((i + 1) >> 1) & 1);
+                if (!ok) break;
+                tc_fence_after();
+              }
+              issue_s(tile, nx);
             }
           }
-          const int tok = token_of(it);
-          // the second half of the row's chunks stores its odd piece first: no bank twice
-          const int sw = c >= CH / 2 ? 1 : 0;
-          *reinterpret_cast<int4*>(dst_of(tile, tok, 2 * c + sw)) =
-              sw ? make_int4(o[4], o[5], o[6], o[7]) : make_int4(o[0], o[1], o[2], o[3]);
-          *reinterpret_cast<int4*>(dst_of(tile, tok, 2 * c + 1 - sw)) =
-              sw ? make_int4(o[0], o[1], o[2], o[3]) : make_int4(o[4], o[5], o[6], o[7]);
+          if (ok) {
+            umma_commit(&v_empty[st]);
+            if (i + 1 < steps) umma_commit(&k_empty[nx]);
+          }
         }
-        return bad;
-      };
-      float sk, sv;
-      int64_t at = locate(w.v_begin, page_of(w.v_begin), sk, sv);
-      load(ka, at, 0);
-      int page_next = page_of(w.v_begin + PW_TOK);
-      for (int i = 0; i < steps; ++i) {
-        const int st = i & 1, v0 = w.v_begin + i * PW_TOK;
-        const bool check = !full_step(v0);
-        load(va, at, plane_step);
-        if (i >= 2) ok = warp_wait(&k_empty[st], ((i >> 1) - 1) & 1, abort_flag);
-        if (!ok) break;
-        store(smem + SM::K + st * SM::TILE, ka, sk, false);
-        publish(i, at);
-        signal(&k_full[st]);
-        const float sv_now = sv;
-        if (i + 1 < steps) {
-          at = locate(v0 + PW_TOK, page_next, sk, sv);
-          load(ka, at, 0);
-          page_next = page_of(v0 + 2 * PW_TOK);
+        if (!ok) {        // leave with no product in flight
+          *abort_flag = 1;
+          umma_commit(drain);
+          mbar_wait(drain, 0);
         }
-        if (i >= 2) ok = warp_wait(&v_empty[st], ((i >> 1) - 1) & 1, abort_flag);
-        if (!ok) break;
-        if (store(smem + SM::V + st * SM::TILE, va, sv_now, check)) odd[st] = i + 1;
-        signal(&v_full[st]);
       }
     } else {
-      auto copy = [&](char* tile, int64_t at, int64_t plane) {
-#pragma unroll
-        for (int it = 0; it < ITS; ++it) {
-          const int64_t o = __shfl_sync(0xffffffffu, at, it * TPI + sub);
-          cp_async16(smem_u32(dst_of(tile, token_of(it), c)),
-                     o >= 0 ? base + o + plane + c * 16 : p.pool, o >= 0);
-        }
-        cp_commit();
+      // ---------------- loaders ----------------
+      const int lw = warp - 8;
+      const int64_t row_step = (int64_t)p.hkv * ROWB, plane_step = row_step * p.ps;
+      const char* base = p.pool + (int64_t)kvh * ROWB;
+      const int c = lane % CH, sub = lane / CH;
+      // load instruction `it` of this warp takes tokens [unit * TPI, + TPI), unit = lw + 7 it;
+      // lane L locates the token that instruction L / TPI loads in place L % TPI
+      auto unit_of = [&](int it) { return lw + PW_LOADERS * it; };
+      const int my_tok = unit_of(lane / TPI) * TPI + lane % TPI;
+      const bool my = lane < ITS * TPI && my_tok < PW_TOK;
+      const int ps_shift = (p.ps & (p.ps - 1)) == 0 ? __ffs(p.ps) - 1 : -1;
+      auto token_t = [&](int v) { return v + (v >= w.n0 ? w.shift : 0); };
+      auto page_of = [&](int v0) -> int {        // page id of this lane's token, -1 past the range
+        const int v = v0 + my_tok;
+        if (!my || v >= w.v_end) return -1;
+        const int t = token_t(v);
+        return ld_early4(kvlist + (ps_shift >= 0 ? t >> ps_shift : t / p.ps));
       };
-      auto finish_v = [&](int i) {    // V of step i has landed: look at it where rows see it in part
-        const int st = i & 1;
-        if (!full_step(w.v_begin + i * PW_TOK)) {
+      auto locate = [&](int i, int page, float& sk, float& sv) -> int64_t {
+        const int v = w.v_begin + i * PW_TOK + my_tok;
+        sk = 0.f;
+        sv = -1.f;
+        if (page < 0 || page >= p.num_pages) {
+          if (my && v < w.v_end) {
+            flag_range_error();
+            gone[i & 3] = i + 1;
+          }
+          return -1;
+        }
+        if constexpr (Q8) {
+          const float* s = p.scale + (int64_t)page * 2 * p.hkv + kvh;
+          sk = ld_early4(s);
+          sv = ld_early4(s + p.hkv);
+        }
+        const int t = token_t(v);
+        return (int64_t)page * 2 * plane_step +
+               (int64_t)(ps_shift >= 0 ? t & (p.ps - 1) : t % p.ps) * row_step;
+      };
+      auto dst_of = [&](char* tile, int tok, int chunk) {   // 16-byte chunk of 8 dims
+        return tile + (chunk >> 3) * PW_HALF + tok * 128 + (((chunk & 7) ^ (tok & 7)) << 4);
+      };
+      auto signal = [&](uint64_t* bar) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+      };
+      bool ok = true;
+      if constexpr (Q8) {
+        int4 ka[ITS], va[ITS];
+        auto load = [&](int4* buf, int64_t at, int64_t plane) {
+#pragma unroll
+          for (int it = 0; it < ITS; ++it) {
+            const int64_t o = __shfl_sync(0xffffffffu, at, it * TPI + sub);
+            buf[it] = o >= 0 ? ld_early16(base + o + plane + c * 16) : make_int4(0, 0, 0, 0);
+          }
+        };
+        auto store = [&](char* tile, const int4* buf, bool check) -> bool {
           bool bad = false;
 #pragma unroll
           for (int it = 0; it < ITS; ++it) {
-            int4* a = reinterpret_cast<int4*>(dst_of(smem + SM::V + st * SM::TILE, token_of(it), c));
-            const int4 x = *a;
-            const int4 z = make_int4(zero_not_finite<T>(x.x), zero_not_finite<T>(x.y),
-                                     zero_not_finite<T>(x.z), zero_not_finite<T>(x.w));
-            if (z.x != x.x || z.y != x.y || z.z != x.z || z.w != x.w) {
-              bad = true;
-              *a = z;
+            if (unit_of(it) >= UNITS) break;
+            const uint32_t wd[4] = {(uint32_t)buf[it].x, (uint32_t)buf[it].y, (uint32_t)buf[it].z,
+                                    (uint32_t)buf[it].w};
+            uint32_t o[8];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              o[2 * x] = e4m3x2_to_h2(wd[x] & 0xffffu);
+              o[2 * x + 1] = e4m3x2_to_h2(wd[x] >> 16);
             }
+            if (check) {
+#pragma unroll
+              for (int x = 0; x < 8; ++x) {
+                const uint32_t z = zero_not_finite<__half>(o[x]);
+                bad |= z != o[x];
+                o[x] = z;
+              }
+            }
+            const int tok = unit_of(it) * TPI + sub;
+            // the second half of the row's chunks stores its odd piece first: no bank twice
+            const int sw = c >= CH / 2 ? 1 : 0;
+            *reinterpret_cast<int4*>(dst_of(tile, tok, 2 * c + sw)) =
+                sw ? make_int4(o[4], o[5], o[6], o[7]) : make_int4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<int4*>(dst_of(tile, tok, 2 * c + 1 - sw)) =
+                sw ? make_int4(o[0], o[1], o[2], o[3]) : make_int4(o[4], o[5], o[6], o[7]);
           }
-          if (bad) odd[st] = i + 1;
+          return bad;
+        };
+        float sk, sv;
+        int64_t at = locate(0, page_of(w.v_begin), sk, sv);
+        load(ka, at, 0);
+        int page_next = page_of(w.v_begin + PW_TOK);
+        for (int i = 0; i < steps; ++i) {
+          const int st = i & 1, v0 = w.v_begin + i * PW_TOK;
+          load(va, at, plane_step);
+          // scales of 0 (blocks never written) stand for values of 0: any will do; a token that is
+          // not there gets an exponent of -inf
+          const float svc = fmaxf(sv, 9.0949470177e-13f);         // 2^-40
+          const float4 entry = sv < 0.f ? make_float4(1.f, -INFINITY, 0.f, 0.f)
+                                        : make_float4(fmaxf(sk, 1e-30f), log2f(svc), 1.f / svc, 0.f);
+          if (i >= 2) ok = warp_wait(&k_empty[st], ((i >> 1) - 1) & 1, abort_flag);
+          if (!ok) break;
+          if (my) tab[(i & 3) * PW_TOK + my_tok] = entry;
+          store(smem + SM::K + st * SM::TILE, ka, false);
+          signal(&k_full[st]);
+          if (i + 1 < steps) {
+            at = locate(i + 1, page_next, sk, sv);
+            load(ka, at, 0);
+            page_next = page_of(v0 + 2 * PW_TOK);
+          }
+          if (i >= 2) ok = warp_wait(&v_empty[st], ((i >> 1) - 1) & 1, abort_flag);
+          if (!ok) break;
+          if (store(smem + SM::V + st * SM::TILE, va, !full_step(v0))) odd[st] = i + 1;
+          signal(&v_full[st]);
         }
-        signal(&v_full[st]);
-      };
-      float sk, sv;
-      int page_next = page_of(w.v_begin);
-      for (int i = 0; i < steps; ++i) {
-        const int st = i & 1, v0 = w.v_begin + i * PW_TOK;
-        const int64_t at = locate(v0, page_next, sk, sv);
-        page_next = page_of(v0 + PW_TOK);
-        if (i >= 2) ok = warp_wait(&k_empty[st], ((i >> 1) - 1) & 1, abort_flag);
-        if (!ok) break;
-        copy(smem + SM::K + st * SM::TILE, at, 0);
-        publish(i, at);
-        if (i > 0) {
-          cp_wait<1>();
-          finish_v(i - 1);
+      } else {
+        auto copy = [&](char* tile, int64_t at, int64_t plane) {
+#pragma unroll
+          for (int it = 0; it < ITS; ++it) {
+            const int64_t o = __shfl_sync(0xffffffffu, at, it * TPI + sub);
+            if (unit_of(it) < UNITS)
+              cp_async16(smem_u32(dst_of(tile, unit_of(it) * TPI + sub, c)),
+                         o >= 0 ? base + o + plane + c * 16 : p.pool, o >= 0);
+          }
+          cp_commit();
+        };
+        auto finish_v = [&](int i) {  // V of step i has landed: look at it where rows see it in part
+          const int st = i & 1;
+          if (!full_step(w.v_begin + i * PW_TOK)) {
+            bool bad = false;
+#pragma unroll 1
+            for (int it = 0; it < ITS; ++it) {
+              if (unit_of(it) >= UNITS) break;
+              int4* a = reinterpret_cast<int4*>(
+                  dst_of(smem + SM::V + st * SM::TILE, unit_of(it) * TPI + sub, c));
+              const int4 x = *a;
+              const int4 z = make_int4(zero_not_finite<T>(x.x), zero_not_finite<T>(x.y),
+                                       zero_not_finite<T>(x.z), zero_not_finite<T>(x.w));
+              if (z.x != x.x || z.y != x.y || z.z != x.z || z.w != x.w) {
+                bad = true;
+                *a = z;
+              }
+            }
+            if (bad) odd[st] = i + 1;
+          }
+          signal(&v_full[st]);
+        };
+        float sk, sv;
+        int page_next = page_of(w.v_begin);
+        for (int i = 0; i < steps; ++i) {
+          const int st = i & 1;
+          const int64_t at = locate(i, page_next, sk, sv);
+          page_next = page_of(w.v_begin + (i + 1) * PW_TOK);
+          if (i >= 2) ok = warp_wait(&k_empty[st], ((i >> 1) - 1) & 1, abort_flag);
+          if (!ok) break;
+          copy(smem + SM::K + st * SM::TILE, at, 0);
+          if (i > 0) {
+            cp_wait<1>();
+            finish_v(i - 1);
+          }
+          // K goes out before V's stage is waited for: that one comes free with the step before last
+          cp_wait<0>();
+          signal(&k_full[st]);
+          if (i >= 2) ok = warp_wait(&v_empty[st], ((i >> 1) - 1) & 1, abort_flag);
+          if (!ok) break;
+          copy(smem + SM::V + st * SM::TILE, at, plane_step);
         }
-        if (i >= 2) ok = warp_wait(&v_empty[st], ((i >> 1) - 1) & 1, abort_flag);
-        if (!ok) break;
-        copy(smem + SM::V + st * SM::TILE, at, plane_step);
-        cp_wait<1>();
-        signal(&k_full[st]);
+        cp_wait<0>();
+        if (ok) finish_v(steps - 1);
       }
-      cp_wait<0>();
-      if (ok) finish_v(steps - 1);
+      if (!ok) *abort_flag = 1;
     }
-    if (!ok) *abort_flag = 1;
   } else {
     // ---------------- softmax: one row per thread ----------------
     const int tile = warp >> 2, row = tid;                 // rows 0..255 of the item
@@ -428,13 +511,17 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
       const uint32_t quad = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t t_s = tmem + tile * 128 + quad, t_o = tmem + 256 + tile * D + quad;
       const int pos = w.pos0 + w.pos_step * (row / g);
-      const float scale = p.scale_log2;
-      // what the row sees, in v: v <= vc and (v < vs or v >= vw).  With a gap the tokens before n0
-      // are the sinks; without one t is v.
+      // factors of scores are never 0: a masked score of -inf stays -inf
+      constexpr float kLeast = 1e-37f;
+      const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f) * (Q8 ? row_scale[row] : 1.f);
+      // groups of 8 tokens lie in one page
+      const bool grouped = p.ps % 8 == 0 && w.v_begin % 8 == 0 &&
+                           (w.shift == 0 || (w.n0 % 8 == 0 && w.shift % 8 == 0));
+      // what the row sees, in v: v <= vc and (v < sink_end or v >= vw); with a gap, v >= n0 is t - shift
       const int vc = !causal ? INT_MAX - 1 : w.shift == 0 ? pos : pos >= w.n0 + w.shift
                                                     ? pos - w.shift : min(pos, w.n0 - 1);
-      const int vs = w.shift == 0 ? w.sink_end : w.n0;
-      const int vw = window ? pos - w.window - w.shift : INT_MIN;
+      const int vw = !window ? INT_MIN : w.shift == 0 ? pos - w.window
+                                                      : max(pos - w.window - w.shift, w.n0);
       float m = kNoMax, l = 0.f;
       bool ok = true, marked = false;
       for (int i = 0; i < steps; ++i) {
@@ -442,44 +529,80 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
         ok = warp_wait(&s_full[tile], i & 1, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        const uint4 ex4 = *reinterpret_cast<const uint4*>(exists + (i & 3) * 4);
-        // a negative scale turns the maximum around: such calls take the masked path throughout
-        const bool full = full_step(v0) && scale >= 0.f && (ex4.x & ex4.y & ex4.z & ex4.w) == ~0u;
-        uint32_t see[4] = {ex4.x, ex4.y, ex4.z, ex4.w};
-        if (!full) {
-          const int kc = (vc >= v0 + PW_TOK ? PW_TOK : vc - v0 + 1), ks = min(vs - v0, PW_TOK);
-          const int kw = vw <= v0 ? 0 : min(vw - v0, PW_TOK);
+        const float4* tb = tab + (i & 3) * PW_TOK;
+        const bool missing = !Q8 && gone[i & 3] == i + 1, cut = !full_step(v0) || missing;
+        uint32_t see[4] = {};
+        if (cut) {
+          const int kc = min(vc >= v0 + PW_TOK ? PW_TOK : vc - v0 + 1, w.v_end - v0);
+          const int ks = min(w.sink_end - v0, PW_TOK), kw = vw <= v0 ? 0 : min(vw - v0, PW_TOK);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            see[j] &= low_bits(kc, j) & (low_bits(ks, j) | ~low_bits(kw, j));
+            see[j] = low_bits(kc, j) & (low_bits(ks, j) | ~low_bits(kw, j));
+          if (missing)                               // a page id out of range: its tokens drop out
+            for (int k = 0; k < min(PW_TOK, w.v_end - v0); ++k) {
+              const int v = v0 + k, t = v + (v >= w.n0 ? w.shift : 0);
+              const int page = kvlist[t / p.ps];
+              if (page < 0 || page >= p.num_pages) {
+                const uint32_t bit = ~(1u << (k & 31));
+                if (k < 32) see[0] &= bit;
+                else if (k < 64) see[1] &= bit;
+                else if (k < 96) see[2] &= bit;
+                else see[3] &= bit;
+              }
+            }
         }
         uint32_t x[64];
-        float mx;
-        if (full) {
-          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        // scores of tokens [64 h, 64 h + 64) of the step, -inf where the row does not see them
+        auto fetch = [&](int h) {
+          tmem_ld32_nw(t_s + 64 * h, x);
+          tmem_ld32_nw(t_s + 64 * h + 32, x + 32);
+          tmem_wait();
+          if (cut) {
+            const uint32_t lo = h ? see[2] : see[0], hi = h ? see[3] : see[1];
 #pragma unroll
-          for (int c0 = 0; c0 < PW_TOK; c0 += 64) {
-            tmem_ld32_nw(t_s + c0, x);
-            tmem_ld32_nw(t_s + c0 + 32, x + 32);
-            tmem_wait();
-#pragma unroll
-            for (int k = 0; k < 64; k += 8)
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                m4[j] = fmaxf(fmaxf(m4[j], __uint_as_float(x[k + j])), __uint_as_float(x[k + 4 + j]));
+            for (int k = 0; k < 32; ++k) {
+              x[k] = (lo >> k) & 1 ? x[k] : 0xff800000u;
+              x[32 + k] = (hi >> k) & 1 ? x[32 + k] : 0xff800000u;
+            }
           }
-          mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * scale;
-        } else {
-          mx = -INFINITY;
+        };
+        const bool by_token = Q8 && !grouped;
+        float mx = -INFINITY;
+        if (by_token) {
 #pragma unroll 1
-          for (int j = 0; j < 4; ++j) {
-            tmem_ld32_nw(t_s + 32 * j, x);
+          for (int c0 = 0; c0 < PW_TOK; c0 += 8) {
+            tmem_ld8_nw(t_s + c0, x);
             tmem_wait();
-            const uint32_t bits = j == 0 ? see[0] : j == 1 ? see[1] : j == 2 ? see[2] : see[3];
+            const uint32_t bits = cut ? see_at(see, c0) : 0xffu;
 #pragma unroll
-            for (int k = 0; k < 32; ++k)
-              mx = fmaxf(mx, (bits >> k) & 1 ? __uint_as_float(x[k]) * scale : -INFINITY);
+            for (int k = 0; k < 8; ++k)
+              if ((bits >> k) & 1)
+                mx = fmaxf(mx, fmaf(__uint_as_float(x[k]), fmaxf(tb[c0 + k].x * scale, kLeast), tb[c0 + k].y));
           }
+        } else {
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            fetch(h);
+            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int k = 0; k < 64; k += 8) {
+              if constexpr (Q8) {
+                float y[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] = __uint_as_float(x[k + j]);
+                const float gm = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])),
+                                       fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
+                const float4 e = tb[64 * h + k];
+                m4[(k >> 3) & 3] = fmaxf(m4[(k >> 3) & 3], fmaf(gm, fmaxf(e.x * scale, kLeast), e.y));
+              } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  m4[j] = fmaxf(fmaxf(m4[j], __uint_as_float(x[k + j])), __uint_as_float(x[k + 4 + j]));
+              }
+            }
+            mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+          }
+          if (!Q8) mx *= scale;
         }
         if (__any_sync(0xffffffffu, mx > m + kLazyMax)) {
           const float to = fmaxf(m, mx), f = ex2(m - to);
@@ -490,65 +613,93 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
             if (!ok) break;
             tc_fence_after();
 #pragma unroll 1
-            for (int c0 = 0; c0 < D; c0 += 32) {
-              tmem_ld32_nw(t_o + c0, x);
+            for (int c0 = 0; c0 < D; c0 += 16) {
+              uint32_t y[16];
+              tmem_ld16_nw(t_o + c0, y);
               tmem_wait();
 #pragma unroll
-              for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * f);
-              tmem_st32(t_o + c0, x);
+              for (int k = 0; k < 16; ++k) y[k] = __float_as_uint(__uint_as_float(y[k]) * f);
+              tmem_st16(t_o + c0, y);
             }
             tmem_wait_st();
           }
         }
-        if (full) {
-          const uint64_t s2 = f2_pack(scale, scale), m2 = f2_pack(-m, -m);
-          uint64_t sum[2] = {0, 0};
+        // ---- P, half by half: P V of the first 64 tokens starts while the others are made ----
+        const uint64_t s2 = f2_pack(scale, scale), m2 = f2_pack(-m, -m);
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          if (by_token) {
+#pragma unroll 1
+            for (int c0 = 64 * h; c0 < 64 * h + 64; c0 += 8) {
+              tmem_ld8_nw(t_s + c0, x);
+              tmem_wait();
+              const uint32_t bits = cut ? see_at(see, c0) : 0xffu;
+              uint32_t pk[4];
 #pragma unroll
-          for (int c0 = 0; c0 < PW_TOK; c0 += 64) {
-            tmem_ld32_nw(t_s + c0, x);
-            tmem_ld32_nw(t_s + c0 + 32, x + 32);
-            tmem_wait();
+              for (int k = 0; k < 8; k += 2) {
+                const float4 e = tb[c0 + k], f = tb[c0 + k + 1];
+                float a = ex2(fmaf(__uint_as_float(x[k]), fmaxf(e.x * scale, kLeast), e.y) - m);
+                float b = ex2(fmaf(__uint_as_float(x[k + 1]), fmaxf(f.x * scale, kLeast), f.y) - m);
+                a = (bits >> k) & 1 ? a : 0.f;
+                b = (bits >> k) & 2 ? b : 0.f;
+                l = fmaf(a, e.z, fmaf(b, f.z, l));
+                pk[k >> 1] = pack2<MT>(a, b);
+              }
+              tmem_st4(t_s + c0 / 2, pk);
+            }
+          } else {
+            fetch(h);
+            uint64_t sum[2] = {0, 0};
 #pragma unroll
-            for (int h = 0; h < 64; h += 32) {
+            for (int c0 = 0; c0 < 64; c0 += 32) {
               uint32_t pk[16];
 #pragma unroll
-              for (int k = h; k < h + 32; k += 2) {
-                float a, b;
-                f2_unpack(f2_fma(f2_pack(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), s2, m2), a, b);
-                a = ex2(a);
-                b = ex2(b);
-                sum[(k >> 1) & 1] = f2_add(sum[(k >> 1) & 1], f2_pack(a, b));
-                pk[(k - h) >> 1] = pack2<T>(a, b);
+              for (int k0 = c0; k0 < c0 + 32; k0 += 8) {
+                uint64_t gs = s2, gm = m2;
+                float inv = 1.f;
+                if constexpr (Q8) {
+                  const float4 e = tb[64 * h + k0];
+                  const float both = fmaxf(e.x * scale, kLeast);
+                  gs = f2_pack(both, both);
+                  gm = f2_pack(e.y - m, e.y - m);
+                  inv = e.z;
+                  sum[0] = sum[1] = 0;
+                }
+#pragma unroll
+                for (int k = k0; k < k0 + 8; k += 2) {
+                  const uint64_t y = f2_pack(__uint_as_float(x[k]), __uint_as_float(x[k + 1]));
+                  float a, b;
+                  f2_unpack(f2_fma(y, gs, gm), a, b);
+                  a = ex2(a);
+                  b = ex2(b);
+                  sum[(k >> 1) & 1] = f2_add(sum[(k >> 1) & 1], f2_pack(a, b));
+                  pk[(k - c0) >> 1] = pack2<MT>(a, b);
+                }
+                if constexpr (Q8) {
+                  float a, b;
+                  f2_unpack(f2_add(sum[0], sum[1]), a, b);
+                  l = fmaf(a + b, inv, l);
+                }
               }
-              tmem_st16(t_s + (c0 + h) / 2, pk);
+              tmem_st16(t_s + 32 * h + c0 / 2, pk);
+            }
+            if constexpr (!Q8) {
+              float a, b;
+              f2_unpack(f2_add(sum[0], sum[1]), a, b);
+              l += a + b;
             }
           }
-          float a, b;
-          f2_unpack(f2_add(sum[0], sum[1]), a, b);
-          l += a + b;
-        } else {
-#pragma unroll 1
-          for (int j = 0; j < 4; ++j) {
-            tmem_ld32_nw(t_s + 32 * j, x);
-            tmem_wait();
-            const uint32_t bits = j == 0 ? see[0] : j == 1 ? see[1] : j == 2 ? see[2] : see[3];
-            uint32_t pk[16];
-#pragma unroll
-            for (int k = 0; k < 32; k += 2) {
-              float a = ex2(fmaf(__uint_as_float(x[k]), scale, -m));
-              float b = ex2(fmaf(__uint_as_float(x[k + 1]), scale, -m));
-              a = (bits >> k) & 1 ? a : 0.f;
-              b = (bits >> k) & 2 ? b : 0.f;
-              l += a + b;
-              pk[k >> 1] = pack2<T>(a, b);
-            }
-            tmem_st16(t_s + 16 * j, pk);
+          if (h == 0) {
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[2 * tile]);
           }
         }
         tmem_wait_st();
         if (!full_step(v0)) {
           // values that are not finite, taken out of V: mark the dims of the rows that see them
-          // (before P is handed over: V's stage and its flag stay until P V of this step is done)
+          // (before the second half of P: V's stage and its flag stay until P V of this step is done)
           ok = warp_wait(&v_full[i & 1], (i >> 1) & 1, abort_flag);
           if (!ok) break;
           if (odd[i & 1] == i + 1) {
@@ -564,13 +715,11 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
                 continue;
               const int64_t r = ((int64_t)page * 2 + 1) * p.ps + t % p.ps;
               const char* src = p.pool + (r * p.hkv + kvh) * ROWB;
-              float s = 1.f;
-              if constexpr (Q8) s = p.scale[((int64_t)page * 2 + 1) * p.hkv + kvh];
               for (int d = 0; d < D; ++d) {
                 float val;
                 if constexpr (Q8) {
                   const uint32_t h2 = e4m3x2_to_h2(*reinterpret_cast<const uint8_t*>(src + d));
-                  val = to_f(from_f<T>(__low2float(*reinterpret_cast<const __half2*>(&h2)) * s));
+                  val = __low2float(*reinterpret_cast<const __half2*>(&h2));
                 } else {
                   val = to_f(reinterpret_cast<const T*>(src)[d]);
                 }
@@ -582,7 +731,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[tile]);
+        if (lane == 0) mbar_arrive(&p_full[2 * tile + 1]);
       }
       // ---- epilogue ----
       if (ok) ok = warp_wait(&o_done[tile], (steps - 1) & 1, abort_flag);

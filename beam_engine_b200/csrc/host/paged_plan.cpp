@@ -213,8 +213,11 @@ extern "C" int be_paged_plan(int num_levels, const int32_t* const* qo_indptr,
       const int64_t pmax = R.pos0 + (int64_t)R.step * (q0 + t.ql - 1);
       const int64_t hi = R.causal ? std::min<int64_t>(R.kv_len, pmax + 1) : R.kv_len;
       if (hi <= 0) continue;                        // sees nothing
-      const int64_t lo = window ? std::max<int64_t>(0, pmin - window_left) : 0;
-      const int64_t s = window ? std::min<int64_t>(R.sink_end, hi) : 0;
+      // where pages are multiples of 8 tokens, so are the ends of the two runs: groups of 8 tokens then
+      // share a page (the kernels mask by position, so the few tokens more are not seen)
+      const int64_t round = page_size % 8 == 0 ? 7 : 0;
+      const int64_t lo = window ? std::max<int64_t>(0, pmin - window_left) & ~round : 0;
+      const int64_t s = window ? std::min<int64_t>((R.sink_end + round) & ~round, hi) : 0;
       if (lo <= s) {
         t.n0 = (int)hi;
         t.shift = 0;
