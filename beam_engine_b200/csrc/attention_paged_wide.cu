@@ -54,13 +54,35 @@ struct PwSmem {
   static constexpr int BYTES = BAR + 256 + 1024;
 };
 
-// D[tmem] (+)= A[tmem] * B[smem], kind::f16
-__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t b,
-                                            uint32_t idesc, uint32_t accumulate) {
+// The elected lane's 1; whole warps call these.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate)
+      "{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r;
+}
+// D[tmem] (+)= A[smem] * B[smem] and D[tmem] (+)= A[tmem] * B[smem], kind::f16
+__device__ __forceinline__ void umma_f16_el(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc,
+                                            uint32_t accumulate, uint32_t el) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(el)
+      : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts_el(uint32_t tmem_d, uint32_t tmem_a, uint64_t b,
+                                               uint32_t idesc, uint32_t accumulate, uint32_t el) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(b), "r"(idesc), "r"(accumulate), "r"(el)
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit_el(uint64_t* bar, uint32_t el) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(
+          smem_u32(bar)), "r"(el)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
@@ -269,68 +291,68 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
   if (warp >= 8) {
     if (warp == 15) {
       // ---------------- issuer ----------------
-      if (lane == 0) {
-        const uint32_t id_s = umma_idesc<MT>(128, PW_TOK, 0), id_o = umma_idesc<MT>(128, D, 1);
-        // descriptors once; per product only a constant is added (what one thread can issue
-        // bounds the rate: 65 clocks per 128 x 128 x 16, 100 with the descriptors made each time)
-        const uint64_t dq = umma_desc(smem_u32(smem + SM::Q), 16, 1024);
-        const uint64_t dk = umma_desc(smem_u32(smem + SM::K), 16, 1024);
-        const uint64_t dv = umma_desc(smem_u32(smem + SM::V), PW_HALF, 1024);
-        auto issue_s = [&](int tile, int stage) {
-          const uint64_t a = dq + tile * (SM::TILE >> 4), b = dk + stage * (SM::TILE >> 4);
-          const uint32_t d = tmem + tile * 128;
+      // The whole warp walks the steps and one elected lane issues: addresses and descriptors
+      // then stay in uniform registers (from a divergent lane every product first moves them there)
+      const uint32_t el = elect_one();
+      const uint32_t id_s = umma_idesc<MT>(128, PW_TOK, 0), id_o = umma_idesc<MT>(128, D, 1);
+      const uint64_t dq = umma_desc(smem_u32(smem + SM::Q), 16, 1024);
+      const uint64_t dk = umma_desc(smem_u32(smem + SM::K), 16, 1024);
+      const uint64_t dv = umma_desc(smem_u32(smem + SM::V), PW_HALF, 1024);
+      auto issue_s = [&](int tile, int stage) {
+        const uint64_t a = dq + tile * (SM::TILE >> 4), b = dk + stage * (SM::TILE >> 4);
+        const uint32_t d = tmem + tile * 128;
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = ((kk >> 2) * PW_HALF + (kk & 3) * 32) >> 4;
-            umma_f16(d, a + off, b + off, id_s, kk > 0);
-          }
-          umma_commit(&s_full[tile]);
-        };
-        auto issue_o = [&](int tile, int stage, int half, bool first) {   // 64 tokens
-          const uint64_t b = dv + stage * (SM::TILE >> 4) + half * (4 * 2048 >> 4);
-          const uint32_t d = tmem + 256 + tile * D, a = tmem + tile * 128 + half * 32;
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            umma_f16_ts(d, a + ks * 8, b + ks * (2048 >> 4), id_o, !(first && half == 0 && ks == 0));
-        };
-        bool ok = mbar_wait(&k_full[0], 0);
-        if (ok) {
-          tc_fence_after();
-          issue_s(0, 0);
-          if (two) issue_s(1, 0);
-          umma_commit(&k_empty[0]);
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = ((kk >> 2) * PW_HALF + (kk & 3) * 32) >> 4;
+          umma_f16_el(d, a + off, b + off, id_s, kk > 0, el);
         }
-        for (int i = 0; ok && i < steps; ++i) {
-          const int st = i & 1, nx = (i + 1) & 1;
-          for (int tile = 0; tile < (two ? 2 : 1); ++tile) {
-            if (tile == 0) ok = ok && mbar_wait(&v_full[st], (i >> 1) & 1);
-            for (int half = 0; half < 2; ++half) {
-              ok = ok && !*abort_flag && mbar_wait(&p_full[2 * tile + half], i & 1);
+        umma_commit_el(&s_full[tile], el);
+      };
+      auto issue_o = [&](int tile, int stage, int half, uint32_t first) {   // 64 tokens
+        const uint64_t b = dv + stage * (SM::TILE >> 4) + half * (4 * 2048 >> 4);
+        const uint32_t d = tmem + 256 + tile * D, a = tmem + tile * 128 + half * 32;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+          umma_f16_ts_el(d, a + ks * 8, b + ks * (2048 >> 4), id_o, ks > 0 ? 1u : first, el);
+      };
+      bool ok = warp_wait(&k_full[0], 0, abort_flag);
+      if (ok) {
+        tc_fence_after();
+        issue_s(0, 0);
+        if (two) issue_s(1, 0);
+        umma_commit_el(&k_empty[0], el);
+      }
+      for (int i = 0; ok && i < steps; ++i) {
+        const int st = i & 1, nx = (i + 1) & 1;
+        ok = warp_wait(&v_full[st], (i >> 1) & 1, abort_flag);
+        for (int tile = 0; ok && tile < (two ? 2 : 1); ++tile) {
+          ok = warp_wait(&p_full[2 * tile], i & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          issue_o(tile, st, 0, i > 0);
+          ok = warp_wait(&p_full[2 * tile + 1], i & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          issue_o(tile, st, 1, 1);
+          umma_commit_el(&o_done[tile], el);
+          if (i + 1 < steps) {
+            if (tile == 0) {
+              ok = warp_wait(&k_full[nx], ((i + 1) >> 1) & 1, abort_flag);
               if (!ok) break;
               tc_fence_after();
-              issue_o(tile, st, half, i == 0);
             }
-            if (!ok) break;
-            umma_commit(&o_done[tile]);
-            if (i + 1 < steps) {
-              if (tile == 0) {
-                ok = mbar_wait(&k_full[nx], ((i + 1) >> 1) & 1);
-                if (!ok) break;
-                tc_fence_after();
-              }
-              issue_s(tile, nx);
-            }
-          }
-          if (ok) {
-            umma_commit(&v_empty[st]);
-            if (i + 1 < steps) umma_commit(&k_empty[nx]);
+            issue_s(tile, nx);
           }
         }
-        if (!ok) {        // leave with no product in flight
-          *abort_flag = 1;
-          umma_commit(drain);
-          mbar_wait(drain, 0);
+        if (ok) {
+          umma_commit_el(&v_empty[st], el);
+          if (i + 1 < steps) umma_commit_el(&k_empty[nx], el);
         }
+      }
+      if (!ok) {        // leave with no product in flight
+        *abort_flag = 1;
+        umma_commit_el(drain, el);
+        mbar_wait(drain, 0);
       }
     } else {
       // ---------------- loaders ----------------
