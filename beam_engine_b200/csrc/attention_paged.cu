@@ -15,16 +15,19 @@
 // range (exact down to 2^-33 of the row's largest value), so both products run in
 // fp16 with fp32 sums; 16-bit caches use their own type.
 //
-// A warp takes 16 tokens at a time straight from global memory into mma.sync
-// fragments; nothing passes through shared memory before the end.  The dims of a
-// fragment may be in any order as long as Q and K (or V and O) agree, so each lane
-// loads 16-byte pieces: lane (r, c) = (lane / 4, lane % 4) holds token r's pieces c, c + 4, ...
-// for S = Q K^T and piece r of tokens 2c, 2c + 1, 2c + 8, 2c + 9 for O = P V; whole
-// rows of a token and head are read by neighbouring lanes.  The next 16 tokens' K is
-// requested once this step's S is done, the next V once its O is done.
+// A warp takes 16 tokens at a time through a ring of its own in shared memory (cp.async by
+// 16 bytes, no barrier between warps) into mma.sync fragments.  The dims of a fragment may be
+// in any order as long as Q and K (or V and O) agree, so a lane reads 16-byte pieces: lane
+// (r, c) = (lane / 4, lane % 4) has token r's pieces c, c + 4, ... for S = Q K^T and piece r of
+// tokens 2c, 2c + 1, 2c + 8, 2c + 9 for O = P V; pieces are swizzled by the token so that both
+// reads hit every bank once.  The ring keeps 3 steps in flight per warp (12 KB at 128 dims in
+// 8 bits, 12 warps per SM); loading straight into registers kept one and ran at a quarter of
+// HBM's rate (1 600 GB/s over 64 requests of up to 4 096 tokens).
 //
 // Bound: HBM.  Four warps of a CTA split the item's tokens and fold their states
 // through shared memory; items that split a sequence leave partial rows for merge_kernel.
+#include <atomic>
+
 #include "common.cuh"
 
 namespace be {
@@ -53,15 +56,13 @@ constexpr float kNoMax = -1e30f;      // running maximum of a row that has seen 
 
 // Loads that stay where they are written: a plain load of constant memory is moved down to its
 // first use, which puts its latency back into every step.
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0));
+}
 __device__ __forceinline__ int4 ld_early16(const void* p) {
   int4 v;
   asm volatile("ld.global.nc.v4.s32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint2 ld_early8(const void* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
   return v;
 }
 __device__ __forceinline__ int ld_early4(const int32_t* p) {
@@ -90,9 +91,20 @@ __device__ __forceinline__ bool word_not_finite(uint32_t w) {
   }
 }
 
+// Ring of one warp: stages of 16 K rows, 16 V rows, 16 + 16 scales and a word of valid tokens.
+template <typename CT, int D>
+struct PnRing {
+  static constexpr int ROWB = D * CacheElt<CT>::bytes;
+  static constexpr int STAGE = 2 * 16 * ROWB + 256;
+  static constexpr int STAGES = ROWB > 128 ? 3 : 4;
+  static constexpr int CTAS = ROWB > 128 ? 2 : 3;      // per SM
+  static constexpr int FOLD = 4 * 16 * (D + 4) * 4;    // the warps' O at the end
+  static constexpr int BYTES = 4 * STAGES * STAGE > FOLD ? 4 * STAGES * STAGE : FOLD;
+};
+
 // T: type of q and out.  CT: E4M3 or T.
 template <typename T, typename CT, int D>
-__global__ void __launch_bounds__(128) paged_narrow_kernel(const PagedParams p) {
+__global__ void __launch_bounds__(128, PnRing<CT, D>::CTAS) paged_narrow_kernel(const PagedParams p) {
   constexpr bool Q8 = std::is_same<CT, E4M3>::value;
   using MT = typename std::conditional<Q8, __half, T>::type;   // type of the products
   constexpr int EB = CacheElt<CT>::bytes;
@@ -104,7 +116,10 @@ __global__ void __launch_bounds__(128) paged_narrow_kernel(const PagedParams p) 
   constexpr int VW = VB / EB;                  // dims per V piece
   constexpr int KS = D / 16, NT = D / 8;       // k-steps of S, column tiles of O
   constexpr int OLD = D + 4;
-  __shared__ __align__(16) float sO[4][16][OLD];
+  using Ring = PnRing<CT, D>;
+  constexpr int CHR = ROWB / 16;               // 16-byte chunks per row
+  extern __shared__ __align__(128) char ring_raw[];
+  float (*sO)[16][OLD] = reinterpret_cast<float (*)[16][OLD]>(ring_raw);
   __shared__ float sM[4][16], sL[4][16];
 
   pdl_wait();
@@ -171,59 +186,48 @@ __global__ void __launch_bounds__(128) paged_narrow_kernel(const PagedParams p) 
   }
 
   const int64_t row_step = (int64_t)p.hkv * ROWB;             // bytes between a page's tokens
-  const int64_t plane_step = row_step * p.ps;
   const char* base = p.pool + (int64_t)kvh * ROWB;
-
-  // Token (lane & 15) of the step that starts at v0: its K row's byte offset (V is a
-  // plane further), or -1 past the range and for a page that does not exist.
-  auto locate = [&](int v0, float& sk, float& sv) -> int64_t {
-    const int v = v0 + (lane & 15);
-    sk = 0.f;
-    sv = 0.f;
+  char* ring = ring_raw + warp * (Ring::STAGES * Ring::STAGE);
+  const int ps_shift = (p.ps & (p.ps - 1)) == 0 ? __ffs(p.ps) - 1 : -1;
+  auto token_t = [&](int v) { return v + (v >= w.n0 ? w.shift : 0); };
+  // place of token t's row in the ring (8-bit rows of 64 dims: two lie in one line of banks, so even
+  // and odd tokens go to different halves) and of its chunk
+  auto row_at = [](int t) { return (ROWB == 64 ? (t >> 1) | ((t & 1) << 3) : t) * ROWB; };
+  auto chunk_at = [](int t, int ch) {
+    return (ROWB == 64 ? ch ^ (((t >> 2) & 1) << 1) : ch ^ ((t & 6) ^ ((t & 1) << 2))) << 4;
+  };
+  auto page_of = [&](int v) -> int {           // page id of token v's step place (lane & 15)
+    v += lane & 15;
     if (v >= w.v_end) return -1;
-    const int t = v + (v >= w.n0 ? w.shift : 0);
-    const int pi = t / p.ps;
-    const int page = kvlist[pi];
-    if (page < 0 || page >= p.num_pages) {
-      flag_range_error();
-      return -1;
-    }
-    if constexpr (Q8) {
-      const float* s = p.scale + (int64_t)page * 2 * p.hkv + kvh;
-      sk = s[0];
-      sv = s[p.hkv];
-    }
-    return (int64_t)page * 2 * plane_step + (int64_t)(t - pi * p.ps) * row_step;
+    const int t = token_t(v);
+    return ld_early4(kvlist + (ps_shift >= 0 ? t >> ps_shift : t / p.ps));
   };
-
-  int4 kraw[2][KP];
-  uint32_t vraw[4][VP * VB / 4];
-  auto load_k = [&](int64_t at) {
+  // Requests the 16 tokens from v0 into stage st; tokens that are not there are zeros.
+  auto issue = [&](int st, int v0, int page) {
+    if (v0 < w.v_end) {
+      char* dst = ring + st * Ring::STAGE;
+      const int v = v0 + (lane & 15);
+      const bool has = page >= 0 && page < p.num_pages;
+      if (!has && v < w.v_end) flag_range_error();
+      const int t = token_t(v);
+      const int row = has ? page * 2 * p.ps + (ps_shift >= 0 ? t & (p.ps - 1) : t % p.ps) : -1;
+      const unsigned valid = __ballot_sync(0xffffffffu, has) & 0xffffu;
+      if (lane == 0) *reinterpret_cast<unsigned*>(dst + 2 * 16 * ROWB + 128) = valid;
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const int64_t o = __shfl_sync(0xffffffffu, at, n * 8 + r);
-#pragma unroll
-      for (int k = 0; k < KP; ++k)
-        kraw[n][k] = o >= 0 ? ld_early16(base + o + k * 64 + c * 16) : make_int4(0, 0, 0, 0);
-    }
-  };
-  auto load_v = [&](int64_t at) {
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const int64_t o = __shfl_sync(0xffffffffu, at, (n >> 1) * 8 + 2 * c + (n & 1));
-      const char* src = base + o + plane_step;
-#pragma unroll
-      for (int k = 0; k < VP; ++k) {
-        if constexpr (VB == 16) {
-          const int4 x = o >= 0 ? ld_early16(src + k * 128 + r * 16) : make_int4(0, 0, 0, 0);
-          vraw[n][4 * k] = x.x; vraw[n][4 * k + 1] = x.y;
-          vraw[n][4 * k + 2] = x.z; vraw[n][4 * k + 3] = x.w;
-        } else {
-          const uint2 x = o >= 0 ? ld_early8(src + r * 8) : make_uint2(0, 0);
-          vraw[n][0] = x.x; vraw[n][1] = x.y;
-        }
+      for (int i = 0; i < 16 * CHR / 32; ++i) {
+        const int k = lane / CHR + i * (32 / CHR), ch = lane % CHR;
+        const int rk = __shfl_sync(0xffffffffu, row, k);
+        const char* src = base + (int64_t)max(rk, 0) * row_step + ch * 16;
+        const uint32_t to = smem_u32(dst + row_at(k) + chunk_at(k, ch));
+        cp_async16(to, src, rk >= 0);
+        cp_async16(to + 16 * ROWB, src + row_step * p.ps, rk >= 0);
+      }
+      if constexpr (Q8) {
+        const float* s = p.scale + (int64_t)max(page, 0) * 2 * p.hkv + kvh + (lane < 16 ? 0 : p.hkv);
+        cp_async4(smem_u32(dst + 2 * 16 * ROWB + lane * 4), has ? s : p.scale, has);
       }
     }
+    cp_commit();
   };
 
   float o[NT][4];
@@ -233,24 +237,31 @@ __global__ void __launch_bounds__(128) paged_narrow_kernel(const PagedParams p) 
   const int pos_r[2] = {w.pos0 + w.pos_step * (r / g), w.pos0 + w.pos_step * ((r + 8) / g)};
   const int pos_hi = w.pos0 + w.pos_step * (w.q_len - 1);
 
-  int v0 = w.v_begin + warp * 16;
-  float sk = 0.f, sv = 0.f;
-  int64_t at = locate(v0, sk, sv);
-  if (v0 < w.v_end) {
-    load_k(at);
-    load_v(at);
+  int v0 = w.v_begin + warp * 16, st = 0;
+  int page_next = page_of(v0);
+#pragma unroll
+  for (int j = 0; j < Ring::STAGES - 1; ++j) {
+    const int page = page_next;
+    page_next = page_of(v0 + 64 * (j + 1));
+    issue(j, v0 + 64 * j, page);
   }
   for (; v0 < w.v_end; v0 += 64) {
-    float sk_next, sv_next;
-    const int64_t at_next = locate(v0 + 64, sk_next, sv_next);
+    cp_wait<Ring::STAGES - 2>();
+    __syncwarp();
+    // the stage read in the step before takes the tokens 3 (2) steps ahead
+    const int page = page_next;
+    page_next = page_of(v0 + 64 * Ring::STAGES);
+    issue(st == 0 ? Ring::STAGES - 1 : st - 1, v0 + 64 * (Ring::STAGES - 1), page);
+    const char* stage = ring + st * Ring::STAGE;
     // ---- S = Q K^T over 2 x 8 tokens ----
     float s[2][4] = {};
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
 #pragma unroll
       for (int k = 0; k < KP; ++k) {
-        const uint32_t wd[4] = {(uint32_t)kraw[n][k].x, (uint32_t)kraw[n][k].y,
-                                (uint32_t)kraw[n][k].z, (uint32_t)kraw[n][k].w};
+        const uint4 x4 = *reinterpret_cast<const uint4*>(stage + row_at(n * 8 + r) +
+                                                         chunk_at(n * 8 + r, k * 4 + c));
+        const uint32_t wd[4] = {x4.x, x4.y, x4.z, x4.w};
         if constexpr (Q8) {
 #pragma unroll
           for (int x = 0; x < 4; ++x)
@@ -262,28 +273,38 @@ __global__ void __launch_bounds__(128) paged_narrow_kernel(const PagedParams p) 
         }
       }
     }
-    load_k(at_next);
     // ---- scores in base 2, masked; x[n][i]: token n * 8 + 2c + (i & 1), row r + 8 (i >> 1) ----
-    const unsigned valid = __ballot_sync(0xffffffffu, at >= 0);
-    const int t_lo = v0 + (v0 >= w.n0 ? w.shift : 0);
-    const int t_hi = v0 + 15 + (v0 + 15 >= w.n0 ? w.shift : 0);
-    const bool full = (valid & 0xffffu) == 0xffffu && (!causal || t_hi <= w.pos0) &&
+    const unsigned valid = *reinterpret_cast<const unsigned*>(stage + 2 * 16 * ROWB + 128);
+    const int t_lo = token_t(v0), t_hi = token_t(v0 + 15);
+    const bool full = valid == 0xffffu && (!causal || t_hi <= w.pos0) &&
                       (!window || t_lo >= pos_hi - w.window || t_hi < w.sink_end);
     float rsv[2][2] = {{1.f, 1.f}, {1.f, 1.f}};
     float mult[2][2] = {{1.f, 1.f}, {1.f, 1.f}}, add[2][2] = {};
     if constexpr (Q8) {
+      const float* sc = reinterpret_cast<const float*>(stage + 2 * 16 * ROWB);
       // a V scale of 0 (a block never written) stands for values of 0: any scale will do
-      const float svc = fmaxf(sv, 9.0949470177e-13f);            // 2^-40
-      const float lsv = log2f(svc), inv = 1.f / svc;
+      if (t_hi - t_lo == 15 && ((p.ps | t_lo) & 15) == 0) {        // one page
+        const float sk = sc[0], svc = fmaxf(sc[16], 9.0949470177e-13f);            // 2^-40
+        const float lsv = log2f(svc), inv = 1.f / svc;
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int src = n * 8 + 2 * c + e;
-          mult[n][e] = __shfl_sync(0xffffffffu, sk, src);
-          add[n][e] = __shfl_sync(0xffffffffu, lsv, src);
-          rsv[n][e] = __shfl_sync(0xffffffffu, inv, src);
-        }
+          for (int e = 0; e < 2; ++e) {
+            mult[n][e] = sk;
+            add[n][e] = lsv;
+            rsv[n][e] = inv;
+          }
+      } else {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float svc = fmaxf(sc[16 + n * 8 + 2 * c + e], 9.0949470177e-13f);
+            mult[n][e] = sc[n * 8 + 2 * c + e];
+            add[n][e] = log2f(svc);
+            rsv[n][e] = 1.f / svc;
+          }
+      }
     }
     bool grew = false;
 #pragma unroll
@@ -328,6 +349,24 @@ __global__ void __launch_bounds__(128) paged_narrow_kernel(const PagedParams p) 
         pf[n][i] = ex2(s[n][i] - m[i >> 1]);
         l[i >> 1] = fmaf(pf[n][i], rsv[n][i & 1], l[i >> 1]);
       }
+    // ---- V fragments' words: tokens 2c, 2c + 1, 2c + 8, 2c + 9 ----
+    uint32_t vraw[4][VP * VB / 4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int t = (n >> 1) * 8 + 2 * c + (n & 1);
+      const char* src = stage + 16 * ROWB + row_at(t);
+#pragma unroll
+      for (int k = 0; k < VP; ++k) {
+        if constexpr (VB == 16) {
+          const uint4 x = *reinterpret_cast<const uint4*>(src + chunk_at(t, k * 8 + r));
+          vraw[n][4 * k] = x.x; vraw[n][4 * k + 1] = x.y;
+          vraw[n][4 * k + 2] = x.z; vraw[n][4 * k + 3] = x.w;
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2*>(src + chunk_at(t, r >> 1) + (r & 1) * 8);
+          vraw[n][0] = x.x; vraw[n][1] = x.y;
+        }
+      }
+    }
     // ---- values that are not finite and not seen by every row: out of the product (0 * NaN is
     // NaN), added to the rows that see them ----
     if (!full) {
@@ -349,9 +388,9 @@ __global__ void __launch_bounds__(128) paged_narrow_kernel(const PagedParams p) 
 #pragma unroll
             for (int k = 0; k < VP * VB / 4; ++k) vraw[n][k] = 0;
         }
+#pragma unroll 1
         for (int k = 0; k < 16; ++k) {
-          const int64_t off = __shfl_sync(0xffffffffu, at, k);
-          if (off < 0) continue;
+          if (!((valid >> k) & 1)) continue;
           const int src = (lane & 28) + ((k & 7) >> 1);
           const float q00 = __shfl_sync(0xffffffffu, pf[0][0], src), q01 = __shfl_sync(0xffffffffu, pf[0][1], src);
           const float q02 = __shfl_sync(0xffffffffu, pf[0][2], src), q03 = __shfl_sync(0xffffffffu, pf[0][3], src);
@@ -359,22 +398,23 @@ __global__ void __launch_bounds__(128) paged_narrow_kernel(const PagedParams p) 
           const float q12 = __shfl_sync(0xffffffffu, pf[1][2], src), q13 = __shfl_sync(0xffffffffu, pf[1][3], src);
           const float p0 = k < 8 ? ((k & 1) ? q01 : q00) : ((k & 1) ? q11 : q10);
           const float p1 = k < 8 ? ((k & 1) ? q03 : q02) : ((k & 1) ? q13 : q12);
-          const char* src_v = base + off + plane_step;
+          const char* row_v = stage + 16 * ROWB + row_at(k);
           bool has = false;
           for (int b = lane * 4; b < ROWB; b += 128)
-            has |= word_not_finite<CT>(*reinterpret_cast<const uint32_t*>(src_v + b));
+            has |= word_not_finite<CT>(*reinterpret_cast<const uint32_t*>(row_v + b));
           if (!__any_sync(0xffffffffu, has)) continue;
 #pragma unroll
           for (int i = 0; i < NT; ++i)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const int d = (i / VW) * 8 * VW + (2 * c + e) * VW + i % VW;
+              const int b = ((i / VW) * 8 * VW + (2 * c + e) * VW + i % VW) * EB;    // byte of the row
+              const char* src_v = row_v + chunk_at(k, b >> 4) + (b & 15);
               float val;
               if constexpr (Q8) {
-                const uint32_t h2 = e4m3x2_to_h2(*reinterpret_cast<const uint8_t*>(src_v + d));
+                const uint32_t h2 = e4m3x2_to_h2(*reinterpret_cast<const uint8_t*>(src_v));
                 val = __low2float(*reinterpret_cast<const __half2*>(&h2));
               } else {
-                val = to_f(reinterpret_cast<const T*>(src_v)[d]);
+                val = to_f(*reinterpret_cast<const T*>(src_v));
               }
               if (p0 > 0.f) o[i][e] = fmaf(p0, val, o[i][e]);
               if (p1 > 0.f) o[i][2 + e] = fmaf(p1, val, o[i][2 + e]);
@@ -402,11 +442,10 @@ __global__ void __launch_bounds__(128) paged_narrow_kernel(const PagedParams p) 
         mma16816<MT>(o[2 * k + 1], pa, prmt(vraw[0][k], vraw[1][k], 0x7632), prmt(vraw[2][k], vraw[3][k], 0x7632));
       }
     }
-    load_v(at_next);
-    at = at_next;
-    sk = sk_next;
-    sv = sv_next;
+    st = st + 1 == Ring::STAGES ? 0 : st + 1;
   }
+  cp_wait<0>();
+  __syncthreads();                             // every ring is read: O goes there
 
   // ---- fold the four warps ----
 #pragma unroll
@@ -466,6 +505,28 @@ __global__ void __launch_bounds__(128) paged_narrow_kernel(const PagedParams p) 
   }
 }
 
+// Raises a kernel's shared-memory limit, once per device.
+template <typename K>
+static int allow_smem(K kernel, int bytes, std::atomic<uint64_t>& ready) {
+  int dev = 0;
+  BE_CUDA_CHECK(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(ready.load() & bit)) {
+    BE_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    ready.fetch_or(bit);
+  }
+  return BE_OK;
+}
+
+template <typename T, typename CT, int D>
+static int paged_narrow_launch(const PagedParams& p, dim3 grid, cudaStream_t st) {
+  static std::atomic<uint64_t> ready{0};
+  const int rc = allow_smem(paged_narrow_kernel<T, CT, D>, PnRing<CT, D>::BYTES, ready);
+  if (rc != BE_OK) return rc;
+  BE_CUDA_CHECK(launch_pdl(paged_narrow_kernel<T, CT, D>, grid, dim3(128), PnRing<CT, D>::BYTES, st, p));
+  return BE_OK;
+}
+
 template <typename T, typename CT, int D>
 static int paged_wide_launch(const PagedParams& p, int max_wide, cudaStream_t st);
 
@@ -484,15 +545,13 @@ static int paged_launch(const PagedParams& p, bool q8, int D, int max_wide, int 
   }
   if (max_narrow > 0) {
     const dim3 grid((unsigned)max_narrow * p.hkv);   // heads of an item next to each other
-    auto go = [&](auto kernel) -> int {
-      BE_CUDA_CHECK(launch_pdl(kernel, grid, dim3(128), 0, st, p));
-      return BE_OK;
-    };
     int rc;
     if (q8)
-      rc = D == 128 ? go(paged_narrow_kernel<T, E4M3, 128>) : go(paged_narrow_kernel<T, E4M3, 64>);
+      rc = D == 128 ? paged_narrow_launch<T, E4M3, 128>(p, grid, st)
+                    : paged_narrow_launch<T, E4M3, 64>(p, grid, st);
     else
-      rc = D == 128 ? go(paged_narrow_kernel<T, T, 128>) : go(paged_narrow_kernel<T, T, 64>);
+      rc = D == 128 ? paged_narrow_launch<T, T, 128>(p, grid, st)
+                    : paged_narrow_launch<T, T, 64>(p, grid, st);
     if (rc != BE_OK) return rc;
   }
   if (max_merge > 0) {

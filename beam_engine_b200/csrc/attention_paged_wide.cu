@@ -31,7 +31,6 @@
 //
 // Every wait is bounded (2 s); one that runs out sets the device status and the abort flag, and all
 // roles leave their loops.
-#include <atomic>
 #include <climits>
 
 #include "common.cuh"
@@ -816,16 +815,10 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
 
 template <typename T, typename CT, int D>
 static int paged_wide_launch(const PagedParams& p, int max_wide, cudaStream_t st) {
+  static std::atomic<uint64_t> ready{0};
   auto kernel = paged_wide_kernel<T, CT, D>;
-  static std::atomic<uint64_t> ready{0};     // per device: the shared-memory limit is set
-  int dev = 0;
-  BE_CUDA_CHECK(cudaGetDevice(&dev));
-  const uint64_t bit = 1ull << (dev & 63);
-  if (!(ready.load() & bit)) {
-    BE_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       PwSmem<D>::BYTES));
-    ready.fetch_or(bit);
-  }
+  const int rc = allow_smem(kernel, PwSmem<D>::BYTES, ready);
+  if (rc != BE_OK) return rc;
   BE_CUDA_CHECK(launch_pdl(kernel, dim3((unsigned)max_wide * p.hkv), dim3(PW_THREADS),
                            PwSmem<D>::BYTES, st, p));
   return BE_OK;

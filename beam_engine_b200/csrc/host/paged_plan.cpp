@@ -89,6 +89,49 @@ int wide_chunk(const std::vector<Tile>& tiles, int64_t total_steps, int sms, int
   return best_chunk;
 }
 
+// Tokens per narrow item.  About 3 CTAs share an SM, so (item, KV head) pairs run 3 x SMs at a time;
+// whole tiles and cuts at fractions of the average share are tried longest first, with 192 tokens'
+// time for a CTA's start and end and 512 for the merge launch that a cut brings.
+int narrow_chunk(const std::vector<Tile>& tiles, int64_t total, int sms, int hkv) {
+  int longest = 0;
+  for (const Tile& t : tiles)
+    if (!t.wide) longest = std::max(longest, t.n);
+  if (longest == 0) return 1 << 28;
+  const int slots = std::max(1, sms * 3 / hkv);
+  const int64_t share = std::max<int64_t>(1, total / slots);
+  int best_chunk = 1 << 28;
+  int64_t best = INT64_MAX;
+  std::vector<int> cost;
+  std::vector<int64_t> busy;
+  for (const double f : {0.0, 1.0, 0.5, 0.34, 0.25, 0.17}) {
+    const int chunk = f == 0.0 ? 1 << 28 : (int)std::max<int64_t>(128, ((int64_t)(share * f) + 63) / 64 * 64);
+    if (f != 0.0 && chunk >= longest) continue;
+    cost.clear();
+    for (const Tile& t : tiles) {
+      if (t.wide) continue;
+      const int ns = (t.n + chunk - 1) / chunk, len = ((t.n + ns - 1) / ns + 63) / 64 * 64;
+      for (int v = 0; v < t.n; v += len) cost.push_back(std::min(len, t.n - v) + 192);
+    }
+    if (cost.size() > 32768) continue;
+    std::sort(cost.begin(), cost.end(), [](int a, int b) { return a > b; });
+    busy.assign(slots, 0);
+    auto later = [](int64_t a, int64_t b) { return a > b; };      // min-heap
+    int64_t end = 0;
+    for (const int c : cost) {
+      std::pop_heap(busy.begin(), busy.end(), later);
+      busy.back() += c;
+      end = std::max(end, busy.back());
+      std::push_heap(busy.begin(), busy.end(), later);
+    }
+    end += f != 0.0 ? 512 : 0;
+    if (end < best) {
+      best = end;
+      best_chunk = chunk;
+    }
+  }
+  return best_chunk;
+}
+
 }  // namespace
 }  // namespace be
 
@@ -213,9 +256,9 @@ extern "C" int be_paged_plan(int num_levels, const int32_t* const* qo_indptr,
       const int64_t pmax = R.pos0 + (int64_t)R.step * (q0 + t.ql - 1);
       const int64_t hi = R.causal ? std::min<int64_t>(R.kv_len, pmax + 1) : R.kv_len;
       if (hi <= 0) continue;                        // sees nothing
-      // where pages are multiples of 8 tokens, so are the ends of the two runs: groups of 8 tokens then
-      // share a page (the kernels mask by position, so the few tokens more are not seen)
-      const int64_t round = page_size % 8 == 0 ? 7 : 0;
+      // where pages are multiples of 16 (8) tokens, so are the ends of the two runs: groups of 16 (8) tokens
+      // then share a page (the kernels mask by position, so the few tokens more are not seen)
+      const int64_t round = page_size % 16 == 0 ? 15 : page_size % 8 == 0 ? 7 : 0;
       const int64_t lo = window ? std::max<int64_t>(0, pmin - window_left) & ~round : 0;
       const int64_t s = window ? std::min<int64_t>((R.sink_end + round) & ~round, hi) : 0;
       if (lo <= s) {
@@ -233,11 +276,8 @@ extern "C" int be_paged_plan(int num_levels, const int32_t* const* qo_indptr,
       tiles.push_back(t);
     }
   }
-  // items: split the narrow tiles so that items x KV heads come to about `target` CTAs
   const int sms = num_sms > 0 ? num_sms : 148;
-  const int64_t target = std::max<int64_t>(1, (int64_t)sms * 3 / num_kv_heads);
-  const int64_t even = (narrow_tokens + target - 1) / std::max<int64_t>(1, target);
-  const int chunk_n = (int)std::min<int64_t>(1 << 28, std::max<int64_t>(256, (even + 63) / 64 * 64));
+  const int chunk_n = narrow_chunk(tiles, narrow_tokens, sms, num_kv_heads);
   const int chunk_w = wide_chunk(tiles, wide_steps, sms, num_kv_heads) * 128;
   struct Item {
     int tile, v0, v1, part;
@@ -246,7 +286,7 @@ extern "C" int be_paged_plan(int num_levels, const int32_t* const* qo_indptr,
   std::vector<int32_t> cover(num_queries, 0);
   for (size_t i = 0; i < tiles.size(); ++i) {
     const Tile& t = tiles[i];
-    const int chunk = t.wide ? chunk_w : chunk_n, unit = t.wide ? 128 : 16;
+    const int chunk = t.wide ? chunk_w : chunk_n, unit = t.wide ? 128 : 64;
     const int nsplit = (t.n + chunk - 1) / chunk;
     const int len = ((t.n + nsplit - 1) / nsplit + unit - 1) / unit * unit;
     for (int v = 0; v < t.n; v += len) {
