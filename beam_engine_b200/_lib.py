@@ -29,6 +29,10 @@ class AttnPlanInfo(C.Structure):
         "page_size", "group_size", "any_slots", "max_item_tokens", "total_tokens", "max_wide_tokens")]
 
 
+class PagedPlanInfo(C.Structure):
+    _fields_ = AttnPlanInfo._fields_ + [("narrow_rows", C.c_int32)]
+
+
 class TilePlanInfo(C.Structure):
     _fields_ = [(n, C.c_int32) for n in (
         "n_tiles", "n_pieces", "n_entries", "n_queries", "off_tiles", "off_pieces", "off_entries",
@@ -86,8 +90,8 @@ _SIGS = {
                                           C.c_int, vp, C.c_int, C.c_int, vp]),
     "be_paged_plan": (C.c_int, [C.c_int, PP32, PP32, PP32, PP32, P32, C.c_int, C.c_int, C.c_int,
                                 C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp, i64,
-                                C.POINTER(AttnPlanInfo)]),
-    "be_paged_attn_run": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp, i64, vp, vp,
+                                C.POINTER(PagedPlanInfo)]),
+    "be_paged_attn_run": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp, i64, vp, vp,
                                     C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, f32, vp,
                                     i64, vp, vp, vp, vp]),
     # host page manager

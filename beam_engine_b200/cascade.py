@@ -34,7 +34,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import AttnPlanInfo, TilePlanInfo, check, lib
+from ._lib import AttnPlanInfo, PagedPlanInfo, TilePlanInfo, check, lib
 from .page_table import (check_pool8, dtype_code, is_8bit, require_cuda, require_same_device,
                          stream_ptr)
 
@@ -232,8 +232,8 @@ class _Plan:
         i = self.info
         with torch.cuda.device(q.device):
             rc = lib().be_paged_attn_run(
-                self.plan_dev, i.n_work_wide, i.n_work - i.n_work_wide, i.n_merge, i.n_parts,
-                i.page_size, q.data_ptr(), q.stride(0), kv.data_ptr(),
+                self.plan_dev, i.n_work_wide, i.n_work - i.n_work_wide, i.narrow_rows, i.n_merge,
+                i.n_parts, i.page_size, q.data_ptr(), q.stride(0), kv.data_ptr(),
                 kv_scale.data_ptr() if kv_scale is not None else None, kv.shape[0], num_qo_heads,
                 num_kv_heads, head_dim, dtype_code(q.dtype),
                 _lib.BE_E4M3 if kv_scale is not None else dtype_code(kv.dtype), sm_scale,
@@ -335,6 +335,7 @@ class MultiLevelCascadeAttentionWrapper:
             return lib().be_cascade_plan(L, *ptrs, _lib.ptr32(ng), nq, page_size, hq, hkv,
                                          1 if causal else 0, split_tokens, ps.num_sms,
                                          C.cast(buf, _lib.P32), cap, info)
+        ps.info = AttnPlanInfo()
         ps.build(fn)
         ps.place(hq, head_dim)
         ps.tinfo = None
@@ -352,6 +353,7 @@ class MultiLevelCascadeAttentionWrapper:
             return lib().be_paged_plan(L, *ptrs, _lib.ptr32(ng), nq, page_size, hq, hkv,
                                        1 if causal else 0, window, sinks, ps.num_sms, buf, cap,
                                        info)
+        ps.info = PagedPlanInfo()
         ps.build(fn)
         ps.place(hq, head_dim)
         ps.tinfo = None

@@ -16,10 +16,13 @@
 // fp16 with fp32 sums; 16-bit caches use their own type.
 //
 // A warp takes 16 tokens at a time through a ring of its own in shared memory (cp.async by
-// 16 bytes, no barrier between warps) into mma.sync fragments.  The dims of a fragment may be
-// in any order as long as Q and K (or V and O) agree, so a lane reads 16-byte pieces: lane
-// (r, c) = (lane / 4, lane % 4) has token r's pieces c, c + 4, ... for S = Q K^T and piece r of
-// tokens 2c, 2c + 1, 2c + 8, 2c + 9 for O = P V; pieces are swizzled by the token so that both
+// 16 bytes, no barrier between warps) into mma.sync fragments, tokens as the fragments' 16 rows and
+// query rows as their 8 columns: S^T = K Q^T and O^T = V^T P^T, so that the few rows of a single
+// token's heads fill half the products that the other way round needs (up to 8 rows; 16 take two
+// blocks).  P^T turns from result to operand by a transpose of 8 x 8 halves.  The dims of a fragment
+// may be in any order as long as Q and K (or V and O) agree, so a lane reads 16-byte pieces: lane
+// (r, c) = (lane / 4, lane % 4) has pieces c, c + 4, ... of tokens r and r + 8 for S and piece r of
+// tokens 2c, 2c + 1, 2c + 8, 2c + 9 for O; pieces are swizzled by the token so that both
 // reads hit every bank once.  The ring keeps 3 steps in flight per warp (12 KB at 128 dims in
 // 8 bits, 12 warps per SM); loading straight into registers kept one and ran at a quarter of
 // HBM's rate (1 600 GB/s over 64 requests of up to 4 096 tokens).
@@ -75,6 +78,22 @@ __device__ __forceinline__ float ld_early4(const float* p) {
   asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
   return v;
 }
+__device__ __forceinline__ float lg2(float x) {      // of normal numbers: the hardware's, exact for 2^n
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// An 8 x 8 block of halves, one row per four lanes, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
   return __byte_perm(a, b, sel);
 }
@@ -92,19 +111,19 @@ __device__ __forceinline__ bool word_not_finite(uint32_t w) {
 }
 
 // Ring of one warp: stages of 16 K rows, 16 V rows, 16 + 16 scales and a word of valid tokens.
-template <typename CT, int D>
+template <typename CT, int D, int NB>
 struct PnRing {
   static constexpr int ROWB = D * CacheElt<CT>::bytes;
   static constexpr int STAGE = 2 * 16 * ROWB + 256;
   static constexpr int STAGES = ROWB > 128 ? 3 : 4;
   static constexpr int CTAS = ROWB > 128 ? 2 : 3;      // per SM
-  static constexpr int FOLD = 4 * 16 * (D + 4) * 4;    // the warps' O at the end
+  static constexpr int FOLD = 4 * 8 * NB * (D + 4) * 4;   // the warps' O at the end
   static constexpr int BYTES = 4 * STAGES * STAGE > FOLD ? 4 * STAGES * STAGE : FOLD;
 };
 
-// T: type of q and out.  CT: E4M3 or T.
-template <typename T, typename CT, int D>
-__global__ void __launch_bounds__(128, PnRing<CT, D>::CTAS) paged_narrow_kernel(const PagedParams p) {
+// T: type of q and out.  CT: E4M3 or T.  NB: blocks of 8 rows (1 or 2).
+template <typename T, typename CT, int D, int NB>
+__global__ void __launch_bounds__(128, PnRing<CT, D, NB>::CTAS) paged_narrow_kernel(const PagedParams p) {
   constexpr bool Q8 = std::is_same<CT, E4M3>::value;
   using MT = typename std::conditional<Q8, __half, T>::type;   // type of the products
   constexpr int EB = CacheElt<CT>::bytes;
@@ -114,16 +133,16 @@ __global__ void __launch_bounds__(128, PnRing<CT, D>::CTAS) paged_narrow_kernel(
   constexpr int VB = ROWB / 8 < 16 ? ROWB / 8 : 16;   // bytes per V piece
   constexpr int VP = ROWB / (8 * VB);          // V pieces per lane and token
   constexpr int VW = VB / EB;                  // dims per V piece
-  constexpr int KS = D / 16, NT = D / 8;       // k-steps of S, column tiles of O
+  constexpr int KS = D / 16;                   // k-steps of S = tiles of 16 dims of O
   constexpr int OLD = D + 4;
-  using Ring = PnRing<CT, D>;
+  using Ring = PnRing<CT, D, NB>;
   constexpr int CHR = ROWB / 16;               // 16-byte chunks per row
   extern __shared__ __align__(128) char ring_raw[];
-  float (*sO)[16][OLD] = reinterpret_cast<float (*)[16][OLD]>(ring_raw);
-  __shared__ float sM[4][16], sL[4][16];
+  float (*sO)[8 * NB][OLD] = reinterpret_cast<float (*)[8 * NB][OLD]>(ring_raw);
+  __shared__ float sM[4][8 * NB], sL[4][8 * NB];
 
   pdl_wait();
-  const be_attn_plan_info* hdr = reinterpret_cast<const be_attn_plan_info*>(p.plan);
+  const be_paged_plan_info* hdr = reinterpret_cast<const be_paged_plan_info*>(p.plan);
   const int n_wide = hdr->n_work_wide;
   const int item = blockIdx.x / p.hkv, kvh = blockIdx.x - item * p.hkv;
   if (item >= hdr->n_work - n_wide) return;
@@ -134,14 +153,18 @@ __global__ void __launch_bounds__(128, PnRing<CT, D>::CTAS) paged_narrow_kernel(
   const int g = p.g, rows = w.q_len * g;
   const bool causal = (w.flags & BE_ITEM_CAUSAL) != 0;
   const bool window = w.window >= 0;
+  if (rows > 8 * NB) {                         // a plan made for higher tiles
+    if (tid == 0) flag_range_error();
+    return;
+  }
 
-  // ---- Q fragments: rows r and r + 8 ----
-  uint32_t qa[KS][4];
-  float row_scale[2];
+  // ---- Q fragments (second operand): row 8 b + r, this lane's D / 4 dims as 16-bit pairs ----
+  uint32_t qb[NB][D / 8];
+  float up_r[NB];                              // 1 / (what the row's products are scaled by)
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int row = r + 8 * h;
-    uint32_t raw[D / 8];                       // this lane's D / 4 dims, 16-bit pairs
+  for (int b = 0; b < NB; ++b) {
+    const int row = r + 8 * b;
+    uint32_t (&raw)[D / 8] = qb[b];
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) raw[i] = 0;
     if (row < rows) {
@@ -156,7 +179,7 @@ __global__ void __launch_bounds__(128, PnRing<CT, D>::CTAS) paged_narrow_kernel(
           raw[o] = v.x; raw[o + 1] = v.y; raw[o + 2] = v.z; raw[o + 3] = v.w;
         }
     }
-    row_scale[h] = p.scale_log2;
+    up_r[b] = p.scale_log2;
     if constexpr (Q8 && std::is_same<T, __nv_bfloat16>::value) {
       float mx = 0.f;
 #pragma unroll
@@ -170,7 +193,7 @@ __global__ void __launch_bounds__(128, PnRing<CT, D>::CTAS) paged_narrow_kernel(
       int e = (int)(__float_as_uint(mx) >> 23) - 127;
       e = mx < INFINITY ? min(max(e, -110), 110) : 0;
       const float up = __uint_as_float((uint32_t)(8 - e + 127) << 23);
-      row_scale[h] *= __uint_as_float((uint32_t)(e - 8 + 127) << 23);
+      up_r[b] *= __uint_as_float((uint32_t)(e - 8 + 127) << 23);
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) {
         const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[i]));
@@ -178,12 +201,18 @@ __global__ void __launch_bounds__(128, PnRing<CT, D>::CTAS) paged_narrow_kernel(
         raw[i] = *reinterpret_cast<const uint32_t*>(&x);
       }
     }
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      qa[s][h] = raw[2 * s];
-      qa[s][2 + h] = raw[2 * s + 1];
-    }
   }
+  // from here a lane's rows are 8 b + 2 c + e: columns of the score fragments
+  float row_scale[NB][2];
+  int pos_r[NB][2];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      row_scale[b][e] = __shfl_sync(0xffffffffu, up_r[b], (2 * c + e) * 4);
+      pos_r[b][e] = w.pos0 + w.pos_step * ((8 * b + 2 * c + e) / g);
+    }
+  const int pos_hi = w.pos0 + w.pos_step * (w.q_len - 1);
 
   const int64_t row_step = (int64_t)p.hkv * ROWB;             // bytes between a page's tokens
   const char* base = p.pool + (int64_t)kvh * ROWB;
@@ -196,12 +225,15 @@ __global__ void __launch_bounds__(128, PnRing<CT, D>::CTAS) paged_narrow_kernel(
   auto chunk_at = [](int t, int ch) {
     return (ROWB == 64 ? ch ^ (((t >> 2) & 1) << 1) : ch ^ ((t & 6) ^ ((t & 1) << 2))) << 4;
   };
-  auto page_of = [&](int v) -> int {           // page id of token v's step place (lane & 15)
+  auto page_of = [&](int v) -> int {           // page id of token v + (lane & 15)
     v += lane & 15;
     if (v >= w.v_end) return -1;
     const int t = token_t(v);
     return ld_early4(kvlist + (ps_shift >= 0 ? t >> ps_shift : t / p.ps));
   };
+  // this lane's part of a step's copies: chunk ch of tokens k0, k0 + 32 / CHR, ...
+  const int k0 = lane / CHR, ch = lane % CHR;
+  const int64_t v_plane = row_step * p.ps;
   // Requests the 16 tokens from v0 into stage st; tokens that are not there are zeros.
   auto issue = [&](int st, int v0, int page) {
     if (v0 < w.v_end) {
@@ -215,12 +247,12 @@ __global__ void __launch_bounds__(128, PnRing<CT, D>::CTAS) paged_narrow_kernel(
       if (lane == 0) *reinterpret_cast<unsigned*>(dst + 2 * 16 * ROWB + 128) = valid;
 #pragma unroll
       for (int i = 0; i < 16 * CHR / 32; ++i) {
-        const int k = lane / CHR + i * (32 / CHR), ch = lane % CHR;
+        const int k = k0 + i * (32 / CHR);
         const int rk = __shfl_sync(0xffffffffu, row, k);
         const char* src = base + (int64_t)max(rk, 0) * row_step + ch * 16;
         const uint32_t to = smem_u32(dst + row_at(k) + chunk_at(k, ch));
         cp_async16(to, src, rk >= 0);
-        cp_async16(to + 16 * ROWB, src + row_step * p.ps, rk >= 0);
+        cp_async16(to + 16 * ROWB, src + v_plane, rk >= 0);
       }
       if constexpr (Q8) {
         const float* s = p.scale + (int64_t)max(page, 0) * 2 * p.hkv + kvh + (lane < 16 ? 0 : p.hkv);
@@ -230,12 +262,17 @@ __global__ void __launch_bounds__(128, PnRing<CT, D>::CTAS) paged_narrow_kernel(
     cp_commit();
   };
 
-  float o[NT][4];
+  // O^T: tile j holds dims i = 2 j and 2 j + 1 of this lane's V pieces (the fragment's rows r and
+  // r + 8), columns 8 b + 2c + {0, 1}
+  float o[NB][KS][4];
+  float m[NB][2], l[NB][2];
 #pragma unroll
-  for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float m[2] = {kNoMax, kNoMax}, l[2] = {0.f, 0.f};
-  const int pos_r[2] = {w.pos0 + w.pos_step * (r / g), w.pos0 + w.pos_step * ((r + 8) / g)};
-  const int pos_hi = w.pos0 + w.pos_step * (w.q_len - 1);
+  for (int b = 0; b < NB; ++b) {
+#pragma unroll
+    for (int j = 0; j < KS; ++j) o[b][j][0] = o[b][j][1] = o[b][j][2] = o[b][j][3] = 0.f;
+    m[b][0] = m[b][1] = kNoMax;
+    l[b][0] = l[b][1] = 0.f;
+  }
 
   int v0 = w.v_begin + warp * 16, st = 0;
   int page_next = page_of(v0);
@@ -253,101 +290,105 @@ __global__ void __launch_bounds__(128, PnRing<CT, D>::CTAS) paged_narrow_kernel(
     page_next = page_of(v0 + 64 * Ring::STAGES);
     issue(st == 0 ? Ring::STAGES - 1 : st - 1, v0 + 64 * (Ring::STAGES - 1), page);
     const char* stage = ring + st * Ring::STAGE;
-    // ---- S = Q K^T over 2 x 8 tokens ----
-    float s[2][4] = {};
+    // ---- S^T = K Q^T: 16 tokens x 8 NB rows; s[b][i]: token r + 8 (i >> 1), row 8 b + 2c + (i & 1) ----
+    float s[NB][4] = {};
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+    for (int k = 0; k < KP; ++k) {
+      const uint4 x0 = *reinterpret_cast<const uint4*>(stage + row_at(r) + chunk_at(r, k * 4 + c));
+      const uint4 x1 = *reinterpret_cast<const uint4*>(stage + row_at(r + 8) + chunk_at(r + 8, k * 4 + c));
+      const uint32_t wa[4] = {x0.x, x0.y, x0.z, x0.w}, wb[4] = {x1.x, x1.y, x1.z, x1.w};
+      if constexpr (Q8) {
 #pragma unroll
-      for (int k = 0; k < KP; ++k) {
-        const uint4 x4 = *reinterpret_cast<const uint4*>(stage + row_at(n * 8 + r) +
-                                                         chunk_at(n * 8 + r, k * 4 + c));
-        const uint32_t wd[4] = {x4.x, x4.y, x4.z, x4.w};
-        if constexpr (Q8) {
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t a[4] = {e4m3x2_to_h2(wa[x] & 0xffffu), e4m3x2_to_h2(wb[x] & 0xffffu),
+                                 e4m3x2_to_h2(wa[x] >> 16), e4m3x2_to_h2(wb[x] >> 16)};
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-            mma16816<MT>(s[n], qa[k * 4 + x], e4m3x2_to_h2(wd[x] & 0xffffu),
-                         e4m3x2_to_h2(wd[x] >> 16));
-        } else {
-          mma16816<MT>(s[n], qa[k * 2], wd[0], wd[1]);
-          mma16816<MT>(s[n], qa[k * 2 + 1], wd[2], wd[3]);
+          for (int b = 0; b < NB; ++b)
+            mma16816<MT>(s[b], a, qb[b][2 * (k * 4 + x)], qb[b][2 * (k * 4 + x) + 1]);
+        }
+      } else {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const uint32_t a[4] = {wa[2 * x], wb[2 * x], wa[2 * x + 1], wb[2 * x + 1]};
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+            mma16816<MT>(s[b], a, qb[b][2 * (k * 2 + x)], qb[b][2 * (k * 2 + x) + 1]);
         }
       }
     }
-    // ---- scores in base 2, masked; x[n][i]: token n * 8 + 2c + (i & 1), row r + 8 (i >> 1) ----
+    // ---- scores in base 2, masked ----
     const unsigned valid = *reinterpret_cast<const unsigned*>(stage + 2 * 16 * ROWB + 128);
     const int t_lo = token_t(v0), t_hi = token_t(v0 + 15);
     const bool full = valid == 0xffffu && (!causal || t_hi <= w.pos0) &&
                       (!window || t_lo >= pos_hi - w.window || t_hi < w.sink_end);
-    float rsv[2][2] = {{1.f, 1.f}, {1.f, 1.f}};
-    float mult[2][2] = {{1.f, 1.f}, {1.f, 1.f}}, add[2][2] = {};
+    float mult[2] = {1.f, 1.f}, add[2] = {0.f, 0.f}, rsv[2] = {1.f, 1.f};   // tokens r, r + 8
     if constexpr (Q8) {
       const float* sc = reinterpret_cast<const float*>(stage + 2 * 16 * ROWB);
       // a V scale of 0 (a block never written) stands for values of 0: any scale will do
-      if (t_hi - t_lo == 15 && ((p.ps | t_lo) & 15) == 0) {        // one page
-        const float sk = sc[0], svc = fmaxf(sc[16], 9.0949470177e-13f);            // 2^-40
-        const float lsv = log2f(svc), inv = 1.f / svc;
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            mult[n][e] = sk;
-            add[n][e] = lsv;
-            rsv[n][e] = inv;
-          }
+      mult[0] = sc[r];
+      const float sv0 = fmaxf(sc[16 + r], 9.0949470177e-13f);            // 2^-40
+      add[0] = lg2(sv0);
+      rsv[0] = rcp(sv0);
+      if (t_hi - t_lo == 15 && ((p.ps | t_lo) & 15) == 0) {              // one page
+        mult[1] = mult[0];
+        add[1] = add[0];
+        rsv[1] = rsv[0];
       } else {
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float svc = fmaxf(sc[16 + n * 8 + 2 * c + e], 9.0949470177e-13f);
-            mult[n][e] = sc[n * 8 + 2 * c + e];
-            add[n][e] = log2f(svc);
-            rsv[n][e] = 1.f / svc;
-          }
+        mult[1] = sc[r + 8];
+        const float sv1 = fmaxf(sc[24 + r], 9.0949470177e-13f);
+        add[1] = lg2(sv1);
+        rsv[1] = rcp(sv1);
       }
     }
     bool grew = false;
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int h = i >> 1, e = i & 1;
-        float x = Q8 ? fmaf(s[n][i], row_scale[h] * mult[n][e], add[n][e]) : s[n][i] * row_scale[h];
+        float x = Q8 ? fmaf(s[b][i], row_scale[b][e] * mult[h], add[h]) : s[b][i] * row_scale[b][e];
         if (!full) {
-          const int k = n * 8 + 2 * c + e, v = v0 + k;
-          const int t = v + (v >= w.n0 ? w.shift : 0);
-          const bool see = ((valid >> k) & 1) && (!causal || t <= pos_r[h]) &&
-                           (!window || t >= pos_r[h] - w.window || t < w.sink_end);
+          const int k = r + 8 * h, t = token_t(v0 + k);
+          const bool see = ((valid >> k) & 1) && (!causal || t <= pos_r[b][e]) &&
+                           (!window || t >= pos_r[b][e] - w.window || t < w.sink_end);
           x = see ? x : -INFINITY;
         }
-        s[n][i] = x;
-        grew |= x > m[h] + kLazyMax;
+        s[b][i] = x;
+        grew |= x > m[b][e] + kLazyMax;
       }
     // ---- the running maximum moves only when a factor would pass 2^8 ----
     if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float mx = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        mx = fmaxf(mx, m[h]);
-        const float f = ex2(m[h] - mx);
-        m[h] = mx;
-        l[h] *= f;
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          o[i][2 * h] *= f;
-          o[i][2 * h + 1] *= f;
+        for (int e = 0; e < 2; ++e) {
+          float mx = fmaxf(s[b][e], s[b][2 + e]);
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          mx = fmaxf(mx, m[b][e]);
+          const float f = ex2(m[b][e] - mx);
+          m[b][e] = mx;
+          l[b][e] *= f;
+#pragma unroll
+          for (int j = 0; j < KS; ++j) {
+            o[b][j][e] *= f;
+            o[b][j][2 + e] *= f;
+          }
         }
-      }
     }
-    float pf[2][4];
+    // P^T as the second operand: the fragment's 8 x 8 blocks of halves, transposed
+    uint32_t pb[NB][2];
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        pf[n][i] = ex2(s[n][i] - m[i >> 1]);
-        l[i >> 1] = fmaf(pf[n][i], rsv[n][i & 1], l[i >> 1]);
+      for (int h = 0; h < 2; ++h) {
+        const float a0 = ex2(s[b][2 * h] - m[b][0]), a1 = ex2(s[b][2 * h + 1] - m[b][1]);
+        l[b][0] = fmaf(a0, rsv[h], l[b][0]);
+        l[b][1] = fmaf(a1, rsv[h], l[b][1]);
+        s[b][2 * h] = a0;
+        s[b][2 * h + 1] = a1;
+        pb[b][h] = transpose8(pack2<MT>(a0, a1));
       }
     // ---- V fragments' words: tokens 2c, 2c + 1, 2c + 8, 2c + 9 ----
     uint32_t vraw[4][VP * VB / 4];
@@ -391,24 +432,21 @@ __global__ void __launch_bounds__(128, PnRing<CT, D>::CTAS) paged_narrow_kernel(
 #pragma unroll 1
         for (int k = 0; k < 16; ++k) {
           if (!((valid >> k) & 1)) continue;
-          const int src = (lane & 28) + ((k & 7) >> 1);
-          const float q00 = __shfl_sync(0xffffffffu, pf[0][0], src), q01 = __shfl_sync(0xffffffffu, pf[0][1], src);
-          const float q02 = __shfl_sync(0xffffffffu, pf[0][2], src), q03 = __shfl_sync(0xffffffffu, pf[0][3], src);
-          const float q10 = __shfl_sync(0xffffffffu, pf[1][0], src), q11 = __shfl_sync(0xffffffffu, pf[1][1], src);
-          const float q12 = __shfl_sync(0xffffffffu, pf[1][2], src), q13 = __shfl_sync(0xffffffffu, pf[1][3], src);
-          const float p0 = k < 8 ? ((k & 1) ? q01 : q00) : ((k & 1) ? q11 : q10);
-          const float p1 = k < 8 ? ((k & 1) ? q03 : q02) : ((k & 1) ? q13 : q12);
           const char* row_v = stage + 16 * ROWB + row_at(k);
           bool has = false;
           for (int b = lane * 4; b < ROWB; b += 128)
             has |= word_not_finite<CT>(*reinterpret_cast<const uint32_t*>(row_v + b));
           if (!__any_sync(0xffffffffu, has)) continue;
+          const int src = (k & 7) * 4 + c;     // the lane with this token's probabilities
 #pragma unroll
-          for (int i = 0; i < NT; ++i)
+          for (int b = 0; b < NB; ++b) {
+            const float a0 = __shfl_sync(0xffffffffu, s[b][0], src), a1 = __shfl_sync(0xffffffffu, s[b][1], src);
+            const float a2 = __shfl_sync(0xffffffffu, s[b][2], src), a3 = __shfl_sync(0xffffffffu, s[b][3], src);
+            const float q0 = k < 8 ? a0 : a2, q1 = k < 8 ? a1 : a3;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int b = ((i / VW) * 8 * VW + (2 * c + e) * VW + i % VW) * EB;    // byte of the row
-              const char* src_v = row_v + chunk_at(k, b >> 4) + (b & 15);
+            for (int i = 0; i < 2 * KS; ++i) {
+              const int at = ((i / VW) * 8 * VW + r * VW + i % VW) * EB;    // byte of the row
+              const char* src_v = row_v + chunk_at(k, at >> 4) + (at & 15);
               float val;
               if constexpr (Q8) {
                 const uint32_t h2 = e4m3x2_to_h2(*reinterpret_cast<const uint8_t*>(src_v));
@@ -416,30 +454,34 @@ __global__ void __launch_bounds__(128, PnRing<CT, D>::CTAS) paged_narrow_kernel(
               } else {
                 val = to_f(*reinterpret_cast<const T*>(src_v));
               }
-              if (p0 > 0.f) o[i][e] = fmaf(p0, val, o[i][e]);
-              if (p1 > 0.f) o[i][2 + e] = fmaf(p1, val, o[i][2 + e]);
+              float* acc = &o[b][i / 2][(i & 1) * 2];
+              if (q0 > 0.f) acc[0] = fmaf(q0, val, acc[0]);
+              if (q1 > 0.f) acc[1] = fmaf(q1, val, acc[1]);
             }
+          }
         }
       }
     }
-    // ---- O += P V ----
-    uint32_t pa[4];
-    pa[0] = pack2<MT>(pf[0][0], pf[0][1]);
-    pa[1] = pack2<MT>(pf[0][2], pf[0][3]);
-    pa[2] = pack2<MT>(pf[1][0], pf[1][1]);
-    pa[3] = pack2<MT>(pf[1][2], pf[1][3]);
+    // ---- O^T += V^T P^T ----
 #pragma unroll
     for (int k = 0; k < VP * VB / 4; ++k) {
       if constexpr (Q8) {
         const uint32_t a01 = prmt(vraw[0][k], vraw[1][k], 0x5140), a23 = prmt(vraw[0][k], vraw[1][k], 0x7362);
         const uint32_t b01 = prmt(vraw[2][k], vraw[3][k], 0x5140), b23 = prmt(vraw[2][k], vraw[3][k], 0x7362);
-        mma16816<MT>(o[4 * k], pa, e4m3x2_to_h2(a01 & 0xffffu), e4m3x2_to_h2(b01 & 0xffffu));
-        mma16816<MT>(o[4 * k + 1], pa, e4m3x2_to_h2(a01 >> 16), e4m3x2_to_h2(b01 >> 16));
-        mma16816<MT>(o[4 * k + 2], pa, e4m3x2_to_h2(a23 & 0xffffu), e4m3x2_to_h2(b23 & 0xffffu));
-        mma16816<MT>(o[4 * k + 3], pa, e4m3x2_to_h2(a23 >> 16), e4m3x2_to_h2(b23 >> 16));
+        const uint32_t x[4] = {e4m3x2_to_h2(a01 & 0xffffu), e4m3x2_to_h2(a01 >> 16),
+                               e4m3x2_to_h2(b01 & 0xffffu), e4m3x2_to_h2(b01 >> 16)};
+        const uint32_t y[4] = {e4m3x2_to_h2(a23 & 0xffffu), e4m3x2_to_h2(a23 >> 16),
+                               e4m3x2_to_h2(b23 & 0xffffu), e4m3x2_to_h2(b23 >> 16)};
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          mma16816<MT>(o[b][2 * k], x, pb[b][0], pb[b][1]);
+          mma16816<MT>(o[b][2 * k + 1], y, pb[b][0], pb[b][1]);
+        }
       } else {
-        mma16816<MT>(o[2 * k], pa, prmt(vraw[0][k], vraw[1][k], 0x5410), prmt(vraw[2][k], vraw[3][k], 0x5410));
-        mma16816<MT>(o[2 * k + 1], pa, prmt(vraw[0][k], vraw[1][k], 0x7632), prmt(vraw[2][k], vraw[3][k], 0x7632));
+        const uint32_t x[4] = {prmt(vraw[0][k], vraw[1][k], 0x5410), prmt(vraw[0][k], vraw[1][k], 0x7632),
+                               prmt(vraw[2][k], vraw[3][k], 0x5410), prmt(vraw[2][k], vraw[3][k], 0x7632)};
+#pragma unroll
+        for (int b = 0; b < NB; ++b) mma16816<MT>(o[b][k], x, pb[b][0], pb[b][1]);
       }
     }
     st = st + 1 == Ring::STAGES ? 0 : st + 1;
@@ -449,24 +491,22 @@ __global__ void __launch_bounds__(128, PnRing<CT, D>::CTAS) paged_narrow_kernel(
 
   // ---- fold the four warps ----
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-    if (c == 0) {
-      sM[warp][r + 8 * h] = m[h];
-      sL[warp][r + 8 * h] = l[h];
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < NT; ++i)
+  for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int d = (i / VW) * 8 * VW + (2 * c + e) * VW + i % VW;
-      sO[warp][r][d] = o[i][e];
-      sO[warp][r + 8][d] = o[i][2 + e];
+#pragma unroll
+      for (int off = 4; off < 32; off *= 2) l[b][e] += __shfl_xor_sync(0xffffffffu, l[b][e], off);
+      if (r == 0) {
+        sM[warp][8 * b + 2 * c + e] = m[b][e];
+        sL[warp][8 * b + 2 * c + e] = l[b][e];
+      }
+#pragma unroll
+      for (int i = 0; i < 2 * KS; ++i)
+        sO[warp][8 * b + 2 * c + e][(i / VW) * 8 * VW + r * VW + i % VW] = o[b][i / 2][(i & 1) * 2 + e];
     }
   __syncthreads();
-  const int row = tid >> 3, d0 = (tid & 7) * (D / 8);
+  constexpr int TPR = 128 / (8 * NB);          // threads per row
+  const int row = tid / TPR, d0 = (tid % TPR) * 4;
   if (row >= rows) return;
   const float mx = fmaxf(fmaxf(sM[0][row], sM[1][row]), fmaxf(sM[2][row], sM[3][row]));
   float f[4], den = 0.f;
@@ -479,7 +519,7 @@ __global__ void __launch_bounds__(128, PnRing<CT, D>::CTAS) paged_narrow_kernel(
   const int qi = row / g, head = kvh * g + row % g;
   const int64_t dst_q = w.part_base < 0 ? w.q_begin + qi : w.part_base + qi;
 #pragma unroll
-  for (int d = d0; d < d0 + D / 8; d += 4) {
+  for (int d = d0; d < D; d += 4 * TPR) {
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -494,7 +534,7 @@ __global__ void __launch_bounds__(128, PnRing<CT, D>::CTAS) paged_narrow_kernel(
     else
       *reinterpret_cast<float4*>(p.mid_o + (dst_q * p.hq + head) * D + d) = acc;
   }
-  if ((tid & 7) == 0) {
+  if (tid % TPR == 0) {
     const float lse = den > 0.f ? (mx + log2f(den)) * kLn2 : den == 0.f ? -INFINITY : den;
     // a NaN partial row is merged as +inf: the merge takes the maximum over its parts, which
     // passes over NaN, and inf - inf makes the row NaN there
@@ -518,12 +558,13 @@ static int allow_smem(K kernel, int bytes, std::atomic<uint64_t>& ready) {
   return BE_OK;
 }
 
-template <typename T, typename CT, int D>
+template <typename T, typename CT, int D, int NB>
 static int paged_narrow_launch(const PagedParams& p, dim3 grid, cudaStream_t st) {
   static std::atomic<uint64_t> ready{0};
-  const int rc = allow_smem(paged_narrow_kernel<T, CT, D>, PnRing<CT, D>::BYTES, ready);
+  constexpr int bytes = PnRing<CT, D, NB>::BYTES;
+  const int rc = allow_smem(paged_narrow_kernel<T, CT, D, NB>, bytes, ready);
   if (rc != BE_OK) return rc;
-  BE_CUDA_CHECK(launch_pdl(paged_narrow_kernel<T, CT, D>, grid, dim3(128), PnRing<CT, D>::BYTES, st, p));
+  BE_CUDA_CHECK(launch_pdl(paged_narrow_kernel<T, CT, D, NB>, grid, dim3(128), bytes, st, p));
   return BE_OK;
 }
 
@@ -532,7 +573,7 @@ static int paged_wide_launch(const PagedParams& p, int max_wide, cudaStream_t st
 
 template <typename T>
 static int paged_launch(const PagedParams& p, bool q8, int D, int max_wide, int max_narrow,
-                        int max_merge, cudaStream_t st) {
+                        int rows, int max_merge, cudaStream_t st) {
   if (max_wide > 0) {
     int rc;
     if (q8)
@@ -545,13 +586,16 @@ static int paged_launch(const PagedParams& p, bool q8, int D, int max_wide, int 
   }
   if (max_narrow > 0) {
     const dim3 grid((unsigned)max_narrow * p.hkv);   // heads of an item next to each other
-    int rc;
-    if (q8)
-      rc = D == 128 ? paged_narrow_launch<T, E4M3, 128>(p, grid, st)
-                    : paged_narrow_launch<T, E4M3, 64>(p, grid, st);
-    else
-      rc = D == 128 ? paged_narrow_launch<T, T, 128>(p, grid, st)
-                    : paged_narrow_launch<T, T, 64>(p, grid, st);
+    auto go = [&](auto elt, auto dim) {
+      using CT = decltype(elt);
+      constexpr int DD = decltype(dim)::value;
+      return rows <= 8 ? paged_narrow_launch<T, CT, DD, 1>(p, grid, st)
+                       : paged_narrow_launch<T, CT, DD, 2>(p, grid, st);
+    };
+    using D128 = std::integral_constant<int, 128>;
+    using D64 = std::integral_constant<int, 64>;
+    const int rc = q8 ? (D == 128 ? go(E4M3{}, D128{}) : go(E4M3{}, D64{}))
+                      : (D == 128 ? go(T{}, D128{}) : go(T{}, D64{}));
     if (rc != BE_OK) return rc;
   }
   if (max_merge > 0) {
@@ -570,13 +614,13 @@ static int paged_launch(const PagedParams& p, bool q8, int D, int max_wide, int 
 using namespace be;
 
 extern "C" int be_paged_attn_run(const int32_t* plan_dev, int max_wide, int max_narrow,
-                                 int max_merge, int max_parts, int page_size, const void* q,
+                                 int narrow_rows, int max_merge, int max_parts, int page_size, const void* q,
                                  int64_t q_row_stride, const void* paged_kv_cache,
                                  const float* kv_scale, int num_pages, int num_qo_heads,
                                  int num_kv_heads, int head_dim, int dtype, int cache_dtype,
                                  float sm_scale, void* out, int64_t out_row_stride, float* lse,
                                  float* mid_o, float* mid_lse, void* stream) {
-  if (max_wide < 0 || max_narrow < 0 || max_merge < 0 || max_parts < 0 || page_size < 1 ||
+  if (max_wide < 0 || max_narrow < 0 || narrow_rows < 0 || narrow_rows > 16 || max_merge < 0 || max_parts < 0 || page_size < 1 ||
       num_pages < 1 || num_kv_heads < 1 || num_kv_heads > 1024 || num_qo_heads < 1 ||
       std::max(max_wide, max_narrow) > (1 << 20) ||
       num_qo_heads % num_kv_heads) {
@@ -626,6 +670,8 @@ extern "C" int be_paged_attn_run(const int32_t* plan_dev, int max_wide, int max_
   p.mid_lse = mid_lse;
   const bool q8 = cache_dtype == BE_E4M3;
   return dtype == BE_BF16
-             ? paged_launch<__nv_bfloat16>(p, q8, head_dim, max_wide, max_narrow, max_merge, (cudaStream_t)stream)
-             : paged_launch<__half>(p, q8, head_dim, max_wide, max_narrow, max_merge, (cudaStream_t)stream);
+             ? paged_launch<__nv_bfloat16>(p, q8, head_dim, max_wide, max_narrow,
+                                           narrow_rows, max_merge, (cudaStream_t)stream)
+             : paged_launch<__half>(p, q8, head_dim, max_wide, max_narrow,
+                                           narrow_rows, max_merge, (cudaStream_t)stream);
 }

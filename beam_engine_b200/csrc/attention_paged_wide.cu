@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
   float* row_scale = reinterpret_cast<float*>(smem + SM::RS);
 
   pdl_wait();
-  const be_attn_plan_info* hdr = reinterpret_cast<const be_attn_plan_info*>(p.plan);
+  const be_paged_plan_info* hdr = reinterpret_cast<const be_paged_plan_info*>(p.plan);
   const int item = blockIdx.x / p.hkv, kvh = blockIdx.x - item * p.hkv;
   if (item >= hdr->n_work_wide) return;
   const be_paged_item w = reinterpret_cast<const be_paged_item*>(p.plan + hdr->off_work)[item];

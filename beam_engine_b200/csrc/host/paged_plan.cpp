@@ -142,7 +142,7 @@ extern "C" int be_paged_plan(int num_levels, const int32_t* const* qo_indptr,
                              const int32_t* const* last_page_len, const int32_t* num_groups,
                              int num_queries, int page_size, int num_qo_heads, int num_kv_heads,
                              int causal_last, int window_left, int num_sinks, int num_sms,
-                             int32_t* plan, int64_t plan_capacity, be_attn_plan_info* info) {
+                             int32_t* plan, int64_t plan_capacity, be_paged_plan_info* info) {
   if (num_levels < 1 || num_queries < 0 || page_size < 1 || num_kv_heads < 1 || num_qo_heads < 1 ||
       num_qo_heads % num_kv_heads || num_sinks < 0 || !info) {
     set_error("be_paged_plan: invalid arguments");
@@ -336,7 +336,7 @@ extern "C" int be_paged_plan(int num_levels, const int32_t* const* qo_indptr,
     if (wa != wb) return wa;
     return items[a].v1 - items[a].v0 > items[b].v1 - items[b].v0;
   });
-  be_attn_plan_info in{};
+  be_paged_plan_info in{};
   in.n_work = (int32_t)items.size();
   for (const Item& it : items) in.n_work_wide += tiles[it.tile].wide ? 1 : 0;
   in.n_queries = num_queries;
@@ -344,6 +344,8 @@ extern "C" int be_paged_plan(int num_levels, const int32_t* const* qo_indptr,
   in.n_merge = (int32_t)mq.size();
   in.page_size = page_size;
   in.group_size = g;
+  for (const Tile& t : tiles)
+    if (!t.wide) in.narrow_rows = std::max(in.narrow_rows, t.ql * g);
   for (const Item& it : items) {
     const int len = it.v1 - it.v0;
     in.max_item_tokens = std::max(in.max_item_tokens, len);

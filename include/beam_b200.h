@@ -395,9 +395,16 @@ int be_attn_tiles_run(const int32_t* plan_dev, int max_pieces, int max_tiles, in
  *   t <= p (last level, causal_last != 0) and, when window_left >= 0,
  *   t >= p - window_left or t < num_sinks.
  * A query that sees nothing gets out = 0, lse = -inf.
- * Plan buffer: header (be_attn_plan_info, BE_PLAN_HEADER_INTS ints), items
+ * Plan buffer: header (be_paged_plan_info, BE_PLAN_HEADER_INTS ints), items
  * (wide ones first), page list, merge lists.
  * ---------------------------------------------------------------------- */
+typedef struct {            /* be_attn_plan_info's fields, then:                    */
+  int32_t n_work, n_work_wide, n_queries, n_parts, n_merge;
+  int32_t off_work, off_qlist, off_kvlist, off_merge_q, off_merge_ptr, off_merge_parts;
+  int32_t total_ints, page_size, group_size, any_slots, max_item_tokens, total_tokens;
+  int32_t max_wide_tokens;
+  int32_t narrow_rows;      /* query-head rows of the highest narrow item (0..16)   */
+} be_paged_plan_info;
 typedef struct {
   int32_t q_begin, q_len;   /* consecutive queries                                  */
   int32_t kv_off;           /* the group's pages in the page list                   */
@@ -418,19 +425,19 @@ int be_paged_plan(int num_levels, const int32_t* const* qo_indptr, const int32_t
                   const int32_t* const* kv_indices, const int32_t* const* last_page_len,
                   const int32_t* num_groups, int num_queries, int page_size, int num_qo_heads,
                   int num_kv_heads, int causal_last, int window_left, int num_sinks, int num_sms,
-                  int32_t* plan, int64_t plan_capacity, be_attn_plan_info* info);
+                  int32_t* plan, int64_t plan_capacity, be_paged_plan_info* info);
 
 /* Runs a be_paged_plan plan in device memory (header included) for one layer.
  * The launch shape depends on the max_* capacities only and the kernels read the plan's counts
  * from its header, so a recorded launch serves every plan with at most
- * max_wide wide and max_narrow narrow items, max_merge merged queries and
- * max_parts partial rows.  dtype (q, out): BE_BF16 or BE_F16; cache_dtype BE_E4M3
+ * max_wide wide and max_narrow narrow items (of up to narrow_rows rows, 0..16), max_merge
+ * merged queries and max_parts partial rows.  dtype (q, out): BE_BF16 or BE_F16; cache_dtype BE_E4M3
  * (kv_scale required) or dtype; head_dim 64 or 128.  q [n][num_qo_heads][head_dim]
  * with q_row_stride elements between queries.  mid_o / mid_lse: float32 scratch of
  * max_parts * num_qo_heads * head_dim and max_parts * num_qo_heads (calls that share
  * them must not overlap on the GPU).                                          */
-int be_paged_attn_run(const int32_t* plan_dev, int max_wide, int max_narrow, int max_merge,
-                      int max_parts, int page_size, const void* q, int64_t q_row_stride,
+int be_paged_attn_run(const int32_t* plan_dev, int max_wide, int max_narrow, int narrow_rows,
+                      int max_merge, int max_parts, int page_size, const void* q, int64_t q_row_stride,
                       const void* paged_kv_cache, const float* kv_scale, int num_pages,
                       int num_qo_heads, int num_kv_heads, int head_dim, int dtype,
                       int cache_dtype, float sm_scale, void* out, int64_t out_row_stride,

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from beam_engine_b200 import _lib
-from beam_engine_b200._lib import AttnPlanInfo, lib
+from beam_engine_b200._lib import PagedPlanInfo, lib
 
 ITEM = np.dtype([(n, np.int32) for n in (
     "q_begin", "q_len", "kv_off", "v_begin", "v_end", "n0", "shift", "pos0", "pos_step",
@@ -20,7 +20,7 @@ def plan(levels, nq, page, hq, hkv, causal=True, window=-1, sinks=0, sms=148, ca
     arrs = [[np.ascontiguousarray(np.asarray(lv[k], np.int32)) for lv in levels] for k in range(4)]
     ng = np.asarray([len(a) - 1 for a in arrs[0]], np.int32)
     ptrs = [(_lib.P32 * max(L, 1))(*[_lib.ptr32(a) for a in grp]) for grp in arrs]
-    info = AttnPlanInfo()
+    info = PagedPlanInfo()
     buf = np.zeros(cap or (1 << 22), np.int32)
     rc = lib().be_paged_plan(L, *ptrs, _lib.ptr32(ng), nq, page, hq, hkv, int(causal), window, sinks,
                              sms, _lib.addr(buf), buf.size, C.byref(info))
@@ -197,12 +197,12 @@ def test_append_arguments(kw, rc):
 
 @pytest.mark.parametrize("kw", [
     dict(dt=_lib.BE_F32), dict(cdt=_lib.BE_F16), dict(d=80), dict(scale=None), dict(hq=258),
-    dict(q=None), dict(q=8), dict(parts=1), dict(qs=4), dict(narrow=-1)])
+    dict(q=None), dict(q=8), dict(parts=1), dict(qs=4), dict(narrow=-1), dict(rows=17)])
 def test_run_refuses(kw):
     a = dict(q=16, qs=512, cache=16, scale=16, hq=4, d=64, dt=_lib.BE_BF16, cdt=_lib.BE_E4M3,
-             parts=0, narrow=1)
+             parts=0, narrow=1, rows=4)
     a.update(kw)
-    rc = lib().be_paged_attn_run(16, 0, a["narrow"], 0, a["parts"], 16, a["q"], a["qs"], a["cache"],
+    rc = lib().be_paged_attn_run(16, 0, a["narrow"], a["rows"], 0, a["parts"], 16, a["q"], a["qs"], a["cache"],
                                  a["scale"], 8, a["hq"], 2, a["d"], a["dt"], a["cdt"], 1.0, 16, 512,
                                  None, None, None, None)
     assert rc == _lib.BE_EINVAL
