@@ -35,8 +35,8 @@ import torch
 
 from . import _lib
 from ._lib import AttnPlanInfo, PagedPlanInfo, TilePlanInfo, check, lib
-from .page_table import (check_pool8, dtype_code, is_8bit, require_cuda, require_same_device,
-                         stream_ptr)
+from .page_table import (_DT, check_pool8, dtype_code, is_8bit, on_device, raw_stream,
+                         require_cuda, require_same_device, stream_ptr)
 
 
 def _i32(x):
@@ -227,19 +227,23 @@ class _Plan:
     def run_paged(self, q, kv, kv_scale, num_qo_heads, num_kv_heads, head_dim, sm_scale, out,
                   lse=None):
         """A be_paged_plan plan (placed like a work-item plan)."""
-        if q.stride(-1) != 1 or q.stride(-2) != head_dim or q.stride(0) % 8 or q.data_ptr() % 16:
+        qs = q.stride()
+        if qs[2] != 1 or qs[1] != head_dim or qs[0] % 8 or q.data_ptr() % 16:
             q = q.contiguous()
+            qs = q.stride()
         i = self.info
-        with torch.cuda.device(q.device):
+        index = q.device.index
+        code = _DT.get(q.dtype, -1)
+        with on_device(index):
             rc = lib().be_paged_attn_run(
                 self.plan_dev, i.n_work_wide, i.n_work - i.n_work_wide, i.narrow_rows, i.n_merge,
-                i.n_parts, i.page_size, q.data_ptr(), q.stride(0), kv.data_ptr(),
-                kv_scale.data_ptr() if kv_scale is not None else None, kv.shape[0], num_qo_heads,
-                num_kv_heads, head_dim, dtype_code(q.dtype),
-                _lib.BE_E4M3 if kv_scale is not None else dtype_code(kv.dtype), sm_scale,
-                out.data_ptr(), out.stride(0), lse.data_ptr() if lse is not None else None,
-                self.mid_o, self.mid_lse, stream_ptr(q.device))
-        check(rc, "be_paged_attn_run")
+                i.n_parts, i.page_size, q.data_ptr(), qs[0], kv.data_ptr(),
+                None if kv_scale is None else kv_scale.data_ptr(), kv.shape[0], num_qo_heads,
+                num_kv_heads, head_dim, code, code if kv_scale is None else _lib.BE_E4M3, sm_scale,
+                out.data_ptr(), out.stride(0), None if lse is None else lse.data_ptr(),
+                self.mid_o, self.mid_lse, raw_stream(index))
+        if rc:
+            check(rc, "be_paged_attn_run")
 
 
 _plan_cap = 4096     # int32 capacity of the next host plan buffer (grows on demand)
@@ -361,28 +365,27 @@ class MultiLevelCascadeAttentionWrapper:
         self.paged = True
 
     def _run_paged(self, q, kv, kv_scale, return_lse, out):
-        n, hq, d = self.num_queries, self.hq, self.d
-        page_size = self._plan.info.page_size
-        if q.shape != (n, hq, d):
-            raise ValueError(f"q must be {(n, hq, d)}, got {tuple(q.shape)}")
-        if kv.dim() != 5 or kv.shape[1:] != (2, page_size, self.hkv, d) or not kv.is_contiguous():
-            raise ValueError(f"paged_kv_cache must be contiguous [pages, 2, {page_size}, "
-                             f"{self.hkv}, {d}], got {tuple(kv.shape)}")
+        n, hq, d = shape = (self.num_queries, self.hq, self.d)
+        dtype, dev, ks = q.dtype, q.device, kv.shape
+        if q.shape != shape:
+            raise ValueError(f"q must be {shape}, got {tuple(q.shape)}")
+        if ks[1:] != (2, self._plan.info.page_size, self.hkv, d) or not kv.is_contiguous():
+            raise ValueError(f"paged_kv_cache must be contiguous [pages, 2, "
+                             f"{self._plan.info.page_size}, {self.hkv}, {d}], got {tuple(ks)}")
         if is_8bit(kv.dtype):
             check_pool8(kv, kv_scale)
             require_same_device(kv, q, kv_scale, self._plan.ws)
-        elif kv_scale is not None or kv.dtype != q.dtype:
-            raise ValueError(f"a cache of {kv.dtype} takes queries of its type (got {q.dtype}) and "
+        elif kv_scale is not None or kv.dtype is not dtype:
+            raise ValueError(f"a cache of {kv.dtype} takes queries of its type (got {dtype}) and "
                              "no kv_scale")
         else:
             require_same_device(kv, q, self._plan.ws)
         if out is None:
-            out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
-        elif (out.shape != (n, hq, d) or out.dtype != q.dtype or out.device != q.device
+            out = torch.empty(shape, dtype=dtype, device=dev)
+        elif (out.shape != shape or out.dtype is not dtype or out.device != dev
               or out.stride(-1) != 1 or out.stride(-2) != d):
-            raise ValueError(f"out must be {q.dtype} {(n, hq, d)} on {q.device} with contiguous "
-                             "heads")
-        lse = torch.empty((n, hq), dtype=torch.float32, device=q.device) if return_lse else None
+            raise ValueError(f"out must be {dtype} {shape} on {dev} with contiguous heads")
+        lse = torch.empty((n, hq), dtype=torch.float32, device=dev) if return_lse else None
         if n:
             self._plan.run_paged(q, kv, kv_scale, hq, self.hkv, d, self.sm_scale, out, lse)
         return (out, lse) if return_lse else out

@@ -48,6 +48,7 @@ struct PagedParams {
   float* lse;
   float* mid_o;
   float* mid_lse;
+  int merge_next;        // the merge is launched next: it may be prepared while these tiles run
 };
 
 struct E4M3 {};          // cache element tag
@@ -142,6 +143,7 @@ __global__ void __launch_bounds__(128, PnRing<CT, D, NB>::CTAS) paged_narrow_ker
   __shared__ float sM[4][8 * NB], sL[4][8 * NB];
 
   pdl_wait();
+  if (p.merge_next) pdl_trigger();   // the merge waits for this grid; another kernel might not
   const be_paged_plan_info* hdr = reinterpret_cast<const be_paged_plan_info*>(p.plan);
   const int n_wide = hdr->n_work_wide;
   const int item = blockIdx.x / p.hkv, kvh = blockIdx.x - item * p.hkv;
@@ -545,6 +547,74 @@ __global__ void __launch_bounds__(128, PnRing<CT, D, NB>::CTAS) paged_narrow_ker
   }
 }
 
+// merge_kernel's work with a CTA per (query, head): four warps take every fourth partial row.
+// A long sequence split over the GPU leaves dozens of parts for a few rows, and one warp
+// walking them is latency alone (cache8-long: 66 us a pass with it, 59 with this).
+template <typename T, int D>
+__global__ void __launch_bounds__(128) paged_merge_kernel(const PagedParams p) {
+  __shared__ __align__(16) float sO[4][D];
+  __shared__ float sM[4], sL[4];
+  pdl_wait();
+  const be_paged_plan_info* hdr = reinterpret_cast<const be_paged_plan_info*>(p.plan);
+  const int b = blockIdx.x / p.hq, head = blockIdx.x - b * p.hq;
+  if (b >= hdr->n_merge) return;
+  const int qi = p.plan[hdr->off_merge_q + b];
+  const int p0 = p.plan[hdr->off_merge_ptr + b], p1 = p.plan[hdr->off_merge_ptr + b + 1];
+  const int32_t* parts = p.plan + hdr->off_merge_parts;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int DL = D / 32;                   // floats per lane
+  float acc[DL] = {}, m = -INFINITY, l = 0.f;
+  for (int k0 = p0 + warp; k0 < p1; k0 += 16) {   // 4 parts of this warp at once
+    float e[4], x[4][DL];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int k = k0 + 4 * u;
+      const int64_t row = k < p1 ? (int64_t)parts[k] * p.hq + head : -1;
+      e[u] = row >= 0 ? p.mid_lse[row] : -INFINITY;
+#pragma unroll
+      for (int d = 0; d < DL; ++d) x[u][d] = row >= 0 ? p.mid_o[row * D + lane * DL + d] : 0.f;
+    }
+    float to = m;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) to = fmaxf(to, e[u]);
+    if (to == -INFINITY) continue;
+    const float f = m == -INFINITY ? 0.f : expf(m - to);
+    m = to;
+    l *= f;
+#pragma unroll
+    for (int d = 0; d < DL; ++d) acc[d] *= f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (e[u] == -INFINITY) continue;         // empty: its row counts for nothing, whatever it holds
+      const float g = expf(e[u] - to);
+      l += g;
+#pragma unroll
+      for (int d = 0; d < DL; ++d) acc[d] = fmaf(g, x[u][d], acc[d]);
+    }
+  }
+#pragma unroll
+  for (int d = 0; d < DL; ++d) sO[warp][lane * DL + d] = acc[d];
+  if (lane == 0) {
+    sM[warp] = m;
+    sL[warp] = l;
+  }
+  __syncthreads();
+  const float mx = fmaxf(fmaxf(sM[0], sM[1]), fmaxf(sM[2], sM[3]));
+  float f[4], den = 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    f[k] = sM[k] == -INFINITY ? 0.f : expf(sM[k] - mx);
+    den += f[k] * sL[k];
+  }
+  for (int d = threadIdx.x; d < D; d += 128) {
+    const float o = f[0] * sO[0][d] + f[1] * sO[1][d] + f[2] * sO[2][d] + f[3] * sO[3][d];
+    reinterpret_cast<T*>(p.out)[qi * p.out_row_stride + (int64_t)head * D + d] =
+        from_f<T>(den != 0.f ? o / den : 0.f);
+  }
+  if (p.lse && threadIdx.x == 0)
+    p.lse[(int64_t)qi * p.hq + head] = den == 0.f ? -INFINITY : mx + logf(den);
+}
+
 // Raises a kernel's shared-memory limit, once per device.
 template <typename K>
 static int allow_smem(K kernel, int bytes, std::atomic<uint64_t>& ready) {
@@ -598,7 +668,13 @@ static int paged_launch(const PagedParams& p, bool q8, int D, int max_wide, int 
                       : (D == 128 ? go(T{}, D128{}) : go(T{}, D64{}));
     if (rc != BE_OK) return rc;
   }
-  if (max_merge > 0) {
+  // a CTA per row while that is a few waves of CTAs, a warp per row for prompts' many rows
+  if (max_merge > 0 && (int64_t)max_merge * p.hq <= 148 * 32) {
+    if (D == 128)
+      BE_CUDA_CHECK(launch_pdl(paged_merge_kernel<T, 128>, dim3(max_merge * p.hq), dim3(128), 0, st, p));
+    else
+      BE_CUDA_CHECK(launch_pdl(paged_merge_kernel<T, 64>, dim3(max_merge * p.hq), dim3(128), 0, st, p));
+  } else if (max_merge > 0) {
     const int items = max_merge * p.hq;
     BE_CUDA_CHECK(launch_pdl(merge_kernel<T>, dim3((items + 3) / 4), dim3(128), 0, st,
                              (const int32_t*)nullptr, (const int32_t*)nullptr,
@@ -668,6 +744,7 @@ extern "C" int be_paged_attn_run(const int32_t* plan_dev, int max_wide, int max_
   p.lse = lse;
   p.mid_o = mid_o;
   p.mid_lse = mid_lse;
+  p.merge_next = max_merge > 0;
   const bool q8 = cache_dtype == BE_E4M3;
   return dtype == BE_BF16
              ? paged_launch<__nv_bfloat16>(p, q8, head_dim, max_wide, max_narrow,

@@ -20,8 +20,8 @@ from __future__ import annotations
 import torch
 
 from ._lib import check, lib
-from .page_table import (_DT, append_rows, check_pool8, dtype_code, is_8bit, require_cuda,
-                         require_same_device, stream_ptr)
+from .page_table import (_DT, _int32, append_rows, check_pool8, dtype_code, is_8bit, on_device,
+                         raw_stream, require_cuda, require_same_device, stream_ptr)
 
 
 def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor,
@@ -35,9 +35,6 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor,
         raise ValueError("only the NHD layout is supported")
     if paged_kv_cache.dim() != 5 or paged_kv_cache.shape[1] != 2:
         raise ValueError("paged_kv_cache must be [pages, 2, page_size, kv_heads, head_dim]")
-    require_cuda(append_key, append_value, paged_kv_cache, batch_indices, positions, kv_indices,
-                 kv_indptr)
-    P, _, ps, H, D = paged_kv_cache.shape
     if not paged_kv_cache.is_contiguous():
         raise ValueError("paged_kv_cache must be contiguous")
     if is_8bit(paged_kv_cache.dtype):
@@ -52,6 +49,9 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor,
                            append_value.to(paged_kv_cache.dtype), batch_indices, positions,
                            paged_kv_cache, None, kv_indices, kv_indptr, rope_inv_freq,
                            rope_positions)
+    require_cuda(append_key, append_value, paged_kv_cache, batch_indices, positions, kv_indices,
+                 kv_indptr)
+    P, _, ps, H, D = paged_kv_cache.shape
     k = append_key.to(paged_kv_cache.dtype)
     v = append_value.to(paged_kv_cache.dtype)
     if k.stride(-1) != 1 or k.stride(-2) != D:
@@ -80,14 +80,14 @@ def read_paged_kv_cache(paged_kv_cache: torch.Tensor, pages: torch.Tensor, kv_sc
     if pages.dim() != 1:
         raise ValueError("pages must be [n]")
     require_same_device(paged_kv_cache, kv_scale, pages)
-    if pages.dtype != torch.int32 or not pages.is_contiguous():
-        pages = pages.to(torch.int32).contiguous()
+    pages = _int32(pages)
     P, _, ps, H, D = paged_kv_cache.shape
-    dev = paged_kv_cache.device
-    out = torch.empty((pages.shape[0], 2, ps, H, D), dtype=dtype, device=dev)
-    with torch.cuda.device(dev):
+    n, dev = pages.shape[0], paged_kv_cache.device
+    out = torch.empty((n, 2, ps, H, D), dtype=dtype, device=dev)
+    with on_device(dev.index):
         rc = lib().be_read_paged_kv8(paged_kv_cache.data_ptr(), kv_scale.data_ptr(),
-                                     pages.data_ptr(), pages.shape[0], P, ps, H, D, out.data_ptr(),
-                                     dtype_code(dtype), stream_ptr(dev))
-    check(rc, "read_paged_kv_cache")
+                                     pages.data_ptr(), n, P, ps, H, D, out.data_ptr(), _DT[dtype],
+                                     raw_stream(dev.index))
+    if rc:
+        check(rc, "read_paged_kv_cache")
     return out

@@ -45,6 +45,27 @@ def stream_ptr(device):
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def raw_stream(index):
+    """The current stream of device ``index`` as an integer (no stream object is made)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+class on_device:
+    """``torch.cuda.device`` that does nothing when the device is the current one already."""
+    __slots__ = ("guard",)
+
+    def __init__(self, index):
+        self.guard = None if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
 def require_cuda(*tensors):
     for t in tensors:
         if not t.is_cuda:
@@ -52,21 +73,28 @@ def require_cuda(*tensors):
 
 
 def require_same_device(first, *tensors):
-    require_cuda(first, *tensors)
+    dev = first.device
+    if dev.type != "cuda":
+        require_cuda(first)
     for t in tensors:
-        if t.device != first.device:
-            raise ValueError(f"tensors on {first.device} and {t.device}")
+        if t.device != dev:
+            require_cuda(t)
+            raise ValueError(f"tensors on {dev} and {t.device}")
 
 
 def check_pool8(pool, scale):
     """A paged cache [pages, 2, page_size, kv_heads, head_dim] of codes with its scales."""
     if scale is None:
         raise ValueError("a float8_e4m3fn cache needs kv_scale [pages, 2, kv_heads]")
-    if (scale.dtype != torch.float32 or not scale.is_contiguous()
+    if (scale.dtype is not torch.float32 or not scale.is_contiguous()
             or scale.shape != (pool.shape[0], 2, pool.shape[3])):
         raise ValueError("kv_scale must be contiguous float32 [pages, 2, kv_heads] "
                          f"({(pool.shape[0], 2, pool.shape[3])}), got {scale.dtype} "
                          f"{tuple(scale.shape)}")
+
+
+def _int32(t):
+    return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
 
 
 def append_rows(key, value, batch_indices, positions, pool, scale, kv_indices, kv_indptr,
@@ -77,36 +105,49 @@ def append_rows(key, value, batch_indices, positions, pool, scale, kv_indices, k
     if key.shape != (n, H, D) or value.shape != (n, H, D):
         raise ValueError(f"rows must be [n, {H}, {D}], got {tuple(key.shape)} and "
                          f"{tuple(value.shape)}")
-    if key.dtype != value.dtype:
+    if key.dtype is not value.dtype:
         raise ValueError(f"keys are {key.dtype}, values {value.dtype}")
-    if key.stride(-1) != 1 or key.stride(-2) != D:
+    ks, vs = key.stride(), value.stride()
+    if ks[2] != 1 or ks[1] != D:
         key = key.contiguous()
-    if value.stride(-1) != 1 or value.stride(-2) != D:
+    if vs[2] != 1 or vs[1] != D:
         value = value.contiguous()
-    for name, t, m in (("batch_indices", batch_indices, n), ("positions", positions, n),
-                       ("rope_positions", rope_positions, n)):
-        if t is not None and t.shape != (m,):
-            raise ValueError(f"{name} must have {m} entries, got {tuple(t.shape)}")
-    ints = [t if t is None or (t.dtype == torch.int32 and t.is_contiguous())
-            else t.to(torch.int32).contiguous()
-            for t in (batch_indices, positions, kv_indices, kv_indptr, rope_positions)]
-    if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.shape != (D // 2,)
-                                 or not inv_freq.is_contiguous()):
-        raise ValueError(f"rope_inv_freq must be contiguous float32 [{D // 2}]")
+    if batch_indices.shape != (n,) or positions.shape != (n,) or (
+            rope_positions is not None and rope_positions.shape != (n,)):
+        raise ValueError(f"batch_indices, positions and rope_positions must have {n} entries")
+    batch_indices, positions = _int32(batch_indices), _int32(positions)
+    kv_indices, kv_indptr = _int32(kv_indices), _int32(kv_indptr)
     dev = pool.device
-    require_same_device(pool, key, value, *[t for t in (*ints, inv_freq, scale) if t is not None])
-    ws = torch.empty(4 * n + 512, dtype=torch.int32, device=dev) if n > 512 else None
-    with torch.cuda.device(dev):
+    same = [key, value, batch_indices, positions, kv_indices, kv_indptr]
+    freq = rope = codes = ws = None
+    ws_ints = 0
+    if inv_freq is not None:
+        if (inv_freq.dtype is not torch.float32 or inv_freq.shape != (D // 2,)
+                or not inv_freq.is_contiguous()):
+            raise ValueError(f"rope_inv_freq must be contiguous float32 [{D // 2}]")
+        same.append(inv_freq)
+        freq = inv_freq.data_ptr()
+        if rope_positions is not None:
+            rope_positions = _int32(rope_positions)
+            same.append(rope_positions)
+            rope = rope_positions.data_ptr()
+    cache_code = _DT.get(pool.dtype, -1)
+    if scale is not None:
+        same.append(scale)
+        codes, cache_code = scale.data_ptr(), _lib.BE_E4M3
+    require_same_device(pool, *same)
+    if n > 512:
+        ws_ints = 4 * n + 512
+        ws = torch.empty(ws_ints, dtype=torch.int32, device=dev)
+    with on_device(dev.index):
         rc = lib().be_rope_append_paged_kv(
-            key.data_ptr(), value.data_ptr(), key.stride(0), value.stride(0), ints[0].data_ptr(),
-            ints[1].data_ptr(), ints[4].data_ptr() if ints[4] is not None else None,
-            ints[2].data_ptr(), ints[3].data_ptr(), n,
-            inv_freq.data_ptr() if inv_freq is not None else None, pool.data_ptr(),
-            scale.data_ptr() if scale is not None else None, P, ps, H, D, dtype_code(key.dtype),
-            _lib.BE_E4M3 if scale is not None else dtype_code(pool.dtype),
-            ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
-            stream_ptr(dev))
-    check(rc, "append_paged_kv_cache")
+            key.data_ptr(), value.data_ptr(), key.stride(0), value.stride(0),
+            batch_indices.data_ptr(), positions.data_ptr(), rope, kv_indices.data_ptr(),
+            kv_indptr.data_ptr(), n, freq, pool.data_ptr(), codes, P, ps, H, D,
+            dtype_code(key.dtype), cache_code, ws.data_ptr() if ws_ints else None, ws_ints,
+            raw_stream(dev.index))
+    if rc:
+        check(rc, "append_paged_kv_cache")
 
 
 class PageTable:
@@ -196,7 +237,7 @@ class PageTable:
             return torch.as_tensor(np.asarray(x, np.int32)).to(dev, non_blocking=True)
         s, d, n = as_dev(src), as_dev(dst), as_dev(lens)
         if self.kv_scale is not None:
-            with torch.cuda.device(dev):
+            with on_device(dev.index):
                 rc = lib().be_fork_tail_copy8(
                     self.kv_cache.data_ptr(), self._layer_stride(), self.kv_scale.data_ptr(),
                     self.kv_scale.stride(0), self.layer_num, self.max_num_pages, self.page_size,
