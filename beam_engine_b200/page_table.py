@@ -137,7 +137,7 @@ def append_rows(key, value, batch_indices, positions, pool, scale, kv_indices, k
         codes, cache_code = scale.data_ptr(), _lib.BE_E4M3
     require_same_device(pool, *same)
     if n > 512:
-        ws_ints = 4 * n + 512
+        ws_ints = 5 * n + 1024
         ws = torch.empty(ws_ints, dtype=torch.int32, device=dev)
     with on_device(dev.index):
         rc = lib().be_rope_append_paged_kv(

@@ -107,7 +107,7 @@ int be_fork_tail_copy_list(void* paged_kv_cache, int64_t pool_layer_stride, int 
  * `positions`).  cache_dtype BE_E4M3 (kv_scale required) or `dtype`
  * (kv_scale NULL).  Rows may come in any order; of two rows for one slot the later
  * one in the call is kept.  Calls with more than 512 rows need a device workspace
- * of 4 * nnz + 512 ints (free to reuse once the call's work is done).
+ * of 5 * nnz + 1024 ints, 8-byte aligned (free to reuse once the call's work is done).
  * head_dim 32, 64, 128 or 256, page_size <= 256, num_kv_heads <= 64.          */
 int be_rope_append_paged_kv(const void* append_key, const void* append_value,
                             int64_t key_row_stride, int64_t value_row_stride,
