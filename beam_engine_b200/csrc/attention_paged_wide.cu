@@ -4,19 +4,22 @@
 // One CTA = one item of be_paged_plan x one KV head: two row tiles of 128 (row r of the
 // item is query r / g, head r % g, so a KV head's tokens are loaded once for its g
 // query heads) against steps of 128 tokens, in one pass with a running maximum:
-//   * loader warps (7): tokens' rows from global memory into the canonical 128-byte
+//   * loader warps (6): tokens' rows from global memory into the canonical 128-byte
 //     swizzle, 16-bit rows by cp.async, 8-bit codes through registers; tokens are addressed one
 //     by one, so any page size and the joint of sinks and window cost nothing;
-//   * one warp issues S = Q K^T (128 x 128 x D) into TMEM and O += P V (128 x D x 128) with
-//     P read from TMEM, alternating between the row tiles so that one tile's softmax
-//     runs under the other's products; P V starts on the first half of P;
-//   * softmax warps (4 per row tile, a thread per row): the maximum, then P written over S, 64 tokens
-//     at a time from TMEM in rolled loops (16 warps in three roles share the instruction cache: with a
-//     row's 128 scores in registers and every loop unrolled, fetching instructions took
-//     half of each step); O is rescaled only when a row's maximum grows by more than 2^8.
-// TMEM: S/P of tile 0 | S/P of tile 1 | O of tile 0 | O of tile 1 = 256 + 2 D columns (512 allocated).
-// A tile's S of step i + 1 overwrites its P of step i: both products come from one thread, and
-// the tensor core runs them in the order of issue.
+//   * a warp per row tile issues S = Q K^T (128 x 64 x D) into TMEM and O += P V (128 x D x 64) with
+//     P read from TMEM, in halves of a step (one warp for both tiles spent 2 560 clocks a half, most
+//     of them between its own waits): a row tile has two buffers of S, so the scores of the next
+//     half are there when its softmax comes to them.  (128 x 128 products with one buffer
+//     left the softmax waiting for P V and S of its own tile, 1 560 of 4 270 clocks a step;
+//     128 x 64 x 16 takes 49 clocks instead of 32, bound by shared memory, 128 x 128 x 16 takes 65.)
+//   * softmax warps (4 per row tile, a thread per row): 64 scores from TMEM to registers, maximum, P
+//     written over S; O is rescaled only when a row's maximum grows by more than 2^8.  Their
+//     loops stay short because 16 warps in three roles share the instruction cache: with 128 scores
+//     per pass and every variant unrolled, fetching instructions took half of each step.
+// TMEM: S/P of tile 0 (two buffers of 64) | of tile 1 | O of tile 0 | O of tile 1 = 256 + 2 D columns
+// (512 allocated).  S of half j + 2 overwrites P of half j: both products come from one thread,
+// and the tensor core runs them in the order of issue.
 //
 // 8-bit caches: as in the narrow kernel the codes become halves by one exact conversion and
 // the scales stay out of the products.  x = s_K (q . c) and log2 s_V joins the exponent, so a group of
@@ -38,8 +41,8 @@
 namespace be {
 
 constexpr int PW_TOK = 128;                    // tokens per step
-constexpr int PW_LOADERS = 7;
-constexpr int PW_THREADS = 16 * 32;            // 8 softmax warps, 7 loader warps, 1 issuer
+constexpr int PW_LOADERS = 6;
+constexpr int PW_THREADS = 16 * 32;            // 8 softmax warps, 6 loader warps, 2 issuers
 constexpr int PW_HALF = PW_TOK * 128;          // 64 dims of 128 rows
 constexpr int PW_STAGES = 2;
 
@@ -145,11 +148,6 @@ __device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t* r) {
                "r"(r[1]), "r"(r[2]), "r"(r[3])
                : "memory");
 }
-// the 8 bits of tokens c0 .. c0 + 7 (c0 a multiple of 8)
-__device__ __forceinline__ uint32_t see_at(const uint32_t (&see)[4], int c0) {
-  const uint32_t w = c0 < 32 ? see[0] : c0 < 64 ? see[1] : c0 < 96 ? see[2] : see[3];
-  return (w >> (c0 & 31)) & 0xffu;
-}
 
 // element x of a 16-bit pair: set to zero if not finite
 template <typename T>
@@ -162,6 +160,7 @@ __device__ __forceinline__ uint32_t zero_not_finite(uint32_t w) {
 
 // Bounded wait of a whole warp: every lane sees the phase, and all agree on the outcome.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
   const bool ok = !*abort_flag && mbar_wait(bar, parity);
   return __all_sync(0xffffffffu, ok);
 }
@@ -185,16 +184,19 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
   uint64_t* v_full = bars + 2;                  // [2]
   uint64_t* k_empty = bars + 4;                 // [2], commit
   uint64_t* v_empty = bars + 6;                 // [2]
-  uint64_t* s_full = bars + 8;                  // [row tile], commit
-  uint64_t* o_done = bars + 10;                 // [row tile], commit
+  uint64_t* s_full = bars + 8;                  // [row tile][half], commit
   uint64_t* p_full = bars + 12;                 // [row tile][half], 4 softmax warps
-  uint64_t* drain = bars + 16;
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bars + 17);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 18);
-  volatile int* odd = reinterpret_cast<volatile int*>(bars + 19);   // [2] per V stage: step + 1
-  volatile int* gone = reinterpret_cast<volatile int*>(bars + 20);  // [4]: step + 1 that misses a page
+  // [row tile][half], commit.  Two P V of a tile can be in flight, so a single barrier's parity could not
+  // tell the one waited for from the one before the last.
+  uint64_t* o_done = bars + 16;
+  uint64_t* drain = bars + 20;                  // [row tile]
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bars + 22);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 23);
+  volatile int* odd = reinterpret_cast<volatile int*>(bars + 24);   // [2] per V stage: step + 1
+  volatile int* gone = reinterpret_cast<volatile int*>(bars + 25);  // [4]: step + 1 that misses a page
   uint32_t* odd_mask = reinterpret_cast<uint32_t*>(smem + SM::ODD);  // [256][2][D / 32]
-  // per token of the last 4 steps (the loaders are at most 2 past the softmax): s_K, log2 s_V, 1 / s_V
+  // per token of the last 4 steps (the loaders are at most 3 past the softmax, and write a step's
+  // entries once V of the third before is used up): s_K, log2 s_V, 1 / s_V
   float4* tab = reinterpret_cast<float4*>(smem + SM::TAB);
   float* row_scale = reinterpret_cast<float*>(smem + SM::RS);
 
@@ -208,12 +210,13 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
   const int g = p.g, rows = w.q_len * g;
   const bool two = rows > 128;
   const int steps = (w.v_end - w.v_begin + PW_TOK - 1) / PW_TOK;
+  const int halves = (w.v_end - w.v_begin + PW_TOK / 2 - 1) / (PW_TOK / 2);
   const bool causal = (w.flags & BE_ITEM_CAUSAL) != 0, window = w.window >= 0;
   const int pos_hi = w.pos0 + w.pos_step * (w.q_len - 1);
-  // whether every row sees every token of the step at v0 (page ids apart)
-  auto full_step = [&](int v0) {
+  // whether every row sees every one of the n tokens from v0 (page ids apart)
+  auto all_see = [&](int v0, int n) {
     const int t_lo = v0 + (v0 >= w.n0 ? w.shift : 0);
-    const int v1 = v0 + PW_TOK - 1, t_hi = v1 + (v1 >= w.n0 ? w.shift : 0);
+    const int v1 = v0 + n - 1, t_hi = v1 + (v1 >= w.n0 ? w.shift : 0);
     return v1 < w.v_end && (!causal || t_hi <= w.pos0) &&
            (!window || t_lo >= pos_hi - w.window || t_hi < w.sink_end);
   };
@@ -222,15 +225,17 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
     for (int s = 0; s < 2; ++s) {
       mbar_init(&k_full[s], PW_LOADERS);
       mbar_init(&v_full[s], PW_LOADERS);
-      mbar_init(&k_empty[s], 1);
-      mbar_init(&v_empty[s], 1);
-      mbar_init(&s_full[s], 1);
-      mbar_init(&o_done[s], 1);
-      mbar_init(&p_full[2 * s], 4);
-      mbar_init(&p_full[2 * s + 1], 4);
+      mbar_init(&k_empty[s], two ? 2 : 1);      // a commit per row tile
+      mbar_init(&v_empty[s], two ? 2 : 1);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&o_done[2 * s + h], 1);
+        mbar_init(&s_full[2 * s + h], 1);
+        mbar_init(&p_full[2 * s + h], 4);
+      }
       odd[s] = gone[s] = gone[2 + s] = 0;
     }
     mbar_init(drain, 1);
+    mbar_init(drain + 1, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -288,70 +293,66 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
   const uint32_t tmem = *tmem_slot;
 
   if (warp >= 8) {
-    if (warp == 15) {
-      // ---------------- issuer ----------------
+    if (warp >= 14) {
+      // ---------------- issuers: warp 14 for row tile 0, warp 15 for row tile 1 ----------------
       // The whole warp walks the steps and one elected lane issues: addresses and descriptors
       // then stay in uniform registers (from a divergent lane every product first moves them there)
       const uint32_t el = elect_one();
-      const uint32_t id_s = umma_idesc<MT>(128, PW_TOK, 0), id_o = umma_idesc<MT>(128, D, 1);
+      const uint32_t id_s = umma_idesc<MT>(128, PW_TOK / 2, 0), id_o = umma_idesc<MT>(128, D, 1);
       const uint64_t dq = umma_desc(smem_u32(smem + SM::Q), 16, 1024);
       const uint64_t dk = umma_desc(smem_u32(smem + SM::K), 16, 1024);
       const uint64_t dv = umma_desc(smem_u32(smem + SM::V), PW_HALF, 1024);
-      auto issue_s = [&](int tile, int stage) {
-        const uint64_t a = dq + tile * (SM::TILE >> 4), b = dk + stage * (SM::TILE >> 4);
-        const uint32_t d = tmem + tile * 128;
+      // half j: tokens [64 (j & 1), + 64) of step j / 2, buffer j & 1 of the tile's S
+      auto issue_s = [&](int tile, int j) {
+        const uint64_t a = dq + tile * (SM::TILE >> 4);
+        const uint64_t b = dk + ((j >> 1) & 1) * (SM::TILE >> 4) + (j & 1) * (64 * 128 >> 4);
+        const uint32_t d = tmem + tile * 128 + (j & 1) * 64;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t off = ((kk >> 2) * PW_HALF + (kk & 3) * 32) >> 4;
           umma_f16_el(d, a + off, b + off, id_s, kk > 0, el);
         }
-        umma_commit_el(&s_full[tile], el);
+        umma_commit_el(&s_full[2 * tile + (j & 1)], el);
       };
-      auto issue_o = [&](int tile, int stage, int half, uint32_t first) {   // 64 tokens
-        const uint64_t b = dv + stage * (SM::TILE >> 4) + half * (4 * 2048 >> 4);
-        const uint32_t d = tmem + 256 + tile * D, a = tmem + tile * 128 + half * 32;
+      auto issue_o = [&](int tile, int j) {
+        const uint64_t b = dv + ((j >> 1) & 1) * (SM::TILE >> 4) + (j & 1) * (4 * 2048 >> 4);
+        const uint32_t d = tmem + 256 + tile * D, a = tmem + tile * 128 + (j & 1) * 64;
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
-          umma_f16_ts_el(d, a + ks * 8, b + ks * (2048 >> 4), id_o, ks > 0 ? 1u : first, el);
+          umma_f16_ts_el(d, a + ks * 8, b + ks * (2048 >> 4), id_o, ks > 0 || j > 0, el);
+        umma_commit_el(&o_done[2 * tile + (j & 1)], el);
       };
-      bool ok = warp_wait(&k_full[0], 0, abort_flag);
-      if (ok) {
+      const int tile = warp - 14;
+      const bool idle = tile == 1 && !two;
+      bool ok = idle || warp_wait(&k_full[0], 0, abort_flag);
+      if (ok && !idle) {
         tc_fence_after();
-        issue_s(0, 0);
-        if (two) issue_s(1, 0);
+        issue_s(tile, 0);
+        if (halves > 1) issue_s(tile, 1);
         umma_commit_el(&k_empty[0], el);
       }
-      for (int i = 0; ok && i < steps; ++i) {
-        const int st = i & 1, nx = (i + 1) & 1;
-        ok = warp_wait(&v_full[st], (i >> 1) & 1, abort_flag);
-        for (int tile = 0; ok && tile < (two ? 2 : 1); ++tile) {
-          ok = warp_wait(&p_full[2 * tile], i & 1, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          issue_o(tile, st, 0, i > 0);
-          ok = warp_wait(&p_full[2 * tile + 1], i & 1, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          issue_o(tile, st, 1, 1);
-          umma_commit_el(&o_done[tile], el);
-          if (i + 1 < steps) {
-            if (tile == 0) {
-              ok = warp_wait(&k_full[nx], ((i + 1) >> 1) & 1, abort_flag);
-              if (!ok) break;
-              tc_fence_after();
-            }
-            issue_s(tile, nx);
+      for (int j = 0; ok && !idle && j < halves; ++j) {
+        const int st = (j >> 1) & 1, nj = j + 2;
+        if ((j & 1) == 0) ok = warp_wait(&v_full[st], (j >> 2) & 1, abort_flag);
+        if (ok) ok = warp_wait(&p_full[2 * tile + (j & 1)], (j >> 1) & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        issue_o(tile, j);
+        if ((j & 1) || j + 1 == halves) umma_commit_el(&v_empty[st], el);
+        if (nj < halves) {
+          if ((nj & 1) == 0) {
+            ok = warp_wait(&k_full[(nj >> 1) & 1], (nj >> 2) & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
           }
-        }
-        if (ok) {
-          umma_commit_el(&v_empty[st], el);
-          if (i + 1 < steps) umma_commit_el(&k_empty[nx], el);
+          issue_s(tile, nj);
+          if ((nj & 1) || nj + 1 == halves) umma_commit_el(&k_empty[(nj >> 1) & 1], el);
         }
       }
       if (!ok) {        // leave with no product in flight
         *abort_flag = 1;
-        umma_commit_el(drain, el);
-        mbar_wait(drain, 0);
+        umma_commit_el(drain + tile, el);
+        mbar_wait(drain + tile, 0);
       }
     } else {
       // ---------------- loaders ----------------
@@ -359,7 +360,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
       const int64_t row_step = (int64_t)p.hkv * ROWB, plane_step = row_step * p.ps;
       const char* base = p.pool + (int64_t)kvh * ROWB;
       const int c = lane % CH, sub = lane / CH;
-      // load instruction `it` of this warp takes tokens [unit * TPI, + TPI), unit = lw + 7 it;
+      // load instruction `it` of this warp takes tokens [unit * TPI, + TPI), unit = lw + 6 it;
       // lane L locates the token that instruction L / TPI loads in place L % TPI
       auto unit_of = [&](int it) { return lw + PW_LOADERS * it; };
       const int my_tok = unit_of(lane / TPI) * TPI + lane % TPI;
@@ -465,7 +466,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
           }
           if (i >= 2) ok = warp_wait(&v_empty[st], ((i >> 1) - 1) & 1, abort_flag);
           if (!ok) break;
-          if (store(smem + SM::V + st * SM::TILE, va, !full_step(v0))) odd[st] = i + 1;
+          if (store(smem + SM::V + st * SM::TILE, va, !all_see(v0, PW_TOK))) odd[st] = i + 1;
           signal(&v_full[st]);
         }
       } else {
@@ -481,7 +482,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
         };
         auto finish_v = [&](int i) {  // V of step i has landed: look at it where rows see it in part
           const int st = i & 1;
-          if (!full_step(w.v_begin + i * PW_TOK)) {
+          if (!all_see(w.v_begin + i * PW_TOK, PW_TOK)) {
             bool bad = false;
 #pragma unroll 1
             for (int it = 0; it < ITS; ++it) {
@@ -545,92 +546,85 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
                                                       : max(pos - w.window - w.shift, w.n0);
       float m = kNoMax, l = 0.f;
       bool ok = true, marked = false;
-      for (int i = 0; i < steps; ++i) {
-        const int v0 = w.v_begin + i * PW_TOK;
-        ok = warp_wait(&s_full[tile], i & 1, abort_flag);
+      for (int j = 0; j < halves; ++j) {
+        const int i = j >> 1, v0 = w.v_begin + j * 64;         // step and first token of the half
+        const uint32_t t_p = t_s + (j & 1) * 64;
+        ok = warp_wait(&s_full[2 * tile + (j & 1)], i & 1, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        const float4* tb = tab + (i & 3) * PW_TOK;
-        const bool missing = !Q8 && gone[i & 3] == i + 1, cut = !full_step(v0) || missing;
-        uint32_t see[4] = {};
+        uint32_t x[64];
+        const bool by_token = Q8 && !grouped;
+        if (!by_token) {
+          tmem_ld32_nw(t_p, x);
+          tmem_ld32_nw(t_p + 32, x + 32);
+        }
+        const float4* tb = tab + (i & 3) * PW_TOK + (j & 1) * 64;
+        const bool missing = !Q8 && gone[i & 3] == i + 1, cut = !all_see(v0, 64) || missing;
+        uint32_t see[2] = {};
         if (cut) {
-          const int kc = min(vc >= v0 + PW_TOK ? PW_TOK : vc - v0 + 1, w.v_end - v0);
-          const int ks = min(w.sink_end - v0, PW_TOK), kw = vw <= v0 ? 0 : min(vw - v0, PW_TOK);
+          const int kc = min(vc >= v0 + 64 ? 64 : vc - v0 + 1, w.v_end - v0);
+          const int ks = min(w.sink_end - v0, 64), kw = vw <= v0 ? 0 : min(vw - v0, 64);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            see[j] = low_bits(kc, j) & (low_bits(ks, j) | ~low_bits(kw, j));
+          for (int k = 0; k < 2; ++k)
+            see[k] = low_bits(kc, k) & (low_bits(ks, k) | ~low_bits(kw, k));
           if (missing)                               // a page id out of range: its tokens drop out
-            for (int k = 0; k < min(PW_TOK, w.v_end - v0); ++k) {
+            for (int k = 0; k < min(64, w.v_end - v0); ++k) {
               const int v = v0 + k, t = v + (v >= w.n0 ? w.shift : 0);
               const int page = kvlist[t / p.ps];
               if (page < 0 || page >= p.num_pages) {
                 const uint32_t bit = ~(1u << (k & 31));
                 if (k < 32) see[0] &= bit;
-                else if (k < 64) see[1] &= bit;
-                else if (k < 96) see[2] &= bit;
-                else see[3] &= bit;
+                else see[1] &= bit;
               }
             }
         }
-        uint32_t x[64];
-        // scores of tokens [64 h, 64 h + 64) of the step, -inf where the row does not see them
-        auto fetch = [&](int h) {
-          tmem_ld32_nw(t_s + 64 * h, x);
-          tmem_ld32_nw(t_s + 64 * h + 32, x + 32);
-          tmem_wait();
-          if (cut) {
-            const uint32_t lo = h ? see[2] : see[0], hi = h ? see[3] : see[1];
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              x[k] = (lo >> k) & 1 ? x[k] : 0xff800000u;
-              x[32 + k] = (hi >> k) & 1 ? x[32 + k] : 0xff800000u;
-            }
-          }
-        };
-        const bool by_token = Q8 && !grouped;
         float mx = -INFINITY;
         if (by_token) {
 #pragma unroll 1
-          for (int c0 = 0; c0 < PW_TOK; c0 += 8) {
-            tmem_ld8_nw(t_s + c0, x);
+          for (int c0 = 0; c0 < 64; c0 += 8) {
+            tmem_ld8_nw(t_p + c0, x);
             tmem_wait();
-            const uint32_t bits = cut ? see_at(see, c0) : 0xffu;
+            const uint32_t bits = cut ? (c0 < 32 ? see[0] : see[1]) >> (c0 & 31) : 0xffu;
 #pragma unroll
             for (int k = 0; k < 8; ++k)
               if ((bits >> k) & 1)
                 mx = fmaxf(mx, fmaf(__uint_as_float(x[k]), fmaxf(tb[c0 + k].x * scale, kLeast), tb[c0 + k].y));
           }
         } else {
-#pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
-            fetch(h);
-            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          tmem_wait();
+          if (cut) {
 #pragma unroll
-            for (int k = 0; k < 64; k += 8) {
-              if constexpr (Q8) {
-                float y[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) y[j] = __uint_as_float(x[k + j]);
-                const float gm = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])),
-                                       fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
-                const float4 e = tb[64 * h + k];
-                m4[(k >> 3) & 3] = fmaxf(m4[(k >> 3) & 3], fmaf(gm, fmaxf(e.x * scale, kLeast), e.y));
-              } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  m4[j] = fmaxf(fmaxf(m4[j], __uint_as_float(x[k + j])), __uint_as_float(x[k + 4 + j]));
-              }
+            for (int k = 0; k < 32; ++k) {
+              x[k] = (see[0] >> k) & 1 ? x[k] : 0xff800000u;             // -inf
+              x[32 + k] = (see[1] >> k) & 1 ? x[32 + k] : 0xff800000u;
             }
-            mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
           }
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int k = 0; k < 64; k += 8) {
+            if constexpr (Q8) {
+              float y[8];
+#pragma unroll
+              for (int u = 0; u < 8; ++u) y[u] = __uint_as_float(x[k + u]);
+              const float gm = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])),
+                                     fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
+              const float4 e = tb[k];
+              m4[(k >> 3) & 3] = fmaxf(m4[(k >> 3) & 3], fmaf(gm, fmaxf(e.x * scale, kLeast), e.y));
+            } else {
+#pragma unroll
+              for (int u = 0; u < 4; ++u)
+                m4[u] = fmaxf(fmaxf(m4[u], __uint_as_float(x[k + u])), __uint_as_float(x[k + 4 + u]));
+            }
+          }
+          mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
           if (!Q8) mx *= scale;
         }
         if (__any_sync(0xffffffffu, mx > m + kLazyMax)) {
           const float to = fmaxf(m, mx), f = ex2(m - to);
           m = to;
           l *= f;
-          if (i > 0) {        // O of the steps before: complete, then rescaled
-            ok = warp_wait(&o_done[tile], (i - 1) & 1, abort_flag);
+          if (j > 0) {        // O of the halves before: complete, then rescaled
+            ok = warp_wait(&o_done[2 * tile + ((j - 1) & 1)], ((j - 1) >> 1) & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll 1
@@ -645,82 +639,72 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
             tmem_wait_st();
           }
         }
-        // ---- P, half by half: P V of the first 64 tokens starts while the others are made ----
-        const uint64_t s2 = f2_pack(scale, scale), m2 = f2_pack(-m, -m);
+        // ---- P over S ----
+        if (by_token) {
 #pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          if (by_token) {
-#pragma unroll 1
-            for (int c0 = 64 * h; c0 < 64 * h + 64; c0 += 8) {
-              tmem_ld8_nw(t_s + c0, x);
-              tmem_wait();
-              const uint32_t bits = cut ? see_at(see, c0) : 0xffu;
-              uint32_t pk[4];
+          for (int c0 = 0; c0 < 64; c0 += 8) {
+            tmem_ld8_nw(t_p + c0, x);
+            tmem_wait();
+            const uint32_t bits = cut ? (c0 < 32 ? see[0] : see[1]) >> (c0 & 31) : 0xffu;
+            uint32_t pk[4];
 #pragma unroll
-              for (int k = 0; k < 8; k += 2) {
-                const float4 e = tb[c0 + k], f = tb[c0 + k + 1];
-                float a = ex2(fmaf(__uint_as_float(x[k]), fmaxf(e.x * scale, kLeast), e.y) - m);
-                float b = ex2(fmaf(__uint_as_float(x[k + 1]), fmaxf(f.x * scale, kLeast), f.y) - m);
-                a = (bits >> k) & 1 ? a : 0.f;
-                b = (bits >> k) & 2 ? b : 0.f;
-                l = fmaf(a, e.z, fmaf(b, f.z, l));
-                pk[k >> 1] = pack2<MT>(a, b);
-              }
-              tmem_st4(t_s + c0 / 2, pk);
+            for (int k = 0; k < 8; k += 2) {
+              const float4 e = tb[c0 + k], f = tb[c0 + k + 1];
+              float a = ex2(fmaf(__uint_as_float(x[k]), fmaxf(e.x * scale, kLeast), e.y) - m);
+              float b = ex2(fmaf(__uint_as_float(x[k + 1]), fmaxf(f.x * scale, kLeast), f.y) - m);
+              a = (bits >> k) & 1 ? a : 0.f;
+              b = (bits >> k) & 2 ? b : 0.f;
+              l = fmaf(a, e.z, fmaf(b, f.z, l));
+              pk[k >> 1] = pack2<MT>(a, b);
             }
-          } else {
-            fetch(h);
-            uint64_t sum[2] = {0, 0};
-#pragma unroll
-            for (int c0 = 0; c0 < 64; c0 += 32) {
-              uint32_t pk[16];
-#pragma unroll
-              for (int k0 = c0; k0 < c0 + 32; k0 += 8) {
-                uint64_t gs = s2, gm = m2;
-                float inv = 1.f;
-                if constexpr (Q8) {
-                  const float4 e = tb[64 * h + k0];
-                  const float both = fmaxf(e.x * scale, kLeast);
-                  gs = f2_pack(both, both);
-                  gm = f2_pack(e.y - m, e.y - m);
-                  inv = e.z;
-                  sum[0] = sum[1] = 0;
-                }
-#pragma unroll
-                for (int k = k0; k < k0 + 8; k += 2) {
-                  const uint64_t y = f2_pack(__uint_as_float(x[k]), __uint_as_float(x[k + 1]));
-                  float a, b;
-                  f2_unpack(f2_fma(y, gs, gm), a, b);
-                  a = ex2(a);
-                  b = ex2(b);
-                  sum[(k >> 1) & 1] = f2_add(sum[(k >> 1) & 1], f2_pack(a, b));
-                  pk[(k - c0) >> 1] = pack2<MT>(a, b);
-                }
-                if constexpr (Q8) {
-                  float a, b;
-                  f2_unpack(f2_add(sum[0], sum[1]), a, b);
-                  l = fmaf(a + b, inv, l);
-                }
-              }
-              tmem_st16(t_s + 32 * h + c0 / 2, pk);
-            }
-            if constexpr (!Q8) {
-              float a, b;
-              f2_unpack(f2_add(sum[0], sum[1]), a, b);
-              l += a + b;
-            }
+            tmem_st4(t_p + c0 / 2, pk);
           }
-          if (h == 0) {
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[2 * tile]);
+        } else {
+          const uint64_t s2 = f2_pack(scale, scale), m2 = f2_pack(-m, -m);
+          uint64_t sum[2] = {0, 0};
+#pragma unroll
+          for (int c0 = 0; c0 < 64; c0 += 32) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int k0 = c0; k0 < c0 + 32; k0 += 8) {
+              uint64_t gs = s2, gm = m2;
+              float inv = 1.f;
+              if constexpr (Q8) {
+                const float4 e = tb[k0];
+                const float both = fmaxf(e.x * scale, kLeast);
+                gs = f2_pack(both, both);
+                gm = f2_pack(e.y - m, e.y - m);
+                inv = e.z;
+                sum[0] = sum[1] = 0;
+              }
+#pragma unroll
+              for (int k = k0; k < k0 + 8; k += 2) {
+                const uint64_t y = f2_pack(__uint_as_float(x[k]), __uint_as_float(x[k + 1]));
+                float a, b;
+                f2_unpack(f2_fma(y, gs, gm), a, b);
+                a = ex2(a);
+                b = ex2(b);
+                sum[(k >> 1) & 1] = f2_add(sum[(k >> 1) & 1], f2_pack(a, b));
+                pk[(k - c0) >> 1] = pack2<MT>(a, b);
+              }
+              if constexpr (Q8) {
+                float a, b;
+                f2_unpack(f2_add(sum[0], sum[1]), a, b);
+                l = fmaf(a + b, inv, l);
+              }
+            }
+            tmem_st16(t_p + c0 / 2, pk);
+          }
+          if constexpr (!Q8) {
+            float a, b;
+            f2_unpack(f2_add(sum[0], sum[1]), a, b);
+            l += a + b;
           }
         }
         tmem_wait_st();
-        if (!full_step(v0)) {
+        if (!all_see(w.v_begin + i * PW_TOK, PW_TOK)) {
           // values that are not finite, taken out of V: mark the dims of the rows that see them
-          // (before the second half of P: V's stage and its flag stay until P V of this step is done)
+          // (before P is handed over: V's stage and its flag stay until P V of this half is done)
           ok = warp_wait(&v_full[i & 1], (i >> 1) & 1, abort_flag);
           if (!ok) break;
           if (odd[i & 1] == i + 1) {
@@ -728,7 +712,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
             if (!marked)
               for (int k = 0; k < 2 * (D / 32); ++k) mask[k] = 0;
             marked = true;
-            for (int k = 0; row < rows && k < min(PW_TOK, w.v_end - v0); ++k) {
+            for (int k = 0; row < rows && k < min(64, w.v_end - v0); ++k) {
               const int v = v0 + k, t = v + (v >= w.n0 ? w.shift : 0);
               const int page = kvlist[t / p.ps];
               if (page < 0 || page >= p.num_pages || (causal && t > pos) ||
@@ -752,10 +736,10 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[2 * tile + 1]);
+        if (lane == 0) mbar_arrive(&p_full[2 * tile + (j & 1)]);
       }
       // ---- epilogue ----
-      if (ok) ok = warp_wait(&o_done[tile], (steps - 1) & 1, abort_flag);
+      if (ok) ok = warp_wait(&o_done[2 * tile + ((halves - 1) & 1)], ((halves - 1) >> 1) & 1, abort_flag);
       if (ok) {
         tc_fence_after();
         const float inv = l != 0.f ? 1.f / l : 0.f;
