@@ -48,6 +48,7 @@ struct PagedParams {
   float* lse;
   float* mid_o;
   float* mid_lse;
+  int out_vec16;         // out's rows are 16-byte aligned
   int merge_next;        // the merge is launched next: it may be prepared while these tiles run
 };
 
@@ -745,6 +746,7 @@ extern "C" int be_paged_attn_run(const int32_t* plan_dev, int max_wide, int max_
   p.mid_o = mid_o;
   p.mid_lse = mid_lse;
   p.merge_next = max_merge > 0;
+  p.out_vec16 = (uintptr_t)out % 16 == 0 && out_row_stride % 8 == 0;
   const bool q8 = cache_dtype == BE_E4M3;
   return dtype == BE_BF16
              ? paged_launch<__nv_bfloat16>(p, q8, head_dim, max_wide, max_narrow,

@@ -190,6 +190,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
   // tell the one waited for from the one before the last.
   uint64_t* o_done = bars + 16;
   uint64_t* drain = bars + 20;                  // [row tile]
+  uint64_t* q_full = bars + 27;                 // the softmax warps
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bars + 22);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 23);
   volatile int* odd = reinterpret_cast<volatile int*>(bars + 24);   // [2] per V stage: step + 1
@@ -203,8 +204,9 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
   pdl_wait();
   const be_paged_plan_info* hdr = reinterpret_cast<const be_paged_plan_info*>(p.plan);
   const int item = blockIdx.x / p.hkv, kvh = blockIdx.x - item * p.hkv;
+  // items follow the header, so both are read at once (the plan holds at least one item here)
+  const be_paged_item w = reinterpret_cast<const be_paged_item*>(p.plan + BE_PLAN_HEADER_INTS)[item];
   if (item >= hdr->n_work_wide) return;
-  const be_paged_item w = reinterpret_cast<const be_paged_item*>(p.plan + hdr->off_work)[item];
   const int32_t* kvlist = p.plan + hdr->off_kvlist + w.kv_off;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = p.g, rows = w.q_len * g;
@@ -235,6 +237,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
       odd[s] = gone[s] = gone[2 + s] = 0;
     }
     mbar_init(drain, 1);
+    mbar_init(q_full, 8);
     mbar_init(drain + 1, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -244,48 +247,6 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
                      smem_u32((const void*)tmem_slot)), "n"(512)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  if (warp < 8) {   // Q rows into shared memory, zeros past the item's rows
-    constexpr int QC = D / 8;
-    // the sign of sm_scale goes into Q, so that the largest score is the largest product
-    const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
-    for (int idx = tid; idx < 256 * QC; idx += 256) {
-      const int r = idx / QC, c = idx % QC;
-      uint32_t x[4] = {0, 0, 0, 0};
-      if (r < rows) {
-        const int4 val = *reinterpret_cast<const int4*>(
-            reinterpret_cast<const T*>(p.q) + (w.q_begin + r / g) * p.q_row_stride +
-            (int64_t)(kvh * g + r % g) * D + c * 8);
-        x[0] = val.x ^ flip; x[1] = val.y ^ flip; x[2] = val.z ^ flip; x[3] = val.w ^ flip;
-      }
-      if constexpr (Q8) {
-        // bf16 rows into half range by a power of two, as in the narrow kernel
-        float back = 1.f;
-        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-          float f[8], mx = 0.f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x[i]));
-            f[2 * i] = y.x;
-            f[2 * i + 1] = y.y;
-            mx = fmaxf(mx, fmaxf(fabsf(y.x), fabsf(y.y)));
-          }
-#pragma unroll
-          for (int off = QC / 2; off; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-          int e = (int)(__float_as_uint(mx) >> 23) - 127;
-          e = mx < INFINITY ? min(max(e, -110), 110) : 0;
-          const float up = __uint_as_float((uint32_t)(8 - e + 127) << 23);
-          back = __uint_as_float((uint32_t)(e - 8 + 127) << 23);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = pack2<__half>(f[2 * i] * up, f[2 * i + 1] * up);
-        }
-        if (c == 0) row_scale[r] = back;
-      }
-      *reinterpret_cast<int4*>(smem + SM::Q + (r >> 7) * SM::TILE + (c >> 3) * PW_HALF +
-                               (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) =
-          make_int4(x[0], x[1], x[2], x[3]);
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
@@ -324,7 +285,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
       };
       const int tile = warp - 14;
       const bool idle = tile == 1 && !two;
-      bool ok = idle || warp_wait(&k_full[0], 0, abort_flag);
+      bool ok = idle || (warp_wait(q_full, 0, abort_flag) && warp_wait(&k_full[0], 0, abort_flag));
       if (ok && !idle) {
         tc_fence_after();
         issue_s(tile, 0);
@@ -528,6 +489,62 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
     }
   } else {
     // ---------------- softmax: one row per thread ----------------
+    // ---- Q rows into shared memory, zeros past the item's rows (8 loads in flight per thread; one
+    // at a time they took 9 us of a CTA's 42 at 18 halves) ----
+    {
+      constexpr int QC = D / 8, QR = 256 / QC, QB = 8;         // chunks per row, rows at once
+      // the sign of sm_scale goes into Q, so that the largest score is the largest product
+      const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+      const int c = tid % QC;
+#pragma unroll 1
+      for (int r0 = tid / QC; r0 < (two ? 256 : 128); r0 += QR * QB) {
+        int4 v[QB];
+#pragma unroll
+        for (int k = 0; k < QB; ++k) {
+          const int r = r0 + k * QR;
+          v[k] = r < rows ? ld_early16(reinterpret_cast<const T*>(p.q) +
+                                       (w.q_begin + r / g) * p.q_row_stride +
+                                       (int64_t)(kvh * g + r % g) * D + c * 8)
+                          : make_int4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < QB; ++k) {
+          const int r = r0 + k * QR;
+          uint32_t x[4] = {v[k].x ^ flip, v[k].y ^ flip, v[k].z ^ flip, v[k].w ^ flip};
+          if constexpr (Q8) {
+            // bf16 rows into half range by a power of two, as in the narrow kernel
+            float back = 1.f;
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+              float f[8], mx = 0.f;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x[i]));
+                f[2 * i] = y.x;
+                f[2 * i + 1] = y.y;
+                mx = fmaxf(mx, fmaxf(fabsf(y.x), fabsf(y.y)));
+              }
+#pragma unroll
+              for (int off = QC / 2; off; off >>= 1)
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+              int e = (int)(__float_as_uint(mx) >> 23) - 127;
+              e = mx < INFINITY ? min(max(e, -110), 110) : 0;
+              const float up = __uint_as_float((uint32_t)(8 - e + 127) << 23);
+              back = __uint_as_float((uint32_t)(e - 8 + 127) << 23);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x[i] = pack2<__half>(f[2 * i] * up, f[2 * i + 1] * up);
+            }
+            if (c == 0) row_scale[r] = back;
+          }
+          *reinterpret_cast<int4*>(smem + SM::Q + (r >> 7) * SM::TILE + (c >> 3) * PW_HALF +
+                                   (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) =
+              make_int4(x[0], x[1], x[2], x[3]);
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+      asm volatile("bar.sync 1, 256;" ::: "memory");           // the rows' scales, among these 8 warps
+    }
     const int tile = warp >> 2, row = tid;                 // rows 0..255 of the item
     if (tile == 0 || two) {
       const uint32_t quad = (uint32_t)((warp & 3) * 32) << 16;
@@ -745,37 +762,67 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
         const float inv = l != 0.f ? 1.f / l : 0.f;
         const int qi = row / g, head = kvh * g + row % g;
         const int64_t dst_q = w.part_base < 0 ? w.q_begin + qi : w.part_base + qi;
+        // through this tile's Q rows (its last product has read them) so that rows leave in whole lines
+        char* mine = smem + SM::Q + tile * SM::TILE + (warp & 3) * 32 * (D * 2);
+        constexpr int RB = D * 2;                              // bytes per row here: D results or D / 2 partials
+        const bool part = w.part_base >= 0;
+#pragma unroll 1
+        for (int h = 0; h < (part ? 2 : 1); ++h) {
+          const int d0 = part ? h * (D / 2) : 0, d1 = part ? d0 + D / 2 : D;
+#pragma unroll 1
+          for (int c0 = d0; c0 < d1; c0 += 32) {
+            uint32_t u[32];
+            tmem_ld32_nw(t_o + c0, u);
+            tmem_wait();
+            float f[32];
 #pragma unroll
-        for (int c0 = 0; c0 < D; c0 += 32) {
-          uint32_t u[32];
-          tmem_ld32_nw(t_o + c0, u);
-          tmem_wait();
-          if (row >= rows) continue;
-          float f[32];
+            for (int k = 0; k < 32; ++k) f[k] = l != 0.f ? __uint_as_float(u[k]) * inv : 0.f;
+            if (marked) {
+              const uint32_t up = odd_mask[row * (2 * (D / 32)) + (c0 >> 5)];
+              const uint32_t dn = odd_mask[row * (2 * (D / 32)) + D / 32 + (c0 >> 5)];
+              if (up | dn)
 #pragma unroll
-          for (int k = 0; k < 32; ++k) f[k] = l != 0.f ? __uint_as_float(u[k]) * inv : 0.f;
-          if (marked) {
-            const uint32_t up = odd_mask[row * (2 * (D / 32)) + (c0 >> 5)];
-            const uint32_t dn = odd_mask[row * (2 * (D / 32)) + D / 32 + (c0 >> 5)];
-            if (up | dn)
+                for (int k = 0; k < 32; ++k) {
+                  if ((up >> k) & 1) f[k] += INFINITY;
+                  if ((dn >> k) & 1) f[k] -= INFINITY;
+                }
+            }
+            // 16-byte chunks, turned by the row so that neither side meets a bank twice
+            if (part) {
 #pragma unroll
-              for (int k = 0; k < 32; ++k) {
-                if ((up >> k) & 1) f[k] += INFINITY;
-                if ((dn >> k) & 1) f[k] -= INFINITY;
+              for (int k = 0; k < 8; ++k)
+                *reinterpret_cast<float4*>(mine + lane * RB + ((((c0 - d0) / 4 + k) ^ (lane & 7)) << 4)) =
+                    make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                *reinterpret_cast<uint4*>(mine + lane * RB + (((c0 / 8 + k) ^ (lane & 7)) << 4)) =
+                    make_uint4(pack2<T>(f[8 * k], f[8 * k + 1]), pack2<T>(f[8 * k + 2], f[8 * k + 3]),
+                               pack2<T>(f[8 * k + 4], f[8 * k + 5]), pack2<T>(f[8 * k + 6], f[8 * k + 7]));
+            }
+          }
+          __syncwarp();
+          constexpr int RC = RB / 16;                          // chunks per row
+#pragma unroll 4
+          for (int x = lane; x < 32 * RC; x += 32) {
+            const int rr = x / RC, ch = x % RC, ir = tile * 128 + (warp & 3) * 32 + rr;
+            if (ir >= rows) continue;
+            const uint4 val = *reinterpret_cast<const uint4*>(mine + rr * RB + ((ch ^ (rr & 7)) << 4));
+            const int iq = ir / g, ih = kvh * g + ir % g;
+            if (part)
+              *reinterpret_cast<uint4*>(p.mid_o + ((int64_t)(w.part_base + iq) * p.hq + ih) * D + d0 +
+                                        ch * 4) = val;
+            else {
+              T* dst = reinterpret_cast<T*>(p.out) + (int64_t)(w.q_begin + iq) * p.out_row_stride +
+                       (int64_t)ih * D + ch * 8;
+              if (p.out_vec16) *reinterpret_cast<uint4*>(dst) = val;
+              else {
+                reinterpret_cast<uint2*>(dst)[0] = make_uint2(val.x, val.y);
+                reinterpret_cast<uint2*>(dst)[1] = make_uint2(val.z, val.w);
               }
+            }
           }
-          if (w.part_base < 0) {
-            T* dst = reinterpret_cast<T*>(p.out) + dst_q * p.out_row_stride + (int64_t)head * D + c0;
-#pragma unroll
-            for (int k = 0; k < 32; k += 4)
-              *reinterpret_cast<uint2*>(dst + k) =
-                  make_uint2(pack2<T>(f[k], f[k + 1]), pack2<T>(f[k + 2], f[k + 3]));
-          } else {
-            float* dst = p.mid_o + (dst_q * p.hq + head) * D + c0;
-#pragma unroll
-            for (int k = 0; k < 32; k += 4)
-              *reinterpret_cast<float4*>(dst + k) = make_float4(f[k], f[k + 1], f[k + 2], f[k + 3]);
-          }
+          __syncwarp();
         }
         if (row < rows) {
           const float lse = l > 0.f ? (m + log2f(l)) * kLn2 : l == 0.f ? -INFINITY : l;

@@ -429,7 +429,8 @@ int be_paged_plan(int num_levels, const int32_t* const* qo_indptr, const int32_t
 
 /* Runs a be_paged_plan plan in device memory (header included) for one layer.
  * The launch shape depends on the max_* capacities only and the kernels read the plan's counts
- * from its header, so a recorded launch serves every plan with at most
+ * from its header (every CTA reads its item before the counts, so the buffer holds at least
+ * BE_PLAN_HEADER_INTS + 16 * max_wide ints), so a recorded launch serves every plan with at most
  * max_wide wide and max_narrow narrow items (of up to narrow_rows rows, 0..16), max_merge
  * merged queries and max_parts partial rows.  dtype (q, out): BE_BF16 or BE_F16; cache_dtype BE_E4M3
  * (kv_scale required) or dtype; head_dim 64 or 128.  q [n][num_qo_heads][head_dim]
