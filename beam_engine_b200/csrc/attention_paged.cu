@@ -285,6 +285,7 @@ __global__ void __launch_bounds__(128, PnRing<CT, D, NB>::CTAS) paged_narrow_ker
     page_next = page_of(v0 + 64 * (j + 1));
     issue(j, v0 + 64 * j, page);
   }
+#pragma unroll 1
   for (; v0 < w.v_end; v0 += 64) {
     cp_wait<Ring::STAGES - 2>();
     __syncwarp();

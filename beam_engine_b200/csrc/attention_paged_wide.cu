@@ -158,10 +158,14 @@ __device__ __forceinline__ uint32_t zero_not_finite(uint32_t w) {
   return w;
 }
 
+// The slow half of a wait, out of line: it would be inlined a dozen times into code that has to fit the
+// instruction caches.
+__device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity); }
+
 // Bounded wait of a whole warp: every lane sees the phase, and all agree on the outcome.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
-  const bool ok = !*abort_flag && mbar_wait(bar, parity);
+  const bool ok = !*abort_flag && wait_on(bar, parity);
   return __all_sync(0xffffffffu, ok);
 }
 
@@ -210,6 +214,9 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
   const int32_t* kvlist = p.plan + hdr->off_kvlist + w.kv_off;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = p.g, rows = w.q_len * g;
+  // row / g for rows below 256 (g <= 128: the error r * 1 / 2^20 stays under 1 / g)
+  const int g_inv = (1 << 20) / g + 1;
+  auto query_of = [&](int r) { return (r * g_inv) >> 20; };
   const bool two = rows > 128;
   const int steps = (w.v_end - w.v_begin + PW_TOK - 1) / PW_TOK;
   const int halves = (w.v_end - w.v_begin + PW_TOK / 2 - 1) / (PW_TOK / 2);
@@ -292,6 +299,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
         if (halves > 1) issue_s(tile, 1);
         umma_commit_el(&k_empty[0], el);
       }
+#pragma unroll 1
       for (int j = 0; ok && !idle && j < halves; ++j) {
         const int st = (j >> 1) & 1, nj = j + 2;
         if ((j & 1) == 0) ok = warp_wait(&v_full[st], (j >> 2) & 1, abort_flag);
@@ -313,7 +321,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
       if (!ok) {        // leave with no product in flight
         *abort_flag = 1;
         umma_commit_el(drain + tile, el);
-        mbar_wait(drain + tile, 0);
+        wait_on(drain + tile, 0);
       }
     } else {
       // ---------------- loaders ----------------
@@ -407,6 +415,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
         int64_t at = locate(0, page_of(w.v_begin), sk, sv);
         load(ka, at, 0);
         int page_next = page_of(w.v_begin + PW_TOK);
+#pragma unroll 1
         for (int i = 0; i < steps; ++i) {
           const int st = i & 1, v0 = w.v_begin + i * PW_TOK;
           load(va, at, plane_step);
@@ -464,6 +473,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
         };
         float sk, sv;
         int page_next = page_of(w.v_begin);
+#pragma unroll 1
         for (int i = 0; i < steps; ++i) {
           const int st = i & 1;
           const int64_t at = locate(i, page_next, sk, sv);
@@ -503,8 +513,8 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
         for (int k = 0; k < QB; ++k) {
           const int r = r0 + k * QR;
           v[k] = r < rows ? ld_early16(reinterpret_cast<const T*>(p.q) +
-                                       (w.q_begin + r / g) * p.q_row_stride +
-                                       (int64_t)(kvh * g + r % g) * D + c * 8)
+                                       (w.q_begin + query_of(r)) * p.q_row_stride +
+                                       (int64_t)(kvh * g + r - query_of(r) * g) * D + c * 8)
                           : make_int4(0, 0, 0, 0);
         }
 #pragma unroll
@@ -549,7 +559,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
     if (tile == 0 || two) {
       const uint32_t quad = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t t_s = tmem + tile * 128 + quad, t_o = tmem + 256 + tile * D + quad;
-      const int pos = w.pos0 + w.pos_step * (row / g);
+      const int pos = w.pos0 + w.pos_step * query_of(row);
       // factors of scores are never 0: a masked score of -inf stays -inf
       constexpr float kLeast = 1e-37f;
       const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f) * (Q8 ? row_scale[row] : 1.f);
@@ -563,6 +573,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
                                                       : max(pos - w.window - w.shift, w.n0);
       float m = kNoMax, l = 0.f;
       bool ok = true, marked = false;
+#pragma unroll 1
       for (int j = 0; j < halves; ++j) {
         const int i = j >> 1, v0 = w.v_begin + j * 64;         // step and first token of the half
         const uint32_t t_p = t_s + (j & 1) * 64;
@@ -585,6 +596,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
           for (int k = 0; k < 2; ++k)
             see[k] = low_bits(kc, k) & (low_bits(ks, k) | ~low_bits(kw, k));
           if (missing)                               // a page id out of range: its tokens drop out
+#pragma unroll 1
             for (int k = 0; k < min(64, w.v_end - v0); ++k) {
               const int v = v0 + k, t = v + (v >= w.n0 ? w.shift : 0);
               const int page = kvlist[t / p.ps];
@@ -729,6 +741,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
             if (!marked)
               for (int k = 0; k < 2 * (D / 32); ++k) mask[k] = 0;
             marked = true;
+#pragma unroll 1
             for (int k = 0; row < rows && k < min(64, w.v_end - v0); ++k) {
               const int v = v0 + k, t = v + (v >= w.n0 ? w.shift : 0);
               const int page = kvlist[t / p.ps];
@@ -737,6 +750,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
                 continue;
               const int64_t r = ((int64_t)page * 2 + 1) * p.ps + t % p.ps;
               const char* src = p.pool + (r * p.hkv + kvh) * ROWB;
+#pragma unroll 1
               for (int d = 0; d < D; ++d) {
                 float val;
                 if constexpr (Q8) {
@@ -760,7 +774,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
       if (ok) {
         tc_fence_after();
         const float inv = l != 0.f ? 1.f / l : 0.f;
-        const int qi = row / g, head = kvh * g + row % g;
+        const int qi = query_of(row), head = kvh * g + row - qi * g;
         const int64_t dst_q = w.part_base < 0 ? w.q_begin + qi : w.part_base + qi;
         // through this tile's Q rows (its last product has read them) so that rows leave in whole lines
         char* mine = smem + SM::Q + tile * SM::TILE + (warp & 3) * 32 * (D * 2);
@@ -781,7 +795,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
               const uint32_t up = odd_mask[row * (2 * (D / 32)) + (c0 >> 5)];
               const uint32_t dn = odd_mask[row * (2 * (D / 32)) + D / 32 + (c0 >> 5)];
               if (up | dn)
-#pragma unroll
+#pragma unroll 4
                 for (int k = 0; k < 32; ++k) {
                   if ((up >> k) & 1) f[k] += INFINITY;
                   if ((dn >> k) & 1) f[k] -= INFINITY;
@@ -803,12 +817,12 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
           }
           __syncwarp();
           constexpr int RC = RB / 16;                          // chunks per row
-#pragma unroll 4
+#pragma unroll 2
           for (int x = lane; x < 32 * RC; x += 32) {
             const int rr = x / RC, ch = x % RC, ir = tile * 128 + (warp & 3) * 32 + rr;
             if (ir >= rows) continue;
             const uint4 val = *reinterpret_cast<const uint4*>(mine + rr * RB + ((ch ^ (rr & 7)) << 4));
-            const int iq = ir / g, ih = kvh * g + ir % g;
+            const int iq = query_of(ir), ih = kvh * g + ir - iq * g;
             if (part)
               *reinterpret_cast<uint4*>(p.mid_o + ((int64_t)(w.part_base + iq) * p.hq + ih) * D + d0 +
                                         ch * 4) = val;
