@@ -28,7 +28,7 @@ from ._lib import check, lib
 from .beam_state import BeamState
 from .beam_strategy import VanillaBeamSearchStrategy
 from .cascade import _Plan, target_pieces, tile_rows_for, tiles_eligible
-from .page_table import PageTable, stream_ptr
+from .page_table import PageTable, is_8bit, stream_ptr
 from .parallel import vocab_parallel_log_softmax_topk
 
 logger = logging.getLogger(__name__)
@@ -65,6 +65,7 @@ class PlannedAttention:
         self.plan = _Plan(workspace)
         self.scale = model.D ** -0.5
         self.kv_list = None
+        self.paged = False         # the plan in place is be_paged_plan's (8-bit pools)
         self.timer = None          # optional (start_event, end_event) list collector
 
     def plan_levels(self, levels, num_queries, causal=True, split_tokens=0):
@@ -75,6 +76,16 @@ class PlannedAttention:
         ptrs = [(_lib.P32 * max(L, 1))(*[_lib.ptr32(a) for a in grp]) for grp in arrs]
         m, ps, p = self.m, self.pt.page_size, self.plan
         self.kv_list = None
+        self.paged = self.pt.kv_scale is not None
+        if self.paged:                     # 8-bit pools: their own plans and kernels
+            def pfn(buf, cap, info):
+                return lib().be_paged_plan(L, *ptrs, _lib.ptr32(ng), num_queries, ps, m.Hq, m.Hkv,
+                                           1 if causal else 0, -1, 0, p.num_sms, buf, cap, info)
+            p.info = _lib.PagedPlanInfo()
+            p.build(pfn)
+            p.place(m.Hq, m.D)
+            p.tinfo = None
+            return
         if (split_tokens == 0 and self.pt.store_dtype != torch.float32
                 and tiles_eligible(m.D, ps, m.Hq, m.Hkv)):
             g = m.Hq // m.Hkv
@@ -133,6 +144,14 @@ class PlannedAttention:
         if t is not None:
             s, e = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
             s.record()
+        if self.paged:
+            self.plan.run_paged(qkv[:, :m.Hq * m.D].view(-1, m.Hq, m.D), self.pt.kv_cache[layer],
+                                self.pt.kv_scale[layer], m.Hq, m.Hkv, m.D, self.scale,
+                                out.view(-1, m.Hq, m.D))
+            if t is not None:
+                e.record()
+                t.append((s, e))
+            return
         if self.plan.tinfo is not None:
             self.plan.run_tiles(qkv[:, :m.Hq * m.D].view(-1, m.Hq, m.D), self.pt.kv_cache[layer],
                                 m.Hq, m.Hkv, m.D, self.scale, out.view(-1, m.Hq, m.D))
@@ -213,7 +232,8 @@ class StepGraph:
     attention runs through ``be_attn_run_fixed_2s``, whose launch shape depends
     only on the capacities (the kernels read the plan's counts from its
     device-side header).  ``kind`` is "cascade" (page-list plans, tensor-core
-    prefix and suffix kernels) or "fasttree" (slot-list plans, general kernel)."""
+    prefix and suffix kernels), "fasttree" (slot-list plans, general kernel) or
+    "paged" (8-bit pools: ``be_paged_attn_run``)."""
 
     def __init__(self, gen, n, k, temperature, caps, kind="cascade"):
         self.gen, self.n, self.k, self.temp = gen, n, k, temperature
@@ -265,7 +285,7 @@ class StepGraph:
             self.sel_h = (torch.empty(nseg * W, dtype=torch.int32).pin_memory(),
                           torch.empty(nseg * W, dtype=torch.int32).pin_memory(),
                           torch.empty(nseg * W, dtype=torch.float64).pin_memory())
-        if kind != "tiles":
+        if kind not in ("tiles", "paged"):
             self.ccaps = _lib.AttnCaps(self.caps["work"], self.caps["wide"], self.caps["merge"], 1,
                                        _lib.BE_CAPS_SLOTS if kind == "fasttree" else 0)
         # suffix tiles on a second stream, overlapping the shared-prefix tiles
@@ -290,6 +310,12 @@ class StepGraph:
                     and info.n_pieces <= c["pieces"] and info.n_tiles <= c["tiles"]
                     and info.n_part_pieces <= c["part_pieces"] and info.total_ints <= c["ints"]
                     and info.tile_rows == c["rows"] and info.cluster == c["cluster"])
+        if self.kind == "paged":
+            return (n == self.n and k == self.k and temperature == self.temp
+                    and info.n_work_wide <= c["wide"]
+                    and info.n_work - info.n_work_wide <= c["narrow"]
+                    and info.narrow_rows <= c["rows"] and info.n_merge <= c["merge"]
+                    and info.n_parts <= c["parts"] and info.total_ints <= c["ints"])
         return (n == self.n and k == self.k and temperature == self.temp
                 and info.n_work <= c["work"] and info.n_work_wide <= c["wide"]
                 and info.n_merge <= c["merge"] and info.n_parts <= c["parts"]
@@ -324,6 +350,17 @@ class StepGraph:
             check(rc, "be_attn_tiles_run")
             self._mark(2 * layer + 1, qkv)
             return
+        if self.kind == "paged":
+            c = self.caps
+            rc = lib().be_paged_attn_run(
+                self.dev_buf.data_ptr() + 4 * self.plan_off, c["wide"], c["narrow"], c["rows"],
+                c["merge"], c["parts"], pt.page_size, qkv.data_ptr(), qkv.stride(0),
+                pt.kv_cache[layer].data_ptr(), pt.kv_scale[layer].data_ptr(), pt.max_num_pages,
+                m.Hq, m.Hkv, m.D, m.dt, _lib.BE_E4M3, m.D ** -0.5, out.data_ptr(), out.stride(0),
+                None, self.mid_o.data_ptr(), self.mid_lse.data_ptr(), stream_ptr(qkv.device))
+            check(rc, "be_paged_attn_run")
+            self._mark(2 * layer + 1, qkv)
+            return
         rc = lib().be_attn_run_fixed_2s(
             self.dev_buf.data_ptr() + 4 * self.plan_off, C.byref(self.ccaps), pt.page_size,
             qkv.data_ptr(), qkv.stride(0), pt.kv_cache[layer].data_ptr(), pt.max_num_pages, m.Hq,
@@ -352,12 +389,18 @@ class StepGraph:
         n = self.n
         d = self.dev_buf
         pt = self.gen.page_table
-        check(lib().be_fork_tail_copy_list(pt.kv_cache.data_ptr(), pt.kv_cache.stride(0),
-                                           pt.layer_num, pt.max_num_pages, pt.page_size,
-                                           pt.head_num, pt.head_dim, _pool_dtype(pt),
-                                           d.data_ptr() + 4 * self.fork_off, n,
-                                           self.gen.attn.plan.num_sms,
-                                           stream_ptr(self.gen.device)), "fork list")
+        if pt.kv_scale is not None:
+            check(lib().be_fork_tail_copy8_list(
+                pt.kv_cache.data_ptr(), pt.kv_cache.stride(0), pt.kv_scale.data_ptr(),
+                pt.kv_scale.stride(0), pt.layer_num, pt.max_num_pages, pt.page_size, pt.head_num,
+                pt.head_dim, d.data_ptr() + 4 * self.fork_off, n, self.gen.attn.plan.num_sms,
+                stream_ptr(self.gen.device)), "fork list")
+        else:
+            check(lib().be_fork_tail_copy_list(
+                pt.kv_cache.data_ptr(), pt.kv_cache.stride(0), pt.layer_num, pt.max_num_pages,
+                pt.page_size, pt.head_num, pt.head_dim, _pool_dtype(pt),
+                d.data_ptr() + 4 * self.fork_off, n, self.gen.attn.plan.num_sms,
+                stream_ptr(self.gen.device)), "fork list")
         logits = self.gen.model.forward(d[0:n], d[n:2 * n], self.gen.page_table, d[2 * n:3 * n],
                                         d[3 * n:4 * n], self)
         v, i = self.gen._logprob_topk(logits, self.k, self.temp)
@@ -452,6 +495,14 @@ class BeamSearchGenerator:
         self.page_size = page_size
         self.kernel_type = kernel_type
         c = model.config
+        # an 8-bit pool (store_dtype=torch.float8_e4m3fn) holds K/V as codes with a scale per
+        # page and head; cascade attention reads them
+        self.cache8 = store_dtype is not None and is_8bit(store_dtype)
+        if self.cache8:
+            if kernel_type != "cascade":
+                raise ValueError("an 8-bit pool takes kernel_type='cascade'")
+            if model.dtype not in (torch.bfloat16, torch.float16) or model.D not in (64, 128):
+                raise ValueError("an 8-bit pool takes a bf16 or fp16 model with head_dim 64 or 128")
         self.page_table = PageTable(layer_num=c["num_hidden_layers"], page_size=page_size,
                                     max_num_pages=max_num_pages, head_num=model.Hkv,
                                     head_dim=model.D, device=self.device,
@@ -462,7 +513,8 @@ class BeamSearchGenerator:
         self.topk_host = None
         self.step_timer = None
         # cascade decode steps replay one CUDA graph (bf16/fp16 pools, page size 16)
-        self.use_graph = (use_graph and kernel_type in ("cascade", "auto") and page_size == 16
+        self.use_graph = (use_graph and kernel_type in ("cascade", "auto")
+                          and (page_size == 16 or self.cache8)
                           and self.page_table.store_dtype != torch.float32)
         # tree steps replay their own graph (slot-list plans, any page size, 2-byte pools)
         self.use_graph_tree = (use_graph and kernel_type in ("fasttree", "auto")
@@ -485,8 +537,9 @@ class BeamSearchGenerator:
                            and self.page_table.store_dtype != torch.float32)
         self.step_graph_tpages = None
         self.step_graph_tiles = None
+        self.step_graph_paged = None  # 8-bit pools
         # cascade steps on the beam-tile kernel (BE_ATTN_TILES=0: the work-item kernels)
-        self.use_tiles = (self.page_table.store_dtype != torch.float32
+        self.use_tiles = (self.page_table.store_dtype != torch.float32 and not self.cache8
                           and tiles_eligible(model.D, page_size, model.Hq, model.Hkv))
         self._beam_width = 1
         # vanilla selection on the device inside the tile step graph (BE_DEVICE_SELECT=0: host)
@@ -713,6 +766,8 @@ class BeamSearchGenerator:
         self._tree_stash = None
         if not self.use_graph or kind != "cascade":
             return self._topk(self.decode_step(state, kind), k, temperature)
+        if getattr(self, "cache8", False):
+            return self._paged_graph_step(state, k, temperature)
         if self.use_tiles:
             got = self._tiles_graph_step(state, k, temperature)
             if got is not None:
@@ -766,6 +821,50 @@ class BeamSearchGenerator:
                 raise RuntimeError("decode step graph sized too small for its own plan")
         if self.plan_hook is not None:
             self.plan_hook(n, info)
+        self._take_fork(sg)
+        return sg.step_filled(sg.plan_off + info.total_ints)
+
+    def _paged_graph_step(self, state: BeamState, k: int, temperature: float):
+        """A cascade decode step over an 8-bit pool, replayed from its graph."""
+        from .cascade import _level_arrays
+        m = self.model
+        n = len(state.leaves)
+        q, wp, wpos, pos = state.step_inputs()
+        L, arrs, ng, ptrs = _level_arrays(state.cascade_levels())
+        info = _lib.PagedPlanInfo()
+        sg = self.step_graph_paged
+
+        def fill(buf_ptr, cap, off):
+            rc = lib().be_paged_plan(L, *ptrs, _lib.ptr32(ng), n, self.page_table.page_size, m.Hq,
+                                     m.Hkv, 1, -1, 0, self.attn.plan.num_sms,
+                                     C.c_void_p(buf_ptr + 4 * off), cap - off, C.byref(info))
+            if rc not in (_lib.BE_OK, _lib.BE_ECAPACITY):
+                check(rc, "be_paged_plan")
+            return rc == _lib.BE_OK
+
+        if not (sg is not None and sg.n == n
+                and fill(sg.host_buf.data_ptr(), sg.slots_off, sg.plan_off)
+                and sg.fits(n, k, temperature, info)):
+            fill(0, 0, 0)                     # sizes only
+            # headroom: items and partial rows keep growing with the beams' suffixes
+            caps = dict(wide=2 * info.n_work_wide + 16,
+                        narrow=3 * (info.n_work - info.n_work_wide) + 2 * n + 64,
+                        rows=16, merge=max(n, 1), parts=3 * info.n_parts + 4 * n + 256,
+                        ints=3 * info.total_ints + 96 * n + 4096)
+            if sg is not None and sg.n == n and sg.k == k and sg.temp == temperature:
+                for key in caps:
+                    caps[key] = max(caps[key], sg.caps[key] * 3 // 2 if key != "rows" else 16)
+            elif sg is not None:
+                self.graph_regrowth.append({"shape": (sg.n, n, sg.k, k)})
+            # every CTA reads its item before the item count
+            caps["ints"] = max(caps["ints"], 32 + 16 * (caps["wide"] + caps["narrow"]) + 64)
+            self.step_graph_paged = sg = StepGraph(self, n, k, temperature, caps, kind="paged")
+            if not fill(sg.host_buf.data_ptr(), sg.slots_off, sg.plan_off):
+                raise RuntimeError("decode step graph sized too small for its own plan")
+        if self.plan_hook is not None:
+            self.plan_hook(n, info)
+        h = sg.host_buf.numpy()
+        h[0:n], h[n:2 * n], h[2 * n:3 * n], h[3 * n:4 * n] = q, pos, wp, wpos
         self._take_fork(sg)
         return sg.step_filled(sg.plan_off + info.total_ints)
 
@@ -996,6 +1095,13 @@ class BeamSearchGenerator:
         cs, cd, cl = copies
         d = self._to_device([cs, cd, cl])
         pt = self.page_table
+        if pt.kv_scale is not None:
+            check(lib().be_fork_tail_copy8(
+                pt.kv_cache.data_ptr(), pt.kv_cache.stride(0), pt.kv_scale.data_ptr(),
+                pt.kv_scale.stride(0), pt.layer_num, pt.max_num_pages, pt.page_size, pt.head_num,
+                pt.head_dim, d[0].data_ptr(), d[1].data_ptr(), d[2].data_ptr(), len(cs),
+                stream_ptr(self.device)), "fork")
+            return
         check(lib().be_fork_tail_copy(pt.kv_cache.data_ptr(), pt.kv_cache.stride(0),
                                       pt.layer_num, pt.max_num_pages, pt.page_size,
                                       pt.head_num, pt.head_dim, _pool_dtype(pt),

@@ -117,6 +117,7 @@ class BeamLlama:
         self.use_lt = mode == "lt" and cuda_bf16           # cuBLASLt, per-shape tuned
         self._gemm_ws = None
         self._lt_ws = None
+        self._append_ws = None    # run lists of large appends into 8-bit pools
         self.comm = None          # PeerAllReduce: fused all-reduce + add + RMSNorm under TP
         self._slot_views = {}
         del weights
@@ -190,7 +191,11 @@ class BeamLlama:
         gu = torch.empty((n, 2 * self.F), dtype=dt, device=dev)
         act = torch.empty((n, self.F), dtype=dt, device=dev)
         delta = torch.empty_like(x)
-        pool = page_table.kv_cache
+        pool, scale = page_table.kv_cache, page_table.kv_scale
+        if scale is not None and n > 512 and (self._append_ws is None
+                                              or self._append_ws.numel() < 5 * n + 1024):
+            self._append_ws = torch.empty(5 * n + 1024, dtype=torch.int32, device=dev)
+        ws = self._append_ws if n > 512 else None
         P, ps = page_table.max_num_pages, page_table.page_size
         have_delta = False
         # fused peer all-reduce: the O / down GEMMs write into this rank's slots and
@@ -203,10 +208,18 @@ class BeamLlama:
                                        self.n_in[i].data_ptr(), h.data_ptr(), n, self.H, self.eps,
                                        self.dt, st), "add_rmsnorm")
             self._mm(h, self.w_qkv[i], qkv)
-            check(L.be_rope_qkv_append(qkv.data_ptr(), self.qkv_width, n, self.Hq, self.Hkv, self.D,
-                                       positions.data_ptr(), self.inv_freq.data_ptr(),
-                                       pool[i].data_ptr(), P, ps, write_pages.data_ptr(),
-                                       write_pos.data_ptr(), 0, self.dt, st), "rope_append")
+            if scale is not None:     # rounded into the 8-bit pages with their blocks' scales
+                check(L.be_rope_qkv_append8(
+                    qkv.data_ptr(), self.qkv_width, n, self.Hq, self.Hkv, self.D,
+                    positions.data_ptr(), self.inv_freq.data_ptr(), pool[i].data_ptr(),
+                    scale[i].data_ptr(), P, ps, write_pages.data_ptr(), write_pos.data_ptr(),
+                    self.dt, ws.data_ptr() if ws is not None else None,
+                    ws.numel() if ws is not None else 0, st), "rope_append8")
+            else:
+                check(L.be_rope_qkv_append(
+                    qkv.data_ptr(), self.qkv_width, n, self.Hq, self.Hkv, self.D,
+                    positions.data_ptr(), self.inv_freq.data_ptr(), pool[i].data_ptr(), P, ps,
+                    write_pages.data_ptr(), write_pos.data_ptr(), 0, self.dt, st), "rope_append")
             attention.run(i, qkv, att)
             if layer_hook is not None:
                 layer_hook(i)
