@@ -13,10 +13,13 @@
 //     half are there when its softmax comes to them.  (128 x 128 products with one buffer
 //     left the softmax waiting for P V and S of its own tile, 1 560 of 4 270 clocks a step;
 //     128 x 64 x 16 takes 49 clocks instead of 32, bound by shared memory, 128 x 128 x 16 takes 65.)
-//   * softmax warps (4 per row tile, a thread per row): 64 scores from TMEM to registers, maximum, P
-//     written over S; O is rescaled only when a row's maximum grows by more than 2^8.  Their
-//     loops stay short because 16 warps in three roles share the instruction cache: with 128 scores
-//     per pass and every variant unrolled, fetching instructions took half of each step.
+//   * softmax warps (8 per row tile, two threads per row with 32 scores of a half each): scores from
+//     TMEM to registers, maximum, P written over S; O is rescaled only when a row's maximum
+//     grows by more than 2^8, so the two threads of a row only agree that it did not (a barrier
+//     with a vote); their sums meet at the end.  One thread per row left a third of the issue slots used
+//     (two softmax warps per scheduler, each a chain of dependent steps).  The loops stay
+//     short because 24 warps in three roles share the instruction cache: with 128 scores per
+//     pass and every variant unrolled, fetching instructions took half of each step.
 // TMEM: S/P of tile 0 (two buffers of 64) | of tile 1 | O of tile 0 | O of tile 1 = 256 + 2 D columns
 // (512 allocated).  S of half j + 2 overwrites P of half j: both products come from one thread,
 // and the tensor core runs them in the order of issue.
@@ -42,7 +45,8 @@ namespace be {
 
 constexpr int PW_TOK = 128;                    // tokens per step
 constexpr int PW_LOADERS = 6;
-constexpr int PW_THREADS = 16 * 32;            // 8 softmax warps, 6 loader warps, 2 issuers
+constexpr int PW_SOFT = 16;                    // softmax warps
+constexpr int PW_THREADS = (PW_SOFT + PW_LOADERS + 2) * 32;   // and 2 issuers
 constexpr int PW_HALF = PW_TOK * 128;          // 64 dims of 128 rows
 constexpr int PW_STAGES = 2;
 
@@ -52,7 +56,8 @@ struct PwSmem {
   static constexpr int Q = 0, K = 2 * TILE, V = K + PW_STAGES * TILE, ODD = V + PW_STAGES * TILE;
   static constexpr int TAB = ODD + 256 * (D / 32) * 8;  // two bit masks of D dims per row
   static constexpr int RS = TAB + 4 * PW_TOK * 16;      // scales of 4 steps' tokens
-  static constexpr int BAR = RS + 256 * 4;              // scales of the rows
+  static constexpr int MX = RS + 256 * 4;               // scales of the rows
+  static constexpr int BAR = MX + 2 * 256 * 4;          // the threads' maxima, then sums
   static constexpr int BYTES = BAR + 256 + 1024;
 };
 
@@ -120,10 +125,18 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// bits [0, n) of the 32 that start at bit 32 * word
-__device__ __forceinline__ uint32_t low_bits(int n, int word) {
-  const int k = min(max(n - 32 * word, 0), 32);
+__device__ __forceinline__ uint32_t low_bits(int n) {         // bits [0, n), n clamped to 0 .. 32
+  const int k = min(max(n, 0), 32);
   return k == 32 ? ~0u : (1u << k) - 1u;
+}
+// Barrier `id` of 256 threads; whether `p` held in one of them.
+__device__ __forceinline__ bool vote256(int id, bool p) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %2, 0;\n"
+      " barrier.cta.red.or.pred q, %1, 256, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(r) : "r"(id), "r"((uint32_t)p) : "memory");
+  return r != 0;
 }
 
 __device__ __forceinline__ void tmem_ld16_nw(uint32_t taddr, uint32_t* r) {
@@ -134,19 +147,6 @@ __device__ __forceinline__ void tmem_ld16_nw(uint32_t taddr, uint32_t* r) {
         "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
         "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
-}
-
-__device__ __forceinline__ void tmem_ld8_nw(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t* r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]),
-               "r"(r[1]), "r"(r[2]), "r"(r[3])
-               : "memory");
 }
 
 // element x of a 16-bit pair: set to zero if not finite
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
   uint64_t* k_empty = bars + 4;                 // [2], commit
   uint64_t* v_empty = bars + 6;                 // [2]
   uint64_t* s_full = bars + 8;                  // [row tile][half], commit
-  uint64_t* p_full = bars + 12;                 // [row tile][half], 4 softmax warps
+  uint64_t* p_full = bars + 12;                 // [row tile][half], 8 softmax warps
   // [row tile][half], commit.  Two P V of a tile can be in flight, so a single barrier's parity could not
   // tell the one waited for from the one before the last.
   uint64_t* o_done = bars + 16;
@@ -199,11 +199,13 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 23);
   volatile int* odd = reinterpret_cast<volatile int*>(bars + 24);   // [2] per V stage: step + 1
   volatile int* gone = reinterpret_cast<volatile int*>(bars + 25);  // [4]: step + 1 that misses a page
+  volatile int* marked = reinterpret_cast<volatile int*>(bars + 28);   // some row's odd_mask is set
   uint32_t* odd_mask = reinterpret_cast<uint32_t*>(smem + SM::ODD);  // [256][2][D / 32]
   // per token of the last 4 steps (the loaders are at most 3 past the softmax, and write a step's
   // entries once V of the third before is used up): s_K, log2 s_V, 1 / s_V
   float4* tab = reinterpret_cast<float4*>(smem + SM::TAB);
   float* row_scale = reinterpret_cast<float*>(smem + SM::RS);
+  float* meet = reinterpret_cast<float*>(smem + SM::MX);             // [2][256]
 
   pdl_wait();
   const be_paged_plan_info* hdr = reinterpret_cast<const be_paged_plan_info*>(p.plan);
@@ -239,14 +241,15 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
       for (int h = 0; h < 2; ++h) {
         mbar_init(&o_done[2 * s + h], 1);
         mbar_init(&s_full[2 * s + h], 1);
-        mbar_init(&p_full[2 * s + h], 4);
+        mbar_init(&p_full[2 * s + h], PW_SOFT / 2);
       }
       odd[s] = gone[s] = gone[2 + s] = 0;
     }
     mbar_init(drain, 1);
-    mbar_init(q_full, 8);
+    mbar_init(q_full, PW_SOFT);
     mbar_init(drain + 1, 1);
     *abort_flag = 0;
+    *marked = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) {
@@ -260,9 +263,9 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp >= 8) {
-    if (warp >= 14) {
-      // ---------------- issuers: warp 14 for row tile 0, warp 15 for row tile 1 ----------------
+  if (warp >= PW_SOFT) {
+    if (warp >= PW_SOFT + PW_LOADERS) {
+      // ---------------- issuers: a warp for each row tile ----------------
       // The whole warp walks the steps and one elected lane issues: addresses and descriptors
       // then stay in uniform registers (from a divergent lane every product first moves them there)
       const uint32_t el = elect_one();
@@ -290,7 +293,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
           umma_f16_ts_el(d, a + ks * 8, b + ks * (2048 >> 4), id_o, ks > 0 || j > 0, el);
         umma_commit_el(&o_done[2 * tile + (j & 1)], el);
       };
-      const int tile = warp - 14;
+      const int tile = warp - (PW_SOFT + PW_LOADERS);
       const bool idle = tile == 1 && !two;
       bool ok = idle || (warp_wait(q_full, 0, abort_flag) && warp_wait(&k_full[0], 0, abort_flag));
       if (ok && !idle) {
@@ -325,7 +328,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
       }
     } else {
       // ---------------- loaders ----------------
-      const int lw = warp - 8;
+      const int lw = warp - PW_SOFT;
       const int64_t row_step = (int64_t)p.hkv * ROWB, plane_step = row_step * p.ps;
       const char* base = p.pool + (int64_t)kvh * ROWB;
       const int c = lane % CH, sub = lane / CH;
@@ -370,139 +373,128 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
         __syncwarp();
         if (lane == 0) mbar_arrive(bar);
       };
-      bool ok = true;
-      if constexpr (Q8) {
-        int4 ka[ITS], va[ITS];
-        auto load = [&](int4* buf, int64_t at, int64_t plane) {
+      // Codes land inside the place of their own row (in its last 128 bytes; where they are 64, odd
+      // tokens in the second 64: no bank twice) and are spread from there over the whole row by the
+      // warp that asked for them.
+      auto land = [&](char* tile, int tok) -> char* {
+        if constexpr (Q8)
+          return tile + (D / 64 - 1) * PW_HALF + tok * 128 + ((c + (CH == 4 ? (tok & 1) * 4 : 0)) << 4);
+        else
+          return dst_of(tile, tok, c);
+      };
+      auto copy = [&](char* tile, int64_t at, int64_t plane) {
 #pragma unroll
-          for (int it = 0; it < ITS; ++it) {
-            const int64_t o = __shfl_sync(0xffffffffu, at, it * TPI + sub);
-            buf[it] = o >= 0 ? ld_early16(base + o + plane + c * 16) : make_int4(0, 0, 0, 0);
+        for (int it = 0; it < ITS; ++it) {
+          const int64_t o = __shfl_sync(0xffffffffu, at, it * TPI + sub);
+          if (unit_of(it) < UNITS)
+            cp_async16(smem_u32(land(tile, unit_of(it) * TPI + sub)),
+                       o >= 0 ? base + o + plane + c * 16 : p.pool, o >= 0);
+        }
+        cp_commit();
+      };
+      // Rows have landed: codes to halves; values that are not finite out if `check`.
+      auto finish = [&](char* tile, bool check) -> bool {
+        bool bad = false;
+        if constexpr (Q8) {
+#pragma unroll 1
+          for (int it0 = 0; it0 < ITS; it0 += 2) {
+            int4 raw[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+              if (unit_of(it0 + u) < UNITS)
+                raw[u] = *reinterpret_cast<const int4*>(land(tile, unit_of(it0 + u) * TPI + sub));
+            __syncwarp();
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              if (unit_of(it0 + u) >= UNITS) break;
+              const uint32_t wd[4] = {(uint32_t)raw[u].x, (uint32_t)raw[u].y, (uint32_t)raw[u].z,
+                                      (uint32_t)raw[u].w};
+              uint32_t o[8];
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                o[2 * x] = e4m3x2_to_h2(wd[x] & 0xffffu);
+                o[2 * x + 1] = e4m3x2_to_h2(wd[x] >> 16);
+              }
+              if (check) {
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                  const uint32_t z = zero_not_finite<__half>(o[x]);
+                  bad |= z != o[x];
+                  o[x] = z;
+                }
+              }
+              const int tok = unit_of(it0 + u) * TPI + sub;
+              // the second half of the row's chunks stores its odd piece first: no bank twice
+              const int sw = c >= CH / 2 ? 1 : 0;
+              *reinterpret_cast<int4*>(dst_of(tile, tok, 2 * c + sw)) =
+                  sw ? make_int4(o[4], o[5], o[6], o[7]) : make_int4(o[0], o[1], o[2], o[3]);
+              *reinterpret_cast<int4*>(dst_of(tile, tok, 2 * c + 1 - sw)) =
+                  sw ? make_int4(o[0], o[1], o[2], o[3]) : make_int4(o[4], o[5], o[6], o[7]);
+            }
           }
-        };
-        auto store = [&](char* tile, const int4* buf, bool check) -> bool {
-          bool bad = false;
-#pragma unroll
+        } else if (check) {
+#pragma unroll 1
           for (int it = 0; it < ITS; ++it) {
             if (unit_of(it) >= UNITS) break;
-            const uint32_t wd[4] = {(uint32_t)buf[it].x, (uint32_t)buf[it].y, (uint32_t)buf[it].z,
-                                    (uint32_t)buf[it].w};
-            uint32_t o[8];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              o[2 * x] = e4m3x2_to_h2(wd[x] & 0xffffu);
-              o[2 * x + 1] = e4m3x2_to_h2(wd[x] >> 16);
+            int4* a = reinterpret_cast<int4*>(land(tile, unit_of(it) * TPI + sub));
+            const int4 x = *a;
+            const int4 z = make_int4(zero_not_finite<T>(x.x), zero_not_finite<T>(x.y),
+                                     zero_not_finite<T>(x.z), zero_not_finite<T>(x.w));
+            if (z.x != x.x || z.y != x.y || z.z != x.z || z.w != x.w) {
+              bad = true;
+              *a = z;
             }
-            if (check) {
-#pragma unroll
-              for (int x = 0; x < 8; ++x) {
-                const uint32_t z = zero_not_finite<__half>(o[x]);
-                bad |= z != o[x];
-                o[x] = z;
-              }
-            }
-            const int tok = unit_of(it) * TPI + sub;
-            // the second half of the row's chunks stores its odd piece first: no bank twice
-            const int sw = c >= CH / 2 ? 1 : 0;
-            *reinterpret_cast<int4*>(dst_of(tile, tok, 2 * c + sw)) =
-                sw ? make_int4(o[4], o[5], o[6], o[7]) : make_int4(o[0], o[1], o[2], o[3]);
-            *reinterpret_cast<int4*>(dst_of(tile, tok, 2 * c + 1 - sw)) =
-                sw ? make_int4(o[0], o[1], o[2], o[3]) : make_int4(o[4], o[5], o[6], o[7]);
           }
-          return bad;
-        };
-        float sk, sv;
-        int64_t at = locate(0, page_of(w.v_begin), sk, sv);
-        load(ka, at, 0);
-        int page_next = page_of(w.v_begin + PW_TOK);
+        }
+        return bad;
+      };
+      auto finish_v = [&](int i) {        // looked at where rows see the step in part
+        if (finish(smem + SM::V + (i & 1) * SM::TILE, !all_see(w.v_begin + i * PW_TOK, PW_TOK)))
+          odd[i & 1] = i + 1;
+        signal(&v_full[i & 1]);
+      };
+      bool ok = true;
+      float sk, sv;
+      int page_next = page_of(w.v_begin);
 #pragma unroll 1
-        for (int i = 0; i < steps; ++i) {
-          const int st = i & 1, v0 = w.v_begin + i * PW_TOK;
-          load(va, at, plane_step);
+      for (int i = 0; i < steps; ++i) {
+        const int st = i & 1;
+        const int64_t at = locate(i, page_next, sk, sv);
+        page_next = page_of(w.v_begin + (i + 1) * PW_TOK);
+        if (i >= 2) ok = warp_wait(&k_empty[st], ((i >> 1) - 1) & 1, abort_flag);
+        if (!ok) break;
+        copy(smem + SM::K + st * SM::TILE, at, 0);
+        if constexpr (Q8) {
           // scales of 0 (blocks never written) stand for values of 0: any will do; a token that is
           // not there gets an exponent of -inf
           const float svc = fmaxf(sv, 9.0949470177e-13f);         // 2^-40
-          const float4 entry = sv < 0.f ? make_float4(1.f, -INFINITY, 0.f, 0.f)
-                                        : make_float4(fmaxf(sk, 1e-30f), log2f(svc), 1.f / svc, 0.f);
-          if (i >= 2) ok = warp_wait(&k_empty[st], ((i >> 1) - 1) & 1, abort_flag);
-          if (!ok) break;
-          if (my) tab[(i & 3) * PW_TOK + my_tok] = entry;
-          store(smem + SM::K + st * SM::TILE, ka, false);
-          signal(&k_full[st]);
-          if (i + 1 < steps) {
-            at = locate(i + 1, page_next, sk, sv);
-            load(ka, at, 0);
-            page_next = page_of(v0 + 2 * PW_TOK);
-          }
-          if (i >= 2) ok = warp_wait(&v_empty[st], ((i >> 1) - 1) & 1, abort_flag);
-          if (!ok) break;
-          if (store(smem + SM::V + st * SM::TILE, va, !all_see(v0, PW_TOK))) odd[st] = i + 1;
-          signal(&v_full[st]);
+          if (my)
+            tab[(i & 3) * PW_TOK + my_tok] =
+                sv < 0.f ? make_float4(1.f, -INFINITY, 0.f, 0.f)
+                         : make_float4(fmaxf(sk, 1e-30f), log2f(svc), 1.f / svc, 0.f);
         }
-      } else {
-        auto copy = [&](char* tile, int64_t at, int64_t plane) {
-#pragma unroll
-          for (int it = 0; it < ITS; ++it) {
-            const int64_t o = __shfl_sync(0xffffffffu, at, it * TPI + sub);
-            if (unit_of(it) < UNITS)
-              cp_async16(smem_u32(dst_of(tile, unit_of(it) * TPI + sub, c)),
-                         o >= 0 ? base + o + plane + c * 16 : p.pool, o >= 0);
-          }
-          cp_commit();
-        };
-        auto finish_v = [&](int i) {  // V of step i has landed: look at it where rows see it in part
-          const int st = i & 1;
-          if (!all_see(w.v_begin + i * PW_TOK, PW_TOK)) {
-            bool bad = false;
-#pragma unroll 1
-            for (int it = 0; it < ITS; ++it) {
-              if (unit_of(it) >= UNITS) break;
-              int4* a = reinterpret_cast<int4*>(
-                  dst_of(smem + SM::V + st * SM::TILE, unit_of(it) * TPI + sub, c));
-              const int4 x = *a;
-              const int4 z = make_int4(zero_not_finite<T>(x.x), zero_not_finite<T>(x.y),
-                                       zero_not_finite<T>(x.z), zero_not_finite<T>(x.w));
-              if (z.x != x.x || z.y != x.y || z.z != x.z || z.w != x.w) {
-                bad = true;
-                *a = z;
-              }
-            }
-            if (bad) odd[st] = i + 1;
-          }
-          signal(&v_full[st]);
-        };
-        float sk, sv;
-        int page_next = page_of(w.v_begin);
-#pragma unroll 1
-        for (int i = 0; i < steps; ++i) {
-          const int st = i & 1;
-          const int64_t at = locate(i, page_next, sk, sv);
-          page_next = page_of(w.v_begin + (i + 1) * PW_TOK);
-          if (i >= 2) ok = warp_wait(&k_empty[st], ((i >> 1) - 1) & 1, abort_flag);
-          if (!ok) break;
-          copy(smem + SM::K + st * SM::TILE, at, 0);
-          if (i > 0) {
-            cp_wait<1>();
-            finish_v(i - 1);
-          }
-          // K goes out before V's stage is waited for: that one comes free with the step before last
-          cp_wait<0>();
-          signal(&k_full[st]);
-          if (i >= 2) ok = warp_wait(&v_empty[st], ((i >> 1) - 1) & 1, abort_flag);
-          if (!ok) break;
-          copy(smem + SM::V + st * SM::TILE, at, plane_step);
+        if (i > 0) {
+          cp_wait<1>();
+          finish_v(i - 1);
         }
+        // K goes out before V's stage is waited for: that one comes free with the step before last
         cp_wait<0>();
-        if (ok) finish_v(steps - 1);
+        finish(smem + SM::K + st * SM::TILE, false);
+        signal(&k_full[st]);
+        if (i >= 2) ok = warp_wait(&v_empty[st], ((i >> 1) - 1) & 1, abort_flag);
+        if (!ok) break;
+        copy(smem + SM::V + st * SM::TILE, at, plane_step);
       }
+      cp_wait<0>();
+      if (ok) finish_v(steps - 1);
       if (!ok) *abort_flag = 1;
     }
   } else {
     // ---------------- softmax: one row per thread ----------------
-    // ---- Q rows into shared memory, zeros past the item's rows (8 loads in flight per thread; one
+    // ---- Q rows into shared memory, zeros past the item's rows (loads in flight together; one
     // at a time they took 9 us of a CTA's 42 at 18 halves) ----
     {
-      constexpr int QC = D / 8, QR = 256 / QC, QB = 8;         // chunks per row, rows at once
+      constexpr int QC = D / 8, QR = PW_SOFT * 32 / QC, QB = 4;   // chunks per row, rows at once
       // the sign of sm_scale goes into Q, so that the largest score is the largest product
       const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
       const int c = tid % QC;
@@ -553,9 +545,12 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
-      asm volatile("bar.sync 1, 256;" ::: "memory");           // the rows' scales, among these 8 warps
+      for (int k = tid; k < 256 * 2 * (D / 32); k += PW_SOFT * 32) odd_mask[k] = 0;
+      asm volatile("bar.sync 1, 512;" ::: "memory");           // the rows' scales and masks
+      static_assert(PW_SOFT * 32 == 512, "barrier count");
     }
-    const int tile = warp >> 2, row = tid;                 // rows 0..255 of the item
+    // rows 0..255 of the item; this thread's scores: tokens [32 part, + 32) of a half
+    const int tile = warp >> 3, part = (warp >> 2) & 1, row = tile * 128 + (warp & 3) * 32 + lane;
     if (tile == 0 || two) {
       const uint32_t quad = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t t_s = tmem + tile * 128 + quad, t_o = tmem + 256 + tile * D + quad;
@@ -563,101 +558,87 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
       // factors of scores are never 0: a masked score of -inf stays -inf
       constexpr float kLeast = 1e-37f;
       const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f) * (Q8 ? row_scale[row] : 1.f);
-      // groups of 8 tokens lie in one page
-      const bool grouped = p.ps % 8 == 0 && w.v_begin % 8 == 0 &&
-                           (w.shift == 0 || (w.n0 % 8 == 0 && w.shift % 8 == 0));
+      // groups of 8 tokens lie in one page, or scales go token by token
+      const bool by_token = Q8 && !( p.ps % 8 == 0 && w.v_begin % 8 == 0 &&
+                           (w.shift == 0 || (w.n0 % 8 == 0 && w.shift % 8 == 0)));
       // what the row sees, in v: v <= vc and (v < sink_end or v >= vw); with a gap, v >= n0 is t - shift
       const int vc = !causal ? INT_MAX - 1 : w.shift == 0 ? pos : pos >= w.n0 + w.shift
                                                     ? pos - w.shift : min(pos, w.n0 - 1);
       const int vw = !window ? INT_MIN : w.shift == 0 ? pos - w.window
                                                       : max(pos - w.window - w.shift, w.n0);
       float m = kNoMax, l = 0.f;
-      bool ok = true, marked = false;
+      // A wait that ran out is told to the row tile's other warps at the barrier of a half, so that all
+      // leave their loop at the same place.
+      bool fail = false;
 #pragma unroll 1
       for (int j = 0; j < halves; ++j) {
-        const int i = j >> 1, v0 = w.v_begin + j * 64;         // step and first token of the half
+        const int i = j >> 1, v0 = w.v_begin + j * 64 + part * 32;      // step; this thread's tokens
         const uint32_t t_p = t_s + (j & 1) * 64;
-        ok = warp_wait(&s_full[2 * tile + (j & 1)], i & 1, abort_flag);
-        if (!ok) break;
+        fail = fail || !warp_wait(&s_full[2 * tile + (j & 1)], i & 1, abort_flag);
         tc_fence_after();
-        uint32_t x[64];
-        const bool by_token = Q8 && !grouped;
-        if (!by_token) {
-          tmem_ld32_nw(t_p, x);
-          tmem_ld32_nw(t_p + 32, x + 32);
-        }
-        const float4* tb = tab + (i & 3) * PW_TOK + (j & 1) * 64;
-        const bool missing = !Q8 && gone[i & 3] == i + 1, cut = !all_see(v0, 64) || missing;
-        uint32_t see[2] = {};
+        uint32_t x[32];
+        tmem_ld32_nw(t_p + part * 32, x);
+        const float4* tb = tab + (i & 3) * PW_TOK + (j & 1) * 64 + part * 32;
+        const bool missing = !Q8 && gone[i & 3] == i + 1, cut = !all_see(v0, 32) || missing;
+        uint32_t see = ~0u;
         if (cut) {
-          const int kc = min(vc >= v0 + 64 ? 64 : vc - v0 + 1, w.v_end - v0);
-          const int ks = min(w.sink_end - v0, 64), kw = vw <= v0 ? 0 : min(vw - v0, 64);
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-            see[k] = low_bits(kc, k) & (low_bits(ks, k) | ~low_bits(kw, k));
+          const int kc = min(vc >= v0 + 32 ? 32 : vc - v0 + 1, w.v_end - v0);
+          const int ks = min(w.sink_end - v0, 32), kw = vw <= v0 ? 0 : min(vw - v0, 32);
+          see = low_bits(kc) & (low_bits(ks) | ~low_bits(kw));
           if (missing)                               // a page id out of range: its tokens drop out
 #pragma unroll 1
-            for (int k = 0; k < min(64, w.v_end - v0); ++k) {
+            for (int k = 0; k < min(32, w.v_end - v0); ++k) {
               const int v = v0 + k, t = v + (v >= w.n0 ? w.shift : 0);
               const int page = kvlist[t / p.ps];
-              if (page < 0 || page >= p.num_pages) {
-                const uint32_t bit = ~(1u << (k & 31));
-                if (k < 32) see[0] &= bit;
-                else see[1] &= bit;
-              }
+              if (page < 0 || page >= p.num_pages) see &= ~(1u << k);
             }
         }
-        float mx = -INFINITY;
-        if (by_token) {
-#pragma unroll 1
-          for (int c0 = 0; c0 < 64; c0 += 8) {
-            tmem_ld8_nw(t_p + c0, x);
-            tmem_wait();
-            const uint32_t bits = cut ? (c0 < 32 ? see[0] : see[1]) >> (c0 & 31) : 0xffu;
+        tmem_wait();
+        if (cut) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              if ((bits >> k) & 1)
-                mx = fmaxf(mx, fmaf(__uint_as_float(x[k]), fmaxf(tb[c0 + k].x * scale, kLeast), tb[c0 + k].y));
+          for (int k = 0; k < 32; ++k) x[k] = (see >> k) & 1 ? x[k] : 0xff800000u;             // -inf
+        }
+        float mx;
+        if (by_token) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            x[k] = __float_as_uint(fmaf(__uint_as_float(x[k]), fmaxf(tb[k].x * scale, kLeast), tb[k].y));
+        }
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (Q8 && !by_token) {
+#pragma unroll
+          for (int k = 0; k < 32; k += 8) {
+            float y[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) y[u] = __uint_as_float(x[k + u]);
+            const float gm = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])),
+                                   fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
+            m4[k >> 3] = fmaf(gm, fmaxf(tb[k].x * scale, kLeast), tb[k].y);
           }
         } else {
-          tmem_wait();
-          if (cut) {
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              x[k] = (see[0] >> k) & 1 ? x[k] : 0xff800000u;             // -inf
-              x[32 + k] = (see[1] >> k) & 1 ? x[32 + k] : 0xff800000u;
-            }
-          }
-          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          for (int k = 0; k < 32; k += 8)
 #pragma unroll
-          for (int k = 0; k < 64; k += 8) {
-            if constexpr (Q8) {
-              float y[8];
-#pragma unroll
-              for (int u = 0; u < 8; ++u) y[u] = __uint_as_float(x[k + u]);
-              const float gm = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])),
-                                     fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
-              const float4 e = tb[k];
-              m4[(k >> 3) & 3] = fmaxf(m4[(k >> 3) & 3], fmaf(gm, fmaxf(e.x * scale, kLeast), e.y));
-            } else {
-#pragma unroll
-              for (int u = 0; u < 4; ++u)
-                m4[u] = fmaxf(fmaxf(m4[u], __uint_as_float(x[k + u])), __uint_as_float(x[k + 4 + u]));
-            }
-          }
-          mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-          if (!Q8) mx *= scale;
+            for (int u = 0; u < 4; ++u)
+              m4[u] = fmaxf(fmaxf(m4[u], __uint_as_float(x[k + u])), __uint_as_float(x[k + 4 + u]));
         }
-        if (__any_sync(0xffffffffu, mx > m + kLazyMax)) {
-          const float to = fmaxf(m, mx), f = ex2(m - to);
+        mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        if (!Q8) mx *= scale;
+        // also: from here on every score of the tile is in registers, P may be written
+        if (vote256(2 + tile, mx > m + kLazyMax || fail)) {
+          meet[part * 256 + row] = mx;
+          if (vote256(2 + tile, fail)) {
+            fail = true;
+            break;
+          }
+          const float to = fmaxf(m, fmaxf(mx, meet[(part ^ 1) * 256 + row])), f = ex2(m - to);
           m = to;
           l *= f;
-          if (j > 0) {        // O of the halves before: complete, then rescaled
-            ok = warp_wait(&o_done[2 * tile + ((j - 1) & 1)], ((j - 1) >> 1) & 1, abort_flag);
-            if (!ok) break;
+          if (j > 0) {        // O of the halves before: complete, then rescaled, half the dims per thread
+            fail = !warp_wait(&o_done[2 * tile + ((j - 1) & 1)], ((j - 1) >> 1) & 1, abort_flag);
             tc_fence_after();
 #pragma unroll 1
-            for (int c0 = 0; c0 < D; c0 += 16) {
+            for (int c0 = part * (D / 2); c0 < (part + 1) * (D / 2); c0 += 16) {
               uint32_t y[16];
               tmem_ld16_nw(t_o + c0, y);
               tmem_wait();
@@ -665,64 +646,47 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
               for (int k = 0; k < 16; ++k) y[k] = __float_as_uint(__uint_as_float(y[k]) * f);
               tmem_st16(t_o + c0, y);
             }
-            tmem_wait_st();
           }
         }
         // ---- P over S ----
+        uint32_t pk[16];
         if (by_token) {
-#pragma unroll 1
-          for (int c0 = 0; c0 < 64; c0 += 8) {
-            tmem_ld8_nw(t_p + c0, x);
-            tmem_wait();
-            const uint32_t bits = cut ? (c0 < 32 ? see[0] : see[1]) >> (c0 & 31) : 0xffu;
-            uint32_t pk[4];
 #pragma unroll
-            for (int k = 0; k < 8; k += 2) {
-              const float4 e = tb[c0 + k], f = tb[c0 + k + 1];
-              float a = ex2(fmaf(__uint_as_float(x[k]), fmaxf(e.x * scale, kLeast), e.y) - m);
-              float b = ex2(fmaf(__uint_as_float(x[k + 1]), fmaxf(f.x * scale, kLeast), f.y) - m);
-              a = (bits >> k) & 1 ? a : 0.f;
-              b = (bits >> k) & 2 ? b : 0.f;
-              l = fmaf(a, e.z, fmaf(b, f.z, l));
-              pk[k >> 1] = pack2<MT>(a, b);
-            }
-            tmem_st4(t_p + c0 / 2, pk);
+          for (int k = 0; k < 32; k += 2) {
+            const float a = ex2(__uint_as_float(x[k]) - m), b = ex2(__uint_as_float(x[k + 1]) - m);
+            l = fmaf(a, tb[k].z, fmaf(b, tb[k + 1].z, l));
+            pk[k >> 1] = pack2<MT>(a, b);
           }
         } else {
           const uint64_t s2 = f2_pack(scale, scale), m2 = f2_pack(-m, -m);
           uint64_t sum[2] = {0, 0};
 #pragma unroll
-          for (int c0 = 0; c0 < 64; c0 += 32) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int k0 = c0; k0 < c0 + 32; k0 += 8) {
-              uint64_t gs = s2, gm = m2;
-              float inv = 1.f;
-              if constexpr (Q8) {
-                const float4 e = tb[k0];
-                const float both = fmaxf(e.x * scale, kLeast);
-                gs = f2_pack(both, both);
-                gm = f2_pack(e.y - m, e.y - m);
-                inv = e.z;
-                sum[0] = sum[1] = 0;
-              }
-#pragma unroll
-              for (int k = k0; k < k0 + 8; k += 2) {
-                const uint64_t y = f2_pack(__uint_as_float(x[k]), __uint_as_float(x[k + 1]));
-                float a, b;
-                f2_unpack(f2_fma(y, gs, gm), a, b);
-                a = ex2(a);
-                b = ex2(b);
-                sum[(k >> 1) & 1] = f2_add(sum[(k >> 1) & 1], f2_pack(a, b));
-                pk[(k - c0) >> 1] = pack2<MT>(a, b);
-              }
-              if constexpr (Q8) {
-                float a, b;
-                f2_unpack(f2_add(sum[0], sum[1]), a, b);
-                l = fmaf(a + b, inv, l);
-              }
+          for (int k0 = 0; k0 < 32; k0 += 8) {
+            uint64_t gs = s2, gm = m2;
+            float inv = 1.f;
+            if constexpr (Q8) {
+              const float4 e = tb[k0];
+              const float both = fmaxf(e.x * scale, kLeast);
+              gs = f2_pack(both, both);
+              gm = f2_pack(e.y - m, e.y - m);
+              inv = e.z;
+              sum[0] = sum[1] = 0;
             }
-            tmem_st16(t_p + c0 / 2, pk);
+#pragma unroll
+            for (int k = k0; k < k0 + 8; k += 2) {
+              const uint64_t y = f2_pack(__uint_as_float(x[k]), __uint_as_float(x[k + 1]));
+              float a, b;
+              f2_unpack(f2_fma(y, gs, gm), a, b);
+              a = ex2(a);
+              b = ex2(b);
+              sum[(k >> 1) & 1] = f2_add(sum[(k >> 1) & 1], f2_pack(a, b));
+              pk[k >> 1] = pack2<MT>(a, b);
+            }
+            if constexpr (Q8) {
+              float a, b;
+              f2_unpack(f2_add(sum[0], sum[1]), a, b);
+              l = fmaf(a + b, inv, l);
+            }
           }
           if constexpr (!Q8) {
             float a, b;
@@ -730,19 +694,16 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
             l += a + b;
           }
         }
+        tmem_st16(t_p + part * 16, pk);
         tmem_wait_st();
         if (!all_see(w.v_begin + i * PW_TOK, PW_TOK)) {
           // values that are not finite, taken out of V: mark the dims of the rows that see them
           // (before P is handed over: V's stage and its flag stay until P V of this half is done)
-          ok = warp_wait(&v_full[i & 1], (i >> 1) & 1, abort_flag);
-          if (!ok) break;
+          fail = fail || !warp_wait(&v_full[i & 1], (i >> 1) & 1, abort_flag);
           if (odd[i & 1] == i + 1) {
             uint32_t* mask = odd_mask + row * (2 * (D / 32));
-            if (!marked)
-              for (int k = 0; k < 2 * (D / 32); ++k) mask[k] = 0;
-            marked = true;
 #pragma unroll 1
-            for (int k = 0; row < rows && k < min(64, w.v_end - v0); ++k) {
+            for (int k = 0; row < rows && k < min(32, w.v_end - v0); ++k) {
               const int v = v0 + k, t = v + (v >= w.n0 ? w.shift : 0);
               const int page = kvlist[t / p.ps];
               if (page < 0 || page >= p.num_pages || (causal && t > pos) ||
@@ -759,9 +720,10 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
                 } else {
                   val = to_f(reinterpret_cast<const T*>(src)[d]);
                 }
-                if (!(val < INFINITY)) mask[d >> 5] |= 1u << (d & 31);
-                if (!(val > -INFINITY)) mask[D / 32 + (d >> 5)] |= 1u << (d & 31);
+                if (!(val < INFINITY)) atomicOr(&mask[d >> 5], 1u << (d & 31));
+                if (!(val > -INFINITY)) atomicOr(&mask[D / 32 + (d >> 5)], 1u << (d & 31));
               }
+              *marked = 1;
             }
           }
         }
@@ -769,66 +731,68 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[2 * tile + (j & 1)]);
       }
-      // ---- epilogue ----
-      if (ok) ok = warp_wait(&o_done[2 * tile + ((halves - 1) & 1)], ((halves - 1) >> 1) & 1, abort_flag);
-      if (ok) {
+      // ---- epilogue: half the dims per thread ----
+      fail = fail || !warp_wait(&o_done[2 * tile + ((halves - 1) & 1)], ((halves - 1) >> 1) & 1, abort_flag);
+      meet[part * 256 + row] = l;
+      if (!vote256(2 + tile, fail)) {
         tc_fence_after();
+        l += meet[(part ^ 1) * 256 + row];
         const float inv = l != 0.f ? 1.f / l : 0.f;
-        const int qi = query_of(row), head = kvh * g + row - qi * g;
-        const int64_t dst_q = w.part_base < 0 ? w.q_begin + qi : w.part_base + qi;
-        // through this tile's Q rows (its last product has read them) so that rows leave in whole lines
-        char* mine = smem + SM::Q + tile * SM::TILE + (warp & 3) * 32 * (D * 2);
-        constexpr int RB = D * 2;                              // bytes per row here: D results or D / 2 partials
-        const bool part = w.part_base >= 0;
+        const bool partial = w.part_base >= 0;
+        // through this tile's Q rows (its last product has read them) so that rows leave in whole lines:
+        // D / 4 dims of fp32 partials or D / 2 of results at a time, in 4 D bytes per warp and row pair
+        constexpr int HD = D / 2, RB = HD * 2;                 // this thread's dims; bytes per row here
+        char* mine = smem + SM::Q + tile * SM::TILE + (warp & 7) * 32 * RB;
+        constexpr int RC = RB / 16;                            // chunks per row: 8 or 4
 #pragma unroll 1
-        for (int h = 0; h < (part ? 2 : 1); ++h) {
-          const int d0 = part ? h * (D / 2) : 0, d1 = part ? d0 + D / 2 : D;
+        for (int h = 0; h < (partial ? 2 : 1); ++h) {
+          const int d0 = part * HD + (partial ? h * (HD / 2) : 0), nd = partial ? HD / 2 : HD;
 #pragma unroll 1
-          for (int c0 = d0; c0 < d1; c0 += 32) {
-            uint32_t u[32];
-            tmem_ld32_nw(t_o + c0, u);
+          for (int c0 = 0; c0 < nd; c0 += 16) {
+            uint32_t u[16];
+            tmem_ld16_nw(t_o + d0 + c0, u);
             tmem_wait();
-            float f[32];
+            float f[16];
 #pragma unroll
-            for (int k = 0; k < 32; ++k) f[k] = l != 0.f ? __uint_as_float(u[k]) * inv : 0.f;
-            if (marked) {
-              const uint32_t up = odd_mask[row * (2 * (D / 32)) + (c0 >> 5)];
-              const uint32_t dn = odd_mask[row * (2 * (D / 32)) + D / 32 + (c0 >> 5)];
-              if (up | dn)
-#pragma unroll 4
-                for (int k = 0; k < 32; ++k) {
-                  if ((up >> k) & 1) f[k] += INFINITY;
-                  if ((dn >> k) & 1) f[k] -= INFINITY;
-                }
+            for (int k = 0; k < 16; ++k) f[k] = l != 0.f ? __uint_as_float(u[k]) * inv : 0.f;
+            if (*marked) {
+              const int d = d0 + c0;
+              const uint32_t up = odd_mask[row * (2 * (D / 32)) + (d >> 5)] >> (d & 31);
+              const uint32_t dn = odd_mask[row * (2 * (D / 32)) + D / 32 + (d >> 5)] >> (d & 31);
+#pragma unroll
+              for (int k = 0; k < 16; ++k) {
+                if ((up >> k) & 1) f[k] += INFINITY;
+                if ((dn >> k) & 1) f[k] -= INFINITY;
+              }
             }
             // 16-byte chunks, turned by the row so that neither side meets a bank twice
-            if (part) {
+            if (partial) {
 #pragma unroll
-              for (int k = 0; k < 8; ++k)
-                *reinterpret_cast<float4*>(mine + lane * RB + ((((c0 - d0) / 4 + k) ^ (lane & 7)) << 4)) =
+              for (int k = 0; k < 4; ++k)
+                *reinterpret_cast<float4*>(mine + lane * RB + (((c0 / 4 + k) ^ (lane & (RC - 1))) << 4)) =
                     make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
             } else {
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                *reinterpret_cast<uint4*>(mine + lane * RB + (((c0 / 8 + k) ^ (lane & 7)) << 4)) =
+              for (int k = 0; k < 2; ++k)
+                *reinterpret_cast<uint4*>(mine + lane * RB + (((c0 / 8 + k) ^ (lane & (RC - 1))) << 4)) =
                     make_uint4(pack2<T>(f[8 * k], f[8 * k + 1]), pack2<T>(f[8 * k + 2], f[8 * k + 3]),
                                pack2<T>(f[8 * k + 4], f[8 * k + 5]), pack2<T>(f[8 * k + 6], f[8 * k + 7]));
             }
           }
           __syncwarp();
-          constexpr int RC = RB / 16;                          // chunks per row
-#pragma unroll 2
-          for (int x = lane; x < 32 * RC; x += 32) {
-            const int rr = x / RC, ch = x % RC, ir = tile * 128 + (warp & 3) * 32 + rr;
+#pragma unroll
+          for (int k = 0; k < RC; ++k) {
+            const int at = lane + 32 * k, rr = at / RC, ch = at % RC;
+            const int ir = tile * 128 + (warp & 3) * 32 + rr;
             if (ir >= rows) continue;
-            const uint4 val = *reinterpret_cast<const uint4*>(mine + rr * RB + ((ch ^ (rr & 7)) << 4));
+            const uint4 val = *reinterpret_cast<const uint4*>(mine + rr * RB + ((ch ^ (rr & (RC - 1))) << 4));
             const int iq = query_of(ir), ih = kvh * g + ir - iq * g;
-            if (part)
+            if (partial)
               *reinterpret_cast<uint4*>(p.mid_o + ((int64_t)(w.part_base + iq) * p.hq + ih) * D + d0 +
                                         ch * 4) = val;
             else {
               T* dst = reinterpret_cast<T*>(p.out) + (int64_t)(w.q_begin + iq) * p.out_row_stride +
-                       (int64_t)ih * D + ch * 8;
+                       (int64_t)ih * D + d0 + ch * 8;
               if (p.out_vec16) *reinterpret_cast<uint4*>(dst) = val;
               else {
                 reinterpret_cast<uint2*>(dst)[0] = make_uint2(val.x, val.y);
@@ -838,9 +802,11 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
           }
           __syncwarp();
         }
-        if (row < rows) {
+        if (row < rows && part == 0) {
+          const int qi = query_of(row), head = kvh * g + row - qi * g;
+          const int64_t dst_q = partial ? w.part_base + qi : w.q_begin + qi;
           const float lse = l > 0.f ? (m + log2f(l)) * kLn2 : l == 0.f ? -INFINITY : l;
-          if (w.part_base >= 0)     // NaN as +inf: see the narrow kernel
+          if (partial)     // NaN as +inf: see the narrow kernel
             p.mid_lse[dst_q * p.hq + head] = l >= 0.f ? lse : INFINITY;
           else if (p.lse)
             p.lse[dst_q * p.hq + head] = lse;
