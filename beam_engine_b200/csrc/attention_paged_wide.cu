@@ -4,9 +4,10 @@
 // One CTA = one item of be_paged_plan x one KV head: two row tiles of 128 (row r of the
 // item is query r / g, head r % g, so a KV head's tokens are loaded once for its g
 // query heads) against steps of 128 tokens, in one pass with a running maximum:
-//   * loader warps (6): tokens' rows from global memory into the canonical 128-byte
-//     swizzle, 16-bit rows by cp.async, 8-bit codes through registers; tokens are addressed one
-//     by one, so any page size and the joint of sinks and window cost nothing;
+//   * loader warps (4; with 8 the registers of the softmax run short, 8-bit prompts 4 % slower): tokens'
+//     rows by cp.async into the canonical 128-byte swizzle, 8-bit codes into the place of
+//     their own row, where the same warp spreads them into halves; tokens are addressed one by
+//     one, so any page size and the joint of sinks and window cost nothing;
 //   * a warp per row tile issues S = Q K^T (128 x 64 x D) into TMEM and O += P V (128 x D x 64) with
 //     P read from TMEM, in halves of a step (one warp for both tiles spent 2 560 clocks a half, most
 //     of them between its own waits): a row tile has two buffers of S, so the scores of the next
@@ -14,22 +15,26 @@
 //     left the softmax waiting for P V and S of its own tile, 1 560 of 4 270 clocks a step;
 //     128 x 64 x 16 takes 49 clocks instead of 32, bound by shared memory, 128 x 128 x 16 takes 65.)
 //   * softmax warps (8 per row tile, two threads per row with 32 scores of a half each): scores from
-//     TMEM to registers, maximum, P written over S; O is rescaled only when a row's maximum
-//     grows by more than 2^8, so the two threads of a row only agree that it did not (a barrier
-//     with a vote); their sums meet at the end.  One thread per row left a third of the issue slots used
-//     (two softmax warps per scheduler, each a chain of dependent steps).  The loops stay
-//     short because 24 warps in three roles share the instruction cache: with 128 scores per
-//     pass and every variant unrolled, fetching instructions took half of each step.
+//     TMEM to registers, maximum, P written over the thread's own scores; P of a half goes out
+//     while the next scores come in.  O is rescaled only when a row's maximum grows by more than
+//     2^8, so the two threads of a row only agree that it did not (a barrier of their two
+//     warps, with a vote); their sums meet at the end.  One thread per row left a third of the
+//     issue slots used, two softmax warps per scheduler in a chain of dependent steps.
+//     The loops stay short because 22 warps in three roles share the instruction cache: with 128
+//     scores per pass and every variant unrolled, fetching instructions took half of each step.
 // TMEM: S/P of tile 0 (two buffers of 64) | of tile 1 | O of tile 0 | O of tile 1 = 256 + 2 D columns
 // (512 allocated).  S of half j + 2 overwrites P of half j: both products come from one thread,
 // and the tensor core runs them in the order of issue.
 //
 // 8-bit caches: as in the narrow kernel the codes become halves by one exact conversion and
 // the scales stay out of the products.  x = s_K (q . c) and log2 s_V joins the exponent, so a group of
-// 8 tokens of one page costs one shared-memory read and three operations per row; scaling
-// the codes themselves on the way to shared memory was 3 times the loaders' work
-// (8 000 clocks a step against 4 600 for a 16-bit cache).  The planner aligns ranges to 8 tokens; pages
-// that are no multiple of 8 take scales token by token.
+// 8 tokens of one page costs one shared-memory read and three operations per row.  The
+// planner aligns ranges to 8 tokens; pages that are no multiple of 8 take scales token by token.
+//
+// Measured: bf16, 8192 tokens, 32 heads on 8, window 1024 + 4: 229 us, 565 TFLOP/s; 8-bit cache, a
+// prompt of 4096 tokens, causal: 209 us, 657 TFLOP/s.  A half takes 2 500 clocks per CTA against
+// 1 280 of the tensor core and 1 024 of the exponentials: the rest is the latency of the softmax's steps
+// (scores out of TMEM 500, exponentials 1 100 while four warps share a scheduler's unit).
 //
 // Values that are not finite: 0 * NaN is NaN in the product, so in steps that some row
 // sees in part the loaders replace them by 0 and the rows that see them mark
@@ -44,9 +49,8 @@
 namespace be {
 
 constexpr int PW_TOK = 128;                    // tokens per step
-constexpr int PW_LOADERS = 6;
-constexpr int PW_SOFT = 16;                    // softmax warps
-constexpr int PW_THREADS = (PW_SOFT + PW_LOADERS + 2) * 32;   // and 2 issuers
+constexpr int PW_SOFT = 16, PW_LOADERS = 4;    // softmax warps, loader warps; and 2 issuers
+constexpr int PW_THREADS = (PW_SOFT + PW_LOADERS + 2) * 32;
 constexpr int PW_HALF = PW_TOK * 128;          // 64 dims of 128 rows
 constexpr int PW_STAGES = 2;
 
@@ -129,13 +133,14 @@ __device__ __forceinline__ uint32_t low_bits(int n) {         // bits [0, n), n 
   const int k = min(max(n, 0), 32);
   return k == 32 ? ~0u : (1u << k) - 1u;
 }
-// Barrier `id` of 256 threads; whether `p` held in one of them.
-__device__ __forceinline__ bool vote256(int id, bool p) {
+// Barrier `id` of N threads; whether `p` held in one of them.
+template <int N>
+__device__ __forceinline__ bool vote(int id, bool p) {
   uint32_t r;
   asm volatile(
       "{\n .reg .pred p, q;\n setp.ne.u32 p, %2, 0;\n"
-      " barrier.cta.red.or.pred q, %1, 256, p;\n selp.u32 %0, 1, 0, q;\n}\n"
-      : "=r"(r) : "r"(id), "r"((uint32_t)p) : "memory");
+      " barrier.cta.red.or.pred q, %1, %3, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(r) : "r"(id), "r"((uint32_t)p), "n"(N) : "memory");
   return r != 0;
 }
 
@@ -159,14 +164,37 @@ __device__ __forceinline__ uint32_t zero_not_finite(uint32_t w) {
 }
 
 // The slow half of a wait, out of line: it would be inlined a dozen times into code that has to fit the
-// instruction caches.
-__device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity); }
+// instruction caches.  The warp sleeps in hardware, up to 20 us at a time: polls without a
+// hint come back after some ten clocks, and 24 waiting warps' polls took half of all issue slots.
+__device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity) {
+  uint64_t t0 = 0;
+  for (uint32_t n = 1;; ++n) {
+    if (mbar_try_sleep(bar, parity, 20000)) return true;
+    if ((n & 15) == 0) {
+      const uint64_t t = gtimer();
+      if (t0 == 0) {
+        t0 = t;
+      } else if (t - t0 > kWaitNs) {
+        atomicCAS(&g_device_status, 0, BE_EDEVICE_TIMEOUT);
+        return false;
+      }
+    }
+  }
+}
 
 // Bounded wait of a whole warp: every lane sees the phase, and all agree on the outcome.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
   const bool ok = !*abort_flag && wait_on(bar, parity);
   return __all_sync(0xffffffffu, ok);
+}
+
+// The same for N threads: one warp polls (`leads`), the others sleep at barrier `id`.
+template <int N>
+__device__ __forceinline__ bool group_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int id,
+                                           bool leads) {
+  const bool fail = leads && !warp_wait(bar, parity, abort_flag);
+  return !vote<N>(id, fail);
 }
 
 template <typename T, typename CT, int D>
@@ -178,11 +206,12 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
   constexpr int CH = ROWB / 16;                 // 16-byte chunks per (token, head) row: 4, 8 or 16
   constexpr int TPI = 32 / CH;                  // tokens per warp and load instruction
   constexpr int UNITS = PW_TOK / TPI;           // such instructions per step, dealt to the warps
-  constexpr int ITS = (UNITS + PW_LOADERS - 1) / PW_LOADERS;
+  constexpr int NL = PW_LOADERS, ITS = UNITS / NL;
+  static_assert(UNITS % NL == 0 && NL * TPI % 8 == 0, "a lane's tokens are the same mod 8");
   static_assert(ITS * TPI <= 32, "a lane locates one token");
   extern __shared__ char smem_raw[];
-  char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                       ~uintptr_t(1023));
+  // (aligned by an offset, so that the compiler still knows it for shared memory)
+  char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SM::BAR);
   uint64_t* k_full = bars;                      // [2], the loader warps
   uint64_t* v_full = bars + 2;                  // [2]
@@ -223,19 +252,24 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
   const int steps = (w.v_end - w.v_begin + PW_TOK - 1) / PW_TOK;
   const int halves = (w.v_end - w.v_begin + PW_TOK / 2 - 1) / (PW_TOK / 2);
   const bool causal = (w.flags & BE_ITEM_CAUSAL) != 0, window = w.window >= 0;
-  const int pos_hi = w.pos0 + w.pos_step * (w.q_len - 1);
+  // the last v that a row at `pos` sees, the first past its sinks; with a gap, v >= n0 is t - shift
+  auto last_of = [&](int pos) {
+    return !causal ? INT_MAX - 1 : w.shift == 0 ? pos : pos >= w.n0 + w.shift ? pos - w.shift : min(pos, w.n0 - 1);
+  };
+  auto first_of = [&](int pos) {
+    return !window ? INT_MIN : w.shift == 0 ? pos - w.window : max(pos - w.window - w.shift, w.n0);
+  };
   // whether every row sees every one of the n tokens from v0 (page ids apart)
+  const int see_end = min(w.v_end, last_of(w.pos0) + 1);
+  const int see_from = first_of(w.pos0 + w.pos_step * (w.q_len - 1));
   auto all_see = [&](int v0, int n) {
-    const int t_lo = v0 + (v0 >= w.n0 ? w.shift : 0);
-    const int v1 = v0 + n - 1, t_hi = v1 + (v1 >= w.n0 ? w.shift : 0);
-    return v1 < w.v_end && (!causal || t_hi <= w.pos0) &&
-           (!window || t_lo >= pos_hi - w.window || t_hi < w.sink_end);
+    return v0 + n <= see_end && (v0 >= see_from || v0 + n <= w.sink_end);
   };
 
   if (tid == 0) {
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&k_full[s], PW_LOADERS);
-      mbar_init(&v_full[s], PW_LOADERS);
+      mbar_init(&k_full[s], NL);
+      mbar_init(&v_full[s], NL);
       mbar_init(&k_empty[s], two ? 2 : 1);      // a commit per row tile
       mbar_init(&v_empty[s], two ? 2 : 1);
       for (int h = 0; h < 2; ++h) {
@@ -264,7 +298,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
   const uint32_t tmem = *tmem_slot;
 
   if (warp >= PW_SOFT) {
-    if (warp >= PW_SOFT + PW_LOADERS) {
+    if (warp >= PW_SOFT + NL) {
       // ---------------- issuers: a warp for each row tile ----------------
       // The whole warp walks the steps and one elected lane issues: addresses and descriptors
       // then stay in uniform registers (from a divergent lane every product first moves them there)
@@ -290,10 +324,10 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
         const uint32_t d = tmem + 256 + tile * D, a = tmem + tile * 128 + (j & 1) * 64;
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
-          umma_f16_ts_el(d, a + ks * 8, b + ks * (2048 >> 4), id_o, ks > 0 || j > 0, el);
+          umma_f16_ts_el(d, a + (ks >> 1) * 32 + (ks & 1) * 8, b + ks * (2048 >> 4), id_o, ks > 0 || j > 0, el);
         umma_commit_el(&o_done[2 * tile + (j & 1)], el);
       };
-      const int tile = warp - (PW_SOFT + PW_LOADERS);
+      const int tile = warp - (PW_SOFT + NL);
       const bool idle = tile == 1 && !two;
       bool ok = idle || (warp_wait(q_full, 0, abort_flag) && warp_wait(&k_full[0], 0, abort_flag));
       if (ok && !idle) {
@@ -329,13 +363,15 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
     } else {
       // ---------------- loaders ----------------
       const int lw = warp - PW_SOFT;
-      const int64_t row_step = (int64_t)p.hkv * ROWB, plane_step = row_step * p.ps;
+      const uint32_t plane = (uint32_t)p.hkv * p.ps;        // rows of ROWB bytes (2^32 of them: 256 GB)
       const char* base = p.pool + (int64_t)kvh * ROWB;
-      const int c = lane % CH, sub = lane / CH;
-      // load instruction `it` of this warp takes tokens [unit * TPI, + TPI), unit = lw + 6 it;
+      // Lane: 16-byte chunk c of token `sub`.  Where a row has 8 chunks of codes, the upper 4 lie with the
+      // neighbouring token: 8 lanes then store halves without meeting a bank twice.
+      const int c = lane % CH, sub = Q8 && CH == 8 ? (lane / CH) ^ (c >> 2) : lane / CH;
+      // load instruction `it` of this warp takes tokens [unit * TPI, + TPI), unit = lw + NL it;
       // lane L locates the token that instruction L / TPI loads in place L % TPI
-      auto unit_of = [&](int it) { return lw + PW_LOADERS * it; };
-      const int my_tok = unit_of(lane / TPI) * TPI + lane % TPI;
+      const int my_tok = (lw + NL * (lane / TPI)) * TPI + lane % TPI;
+      const int tok0 = lw * TPI + sub;              // this lane's tokens: tok0 + NL TPI it
       const bool my = lane < ITS * TPI && my_tok < PW_TOK;
       const int ps_shift = (p.ps & (p.ps - 1)) == 0 ? __ffs(p.ps) - 1 : -1;
       auto token_t = [&](int v) { return v + (v >= w.n0 ? w.shift : 0); };
@@ -345,7 +381,8 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
         const int t = token_t(v);
         return ld_early4(kvlist + (ps_shift >= 0 ? t >> ps_shift : t / p.ps));
       };
-      auto locate = [&](int i, int page, float& sk, float& sv) -> int64_t {
+      constexpr uint32_t kNone = ~0u;
+      auto locate = [&](int i, int page, float& sk, float& sv) -> uint32_t {
         const int v = w.v_begin + i * PW_TOK + my_tok;
         sk = 0.f;
         sv = -1.f;
@@ -354,7 +391,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
             flag_range_error();
             gone[i & 3] = i + 1;
           }
-          return -1;
+          return kNone;
         }
         if constexpr (Q8) {
           const float* s = p.scale + (int64_t)page * 2 * p.hkv + kvh;
@@ -362,11 +399,11 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
           sv = ld_early4(s + p.hkv);
         }
         const int t = token_t(v);
-        return (int64_t)page * 2 * plane_step +
-               (int64_t)(ps_shift >= 0 ? t & (p.ps - 1) : t % p.ps) * row_step;
+        return (uint32_t)page * 2 * plane +
+               (uint32_t)(ps_shift >= 0 ? t & (p.ps - 1) : t % p.ps) * p.hkv;
       };
-      auto dst_of = [&](char* tile, int tok, int chunk) {   // 16-byte chunk of 8 dims
-        return tile + (chunk >> 3) * PW_HALF + tok * 128 + (((chunk & 7) ^ (tok & 7)) << 4);
+      auto dst_of = [&](int tok, int chunk) -> uint32_t {   // 16-byte chunk of 8 dims
+        return (chunk >> 3) * PW_HALF + tok * 128 + (((chunk & 7) ^ (tok & 7)) << 4);
       };
       auto signal = [&](uint64_t* bar) {
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -376,37 +413,33 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
       // Codes land inside the place of their own row (in its last 128 bytes; where they are 64, odd
       // tokens in the second 64: no bank twice) and are spread from there over the whole row by the
       // warp that asked for them.
-      auto land = [&](char* tile, int tok) -> char* {
-        if constexpr (Q8)
-          return tile + (D / 64 - 1) * PW_HALF + tok * 128 + ((c + (CH == 4 ? (tok & 1) * 4 : 0)) << 4);
-        else
-          return dst_of(tile, tok, c);
-      };
-      auto copy = [&](char* tile, int64_t at, int64_t plane) {
+      // (the offset of a 16-byte chunk is the same for all tokens of a lane but for 128 bytes per token)
+      const uint32_t at_raw = Q8 ? (D / 64 - 1) * PW_HALF + tok0 * 128 + ((c + (CH == 4 ? (tok0 & 1) * 4 : 0)) << 4)
+                                 : dst_of(tok0, c);
+      constexpr uint32_t NEXT = NL * TPI * 128;
+      auto copy = [&](char* tile, uint32_t at, uint32_t more) {
+        const uint32_t dst = smem_u32(tile) + at_raw;
 #pragma unroll
         for (int it = 0; it < ITS; ++it) {
-          const int64_t o = __shfl_sync(0xffffffffu, at, it * TPI + sub);
-          if (unit_of(it) < UNITS)
-            cp_async16(smem_u32(land(tile, unit_of(it) * TPI + sub)),
-                       o >= 0 ? base + o + plane + c * 16 : p.pool, o >= 0);
+          const uint32_t o = __shfl_sync(0xffffffffu, at, it * TPI + sub);
+          cp_async16(dst + it * NEXT, o != kNone ? base + (uint64_t)(o + more) * ROWB + c * 16 : p.pool, o != kNone);
         }
         cp_commit();
       };
       // Rows have landed: codes to halves; values that are not finite out if `check`.
+      const uint32_t at0 = dst_of(tok0, 2 * c), at1 = dst_of(tok0, 2 * c + 1);
       auto finish = [&](char* tile, bool check) -> bool {
         bool bad = false;
         if constexpr (Q8) {
+          constexpr int B = ITS < 2 ? 1 : 2;
 #pragma unroll 1
-          for (int it0 = 0; it0 < ITS; it0 += 2) {
-            int4 raw[2];
+          for (int it = 0; it < ITS; it += B, tile += B * NEXT) {
+            int4 raw[B];
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-              if (unit_of(it0 + u) < UNITS)
-                raw[u] = *reinterpret_cast<const int4*>(land(tile, unit_of(it0 + u) * TPI + sub));
+            for (int u = 0; u < B; ++u) raw[u] = *reinterpret_cast<const int4*>(tile + at_raw + u * NEXT);
             __syncwarp();
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              if (unit_of(it0 + u) >= UNITS) break;
+            for (int u = 0; u < B; ++u) {
               const uint32_t wd[4] = {(uint32_t)raw[u].x, (uint32_t)raw[u].y, (uint32_t)raw[u].z,
                                       (uint32_t)raw[u].w};
               uint32_t o[8];
@@ -423,20 +456,14 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
                   o[x] = z;
                 }
               }
-              const int tok = unit_of(it0 + u) * TPI + sub;
-              // the second half of the row's chunks stores its odd piece first: no bank twice
-              const int sw = c >= CH / 2 ? 1 : 0;
-              *reinterpret_cast<int4*>(dst_of(tile, tok, 2 * c + sw)) =
-                  sw ? make_int4(o[4], o[5], o[6], o[7]) : make_int4(o[0], o[1], o[2], o[3]);
-              *reinterpret_cast<int4*>(dst_of(tile, tok, 2 * c + 1 - sw)) =
-                  sw ? make_int4(o[0], o[1], o[2], o[3]) : make_int4(o[4], o[5], o[6], o[7]);
+              *reinterpret_cast<int4*>(tile + at0 + u * NEXT) = make_int4(o[0], o[1], o[2], o[3]);
+              *reinterpret_cast<int4*>(tile + at1 + u * NEXT) = make_int4(o[4], o[5], o[6], o[7]);
             }
           }
         } else if (check) {
 #pragma unroll 1
           for (int it = 0; it < ITS; ++it) {
-            if (unit_of(it) >= UNITS) break;
-            int4* a = reinterpret_cast<int4*>(land(tile, unit_of(it) * TPI + sub));
+            int4* a = reinterpret_cast<int4*>(tile + at_raw + it * NEXT);
             const int4 x = *a;
             const int4 z = make_int4(zero_not_finite<T>(x.x), zero_not_finite<T>(x.y),
                                      zero_not_finite<T>(x.z), zero_not_finite<T>(x.w));
@@ -459,10 +486,12 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
 #pragma unroll 1
       for (int i = 0; i < steps; ++i) {
         const int st = i & 1;
-        const int64_t at = locate(i, page_next, sk, sv);
+        const uint32_t at = locate(i, page_next, sk, sv);
         page_next = page_of(w.v_begin + (i + 1) * PW_TOK);
-        if (i >= 2) ok = warp_wait(&k_empty[st], ((i >> 1) - 1) & 1, abort_flag);
-        if (!ok) break;
+        if (i >= 2 && !group_wait<NL * 32>(&k_empty[st], ((i >> 1) - 1) & 1, abort_flag, 10, lw == 0)) {
+          ok = false;
+          break;
+        }
         copy(smem + SM::K + st * SM::TILE, at, 0);
         if constexpr (Q8) {
           // scales of 0 (blocks never written) stand for values of 0: any will do; a token that is
@@ -481,16 +510,18 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
         cp_wait<0>();
         finish(smem + SM::K + st * SM::TILE, false);
         signal(&k_full[st]);
-        if (i >= 2) ok = warp_wait(&v_empty[st], ((i >> 1) - 1) & 1, abort_flag);
-        if (!ok) break;
-        copy(smem + SM::V + st * SM::TILE, at, plane_step);
+        if (i >= 2 && !group_wait<NL * 32>(&v_empty[st], ((i >> 1) - 1) & 1, abort_flag, 10, lw == 0)) {
+          ok = false;
+          break;
+        }
+        copy(smem + SM::V + st * SM::TILE, at, plane);
       }
       cp_wait<0>();
       if (ok) finish_v(steps - 1);
       if (!ok) *abort_flag = 1;
     }
   } else {
-    // ---------------- softmax: one row per thread ----------------
+    // ---------------- softmax: two threads per row ----------------
     // ---- Q rows into shared memory, zeros past the item's rows (loads in flight together; one
     // at a time they took 9 us of a CTA's 42 at 18 halves) ----
     {
@@ -561,23 +592,63 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
       // groups of 8 tokens lie in one page, or scales go token by token
       const bool by_token = Q8 && !( p.ps % 8 == 0 && w.v_begin % 8 == 0 &&
                            (w.shift == 0 || (w.n0 % 8 == 0 && w.shift % 8 == 0)));
-      // what the row sees, in v: v <= vc and (v < sink_end or v >= vw); with a gap, v >= n0 is t - shift
-      const int vc = !causal ? INT_MAX - 1 : w.shift == 0 ? pos : pos >= w.n0 + w.shift
-                                                    ? pos - w.shift : min(pos, w.n0 - 1);
-      const int vw = !window ? INT_MIN : w.shift == 0 ? pos - w.window
-                                                      : max(pos - w.window - w.shift, w.n0);
+      // what the row sees, in v: v <= vc and (v < sink_end or v >= vw)
+      const int vc = last_of(pos), vw = first_of(pos);
+      const int pair = 2 + tile * 4 + (warp & 3);     // barrier of the two warps with these rows
       float m = kNoMax, l = 0.f;
-      // A wait that ran out is told to the row tile's other warps at the barrier of a half, so that all
-      // leave their loop at the same place.
+      // A wait that ran out is told to the warp with the rows' other scores at the barrier of a half, so
+      // that both leave their loop at the same place.
       bool fail = false;
 #pragma unroll 1
-      for (int j = 0; j < halves; ++j) {
+      for (int j = 0;; ++j) {
         const int i = j >> 1, v0 = w.v_begin + j * 64 + part * 32;      // step; this thread's tokens
-        const uint32_t t_p = t_s + (j & 1) * 64;
-        fail = fail || !warp_wait(&s_full[2 * tile + (j & 1)], i & 1, abort_flag);
-        tc_fence_after();
+        // this thread's columns: 32 scores, then its P in the first 16 of them
+        const uint32_t t_p = t_s + (j & 1) * 64 + part * 32;
         uint32_t x[32];
-        tmem_ld32_nw(t_p + part * 32, x);
+        if (j < halves) {
+          fail = fail || !warp_wait(&s_full[2 * tile + (j & 1)], i & 1, abort_flag);
+          tc_fence_after();
+          tmem_ld32_nw(t_p, x);
+        }
+        if (j > 0) {                       // P of the half before goes out while the scores come in
+          tmem_wait_st();
+          const int i = (j - 1) >> 1, v0 = w.v_begin + (j - 1) * 64 + part * 32;
+          if (!all_see(w.v_begin + i * PW_TOK, PW_TOK)) {
+            // values that are not finite, taken out of V: mark the dims of the rows that see them
+            // (before P is handed over: V's stage and its flag stay until P V of this half is done)
+            fail = fail || !warp_wait(&v_full[i & 1], (i >> 1) & 1, abort_flag);
+            if (odd[i & 1] == i + 1) {
+              uint32_t* mask = odd_mask + row * (2 * (D / 32));
+#pragma unroll 1
+              for (int k = 0; row < rows && k < min(32, w.v_end - v0); ++k) {
+                const int v = v0 + k, t = v + (v >= w.n0 ? w.shift : 0);
+                const int page = kvlist[t / p.ps];
+                if (page < 0 || page >= p.num_pages || (causal && t > pos) ||
+                    (window && t < pos - w.window && t >= w.sink_end))
+                  continue;
+                const int64_t r = ((int64_t)page * 2 + 1) * p.ps + t % p.ps;
+                const char* src = p.pool + (r * p.hkv + kvh) * ROWB;
+#pragma unroll 1
+                for (int d = 0; d < D; ++d) {
+                  float val;
+                  if constexpr (Q8) {
+                    const uint32_t h2 = e4m3x2_to_h2(*reinterpret_cast<const uint8_t*>(src + d));
+                    val = __low2float(*reinterpret_cast<const __half2*>(&h2));
+                  } else {
+                    val = to_f(reinterpret_cast<const T*>(src)[d]);
+                  }
+                  if (!(val < INFINITY)) atomicOr(&mask[d >> 5], 1u << (d & 31));
+                  if (!(val > -INFINITY)) atomicOr(&mask[D / 32 + (d >> 5)], 1u << (d & 31));
+                }
+                *marked = 1;
+              }
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[2 * tile + ((j - 1) & 1)]);
+        }
+        if (j == halves) break;
         const float4* tb = tab + (i & 3) * PW_TOK + (j & 1) * 64 + part * 32;
         const bool missing = !Q8 && gone[i & 3] == i + 1, cut = !all_see(v0, 32) || missing;
         uint32_t see = ~0u;
@@ -624,10 +695,9 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
         }
         mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         if (!Q8) mx *= scale;
-        // also: from here on every score of the tile is in registers, P may be written
-        if (vote256(2 + tile, mx > m + kLazyMax || fail)) {
+        if (vote<64>(pair, mx > m + kLazyMax || fail)) {
           meet[part * 256 + row] = mx;
-          if (vote256(2 + tile, fail)) {
+          if (vote<64>(pair, fail)) {
             fail = true;
             break;
           }
@@ -694,47 +764,12 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
             l += a + b;
           }
         }
-        tmem_st16(t_p + part * 16, pk);
-        tmem_wait_st();
-        if (!all_see(w.v_begin + i * PW_TOK, PW_TOK)) {
-          // values that are not finite, taken out of V: mark the dims of the rows that see them
-          // (before P is handed over: V's stage and its flag stay until P V of this half is done)
-          fail = fail || !warp_wait(&v_full[i & 1], (i >> 1) & 1, abort_flag);
-          if (odd[i & 1] == i + 1) {
-            uint32_t* mask = odd_mask + row * (2 * (D / 32));
-#pragma unroll 1
-            for (int k = 0; row < rows && k < min(32, w.v_end - v0); ++k) {
-              const int v = v0 + k, t = v + (v >= w.n0 ? w.shift : 0);
-              const int page = kvlist[t / p.ps];
-              if (page < 0 || page >= p.num_pages || (causal && t > pos) ||
-                  (window && t < pos - w.window && t >= w.sink_end))
-                continue;
-              const int64_t r = ((int64_t)page * 2 + 1) * p.ps + t % p.ps;
-              const char* src = p.pool + (r * p.hkv + kvh) * ROWB;
-#pragma unroll 1
-              for (int d = 0; d < D; ++d) {
-                float val;
-                if constexpr (Q8) {
-                  const uint32_t h2 = e4m3x2_to_h2(*reinterpret_cast<const uint8_t*>(src + d));
-                  val = __low2float(*reinterpret_cast<const __half2*>(&h2));
-                } else {
-                  val = to_f(reinterpret_cast<const T*>(src)[d]);
-                }
-                if (!(val < INFINITY)) atomicOr(&mask[d >> 5], 1u << (d & 31));
-                if (!(val > -INFINITY)) atomicOr(&mask[D / 32 + (d >> 5)], 1u << (d & 31));
-              }
-              *marked = 1;
-            }
-          }
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[2 * tile + (j & 1)]);
+        tmem_st16(t_p, pk);
       }
       // ---- epilogue: half the dims per thread ----
       fail = fail || !warp_wait(&o_done[2 * tile + ((halves - 1) & 1)], ((halves - 1) >> 1) & 1, abort_flag);
       meet[part * 256 + row] = l;
-      if (!vote256(2 + tile, fail)) {
+      if (!vote<64>(pair, fail)) {
         tc_fence_after();
         l += meet[(part ^ 1) * 256 + row];
         const float inv = l != 0.f ? 1.f / l : 0.f;
