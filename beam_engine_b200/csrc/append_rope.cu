@@ -576,6 +576,10 @@ static int rope_append_check(const char* fn, const RopeAppend& a, int dtype, int
     set_error("%s: %d rows need a workspace of %lld ints", fn, a.n, 5ll * a.n + 1024);
     return BE_ECAPACITY;
   }
+  if (a.n > ROPE_SCAN_ROWS && (uintptr_t)workspace % 8) {
+    set_error("%s: the workspace must be 8-byte aligned", fn);
+    return BE_EINVAL;
+  }
   return BE_OK;
 }
 

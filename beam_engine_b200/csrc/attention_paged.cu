@@ -705,6 +705,12 @@ extern "C" int be_paged_attn_run(const int32_t* plan_dev, int max_wide, int max_
     set_error("be_paged_attn_run: invalid shape");
     return BE_EINVAL;
   }
+  // kernels number a pool's token rows in 31 bits, its (token, head) rows in 32
+  const int64_t token_rows = (int64_t)num_pages * 2 * std::min(page_size, 1 << 24);
+  if (token_rows > INT32_MAX || token_rows * num_kv_heads >= UINT32_MAX) {
+    set_error("be_paged_attn_run: a pool of %d pages of %d tokens is too large", num_pages, page_size);
+    return BE_EINVAL;
+  }
   if ((dtype != BE_BF16 && dtype != BE_F16) || (cache_dtype != BE_E4M3 && cache_dtype != dtype)) {
     set_error("be_paged_attn_run: queries are bf16 or fp16, the cache e4m3 or of their type");
     return BE_EINVAL;

@@ -190,20 +190,22 @@ def _append(**kw):
     (dict(cdt=_lib.BE_BF16), _lib.BE_EINVAL), (dict(k=None), _lib.BE_EINVAL),
     (dict(b=None), _lib.BE_EINVAL), (dict(n=-1), _lib.BE_EINVAL), (dict(dt=_lib.BE_E4M3), _lib.BE_EINVAL),
     (dict(cache=20), _lib.BE_EINVAL), (dict(n=513), _lib.BE_ECAPACITY),
-    (dict(n=513, ws=16, wn=100), _lib.BE_ECAPACITY), (dict(n=0), _lib.BE_OK)])
+    (dict(n=513, ws=16, wn=100), _lib.BE_ECAPACITY), (dict(n=513, ws=20, wn=4096), _lib.BE_EINVAL),
+    (dict(n=0), _lib.BE_OK)])
 def test_append_arguments(kw, rc):
     assert _append(**kw) == rc
 
 
 @pytest.mark.parametrize("kw", [
     dict(dt=_lib.BE_F32), dict(cdt=_lib.BE_F16), dict(d=80), dict(scale=None), dict(hq=258),
-    dict(q=None), dict(q=8), dict(parts=1), dict(qs=4), dict(narrow=-1), dict(rows=17)])
+    dict(q=None), dict(q=8), dict(parts=1), dict(qs=4), dict(narrow=-1), dict(rows=17),
+    dict(pages=1 << 26), dict(pages=2 ** 31 - 1)])
 def test_run_refuses(kw):
     a = dict(q=16, qs=512, cache=16, scale=16, hq=4, d=64, dt=_lib.BE_BF16, cdt=_lib.BE_E4M3,
-             parts=0, narrow=1, rows=4)
+             parts=0, narrow=1, rows=4, pages=8)
     a.update(kw)
     rc = lib().be_paged_attn_run(16, 0, a["narrow"], a["rows"], 0, a["parts"], 16, a["q"], a["qs"], a["cache"],
-                                 a["scale"], 8, a["hq"], 2, a["d"], a["dt"], a["cdt"], 1.0, 16, 512,
+                                 a["scale"], a["pages"], a["hq"], 2, a["d"], a["dt"], a["cdt"], 1.0, 16, 512,
                                  None, None, None, None)
     assert rc == _lib.BE_EINVAL
 
