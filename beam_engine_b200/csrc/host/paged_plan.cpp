@@ -36,12 +36,15 @@ struct Tile {           // a run's queries [q0, q0 + ql) and the tokens they see
   int n0, shift;        // virtual index: t = v + (v >= n0 ? shift : 0)
   int n;                // tokens seen by some query
   bool wide;
+  bool alone;           // no other tile of its queries
 };
 
 // Steps of 128 tokens per wide item.  One CTA (item x KV head) occupies an SM, so what counts is
 // when the last SM is done if CTAs go longest first to whichever SM is free: that is tried for
-// whole tiles and for cuts at fractions of the average load, with 2 steps' time for a CTA's start
-// and end, one more for writing partial rows and 3 for their merge.
+// whole tiles and for cuts at fractions of the average load, with 3 steps' time for a CTA's start
+// and end (7.7 us against 2.8 us a step), and where the cut is what makes rows partial one more
+// for writing them and 3 for their merge.  (8 prefixes of 1024 tokens under 16 beams each, 8 KV heads:
+// whole tiles leave 84 of 148 SMs idle.)
 int wide_chunk(const std::vector<Tile>& tiles, int64_t total_steps, int sms, int hkv) {
   int longest = 0;
   int64_t n = 0;
@@ -51,13 +54,13 @@ int wide_chunk(const std::vector<Tile>& tiles, int64_t total_steps, int sms, int
       ++n;
     }
   if (n == 0 || n * hkv > 8 * (int64_t)sms) return 1 << 20;   // many CTAs: even as they are
-  const int64_t load = std::max<int64_t>(1, total_steps * hkv / sms);
+  const double load = std::max(1.0, (double)total_steps * hkv / sms);
   int best_chunk = 1 << 20;
   int64_t best = INT64_MAX;
   std::vector<int> cost;
   std::vector<int64_t> busy;
   for (const double f : {0.0, 1.0, 0.5, 0.34, 0.25, 0.125}) {
-    const int chunk = f == 0.0 ? 1 << 20 : (int)std::max<int64_t>(1, (int64_t)(load * f + 0.999));
+    const int chunk = f == 0.0 ? 1 << 20 : std::max(1, (int)(load * f + 0.999));
     if (f != 0.0 && chunk >= longest) continue;
     cost.clear();
     bool split = false;
@@ -65,9 +68,10 @@ int wide_chunk(const std::vector<Tile>& tiles, int64_t total_steps, int sms, int
       if (!t.wide) continue;
       const int steps = (t.n + 127) / 128, ns = (steps + chunk - 1) / chunk;
       const int len = (steps + ns - 1) / ns;
-      split = split || ns > 1;
+      const bool partial = ns > 1 && t.alone;
+      split = split || partial;
       for (int s = 0; s < steps; s += len)
-        for (int h = 0; h < hkv; ++h) cost.push_back(std::min(len, steps - s) + 2 + (ns > 1));
+        for (int h = 0; h < hkv; ++h) cost.push_back(std::min(len, steps - s) + 3 + partial);
     }
     if (cost.size() > 65536) continue;
     std::sort(cost.begin(), cost.end(), [](int a, int b) { return a > b; });
@@ -276,6 +280,13 @@ extern "C" int be_paged_plan(int num_levels, const int32_t* const* qo_indptr,
       tiles.push_back(t);
     }
   }
+  std::vector<int32_t> cover(num_queries, 0);
+  for (const Tile& t : tiles)
+    for (int q = 0; q < t.ql; ++q) cover[runs[t.run].q_begin + t.q0 + q]++;
+  for (Tile& t : tiles) {
+    t.alone = true;
+    for (int q = 0; q < t.ql; ++q) t.alone = t.alone && cover[runs[t.run].q_begin + t.q0 + q] == 1;
+  }
   const int sms = num_sms > 0 ? num_sms : 148;
   const int chunk_n = narrow_chunk(tiles, narrow_tokens, sms, num_kv_heads);
   const int chunk_w = wide_chunk(tiles, wide_steps, sms, num_kv_heads) * 128;
@@ -283,7 +294,7 @@ extern "C" int be_paged_plan(int num_levels, const int32_t* const* qo_indptr,
     int tile, v0, v1, part;
   };
   std::vector<Item> items;
-  std::vector<int32_t> cover(num_queries, 0);
+  cover.assign(num_queries, 0);
   for (size_t i = 0; i < tiles.size(); ++i) {
     const Tile& t = tiles[i];
     const int chunk = t.wide ? chunk_w : chunk_n, unit = t.wide ? 128 : 64;
