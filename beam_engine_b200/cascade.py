@@ -306,7 +306,8 @@ class MultiLevelCascadeAttentionWrapper:
         self._levels_args = (L, ptrs, ng, nq, page_size, num_qo_heads, num_kv_heads, causal,
                              split_tokens, head_dim, arrs)
         self.tiles = False
-        self._window = (window_left if window_left >= 0 else -1, num_sinks)
+        most = 2 ** 31 - 1                   # tokens are counted in int32
+        self._window = (min(window_left, most) if window_left >= 0 else -1, min(num_sinks, most))
         self.paged = window_left >= 0 or (kv_data_type is not None and is_8bit(kv_data_type))
         if self.paged:
             self._plan_paged()
@@ -395,6 +396,9 @@ class MultiLevelCascadeAttentionWrapper:
         if q.shape[0] != self.num_queries:
             raise ValueError(f"q has {q.shape[0]} rows, plan has {self.num_queries} queries")
         if is_8bit(paged_kv_cache.dtype) and not self.paged:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("plan with kv_data_type=torch.float8_e4m3fn before capturing a "
+                                   "run over an 8-bit cache")
             self._plan_paged()               # 8-bit caches run on their own plan
         if self.paged:
             return self._run_paged(q, paged_kv_cache, kv_scale, return_lse, out)

@@ -117,7 +117,6 @@ class BeamLlama:
         self.use_lt = mode == "lt" and cuda_bf16           # cuBLASLt, per-shape tuned
         self._gemm_ws = None
         self._lt_ws = None
-        self._append_ws = None    # run lists of large appends into 8-bit pools
         self.comm = None          # PeerAllReduce: fused all-reduce + add + RMSNorm under TP
         self._slot_views = {}
         del weights
@@ -192,10 +191,10 @@ class BeamLlama:
         act = torch.empty((n, self.F), dtype=dt, device=dev)
         delta = torch.empty_like(x)
         pool, scale = page_table.kv_cache, page_table.kv_scale
-        if scale is not None and n > 512 and (self._append_ws is None
-                                              or self._append_ws.numel() < 5 * n + 1024):
-            self._append_ws = torch.empty(5 * n + 1024, dtype=torch.int32, device=dev)
-        ws = self._append_ws if n > 512 else None
+        # run lists of large appends into 8-bit pools (this call's own: a recorded step keeps its)
+        ws = None
+        if scale is not None and n > 512:
+            ws = torch.empty(5 * n + 1024, dtype=torch.int32, device=dev)
         P, ps = page_table.max_num_pages, page_table.page_size
         have_delta = False
         # fused peer all-reduce: the O / down GEMMs write into this rank's slots and

@@ -132,3 +132,22 @@ def test_refusals():
     with pytest.raises(ValueError, match="bf16"):
         BeamSearchGenerator(BeamLlama(TINY, dtype=torch.float32, seed=0), None,
                             VanillaBeamSearchStrategy(), store_dtype=F8)
+
+
+def test_prompts_of_more_rows_than_one_scan():
+    """600 prompt rows in one call (the append sorts them into runs first): the pool's first layer
+    holds the codes and scales that the same prompts leave one by one."""
+    long = [[int(x) for x in np.random.default_rng(9 + i).integers(0, 1024, 300)] for i in range(2)]
+    both = engine(page_size=16, use_graph=False)
+    both.prefill(BeamState(4, both.page_table), long)
+    for i, p in enumerate(long):
+        one = engine(page_size=16, use_graph=False)
+        one.prefill(BeamState(4, one.page_table), [p])
+        n = 18                                             # 18 full pages of 19
+        a = both.page_table.kv_cache[0, i * 19:i * 19 + n].view(torch.uint8)
+        sa, sb = both.page_table.kv_scale[0, i * 19:i * 19 + n], one.page_table.kv_scale[0, :n]
+        # the projections of 600 and of 300 rows may be summed in another order: nearly all codes agree
+        assert (sa == sb).float().mean() > 0.99
+        assert (a == one.page_table.kv_cache[0, :n].view(torch.uint8)).float().mean() > 0.97
+    res = engine(page_size=16).generate_ids(long, 4, max_new_tokens=4)
+    assert len(res) == 2

@@ -682,3 +682,60 @@ def test_append_then_attend_as_a_decode_loop_does(dt):
         values = read_paged_kv_cache(pool, i32(np.arange(P)), scale, torch.float32)
         ref = reference(q, values, None, [0, used], pages[:used], [at], [0, n], True, 40, 4, d ** -0.5)
         compare(out, lse, ref, dt, u_of(dt, True, n * 4))
+
+
+def test_windows_beyond_int32_see_everything():
+    from beam_engine_b200.cascade import BatchPrefillWithPagedKVCacheWrapper
+    outs = []
+    pool, _ = make_pool(8, 16, 2, 64, torch.bfloat16, False, 1)
+    q = torch.randn((6, 4, 64), device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).bfloat16()
+    for window, sinks in ((10 ** 6, 0), (2 ** 32 + 5, 0), (0, 2 ** 32 + 1)):
+        w = BatchPrefillWithPagedKVCacheWrapper(torch.empty(8 << 20, dtype=torch.uint8, device="cuda"))
+        w.plan([0, 6], [0, 6], [5, 1, 2, 7, 0, 3], [9], 4, 2, 64, 16, causal=True, window_left=window,
+               num_sinks=sinks)
+        outs.append(w.run(q, pool))
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+def test_capture_needs_a_plan_for_the_cache():
+    from beam_engine_b200.cascade import BatchPrefillWithPagedKVCacheWrapper
+    pool, scale = make_pool(4, 16, 2, 64, torch.bfloat16, True, 1)
+    q = torch.zeros((2, 4, 64), device="cuda", dtype=torch.bfloat16)
+    w = BatchPrefillWithPagedKVCacheWrapper(torch.empty(8 << 20, dtype=torch.uint8, device="cuda"))
+    w.plan([0, 2], [0, 2], [1, 2], [9], 4, 2, 64, 16, causal=True)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(RuntimeError, match="kv_data_type"):
+            w.run(q, pool, kv_scale=scale)
+
+
+def test_two_graphs_with_workspaces_of_their_own_replayed_together():
+    """Two captured calls on two streams, replayed at once, give what each gives alone."""
+    from beam_engine_b200.cascade import BatchPrefillWithPagedKVCacheWrapper
+    calls = []
+    for seed, (qo, kv) in enumerate((([0, 1, 2], [3000, 2000]), ([0, 40, 41], [700, 2500]))):
+        ptr = np.concatenate([[0], np.cumsum([-(-k // 16) for k in kv])]).tolist()
+        pool, scale = make_pool(ptr[-1], 16, 2, 128, torch.bfloat16, True, seed)
+        pages = np.random.default_rng(seed).permutation(ptr[-1]).tolist()
+        q = torch.randn((qo[-1], 8, 128), device="cuda",
+                        generator=torch.Generator(device="cuda").manual_seed(seed)).bfloat16()
+        w = BatchPrefillWithPagedKVCacheWrapper(torch.empty(64 << 20, dtype=torch.uint8, device="cuda"))
+        w.plan(qo, ptr, pages, [(k - 1) % 16 + 1 for k in kv], 8, 2, 128, 16, causal=True, kv_data_type=F8)
+        want = w.run(q, pool, kv_scale=scale)
+        out = torch.empty_like(want)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            w.run(q, pool, kv_scale=scale, out=out)
+        calls.append((g, out, want, torch.cuda.Stream(), (w, q, pool, scale)))
+    for _ in range(5):
+        for g, out, _, st, _ in calls:
+            with torch.cuda.stream(st):
+                out.zero_()
+                for _ in range(3):
+                    g.replay()
+    torch.cuda.synchronize()
+    for _, out, want, _, _ in calls:
+        assert torch.equal(out, want)
+    assert status() == 0
