@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libbeam_b200.so")
 _lib = None
@@ -27,6 +28,12 @@ class AttnPlanInfo(C.Structure):
         "n_work", "n_work_wide", "n_queries", "n_parts", "n_merge", "off_work", "off_qlist",
         "off_kvlist", "off_merge_q", "off_merge_ptr", "off_merge_parts", "total_ints",
         "page_size", "group_size", "any_slots", "max_item_tokens", "total_tokens", "max_wide_tokens")]
+
+
+# Argument blocks of calls made every step, packed in one go (22 and 24 arguments converted one by one
+# took ctypes 5 us a call): the fields of be_rope_append_args and be_paged_attn_args in order.
+ROPE_APPEND_ARGS = struct.Struct("<2Q2q9QqQ8i")
+PAGED_ATTN_ARGS = struct.Struct("<2Qq3Qq4Q12ifi")
 
 
 class PagedPlanInfo(C.Structure):
@@ -77,9 +84,7 @@ _SIGS = {
     "be_attn_run_fixed_2s": (C.c_int, [vp, vp, C.c_int, vp, i64, vp, C.c_int, C.c_int, C.c_int,
                                     C.c_int, C.c_int, f32, vp, i64, vp, vp, vp, vp, vp, vp]),
     # 8-bit pools, windowed attention
-    "be_rope_append_paged_kv": (C.c_int, [vp, vp, i64, i64, vp, vp, vp, vp, vp, C.c_int, vp, vp, vp,
-                                          C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp,
-                                          i64, vp]),
+    "be_rope_append_paged_kv": (C.c_int, [vp]),      # ROPE_APPEND_ARGS
     "be_rope_qkv_append8": (C.c_int, [vp, i64, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, vp, vp,
                                       C.c_int, C.c_int, vp, vp, C.c_int, vp, i64, vp]),
     "be_read_paged_kv8": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp,
@@ -91,9 +96,7 @@ _SIGS = {
     "be_paged_plan": (C.c_int, [C.c_int, PP32, PP32, PP32, PP32, P32, C.c_int, C.c_int, C.c_int,
                                 C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp, i64,
                                 C.POINTER(PagedPlanInfo)]),
-    "be_paged_attn_run": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp, i64, vp, vp,
-                                    C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, f32, vp,
-                                    i64, vp, vp, vp, vp]),
+    "be_paged_attn_run": (C.c_int, [vp]),            # PAGED_ATTN_ARGS
     # host page manager
     "be_trie_create": (vp, [C.c_int, C.c_int]),
     "be_trie_destroy": (None, [vp]),

@@ -28,7 +28,7 @@ from ._lib import check, lib
 from .beam_state import BeamState
 from .beam_strategy import VanillaBeamSearchStrategy
 from .cascade import _Plan, target_pieces, tile_rows_for, tiles_eligible
-from .page_table import PageTable, is_8bit, stream_ptr
+from .page_table import PageTable, is_8bit, raw_stream, stream_ptr
 from .parallel import vocab_parallel_log_softmax_topk
 
 logger = logging.getLogger(__name__)
@@ -352,12 +352,13 @@ class StepGraph:
             return
         if self.kind == "paged":
             c = self.caps
-            rc = lib().be_paged_attn_run(
-                self.dev_buf.data_ptr() + 4 * self.plan_off, c["wide"], c["narrow"], c["rows"],
-                c["merge"], c["parts"], pt.page_size, qkv.data_ptr(), qkv.stride(0),
-                pt.kv_cache[layer].data_ptr(), pt.kv_scale[layer].data_ptr(), pt.max_num_pages,
-                m.Hq, m.Hkv, m.D, m.dt, _lib.BE_E4M3, m.D ** -0.5, out.data_ptr(), out.stride(0),
-                None, self.mid_o.data_ptr(), self.mid_lse.data_ptr(), stream_ptr(qkv.device))
+            rc = lib().be_paged_attn_run(_lib.PAGED_ATTN_ARGS.pack(
+                self.dev_buf.data_ptr() + 4 * self.plan_off, qkv.data_ptr(), qkv.stride(0),
+                pt.kv_cache[layer].data_ptr(), pt.kv_scale[layer].data_ptr(), out.data_ptr(),
+                out.stride(0), 0, self.mid_o.data_ptr(), self.mid_lse.data_ptr(),
+                raw_stream(qkv.device.index), c["wide"], c["narrow"], c["rows"], c["merge"],
+                c["parts"], pt.page_size, pt.max_num_pages, m.Hq, m.Hkv, m.D, m.dt, _lib.BE_E4M3,
+                m.D ** -0.5, 0))
             check(rc, "be_paged_attn_run")
             self._mark(2 * layer + 1, qkv)
             return

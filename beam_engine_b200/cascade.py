@@ -35,7 +35,7 @@ import torch
 
 from . import _lib
 from ._lib import AttnPlanInfo, PagedPlanInfo, TilePlanInfo, check, lib
-from .page_table import (_DT, check_pool8, dtype_code, is_8bit, on_device, raw_stream,
+from .page_table import (_DT, check_pool8, dtype_code, is_8bit, raw_stream,
                          require_cuda, require_same_device, stream_ptr)
 
 
@@ -234,14 +234,18 @@ class _Plan:
         i = self.info
         index = q.device.index
         code = _DT.get(q.dtype, -1)
-        with on_device(index):
-            rc = lib().be_paged_attn_run(
-                self.plan_dev, i.n_work_wide, i.n_work - i.n_work_wide, i.narrow_rows, i.n_merge,
-                i.n_parts, i.page_size, q.data_ptr(), qs[0], kv.data_ptr(),
-                None if kv_scale is None else kv_scale.data_ptr(), kv.shape[0], num_qo_heads,
-                num_kv_heads, head_dim, code, code if kv_scale is None else _lib.BE_E4M3, sm_scale,
-                out.data_ptr(), out.stride(0), None if lse is None else lse.data_ptr(),
-                self.mid_o, self.mid_lse, raw_stream(index))
+        ks, cache_code = (0, code) if kv_scale is None else (kv_scale.data_ptr(), _lib.BE_E4M3)
+        args = _lib.PAGED_ATTN_ARGS.pack(
+            self.plan_dev, q.data_ptr(), qs[0], kv.data_ptr(), ks, out.data_ptr(), out.stride(0),
+            0 if lse is None else lse.data_ptr(), self.mid_o, self.mid_lse, raw_stream(index),
+            i.n_work_wide, i.n_work - i.n_work_wide, i.narrow_rows, i.n_merge, i.n_parts,
+            i.page_size, kv.shape[0], num_qo_heads, num_kv_heads, head_dim, code, cache_code,
+            sm_scale, 0)
+        if torch.cuda.current_device() == index:
+            rc = lib().be_paged_attn_run(args)
+        else:
+            with torch.cuda.device(index):
+                rc = lib().be_paged_attn_run(args)
         if rc:
             check(rc, "be_paged_attn_run")
 
@@ -381,12 +385,12 @@ class MultiLevelCascadeAttentionWrapper:
                              "no kv_scale")
         else:
             require_same_device(kv, q, self._plan.ws)
-        if out is None:
-            out = torch.empty(shape, dtype=dtype, device=dev)
+        if out is None:              # (new_empty takes 1 us less than torch.empty)
+            out = q.new_empty(shape)
         elif (out.shape != shape or out.dtype is not dtype or out.device != dev
               or out.stride(-1) != 1 or out.stride(-2) != d):
             raise ValueError(f"out must be {dtype} {shape} on {dev} with contiguous heads")
-        lse = torch.empty((n, hq), dtype=torch.float32, device=dev) if return_lse else None
+        lse = q.new_empty((n, hq), dtype=torch.float32) if return_lse else None
         if n:
             self._plan.run_paged(q, kv, kv_scale, hq, self.hkv, d, self.sm_scale, out, lse)
         return (out, lse) if return_lse else out

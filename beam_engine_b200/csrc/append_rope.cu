@@ -589,41 +589,38 @@ static int rope_append_check(const char* fn, const RopeAppend& a, int dtype, int
 
 using namespace be;
 
-extern "C" int be_rope_append_paged_kv(const void* append_key, const void* append_value,
-                                       int64_t key_row_stride, int64_t value_row_stride,
-                                       const int32_t* batch_indices, const int32_t* positions,
-                                       const int32_t* rope_positions, const int32_t* kv_indices,
-                                       const int32_t* kv_indptr, int nnz, const float* inv_freq,
-                                       void* paged_kv_cache, float* kv_scale, int num_pages,
-                                       int page_size, int num_kv_heads, int head_dim, int dtype,
-                                       int cache_dtype, int32_t* workspace,
-                                       int64_t workspace_ints, void* stream) {
-  RopeAppend a{};
-  a.k = (const char*)append_key;
-  a.v = (const char*)append_value;
-  a.k_stride = key_row_stride;
-  a.v_stride = value_row_stride;
-  a.batch = batch_indices;
-  a.pos = positions;
-  a.rope_pos = rope_positions ? rope_positions : positions;
-  a.kv_indices = kv_indices;
-  a.kv_indptr = kv_indptr;
-  a.inv_freq = inv_freq;
-  a.cache = (char*)paged_kv_cache;
-  a.scale = kv_scale;
-  a.n = nnz;
-  a.num_pages = num_pages;
-  a.ps = page_size;
-  a.hkv = num_kv_heads;
-  a.D = head_dim;
-  if (nnz > 0 && !batch_indices) {
+extern "C" int be_rope_append_paged_kv(const be_rope_append_args* args) {
+  if (!args) {
     set_error("be_rope_append_paged_kv: null pointer");
     return BE_EINVAL;
   }
-  const int rc = rope_append_check("be_rope_append_paged_kv", a, dtype, cache_dtype, workspace,
-                                   workspace_ints);
-  if (rc != BE_OK || nnz == 0) return rc;
-  return rope_append_launch(a, dtype, workspace, (cudaStream_t)stream);
+  const be_rope_append_args& g = *args;
+  RopeAppend a{};
+  a.k = (const char*)g.append_key;
+  a.v = (const char*)g.append_value;
+  a.k_stride = g.key_row_stride;
+  a.v_stride = g.value_row_stride;
+  a.batch = g.batch_indices;
+  a.pos = g.positions;
+  a.rope_pos = g.rope_positions ? g.rope_positions : g.positions;
+  a.kv_indices = g.kv_indices;
+  a.kv_indptr = g.kv_indptr;
+  a.inv_freq = g.inv_freq;
+  a.cache = (char*)g.paged_kv_cache;
+  a.scale = g.kv_scale;
+  a.n = g.nnz;
+  a.num_pages = g.num_pages;
+  a.ps = g.page_size;
+  a.hkv = g.num_kv_heads;
+  a.D = g.head_dim;
+  if (a.n > 0 && !a.batch) {
+    set_error("be_rope_append_paged_kv: null pointer");
+    return BE_EINVAL;
+  }
+  const int rc = rope_append_check("be_rope_append_paged_kv", a, g.dtype, g.cache_dtype, g.workspace,
+                                   g.workspace_ints);
+  if (rc != BE_OK || a.n == 0) return rc;
+  return rope_append_launch(a, g.dtype, g.workspace, (cudaStream_t)g.stream);
 }
 
 extern "C" int be_rope_qkv_append8(void* qkv, int64_t row_stride, int n, int num_qo_heads,

@@ -693,15 +693,17 @@ static int paged_launch(const PagedParams& p, bool q8, int D, int max_wide, int 
 
 using namespace be;
 
-extern "C" int be_paged_attn_run(const int32_t* plan_dev, int max_wide, int max_narrow,
-                                 int narrow_rows, int max_merge, int max_parts, int page_size, const void* q,
-                                 int64_t q_row_stride, const void* paged_kv_cache,
-                                 const float* kv_scale, int num_pages, int num_qo_heads,
-                                 int num_kv_heads, int head_dim, int dtype, int cache_dtype,
-                                 float sm_scale, void* out, int64_t out_row_stride, float* lse,
-                                 float* mid_o, float* mid_lse, void* stream) {
-  if (max_wide < 0 || max_narrow < 0 || narrow_rows < 0 || narrow_rows > 16 || max_merge < 0 || max_parts < 0 || page_size < 1 ||
-      num_pages < 1 || num_kv_heads < 1 || num_kv_heads > 1024 || num_qo_heads < 1 ||
+extern "C" int be_paged_attn_run(const be_paged_attn_args* args) {
+  if (!args) {
+    set_error("be_paged_attn_run: null pointer");
+    return BE_EINVAL;
+  }
+  const be_paged_attn_args& a = *args;
+  const int max_wide = a.max_wide, max_narrow = a.max_narrow, max_merge = a.max_merge;
+  const int page_size = a.page_size, num_pages = a.num_pages, head_dim = a.head_dim;
+  const int num_qo_heads = a.num_qo_heads, num_kv_heads = a.num_kv_heads, dtype = a.dtype;
+  if (max_wide < 0 || max_narrow < 0 || a.narrow_rows < 0 || a.narrow_rows > 16 || max_merge < 0 ||
+      a.max_parts < 0 || page_size < 1 || num_pages < 1 || num_kv_heads < 1 || num_kv_heads > 1024 || num_qo_heads < 1 ||
       std::max(max_wide, max_narrow) > (1 << 20) ||
       num_qo_heads % num_kv_heads) {
     set_error("be_paged_attn_run: invalid shape");
@@ -713,7 +715,7 @@ extern "C" int be_paged_attn_run(const int32_t* plan_dev, int max_wide, int max_
     set_error("be_paged_attn_run: a pool of %d pages of %d tokens is too large", num_pages, page_size);
     return BE_EINVAL;
   }
-  if ((dtype != BE_BF16 && dtype != BE_F16) || (cache_dtype != BE_E4M3 && cache_dtype != dtype)) {
+  if ((dtype != BE_BF16 && dtype != BE_F16) || (a.cache_dtype != BE_E4M3 && a.cache_dtype != dtype)) {
     set_error("be_paged_attn_run: queries are bf16 or fp16, the cache e4m3 or of their type");
     return BE_EINVAL;
   }
@@ -727,39 +729,39 @@ extern "C" int be_paged_attn_run(const int32_t* plan_dev, int max_wide, int max_
     return BE_EINVAL;
   }
   if (max_wide + max_narrow + max_merge == 0) return BE_OK;
-  if (!plan_dev || !q || !paged_kv_cache || !out || (max_parts > 0 && (!mid_o || !mid_lse)) ||
-      (cache_dtype == BE_E4M3) != (kv_scale != nullptr)) {
+  if (!a.plan_dev || !a.q || !a.paged_kv_cache || !a.out || (a.max_parts > 0 && (!a.mid_o || !a.mid_lse)) ||
+      (a.cache_dtype == BE_E4M3) != (a.kv_scale != nullptr)) {
     set_error("be_paged_attn_run: null pointer (an 8-bit cache needs kv_scale, another has none)");
     return BE_EINVAL;
   }
-  if (((uintptr_t)q | (uintptr_t)paged_kv_cache | (uintptr_t)mid_o) % 16 || (uintptr_t)out % 8 ||
-      q_row_stride % 8 || out_row_stride % 4) {
+  if (((uintptr_t)a.q | (uintptr_t)a.paged_kv_cache | (uintptr_t)a.mid_o) % 16 || (uintptr_t)a.out % 8 ||
+      a.q_row_stride % 8 || a.out_row_stride % 4) {
     set_error("be_paged_attn_run: q and the cache must be 16-byte aligned, out 8-byte");
     return BE_EINVAL;
   }
   PagedParams p;
-  p.plan = plan_dev;
-  p.q = (const char*)q;
-  p.q_row_stride = q_row_stride;
-  p.pool = (const char*)paged_kv_cache;
-  p.scale = kv_scale;
+  p.plan = a.plan_dev;
+  p.q = (const char*)a.q;
+  p.q_row_stride = a.q_row_stride;
+  p.pool = (const char*)a.paged_kv_cache;
+  p.scale = a.kv_scale;
   p.num_pages = num_pages;
   p.ps = page_size;
   p.hq = num_qo_heads;
   p.hkv = num_kv_heads;
   p.g = num_qo_heads / num_kv_heads;
-  p.scale_log2 = sm_scale * kLog2e;
-  p.out = (char*)out;
-  p.out_row_stride = out_row_stride;
-  p.lse = lse;
-  p.mid_o = mid_o;
-  p.mid_lse = mid_lse;
+  p.scale_log2 = a.sm_scale * kLog2e;
+  p.out = (char*)a.out;
+  p.out_row_stride = a.out_row_stride;
+  p.lse = a.lse;
+  p.mid_o = a.mid_o;
+  p.mid_lse = a.mid_lse;
   p.merge_next = max_merge > 0;
-  p.out_vec16 = (uintptr_t)out % 16 == 0 && out_row_stride % 8 == 0;
-  const bool q8 = cache_dtype == BE_E4M3;
+  p.out_vec16 = (uintptr_t)a.out % 16 == 0 && a.out_row_stride % 8 == 0;
+  const bool q8 = a.cache_dtype == BE_E4M3;
   return dtype == BE_BF16
              ? paged_launch<__nv_bfloat16>(p, q8, head_dim, max_wide, max_narrow,
-                                           narrow_rows, max_merge, (cudaStream_t)stream)
+                                           a.narrow_rows, max_merge, (cudaStream_t)a.stream)
              : paged_launch<__half>(p, q8, head_dim, max_wide, max_narrow,
-                                           narrow_rows, max_merge, (cudaStream_t)stream);
+                                           a.narrow_rows, max_merge, (cudaStream_t)a.stream);
 }

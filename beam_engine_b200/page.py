@@ -83,7 +83,7 @@ def read_paged_kv_cache(paged_kv_cache: torch.Tensor, pages: torch.Tensor, kv_sc
     pages = _int32(pages)
     P, _, ps, H, D = paged_kv_cache.shape
     n, dev = pages.shape[0], paged_kv_cache.device
-    out = torch.empty((n, 2, ps, H, D), dtype=dtype, device=dev)
+    out = paged_kv_cache.new_empty((n, 2, ps, H, D), dtype=dtype)
     with on_device(dev.index):
         rc = lib().be_read_paged_kv8(paged_kv_cache.data_ptr(), kv_scale.data_ptr(),
                                      pages.data_ptr(), n, P, ps, H, D, out.data_ptr(), _DT[dtype],

@@ -119,8 +119,7 @@ def append_rows(key, value, batch_indices, positions, pool, scale, kv_indices, k
     kv_indices, kv_indptr = _int32(kv_indices), _int32(kv_indptr)
     dev = pool.device
     same = [key, value, batch_indices, positions, kv_indices, kv_indptr]
-    freq = rope = codes = ws = None
-    ws_ints = 0
+    freq = rope = codes = ws_ints = 0
     if inv_freq is not None:
         if (inv_freq.dtype is not torch.float32 or inv_freq.shape != (D // 2,)
                 or not inv_freq.is_contiguous()):
@@ -139,13 +138,16 @@ def append_rows(key, value, batch_indices, positions, pool, scale, kv_indices, k
     if n > 512:
         ws_ints = 5 * n + 1024
         ws = torch.empty(ws_ints, dtype=torch.int32, device=dev)
-    with on_device(dev.index):
-        rc = lib().be_rope_append_paged_kv(
-            key.data_ptr(), value.data_ptr(), key.stride(0), value.stride(0),
-            batch_indices.data_ptr(), positions.data_ptr(), rope, kv_indices.data_ptr(),
-            kv_indptr.data_ptr(), n, freq, pool.data_ptr(), codes, P, ps, H, D,
-            dtype_code(key.dtype), cache_code, ws.data_ptr() if ws_ints else None, ws_ints,
-            raw_stream(dev.index))
+    args = _lib.ROPE_APPEND_ARGS.pack(
+        key.data_ptr(), value.data_ptr(), key.stride(0), value.stride(0), batch_indices.data_ptr(),
+        positions.data_ptr(), rope, kv_indices.data_ptr(), kv_indptr.data_ptr(), freq,
+        pool.data_ptr(), codes, ws.data_ptr() if ws_ints else 0, ws_ints, raw_stream(dev.index), n,
+        P, ps, H, D, dtype_code(key.dtype), cache_code, 0)
+    if torch.cuda.current_device() == dev.index:
+        rc = lib().be_rope_append_paged_kv(args)
+    else:
+        with torch.cuda.device(dev.index):
+            rc = lib().be_rope_append_paged_kv(args)
     if rc:
         check(rc, "append_paged_kv_cache")
 

@@ -109,14 +109,19 @@ int be_fork_tail_copy_list(void* paged_kv_cache, int64_t pool_layer_stride, int 
  * one in the call is kept.  Calls with more than 512 rows need a device workspace
  * of 5 * nnz + 1024 ints, 8-byte aligned (free to reuse once the call's work is done).
  * head_dim 32, 64, 128 or 256, page_size <= 256, num_kv_heads <= 64.          */
-int be_rope_append_paged_kv(const void* append_key, const void* append_value,
-                            int64_t key_row_stride, int64_t value_row_stride,
-                            const int32_t* batch_indices, const int32_t* positions,
-                            const int32_t* rope_positions, const int32_t* kv_indices,
-                            const int32_t* kv_indptr, int nnz, const float* inv_freq,
-                            void* paged_kv_cache, float* kv_scale, int num_pages, int page_size,
-                            int num_kv_heads, int head_dim, int dtype, int cache_dtype,
-                            int32_t* workspace, int64_t workspace_ints, void* stream);
+typedef struct be_rope_append_args {
+  const void *append_key, *append_value; /* rows [nnz][num_kv_heads][head_dim] */
+  int64_t key_row_stride, value_row_stride;            /* elements between rows */
+  const int32_t *batch_indices, *positions, *rope_positions, *kv_indices, *kv_indptr;
+  const float* inv_freq;
+  void* paged_kv_cache;
+  float* kv_scale;
+  int32_t* workspace;
+  int64_t workspace_ints;
+  void* stream;
+  int32_t nnz, num_pages, page_size, num_kv_heads, head_dim, dtype, cache_dtype, reserved;
+} be_rope_append_args;
+int be_rope_append_paged_kv(const be_rope_append_args* args);
 
 /* Pages of an 8-bit pool as values: out [n][2][page_size][num_kv_heads][head_dim]
  * in out_dtype.  A page id out of range is flagged and reads as zeros.        */
@@ -437,12 +442,22 @@ int be_paged_plan(int num_levels, const int32_t* const* qo_indptr, const int32_t
  * with q_row_stride elements between queries.  mid_o / mid_lse: float32 scratch of
  * max_parts * num_qo_heads * head_dim and max_parts * num_qo_heads (calls that share
  * them must not overlap on the GPU).                                          */
-int be_paged_attn_run(const int32_t* plan_dev, int max_wide, int max_narrow, int narrow_rows,
-                      int max_merge, int max_parts, int page_size, const void* q, int64_t q_row_stride,
-                      const void* paged_kv_cache, const float* kv_scale, int num_pages,
-                      int num_qo_heads, int num_kv_heads, int head_dim, int dtype,
-                      int cache_dtype, float sm_scale, void* out, int64_t out_row_stride,
-                      float* lse, float* mid_o, float* mid_lse, void* stream);
+typedef struct be_paged_attn_args {
+  const int32_t* plan_dev;
+  const void* q;
+  int64_t q_row_stride;
+  const void* paged_kv_cache;
+  const float* kv_scale;
+  void* out;
+  int64_t out_row_stride;
+  float *lse /* or NULL */, *mid_o, *mid_lse;
+  void* stream;
+  int32_t max_wide, max_narrow, narrow_rows, max_merge, max_parts, page_size, num_pages,
+      num_qo_heads, num_kv_heads, head_dim, dtype, cache_dtype;
+  float sm_scale;
+  int32_t reserved;
+} be_paged_attn_args;
+int be_paged_attn_run(const be_paged_attn_args* args);
 
 /* ------------------------------------------------------------------------
  * Decoder-layer kernels of the model runner (the reference runs these as

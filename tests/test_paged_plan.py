@@ -178,10 +178,10 @@ def _append(**kw):
     a = dict(k=16, v=16, ks=1, vs=1, b=16, pos=16, rp=None, ki=16, kp=16, n=4, f=None, cache=16,
              scale=16, pages=8, ps=16, h=2, d=64, dt=_lib.BE_BF16, cdt=_lib.BE_E4M3, ws=None, wn=0)
     a.update(kw)
+    order = "k v ks vs b pos rp ki kp f cache scale ws wn stream n pages ps h d dt cdt".split()
+    a["stream"] = 0
     return lib().be_rope_append_paged_kv(
-        a["k"], a["v"], a["ks"], a["vs"], a["b"], a["pos"], a["rp"], a["ki"], a["kp"], a["n"],
-        a["f"], a["cache"], a["scale"], a["pages"], a["ps"], a["h"], a["d"], a["dt"], a["cdt"],
-        a["ws"], a["wn"], None)
+        _lib.ROPE_APPEND_ARGS.pack(*[a[x] or 0 for x in order], 0))
 
 
 @pytest.mark.parametrize("kw,rc", [
@@ -204,9 +204,9 @@ def test_run_refuses(kw):
     a = dict(q=16, qs=512, cache=16, scale=16, hq=4, d=64, dt=_lib.BE_BF16, cdt=_lib.BE_E4M3,
              parts=0, narrow=1, rows=4, pages=8)
     a.update(kw)
-    rc = lib().be_paged_attn_run(16, 0, a["narrow"], a["rows"], 0, a["parts"], 16, a["q"], a["qs"], a["cache"],
-                                 a["scale"], a["pages"], a["hq"], 2, a["d"], a["dt"], a["cdt"], 1.0, 16, 512,
-                                 None, None, None, None)
+    rc = lib().be_paged_attn_run(_lib.PAGED_ATTN_ARGS.pack(
+        16, a["q"] or 0, a["qs"], a["cache"], a["scale"] or 0, 16, 512, 0, 0, 0, 0, 0, a["narrow"],
+        a["rows"], 0, a["parts"], 16, a["pages"], a["hq"], 2, a["d"], a["dt"], a["cdt"], 1.0, 0))
     assert rc == _lib.BE_EINVAL
 
 
@@ -221,3 +221,25 @@ def test_host_tensors_are_refused():
         read_paged_kv_cache(pool, one, scale)
     with pytest.raises(ValueError, match="float8"):
         read_paged_kv_cache(torch.zeros((2, 2, 16, 2, 64)), one, scale)
+
+
+def test_argument_blocks_match_the_header():
+    """The packed blocks have the sizes that the C structs of the header have, and no block is refused."""
+    import os
+    import re
+    src = open(os.path.join(os.path.dirname(__file__), "..", "include", "beam_b200.h")).read()
+    src = re.sub(r"/\*.*?\*/", "", src, flags=re.S)
+    for name, packed in (("be_rope_append_args", _lib.ROPE_APPEND_ARGS),
+                         ("be_paged_attn_args", _lib.PAGED_ATTN_ARGS)):
+        body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), src, re.S).group(1)
+        fmt = ""
+        for decl in body.split(";"):
+            fields = decl.strip()
+            if fields:
+                kind = "Q" if "*" in fields else "q" if "int64_t" in fields else "f" if "float" in fields else "i"
+                fmt += kind * len(fields.split(","))
+        assert packed.size == sum({"Q": 8, "q": 8, "i": 4, "f": 4}[c] for c in fmt)
+        plain = re.sub(r"(\d+)(\w)", lambda m: m.group(2) * int(m.group(1)), packed.format[1:])
+        assert plain == fmt
+    assert lib().be_paged_attn_run(None) == _lib.BE_EINVAL
+    assert lib().be_rope_append_paged_kv(None) == _lib.BE_EINVAL
