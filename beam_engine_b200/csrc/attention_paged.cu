@@ -23,13 +23,12 @@
 // may be in any order as long as Q and K (or V and O) agree, so a lane reads 16-byte pieces: lane
 // (r, c) = (lane / 4, lane % 4) has pieces c, c + 4, ... of tokens r and r + 8 for S and piece r of
 // tokens 2c, 2c + 1, 2c + 8, 2c + 9 for O; pieces are swizzled by the token so that both
-// reads hit every bank once.  The ring keeps 3 steps in flight per warp (12 KB at 128 dims in
-// 8 bits, 12 warps per SM); loading straight into registers kept one and ran at a quarter of
+// reads hit every bank once.  The ring keeps 2 or 3 steps in flight per warp (8 KB at 128 dims in
+// 8 bits, 16 warps per SM); loading straight into registers kept one and ran at a quarter of
 // HBM's rate (1 600 GB/s over 64 requests of up to 4 096 tokens).
 //
-// Bound: HBM.  64 requests, window 4096 + 4 of 16 000 tokens, bf16: 178 us, 6.0 TB/s; 64 requests of up to
-// 4 096 tokens in 8 bits: 90 us, 4.5 TB/s (half as many bytes per instruction; 162 registers allow 12
-// warps per SM, which issue in half of all cycles).  Four warps of a CTA split the item's tokens and fold their states
+// Bound: HBM.  64 requests, window 4096 + 4 of 16 000 tokens, bf16: 172 us, 6.3 TB/s; 64 requests of up to
+// 4 096 tokens in 8 bits: 89 us, 4.6 TB/s (half as many bytes per instruction).  Four warps of a CTA split the item's tokens and fold their states
 // through shared memory; items that split a sequence leave partial rows for merge_kernel.
 #include <atomic>
 
@@ -119,8 +118,10 @@ template <typename CT, int D, int NB>
 struct PnRing {
   static constexpr int ROWB = D * CacheElt<CT>::bytes;
   static constexpr int STAGE = 2 * 16 * ROWB + 256;
-  static constexpr int STAGES = ROWB > 128 ? 3 : 4;
-  static constexpr int CTAS = ROWB > 128 ? 2 : 3;      // per SM
+  // up to 8 rows of 128 bytes: 4 CTAs per SM with 2 steps ahead beat 3 CTAs with 3 (shared prefixes with
+  // 128 suffixes 38 us against 41; one sequence of 131 072 tokens 60.6 against 59)
+  static constexpr int STAGES = ROWB <= 128 && NB == 2 ? 4 : 3;
+  static constexpr int CTAS = ROWB > 128 ? 2 : NB == 1 ? 4 : 3;      // per SM
   static constexpr int FOLD = 4 * 8 * NB * (D + 4) * 4;   // the warps' O at the end
   static constexpr int BYTES = 4 * STAGES * STAGE > FOLD ? 4 * STAGES * STAGE : FOLD;
 };

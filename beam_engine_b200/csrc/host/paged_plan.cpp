@@ -93,7 +93,8 @@ int wide_chunk(const std::vector<Tile>& tiles, int64_t total_steps, int sms, int
   return best_chunk;
 }
 
-// Tokens per narrow item.  About 3 CTAs share an SM, so (item, KV head) pairs run 3 x SMs at a time;
+// Tokens per narrow item.  (item, KV head) pairs run up to 4 x SMs at a time (window 4096 over 64 requests,
+// bf16: 172 us planned for 4 per SM, 185 for 3 or 6);
 // whole tiles and cuts at fractions of the average share are tried longest first, with 192 tokens'
 // time for a CTA's start and end and 512 for the merge launch that a cut brings.
 int narrow_chunk(const std::vector<Tile>& tiles, int64_t total, int sms, int hkv) {
@@ -101,7 +102,7 @@ int narrow_chunk(const std::vector<Tile>& tiles, int64_t total, int sms, int hkv
   for (const Tile& t : tiles)
     if (!t.wide) longest = std::max(longest, t.n);
   if (longest == 0) return 1 << 28;
-  const int slots = std::max(1, sms * 3 / hkv);
+  const int slots = std::max(1, sms * 4 / hkv);
   const int64_t share = std::max<int64_t>(1, total / slots);
   int best_chunk = 1 << 28;
   int64_t best = INT64_MAX;
