@@ -231,38 +231,46 @@ __global__ void __launch_bounds__(128, PnRing<CT, D, NB>::CTAS) paged_narrow_ker
   auto chunk_at = [](int t, int ch) {
     return (ROWB == 64 ? ch ^ (((t >> 2) & 1) << 1) : ch ^ ((t & 6) ^ ((t & 1) << 2))) << 4;
   };
-  auto page_of = [&](int v) -> int {           // page id of token v + (lane & 15)
-    v += lane & 15;
-    if (v >= w.v_end) return -1;
-    const int t = token_t(v);
+  auto page_of = [&](int v) -> int {           // page id of token v + (lane & 15), if it is there
+    const int t = token_t(min(v + (lane & 15), w.v_end - 1));
     return ld_early4(kvlist + (ps_shift >= 0 ? t >> ps_shift : t / p.ps));
   };
-  // this lane's part of a step's copies: chunk ch of tokens k0, k0 + 32 / CHR, ...
+  // this lane's part of a step's copies: chunk ch of tokens k0, k0 + KSTEP, ...
+  constexpr int KSTEP = 32 / CHR, COPIES = 16 / KSTEP;
   const int k0 = lane / CHR, ch = lane % CHR;
+  const uint32_t step_bytes = (uint32_t)row_step;
   const int64_t v_plane = row_step * p.ps;
+  const char* src0 = base + ch * 16;
+  // (the compiler does not see that the swizzle of a lane's tokens has few values)
+  uint32_t copy_at[COPIES > 1 ? 2 : 1];
+#pragma unroll
+  for (int i = 0; i < (COPIES > 1 ? 2 : 1); ++i)
+    copy_at[i] = smem_u32(ring) + row_at(k0 + i * KSTEP) + chunk_at(k0 + i * KSTEP, ch);
+  constexpr bool TWO = ROWB == 128;            // tokens 2 KSTEP = 8 apart: the same swizzle
   // Requests the 16 tokens from v0 into stage st; tokens that are not there are zeros.
   auto issue = [&](int st, int v0, int page) {
     if (v0 < w.v_end) {
       char* dst = ring + st * Ring::STAGE;
-      const int v = v0 + (lane & 15);
-      const bool has = page >= 0 && page < p.num_pages;
-      if (!has && v < w.v_end) flag_range_error();
-      const int t = token_t(v);
-      const int row = has ? page * 2 * p.ps + (ps_shift >= 0 ? t & (p.ps - 1) : t % p.ps) : -1;
+      const int v = v0 + (lane & 15), t = token_t(v);
+      const bool has = v < w.v_end && (unsigned)page < (unsigned)p.num_pages;
+      const int row = has ? page * 2 * p.ps + (ps_shift >= 0 ? t & (p.ps - 1) : t % p.ps) : 0;
       const unsigned valid = __ballot_sync(0xffffffffu, has) & 0xffffu;
+      if (valid != (w.v_end - v0 >= 16 ? 0xffffu : (1u << (w.v_end - v0)) - 1u)) flag_range_error();
       if (lane == 0) *reinterpret_cast<unsigned*>(dst + 2 * 16 * ROWB + 128) = valid;
 #pragma unroll
-      for (int i = 0; i < 16 * CHR / 32; ++i) {
-        const int k = k0 + i * (32 / CHR);
-        const int rk = __shfl_sync(0xffffffffu, row, k);
-        const char* src = base + (int64_t)max(rk, 0) * row_step + ch * 16;
-        const uint32_t to = smem_u32(dst + row_at(k) + chunk_at(k, ch));
-        cp_async16(to, src, rk >= 0);
-        cp_async16(to + 16 * ROWB, src + v_plane, rk >= 0);
+      for (int i = 0; i < COPIES; ++i) {
+        const int k = k0 + i * KSTEP;
+        const uint32_t rk = __shfl_sync(0xffffffffu, (uint32_t)row, k);
+        const char* src = src0 + (uint64_t)rk * step_bytes;
+        const uint32_t to = TWO ? copy_at[i & 1] + st * Ring::STAGE + (i >> 1) * (2 * KSTEP * ROWB)
+                                : smem_u32(dst + row_at(k) + chunk_at(k, ch));
+        const bool there = (valid >> k) & 1;
+        cp_async16(to, src, there);
+        cp_async16(to + 16 * ROWB, src + v_plane, there);
       }
       if constexpr (Q8) {
-        const float* s = p.scale + (int64_t)max(page, 0) * 2 * p.hkv + kvh + (lane < 16 ? 0 : p.hkv);
-        cp_async4(smem_u32(dst + 2 * 16 * ROWB + lane * 4), has ? s : p.scale, has);
+        const float* s = p.scale + (has ? (int64_t)page * 2 * p.hkv + kvh + (lane < 16 ? 0 : p.hkv) : 0);
+        cp_async4(smem_u32(dst + 2 * 16 * ROWB + lane * 4), s, has);
       }
     }
     cp_commit();
@@ -288,6 +296,7 @@ __global__ void __launch_bounds__(128, PnRing<CT, D, NB>::CTAS) paged_narrow_ker
     page_next = page_of(v0 + 64 * (j + 1));
     issue(j, v0 + 64 * j, page);
   }
+  const int k_at = row_at(r) + chunk_at(r, c);
 #pragma unroll 1
   for (; v0 < w.v_end; v0 += 64) {
     cp_wait<Ring::STAGES - 2>();
@@ -301,8 +310,11 @@ __global__ void __launch_bounds__(128, PnRing<CT, D, NB>::CTAS) paged_narrow_ker
     float s[NB][4] = {};
 #pragma unroll
     for (int k = 0; k < KP; ++k) {
-      const uint4 x0 = *reinterpret_cast<const uint4*>(stage + row_at(r) + chunk_at(r, k * 4 + c));
-      const uint4 x1 = *reinterpret_cast<const uint4*>(stage + row_at(r + 8) + chunk_at(r + 8, k * 4 + c));
+      const int at = ROWB == 64 ? 0 : k_at ^ (k * 64);       // pieces 4 apart: one bit of the chunk
+      const uint4 x0 = *reinterpret_cast<const uint4*>(
+          stage + (ROWB == 64 ? row_at(r) + chunk_at(r, k * 4 + c) : at));
+      const uint4 x1 = *reinterpret_cast<const uint4*>(
+          stage + (ROWB == 64 ? row_at(r + 8) + chunk_at(r + 8, k * 4 + c) : at + 8 * ROWB));
       const uint32_t wa[4] = {x0.x, x0.y, x0.z, x0.w}, wb[4] = {x1.x, x1.y, x1.z, x1.w};
       if constexpr (Q8) {
 #pragma unroll
