@@ -27,8 +27,9 @@
 // 8 bits, 16 warps per SM); loading straight into registers kept one and ran at a quarter of
 // HBM's rate (1 600 GB/s over 64 requests of up to 4 096 tokens).
 //
-// Bound: HBM.  64 requests, window 4096 + 4 of 16 000 tokens, bf16: 172 us, 6.3 TB/s; 64 requests of up to
-// 4 096 tokens in 8 bits: 89 us, 4.6 TB/s (half as many bytes per instruction).  Four warps of a CTA split the item's tokens and fold their states
+// Bound: HBM.  64 requests, window 4096 + 4 of 16 000 tokens, bf16: 159 us, 6.75 TB/s; 64 requests of up to
+// 4 096 tokens in 8 bits: 86 us, 4.7 TB/s (half as many bytes per instruction: 412 for 16 tokens' K and
+// V, 64 of them conversions).  Four warps of a CTA split the item's tokens and fold their states
 // through shared memory; items that split a sequence leave partial rows for merge_kernel.
 #include <atomic>
 
@@ -119,7 +120,7 @@ struct PnRing {
   static constexpr int ROWB = D * CacheElt<CT>::bytes;
   static constexpr int STAGE = 2 * 16 * ROWB + 256;
   // up to 8 rows of 128 bytes: 4 CTAs per SM with 2 steps ahead beat 3 CTAs with 3 (shared prefixes with
-  // 128 suffixes 38 us against 41; one sequence of 131 072 tokens 60.6 against 59)
+  // 128 suffixes 38 us against 41; one sequence of 131 072 tokens 3 % slower)
   static constexpr int STAGES = ROWB <= 128 && NB == 2 ? 4 : 3;
   static constexpr int CTAS = ROWB > 128 ? 2 : NB == 1 ? 4 : 3;      // per SM
   static constexpr int FOLD = 4 * 8 * NB * (D + 4) * 4;   // the warps' O at the end
@@ -566,7 +567,7 @@ __global__ void __launch_bounds__(128, PnRing<CT, D, NB>::CTAS) paged_narrow_ker
 
 // merge_kernel's work with a CTA per (query, head): four warps take every fourth partial row.
 // A long sequence split over the GPU leaves dozens of parts for a few rows, and one warp
-// walking them is latency alone (one sequence of 131 072 tokens, 8-bit: 66 us with it, 59 with this).
+// walking them is latency alone (one sequence of 131 072 tokens, 8-bit, when this came: 66 us with it, 59 with this).
 template <typename T, int D>
 __global__ void __launch_bounds__(128) paged_merge_kernel(const PagedParams p) {
   __shared__ __align__(16) float sO[4][D];

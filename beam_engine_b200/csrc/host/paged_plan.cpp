@@ -94,7 +94,7 @@ int wide_chunk(const std::vector<Tile>& tiles, int64_t total_steps, int sms, int
 }
 
 // Tokens per narrow item.  (item, KV head) pairs run up to 4 x SMs at a time (window 4096 over 64 requests,
-// bf16: 172 us planned for 4 per SM, 185 for 3 or 6);
+// bf16, when this came: 172 us planned for 4 per SM, 185 for 3 or 6);
 // whole tiles and cuts at fractions of the average share are tried longest first, with 192 tokens'
 // time for a CTA's start and end and 512 for the merge launch that a cut brings.
 int narrow_chunk(const std::vector<Tile>& tiles, int64_t total, int sms, int hkv) {
