@@ -7,13 +7,19 @@
 // 8-bit caches hold codes: k_t = s_K c_t, v_t = s_V d_t with one scale per (page,
 // KV head).  The codes become halves by one exact conversion per pair and the
 // scales never touch them: s_K multiplies the score (it joins sm_scale), and s_V
-// goes into the exponent,
-//   sum_t exp(x_t) s_V,t d_t = sum_t 2^(x'_t + log2 s_V,t) d_t,  x' = x log2(e),
-// so the running maximum is over x' + log2 s_V, every factor of the second product
-// is at most 2^8, and the denominator is the sum of those factors divided by s_V.
+// goes into the exponent, against a unit u = 2^lref that a warp's O is kept in,
+//   sum_t exp(x_t) s_V,t d_t = u sum_t 2^(x'_t + a_t) d_t,  a = log2(s_V / u),  x' = x log2(e),
+// and the denominator is the sum of those factors times 2^-a.  The factors are fp16 (steps of 2^-24 at
+// least), so a must not take range from x': a stays in [0, 7], and the running maximum
+// is taken 7 lower.  A token whose x' is the largest then has a factor of 1 or more whatever the
+// scales of other pages are (which a value in another dim, or of a token that is not seen,
+// may have set), and no factor passes 2^11.  Pages outside [u, 2^7 u] move u: O is
+// multiplied by the old unit over the new one, an exact power of two in fp32.  Tokens of one step that
+// no single u holds are taken in turns.  Scales may span 2^-40 to 2^40 (O stays below 2^127 when u
+// falls that far: factors of 2^11 of codes of 2^9 over 2^18 tokens are 2^38).
 // bf16 queries of an 8-bit cache are scaled per row by a power of two into half
-// range (exact down to 2^-33 of the row's largest value), so both products run in
-// fp16 with fp32 sums; 16-bit caches use their own type.
+// range (exact down to 2^-25 of the row's largest value: 8 significant bits above fp16's smallest
+// step), so both products run in fp16 with fp32 sums; 16-bit caches use their own type.
 //
 // A warp takes 16 tokens at a time through a ring of its own in shared memory (cp.async by
 // 16 bytes, no barrier between warps) into mma.sync fragments, tokens as the fragments' 16 rows and
@@ -59,6 +65,8 @@ template <typename CT> struct CacheElt { static constexpr int bytes = 2; };
 template <> struct CacheElt<E4M3> { static constexpr int bytes = 1; };
 
 constexpr float kLazyMax = 8.f;       // factors up to 2^8 before O is rescaled
+constexpr float kUnitSpan = 7.f;      // log2 of the V scales that one unit of O serves (8-bit caches)
+constexpr float kLazyMax8 = 4.f;      // narrow tiles over 8 bits: factors up to 2^(7 + 4)
 constexpr float kNoMax = -1e30f;      // running maximum of a row that has seen nothing
 
 // Loads that stay where they are written: a plain load of constant memory is moved down to its
@@ -85,11 +93,6 @@ __device__ __forceinline__ float ld_early4(const float* p) {
 __device__ __forceinline__ float lg2(float x) {      // of normal numbers: the hardware's, exact for 2^n
   float y;
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float rcp(float x) {
-  float y;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 // An 8 x 8 block of halves, one row per four lanes, transposed.
@@ -145,7 +148,7 @@ __global__ void __launch_bounds__(128, PnRing<CT, D, NB>::CTAS) paged_narrow_ker
   constexpr int CHR = ROWB / 16;               // 16-byte chunks per row
   extern __shared__ __align__(128) char ring_raw[];
   float (*sO)[8 * NB][OLD] = reinterpret_cast<float (*)[8 * NB][OLD]>(ring_raw);
-  __shared__ float sM[4][8 * NB], sL[4][8 * NB];
+  __shared__ float sM[4][8 * NB], sL[4][8 * NB], sU[4];
 
   pdl_wait();
   if (p.merge_next) pdl_trigger();   // the merge waits for this grid; another kernel might not
@@ -289,6 +292,8 @@ __global__ void __launch_bounds__(128, PnRing<CT, D, NB>::CTAS) paged_narrow_ker
     l[b][0] = l[b][1] = 0.f;
   }
 
+  constexpr float kHead = Q8 ? kUnitSpan : 0.f, kLazy = Q8 ? kLazyMax8 : kLazyMax;
+  float lref = -1000.f;                        // log2 of O's unit: the first step sets it
   int v0 = w.v_begin + warp * 16, st = 0;
   int page_next = page_of(v0);
 #pragma unroll
@@ -307,202 +312,242 @@ __global__ void __launch_bounds__(128, PnRing<CT, D, NB>::CTAS) paged_narrow_ker
     page_next = page_of(v0 + 64 * Ring::STAGES);
     issue(st == 0 ? Ring::STAGES - 1 : st - 1, v0 + 64 * (Ring::STAGES - 1), page);
     const char* stage = ring + st * Ring::STAGE;
-    // ---- S^T = K Q^T: 16 tokens x 8 NB rows; s[b][i]: token r + 8 (i >> 1), row 8 b + 2c + (i & 1) ----
-    float s[NB][4] = {};
+    unsigned turn = 0xffffu, later = 0;        // tokens of this pass over the step; of passes to come
+    for (;;) {
+      // ---- S^T = K Q^T: 16 tokens x 8 NB rows; s[b][i]: token r + 8 (i >> 1), row 8 b + 2c + (i & 1) ----
+      float s[NB][4] = {};
 #pragma unroll
-    for (int k = 0; k < KP; ++k) {
-      const int at = ROWB == 64 ? 0 : k_at ^ (k * 64);       // pieces 4 apart: one bit of the chunk
-      const uint4 x0 = *reinterpret_cast<const uint4*>(
-          stage + (ROWB == 64 ? row_at(r) + chunk_at(r, k * 4 + c) : at));
-      const uint4 x1 = *reinterpret_cast<const uint4*>(
-          stage + (ROWB == 64 ? row_at(r + 8) + chunk_at(r + 8, k * 4 + c) : at + 8 * ROWB));
-      const uint32_t wa[4] = {x0.x, x0.y, x0.z, x0.w}, wb[4] = {x1.x, x1.y, x1.z, x1.w};
+      for (int k = 0; k < KP; ++k) {
+        const int at = ROWB == 64 ? 0 : k_at ^ (k * 64);       // pieces 4 apart: one bit of the chunk
+        const uint4 x0 = *reinterpret_cast<const uint4*>(
+            stage + (ROWB == 64 ? row_at(r) + chunk_at(r, k * 4 + c) : at));
+        const uint4 x1 = *reinterpret_cast<const uint4*>(
+            stage + (ROWB == 64 ? row_at(r + 8) + chunk_at(r + 8, k * 4 + c) : at + 8 * ROWB));
+        const uint32_t wa[4] = {x0.x, x0.y, x0.z, x0.w}, wb[4] = {x1.x, x1.y, x1.z, x1.w};
+        if constexpr (Q8) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const uint32_t a[4] = {e4m3x2_to_h2(wa[x] & 0xffffu), e4m3x2_to_h2(wb[x] & 0xffffu),
+                                   e4m3x2_to_h2(wa[x] >> 16), e4m3x2_to_h2(wb[x] >> 16)};
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+              mma16816<MT>(s[b], a, qb[b][2 * (k * 4 + x)], qb[b][2 * (k * 4 + x) + 1]);
+          }
+        } else {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const uint32_t a[4] = {wa[2 * x], wb[2 * x], wa[2 * x + 1], wb[2 * x + 1]};
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+              mma16816<MT>(s[b], a, qb[b][2 * (k * 2 + x)], qb[b][2 * (k * 2 + x) + 1]);
+          }
+        }
+      }
+      // ---- scores in base 2, masked ----
+      const unsigned valid = *reinterpret_cast<const unsigned*>(stage + 2 * 16 * ROWB + 128) & turn;
+      const int t_lo = token_t(v0), t_hi = token_t(v0 + 15);
+      const bool full = valid == 0xffffu && (!causal || t_hi <= w.pos0) &&
+                        (!window || t_lo >= pos_hi - w.window || t_hi < w.sink_end);
+      float mult[2] = {1.f, 1.f}, add[2] = {0.f, 0.f}, rsv[2] = {1.f, 1.f};   // tokens r, r + 8
+      bool grew = false;
       if constexpr (Q8) {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const uint32_t a[4] = {e4m3x2_to_h2(wa[x] & 0xffffu), e4m3x2_to_h2(wb[x] & 0xffffu),
-                                 e4m3x2_to_h2(wa[x] >> 16), e4m3x2_to_h2(wb[x] >> 16)};
-#pragma unroll
-          for (int b = 0; b < NB; ++b)
-            mma16816<MT>(s[b], a, qb[b][2 * (k * 4 + x)], qb[b][2 * (k * 4 + x) + 1]);
+        const float* sc = reinterpret_cast<const float*>(stage + 2 * 16 * ROWB);
+        // a V scale of 0 (a block never written) stands for values of 0: any scale will do
+        mult[0] = sc[r];
+        add[0] = lg2(fmaxf(sc[16 + r], 9.0949470177e-13f)) - lref;         // 2^-40
+        rsv[0] = ex2(-add[0]);
+        if (t_hi - t_lo == 15 && ((p.ps | t_lo) & 15) == 0) {              // one page
+          mult[1] = mult[0];
+          add[1] = add[0];
+          rsv[1] = rsv[0];
+        } else {
+          mult[1] = sc[r + 8];
+          add[1] = lg2(fmaxf(sc[24 + r], 9.0949470177e-13f)) - lref;
+          rsv[1] = ex2(-add[1]);
         }
-      } else {
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const uint32_t a[4] = {wa[2 * x], wb[2 * x], wa[2 * x + 1], wb[2 * x + 1]};
-#pragma unroll
-          for (int b = 0; b < NB; ++b)
-            mma16816<MT>(s[b], a, qb[b][2 * (k * 2 + x)], qb[b][2 * (k * 2 + x) + 1]);
-        }
+        grew = fabsf(add[0] - 0.5f * kUnitSpan) > 0.5f * kUnitSpan ||
+               fabsf(add[1] - 0.5f * kUnitSpan) > 0.5f * kUnitSpan;
       }
-    }
-    // ---- scores in base 2, masked ----
-    const unsigned valid = *reinterpret_cast<const unsigned*>(stage + 2 * 16 * ROWB + 128);
-    const int t_lo = token_t(v0), t_hi = token_t(v0 + 15);
-    const bool full = valid == 0xffffu && (!causal || t_hi <= w.pos0) &&
-                      (!window || t_lo >= pos_hi - w.window || t_hi < w.sink_end);
-    float mult[2] = {1.f, 1.f}, add[2] = {0.f, 0.f}, rsv[2] = {1.f, 1.f};   // tokens r, r + 8
-    if constexpr (Q8) {
-      const float* sc = reinterpret_cast<const float*>(stage + 2 * 16 * ROWB);
-      // a V scale of 0 (a block never written) stands for values of 0: any scale will do
-      mult[0] = sc[r];
-      const float sv0 = fmaxf(sc[16 + r], 9.0949470177e-13f);            // 2^-40
-      add[0] = lg2(sv0);
-      rsv[0] = rcp(sv0);
-      if (t_hi - t_lo == 15 && ((p.ps | t_lo) & 15) == 0) {              // one page
-        mult[1] = mult[0];
-        add[1] = add[0];
-        rsv[1] = rsv[0];
-      } else {
-        mult[1] = sc[r + 8];
-        const float sv1 = fmaxf(sc[24 + r], 9.0949470177e-13f);
-        add[1] = lg2(sv1);
-        rsv[1] = rcp(sv1);
-      }
-    }
-    bool grew = false;
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int h = i >> 1, e = i & 1;
-        float x = Q8 ? fmaf(s[b][i], row_scale[b][e] * mult[h], add[h]) : s[b][i] * row_scale[b][e];
-        if (!full) {
-          const int k = r + 8 * h, t = token_t(v0 + k);
-          const bool see = ((valid >> k) & 1) && (!causal || t <= pos_r[b][e]) &&
-                           (!window || t >= pos_r[b][e] - w.window || t < w.sink_end);
-          x = see ? x : -INFINITY;
-        }
-        s[b][i] = x;
-        grew |= x > m[b][e] + kLazyMax;
-      }
-    // ---- the running maximum moves only when a factor would pass 2^8 ----
-    if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float mx = fmaxf(s[b][e], s[b][2 + e]);
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          mx = fmaxf(mx, m[b][e]);
-          const float f = ex2(m[b][e] - mx);
-          m[b][e] = mx;
-          l[b][e] *= f;
+        for (int i = 0; i < 4; ++i) {
+          const int h = i >> 1, e = i & 1;
+          float x = Q8 ? fmaf(s[b][i], row_scale[b][e] * mult[h], add[h]) : s[b][i] * row_scale[b][e];
+          if (!full) {
+            const int k = r + 8 * h, t = token_t(v0 + k);
+            const bool see = ((valid >> k) & 1) && (!causal || t <= pos_r[b][e]) &&
+                             (!window || t >= pos_r[b][e] - w.window || t < w.sink_end);
+            x = see ? x : -INFINITY;
+          }
+          s[b][i] = x;
+          grew |= x > m[b][e] + (kHead + kLazy);
+        }
+      // ---- O's unit moves when a page's scale leaves its span, the running maximum only when a factor
+      // would pass 2^8 (2^11) ----
+      if (__any_sync(0xffffffffu, grew)) {
+        if constexpr (Q8) {
+          const bool has0 = (valid >> r) & 1, has1 = (valid >> (r + 8)) & 1;
+          float lo = fminf(has0 ? add[0] : INFINITY, has1 ? add[1] : INFINITY);
+          float hi = fmaxf(has0 ? add[0] : -INFINITY, has1 ? add[1] : -INFINITY);
 #pragma unroll
-          for (int j = 0; j < KS; ++j) {
-            o[b][j][e] *= f;
-            o[b][j][2 + e] *= f;
+          for (int off = 4; off < 32; off *= 2) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+          }
+          if (lo <= hi && (lo < 0.f || hi > kUnitSpan)) {       // the same in every lane
+            // the tokens' span in the middle of the new unit's; from the smallest if it is wider: the
+            // tokens past it wait for a turn of their own
+            const float from = floorf(lo), slack = kUnitSpan - (hi - from);
+            const float by = slack >= 0.f ? from - floorf(0.5f * slack) : from;
+            const float f = ex2(fminf(-by, 126.f));
+            lref += by;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+              for (int j = 0; j < KS; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[b][j][i] *= f;
+            // (lanes of one r agree: lane 4 r tells of tokens r and r + 8)
+            unsigned out = __ballot_sync(0xffffffffu, c == 0 && has0 && add[0] - by > kUnitSpan) |
+                           __ballot_sync(0xffffffffu, c == 1 && has1 && add[1] - by > kUnitSpan);
+            unsigned wait = 0;
+            for (int k = 0; k < 8; ++k)
+              wait |= ((out >> (4 * k)) & 1) << k | ((out >> (4 * k + 1)) & 1) << (k + 8);
+            later |= wait;
+            turn = valid & ~wait;
+            continue;                                           // the scores again, in the new unit
           }
         }
-    }
-    // P^T as the second operand: the fragment's 8 x 8 blocks of halves, transposed
-    uint32_t pb[NB][2];
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float a0 = ex2(s[b][2 * h] - m[b][0]), a1 = ex2(s[b][2 * h + 1] - m[b][1]);
-        l[b][0] = fmaf(a0, rsv[h], l[b][0]);
-        l[b][1] = fmaf(a1, rsv[h], l[b][1]);
-        s[b][2 * h] = a0;
-        s[b][2 * h + 1] = a1;
-        pb[b][h] = transpose8(pack2<MT>(a0, a1));
+          for (int e = 0; e < 2; ++e) {
+            float mx = fmaxf(s[b][e], s[b][2 + e]);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            mx = fmaxf(mx - kHead, m[b][e]);
+            const float f = ex2(m[b][e] - mx);
+            m[b][e] = mx;
+            l[b][e] *= f;
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+              o[b][j][e] *= f;
+              o[b][j][2 + e] *= f;
+            }
+          }
       }
-    // ---- V fragments' words: tokens 2c, 2c + 1, 2c + 8, 2c + 9 ----
-    uint32_t vraw[4][VP * VB / 4];
+      // P^T as the second operand: the fragment's 8 x 8 blocks of halves, transposed
+      uint32_t pb[NB][2];
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const int t = (n >> 1) * 8 + 2 * c + (n & 1);
-      const char* src = stage + 16 * ROWB + row_at(t);
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int k = 0; k < VP; ++k) {
-        if constexpr (VB == 16) {
-          const uint4 x = *reinterpret_cast<const uint4*>(src + chunk_at(t, k * 8 + r));
-          vraw[n][4 * k] = x.x; vraw[n][4 * k + 1] = x.y;
-          vraw[n][4 * k + 2] = x.z; vraw[n][4 * k + 3] = x.w;
-        } else {
-          const uint2 x = *reinterpret_cast<const uint2*>(src + chunk_at(t, r >> 1) + (r & 1) * 8);
-          vraw[n][0] = x.x; vraw[n][1] = x.y;
+        for (int h = 0; h < 2; ++h) {
+          const float a0 = ex2(s[b][2 * h] - m[b][0]), a1 = ex2(s[b][2 * h + 1] - m[b][1]);
+          l[b][0] = fmaf(a0, rsv[h], l[b][0]);
+          l[b][1] = fmaf(a1, rsv[h], l[b][1]);
+          s[b][2 * h] = a0;
+          s[b][2 * h + 1] = a1;
+          pb[b][h] = transpose8(pack2<MT>(a0, a1));
+        }
+      // ---- V fragments' words: tokens 2c, 2c + 1, 2c + 8, 2c + 9 ----
+      uint32_t vraw[4][VP * VB / 4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int t = (n >> 1) * 8 + 2 * c + (n & 1);
+        const char* src = stage + 16 * ROWB + row_at(t);
+#pragma unroll
+        for (int k = 0; k < VP; ++k) {
+          if constexpr (VB == 16) {
+            const uint4 x = *reinterpret_cast<const uint4*>(src + chunk_at(t, k * 8 + r));
+            vraw[n][4 * k] = x.x; vraw[n][4 * k + 1] = x.y;
+            vraw[n][4 * k + 2] = x.z; vraw[n][4 * k + 3] = x.w;
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(src + chunk_at(t, r >> 1) + (r & 1) * 8);
+            vraw[n][0] = x.x; vraw[n][1] = x.y;
+          }
         }
       }
-    }
-    // ---- values that are not finite and not seen by every row: out of the product (0 * NaN is
-    // NaN), added to the rows that see them ----
-    if (!full) {
-      bool odd = false;
+      // ---- values that are not finite and not seen by every row: out of the product (0 * NaN is
+      // NaN), added to the rows that see them ----
+      if (!full) {
+        bool odd = false;
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+        for (int n = 0; n < 4; ++n)
 #pragma unroll
-        for (int k = 0; k < VP * VB / 4; ++k) odd |= word_not_finite<CT>(vraw[n][k]);
-      if (__any_sync(0xffffffffu, odd)) {
+          for (int k = 0; k < VP * VB / 4; ++k) odd |= word_not_finite<CT>(vraw[n][k]);
+        if (__any_sync(0xffffffffu, odd)) {
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          bool mine = false;
+          for (int n = 0; n < 4; ++n) {
+            bool mine = false;
 #pragma unroll
-          for (int k = 0; k < VP * VB / 4; ++k) mine |= word_not_finite<CT>(vraw[n][k]);
-          // the token's row is spread over the lanes with this c
-          unsigned any = __ballot_sync(0xffffffffu, mine);
-          any &= 0x11111111u << c;
-          if (any)
+            for (int k = 0; k < VP * VB / 4; ++k) mine |= word_not_finite<CT>(vraw[n][k]);
+            // the token's row is spread over the lanes with this c
+            unsigned any = __ballot_sync(0xffffffffu, mine);
+            any &= 0x11111111u << c;
+            if (any)
 #pragma unroll
-            for (int k = 0; k < VP * VB / 4; ++k) vraw[n][k] = 0;
-        }
+              for (int k = 0; k < VP * VB / 4; ++k) vraw[n][k] = 0;
+          }
 #pragma unroll 1
-        for (int k = 0; k < 16; ++k) {
-          if (!((valid >> k) & 1)) continue;
-          const char* row_v = stage + 16 * ROWB + row_at(k);
-          bool has = false;
-          for (int b = lane * 4; b < ROWB; b += 128)
-            has |= word_not_finite<CT>(*reinterpret_cast<const uint32_t*>(row_v + b));
-          if (!__any_sync(0xffffffffu, has)) continue;
-          const int src = (k & 7) * 4 + c;     // the lane with this token's probabilities
+          for (int k = 0; k < 16; ++k) {
+            if (!((valid >> k) & 1)) continue;
+            const char* row_v = stage + 16 * ROWB + row_at(k);
+            bool has = false;
+            for (int b = lane * 4; b < ROWB; b += 128)
+              has |= word_not_finite<CT>(*reinterpret_cast<const uint32_t*>(row_v + b));
+            if (!__any_sync(0xffffffffu, has)) continue;
+            const int src = (k & 7) * 4 + c;     // the lane with this token's probabilities
 #pragma unroll
-          for (int b = 0; b < NB; ++b) {
-            const float a0 = __shfl_sync(0xffffffffu, s[b][0], src), a1 = __shfl_sync(0xffffffffu, s[b][1], src);
-            const float a2 = __shfl_sync(0xffffffffu, s[b][2], src), a3 = __shfl_sync(0xffffffffu, s[b][3], src);
-            const float q0 = k < 8 ? a0 : a2, q1 = k < 8 ? a1 : a3;
+            for (int b = 0; b < NB; ++b) {
+              const float a0 = __shfl_sync(0xffffffffu, s[b][0], src), a1 = __shfl_sync(0xffffffffu, s[b][1], src);
+              const float a2 = __shfl_sync(0xffffffffu, s[b][2], src), a3 = __shfl_sync(0xffffffffu, s[b][3], src);
+              const float q0 = k < 8 ? a0 : a2, q1 = k < 8 ? a1 : a3;
 #pragma unroll
-            for (int i = 0; i < 2 * KS; ++i) {
-              const int at = ((i / VW) * 8 * VW + r * VW + i % VW) * EB;    // byte of the row
-              const char* src_v = row_v + chunk_at(k, at >> 4) + (at & 15);
-              float val;
-              if constexpr (Q8) {
-                const uint32_t h2 = e4m3x2_to_h2(*reinterpret_cast<const uint8_t*>(src_v));
-                val = __low2float(*reinterpret_cast<const __half2*>(&h2));
-              } else {
-                val = to_f(*reinterpret_cast<const T*>(src_v));
+              for (int i = 0; i < 2 * KS; ++i) {
+                const int at = ((i / VW) * 8 * VW + r * VW + i % VW) * EB;    // byte of the row
+                const char* src_v = row_v + chunk_at(k, at >> 4) + (at & 15);
+                float val;
+                if constexpr (Q8) {
+                  const uint32_t h2 = e4m3x2_to_h2(*reinterpret_cast<const uint8_t*>(src_v));
+                  val = __low2float(*reinterpret_cast<const __half2*>(&h2));
+                } else {
+                  val = to_f(*reinterpret_cast<const T*>(src_v));
+                }
+                float* acc = &o[b][i / 2][(i & 1) * 2];
+                if (q0 > 0.f) acc[0] = fmaf(q0, val, acc[0]);
+                if (q1 > 0.f) acc[1] = fmaf(q1, val, acc[1]);
               }
-              float* acc = &o[b][i / 2][(i & 1) * 2];
-              if (q0 > 0.f) acc[0] = fmaf(q0, val, acc[0]);
-              if (q1 > 0.f) acc[1] = fmaf(q1, val, acc[1]);
             }
           }
         }
       }
-    }
-    // ---- O^T += V^T P^T ----
+      // ---- O^T += V^T P^T ----
 #pragma unroll
-    for (int k = 0; k < VP * VB / 4; ++k) {
-      if constexpr (Q8) {
-        const uint32_t a01 = prmt(vraw[0][k], vraw[1][k], 0x5140), a23 = prmt(vraw[0][k], vraw[1][k], 0x7362);
-        const uint32_t b01 = prmt(vraw[2][k], vraw[3][k], 0x5140), b23 = prmt(vraw[2][k], vraw[3][k], 0x7362);
-        const uint32_t x[4] = {e4m3x2_to_h2(a01 & 0xffffu), e4m3x2_to_h2(a01 >> 16),
-                               e4m3x2_to_h2(b01 & 0xffffu), e4m3x2_to_h2(b01 >> 16)};
-        const uint32_t y[4] = {e4m3x2_to_h2(a23 & 0xffffu), e4m3x2_to_h2(a23 >> 16),
-                               e4m3x2_to_h2(b23 & 0xffffu), e4m3x2_to_h2(b23 >> 16)};
+      for (int k = 0; k < VP * VB / 4; ++k) {
+        if constexpr (Q8) {
+          const uint32_t a01 = prmt(vraw[0][k], vraw[1][k], 0x5140), a23 = prmt(vraw[0][k], vraw[1][k], 0x7362);
+          const uint32_t b01 = prmt(vraw[2][k], vraw[3][k], 0x5140), b23 = prmt(vraw[2][k], vraw[3][k], 0x7362);
+          const uint32_t x[4] = {e4m3x2_to_h2(a01 & 0xffffu), e4m3x2_to_h2(a01 >> 16),
+                                 e4m3x2_to_h2(b01 & 0xffffu), e4m3x2_to_h2(b01 >> 16)};
+          const uint32_t y[4] = {e4m3x2_to_h2(a23 & 0xffffu), e4m3x2_to_h2(a23 >> 16),
+                                 e4m3x2_to_h2(b23 & 0xffffu), e4m3x2_to_h2(b23 >> 16)};
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          mma16816<MT>(o[b][2 * k], x, pb[b][0], pb[b][1]);
-          mma16816<MT>(o[b][2 * k + 1], y, pb[b][0], pb[b][1]);
+          for (int b = 0; b < NB; ++b) {
+            mma16816<MT>(o[b][2 * k], x, pb[b][0], pb[b][1]);
+            mma16816<MT>(o[b][2 * k + 1], y, pb[b][0], pb[b][1]);
+          }
+        } else {
+          const uint32_t x[4] = {prmt(vraw[0][k], vraw[1][k], 0x5410), prmt(vraw[0][k], vraw[1][k], 0x7632),
+                                 prmt(vraw[2][k], vraw[3][k], 0x5410), prmt(vraw[2][k], vraw[3][k], 0x7632)};
+#pragma unroll
+          for (int b = 0; b < NB; ++b) mma16816<MT>(o[b][k], x, pb[b][0], pb[b][1]);
         }
-      } else {
-        const uint32_t x[4] = {prmt(vraw[0][k], vraw[1][k], 0x5410), prmt(vraw[0][k], vraw[1][k], 0x7632),
-                               prmt(vraw[2][k], vraw[3][k], 0x5410), prmt(vraw[2][k], vraw[3][k], 0x7632)};
-#pragma unroll
-        for (int b = 0; b < NB; ++b) mma16816<MT>(o[b][k], x, pb[b][0], pb[b][1]);
       }
+      if (!Q8 || later == 0) break;
+      turn = later;
+      later = 0;
     }
     st = st + 1 == Ring::STAGES ? 0 : st + 1;
   }
@@ -516,6 +561,7 @@ __global__ void __launch_bounds__(128, PnRing<CT, D, NB>::CTAS) paged_narrow_ker
     for (int e = 0; e < 2; ++e) {
 #pragma unroll
       for (int off = 4; off < 32; off *= 2) l[b][e] += __shfl_xor_sync(0xffffffffu, l[b][e], off);
+      if (lane == 0 && b == 0 && e == 0) sU[warp] = Q8 ? ex2(lref) : 1.f;
       if (r == 0) {
         sM[warp][8 * b + 2 * c + e] = m[b][e];
         sL[warp][8 * b + 2 * c + e] = l[b][e];
@@ -534,6 +580,7 @@ __global__ void __launch_bounds__(128, PnRing<CT, D, NB>::CTAS) paged_narrow_ker
   for (int k = 0; k < 4; ++k) {
     f[k] = ex2(sM[k][row] - mx);
     den += f[k] * sL[k][row];
+    if constexpr (Q8) f[k] *= sU[k];
   }
   const float inv = den != 0.f ? 1.f / den : 0.f;
   const int qi = row / g, head = kvh * g + row % g;

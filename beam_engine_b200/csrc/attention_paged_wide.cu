@@ -26,8 +26,15 @@
 // (512 allocated).  S of half j + 2 overwrites P of half j: both products come from one thread,
 // and the tensor core runs them in the order of issue.
 //
-// 8-bit caches: as in the narrow kernel the codes become halves by one exact conversion and
-// the scales stay out of the products.  x = s_K (q . c) and log2 s_V joins the exponent, so a group of
+// 8-bit caches: as in the narrow kernel the codes become halves by one exact conversion.  s_K multiplies
+// the score.  s_V = 2^E mu with mu in [1, 2): the loaders multiply V's halves by 2^(E - u), u the largest E of
+// the first step's tokens, which is exact from 2^-15 (codes down to 2^-9, fp16 down to 2^-24) to 2^7
+// (448 * 2^7 = 57 344), and log2 mu joins the exponent.  P then has fp16's range to itself (2^-24 to 2^15), whatever the
+// scales of other pages are.  Values of tokens outside those 23 binary orders are 0 in that pass over the
+// item's tokens, and where one has a code that is not 0 the item is walked again for it: a pass
+// per 23 orders, from the lowest up (O times 2^-23 per window in between), with the maximum and
+// sum of the first.  (log2 s_V as a whole in the exponent would need no pass, but a page whose scale is
+// 2^25 above the others' takes their factors below fp16's smallest.)  A group of
 // 8 tokens of one page costs one shared-memory read and three operations per row.  The
 // planner aligns ranges to 8 tokens; pages that are no multiple of 8 take scales token by token.
 //
@@ -53,6 +60,8 @@ constexpr int PW_SOFT = 16, PW_LOADERS = 4;    // softmax warps, loader warps; a
 constexpr int PW_THREADS = (PW_SOFT + PW_LOADERS + 2) * 32;
 constexpr int PW_HALF = PW_TOK * 128;          // 64 dims of 128 rows
 constexpr int PW_STAGES = 2;
+// exponents of V scales that one pass serves, relative to its unit
+constexpr int PW_LOW = -15, PW_SPAN = 23;
 
 template <int D>
 struct PwSmem {
@@ -62,7 +71,7 @@ struct PwSmem {
   static constexpr int RS = TAB + 4 * PW_TOK * 16;      // scales of 4 steps' tokens
   static constexpr int MX = RS + 256 * 4;               // scales of the rows
   static constexpr int BAR = MX + 2 * 256 * 4;          // the threads' maxima, then sums
-  static constexpr int BYTES = BAR + 256 + 1024;
+  static constexpr int BYTES = BAR + 256 + 1024;        // (32 slots of 8 bytes; the alignment)
 };
 
 // The elected lane's 1; whole warps call these.
@@ -149,6 +158,12 @@ __device__ __forceinline__ void tmem_ld16_nw(uint32_t taddr, uint32_t* r) {
       : "r"(taddr));
 }
 
+__device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
 // element x of a 16-bit pair: set to zero if not finite
 template <typename T>
 __device__ __forceinline__ uint32_t zero_not_finite(uint32_t w) {
@@ -224,9 +239,11 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
   volatile int* odd = reinterpret_cast<volatile int*>(bars + 24);   // [2] per V stage: step + 1
   volatile int* gone = reinterpret_cast<volatile int*>(bars + 25);  // [4]: step + 1 that misses a page
   volatile int* marked = reinterpret_cast<volatile int*>(bars + 28);   // some row's odd_mask is set
+  volatile int* unit = reinterpret_cast<volatile int*>(bars + 29);      // u of the first pass
+  volatile uint32_t* needed = reinterpret_cast<volatile uint32_t*>(bars + 30);   // windows: bit 16 + k
   uint32_t* odd_mask = reinterpret_cast<uint32_t*>(smem + SM::ODD);  // [256][2][D / 32]
   // per token of the last 4 steps (the loaders are at most 3 past the softmax, and write a step's
-  // entries once V of the third before is used up): s_K, log2 s_V, 1 / s_V
+  // entries once V of the third before is used up): s_K, log2 mu, 1 / mu
   float4* tab = reinterpret_cast<float4*>(smem + SM::TAB);
   float* row_scale = reinterpret_cast<float*>(smem + SM::RS);
   float* meet = reinterpret_cast<float*>(smem + SM::MX);             // [2][256]
@@ -261,6 +278,29 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
     return v0 + n <= see_end && (v0 >= see_from || v0 + n <= w.sink_end);
   };
 
+  // Passes.  Steps count on over them, and so do the phases of the barriers: step i of a pass is
+  // done + i; the barriers of even and odd halves start a pass with the phases in bits 0 and 1 of `ph`.
+  auto phase = [](int ph, int j) { return ((ph >> (j & 1)) ^ (j >> 1)) & 1; };
+  const int ph_step = (steps & 1) | (halves & 2);
+  // (no page at all in the first step: any unit)
+  auto first_unit = [&]() -> int { return *unit == INT_MIN ? 0 : *unit; };
+  // The pass after the one for window k (all roles come to the same: the windows needed are known with
+  // the last V tile of a pass): 0 none, 1 for a higher window, 2 for the lowest of all with O begun anew.
+  // The first pass is for window 0, whatever the others are; O only ever moves to larger units, where
+  // what fp32 loses at its lower end is nothing beside what any token adds.
+  auto next_pass = [&](int& k, bool& anew) -> int {
+    const uint32_t need = *needed;
+    if (!anew && (need & 0xffffu)) {
+      anew = true;
+      k = __ffs(need) - 17;
+      return 2;
+    }
+    const uint32_t up = (need | (anew ? 1u << 16 : 0u)) & ~((2u << (k + 16)) - 1u);
+    if (!up) return 0;
+    k = __ffs(up) - 17;
+    return 1;
+  };
+
   if (tid == 0) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(&k_full[s], NL);
@@ -279,6 +319,8 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
     mbar_init(drain + 1, 1);
     *abort_flag = 0;
     *marked = 0;
+    *unit = INT_MIN;
+    *needed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) {
@@ -302,10 +344,12 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
       const uint64_t dq = umma_desc(smem_u32(smem + SM::Q), 16, 1024);
       const uint64_t dk = umma_desc(smem_u32(smem + SM::K), 16, 1024);
       const uint64_t dv = umma_desc(smem_u32(smem + SM::V), PW_HALF, 1024);
+      int done = 0, ph = 0, win = 0;
+      bool anew = false, carry = false;
       // half j: tokens [64 (j & 1), + 64) of step j / 2, buffer j & 1 of the tile's S
       auto issue_s = [&](int tile, int j) {
         const uint64_t a = dq + tile * (SM::TILE >> 4);
-        const uint64_t b = dk + ((j >> 1) & 1) * (SM::TILE >> 4) + (j & 1) * (64 * 128 >> 4);
+        const uint64_t b = dk + ((done + (j >> 1)) & 1) * (SM::TILE >> 4) + (j & 1) * (64 * 128 >> 4);
         const uint32_t d = tmem + tile * 128 + (j & 1) * 64;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
@@ -315,40 +359,51 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
         umma_commit_el(&s_full[2 * tile + (j & 1)], el);
       };
       auto issue_o = [&](int tile, int j) {
-        const uint64_t b = dv + ((j >> 1) & 1) * (SM::TILE >> 4) + (j & 1) * (4 * 2048 >> 4);
+        const uint64_t b = dv + ((done + (j >> 1)) & 1) * (SM::TILE >> 4) + (j & 1) * (4 * 2048 >> 4);
         const uint32_t d = tmem + 256 + tile * D, a = tmem + tile * 128 + (j & 1) * 64;
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
-          umma_f16_ts_el(d, a + (ks >> 1) * 32 + (ks & 1) * 8, b + ks * (2048 >> 4), id_o, ks > 0 || j > 0, el);
+          umma_f16_ts_el(d, a + (ks >> 1) * 32 + (ks & 1) * 8, b + ks * (2048 >> 4), id_o,
+                         ks > 0 || j > 0 || carry, el);
         umma_commit_el(&o_done[2 * tile + (j & 1)], el);
       };
       const int tile = warp - (PW_SOFT + NL);
       const bool idle = tile == 1 && !two;
-      bool ok = idle || (warp_wait(q_full, 0, abort_flag) && warp_wait(&k_full[0], 0, abort_flag));
-      if (ok && !idle) {
+      bool ok = idle || warp_wait(q_full, 0, abort_flag);
+#pragma unroll 1
+      while (ok && !idle) {
+        ok = warp_wait(&k_full[done & 1], (done >> 1) & 1, abort_flag);
+        if (!ok) break;
         tc_fence_after();
         issue_s(tile, 0);
         if (halves > 1) issue_s(tile, 1);
-        umma_commit_el(&k_empty[0], el);
-      }
+        umma_commit_el(&k_empty[done & 1], el);
 #pragma unroll 1
-      for (int j = 0; ok && !idle && j < halves; ++j) {
-        const int st = (j >> 1) & 1, nj = j + 2;
-        if ((j & 1) == 0) ok = warp_wait(&v_full[st], (j >> 2) & 1, abort_flag);
-        if (ok) ok = warp_wait(&p_full[2 * tile + (j & 1)], (j >> 1) & 1, abort_flag);
-        if (!ok) break;
-        tc_fence_after();
-        issue_o(tile, j);
-        if ((j & 1) || j + 1 == halves) umma_commit_el(&v_empty[st], el);
-        if (nj < halves) {
-          if ((nj & 1) == 0) {
-            ok = warp_wait(&k_full[(nj >> 1) & 1], (nj >> 2) & 1, abort_flag);
-            if (!ok) break;
-            tc_fence_after();
+        for (int j = 0; j < halves; ++j) {
+          const int i = done + (j >> 1), st = i & 1, nj = j + 2;
+          if ((j & 1) == 0) ok = warp_wait(&v_full[st], (i >> 1) & 1, abort_flag);
+          if (ok) ok = warp_wait(&p_full[2 * tile + (j & 1)], phase(ph, j), abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          issue_o(tile, j);
+          if ((j & 1) || j + 1 == halves) umma_commit_el(&v_empty[st], el);
+          if (nj < halves) {
+            const int ni = i + 1;
+            if ((nj & 1) == 0) {
+              ok = warp_wait(&k_full[ni & 1], (ni >> 1) & 1, abort_flag);
+              if (!ok) break;
+              tc_fence_after();
+            }
+            issue_s(tile, nj);
+            if ((nj & 1) || nj + 1 == halves) umma_commit_el(&k_empty[ni & 1], el);
           }
-          issue_s(tile, nj);
-          if ((nj & 1) || nj + 1 == halves) umma_commit_el(&k_empty[(nj >> 1) & 1], el);
         }
+        if (!ok || !Q8) break;
+        const int next = next_pass(win, anew);
+        if (next == 0) break;
+        carry = next == 1;
+        done += steps;
+        ph ^= ph_step;
       }
       if (!ok) {        // leave with no product in flight
         *abort_flag = 1;
@@ -384,7 +439,7 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
         if (page < 0 || page >= p.num_pages) {
           if (my && v < w.v_end) {
             flag_range_error();
-            gone[i & 3] = i + 1;
+            gone[i & 3] = i + 1;                // (16-bit caches look at it: they take one pass)
           }
           return kNone;
         }
@@ -421,9 +476,44 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
         }
         cp_commit();
       };
-      // Rows have landed: codes to halves; values that are not finite out if `check`.
+      // 8-bit V rows: 2^(E - u) of this lane's token as two halves (0: of another pass) and the bit
+      // of its window; of this step and of the one before, whose rows land meanwhile.
+      int done = 0, win = 0;
+      bool anew = false;
+      uint32_t mul = 0, mul_v = 0;
+      int bit = 0, bit_v = 0;
+      bool some = false, some_v = false;        // a token of the warp's is of another pass
+      auto weigh = [&](float sv, bool first) {
+        const int e = (int)(__float_as_uint(fmaxf(sv, 9.0949470177e-13f)) >> 23) - 127;      // 2^-40
+        const bool has = my && sv >= 0.f;
+        if (first) {
+          const int top = __reduce_max_sync(0xffffffffu, has ? e : INT_MIN);
+          if (lane == 0) atomicMax(const_cast<int*>(unit), top);
+          vote<NL * 32>(10, false);
+        }
+        const int d = has ? e - first_unit() - win * PW_SPAN : 0;
+        const bool in = d >= PW_LOW && d < PW_LOW + PW_SPAN;
+        mul = !in ? 0u : d < -14 ? 0x02000200u : (uint32_t)(d + 15) * 0x04000400u;
+        bit = has ? (e - first_unit() - PW_LOW + 16 * PW_SPAN) / PW_SPAN : 16;
+        some = __any_sync(0xffffffffu, !in);
+      };
+      // Codes of tokens of another pass: 0, and their window asked for where they are not 0.
+      auto put_off = [&](char* tile) {
+#pragma unroll 1
+        for (int it = 0; it < ITS; ++it) {
+          const uint32_t h = __shfl_sync(0xffffffffu, mul_v, it * TPI + sub);
+          const int b = __shfl_sync(0xffffffffu, bit_v, it * TPI + sub);
+          if (h == 0) {
+            int4* a = reinterpret_cast<int4*>(tile + at_raw + it * NEXT);
+            const int4 x = *a;
+            if ((x.x | x.y | x.z | x.w) & 0x7f7f7f7f) atomicOr(const_cast<uint32_t*>(needed), 1u << b);
+            *a = make_int4(0, 0, 0, 0);
+          }
+        }
+      };
+      // Rows have landed: codes to halves, V's times 2^(E - u); values that are not finite out if `check`.
       const uint32_t at0 = dst_of(tok0, 2 * c), at1 = dst_of(tok0, 2 * c + 1);
-      auto finish = [&](char* tile, bool check) -> bool {
+      auto finish = [&](char* tile, bool check, bool v) -> bool {
         bool bad = false;
         if constexpr (Q8) {
           constexpr int B = ITS < 2 ? 1 : 2;
@@ -442,6 +532,11 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
               for (int x = 0; x < 4; ++x) {
                 o[2 * x] = e4m3x2_to_h2(wd[x] & 0xffffu);
                 o[2 * x + 1] = e4m3x2_to_h2(wd[x] >> 16);
+              }
+              if (v) {
+                const uint32_t f = __shfl_sync(0xffffffffu, mul_v, (it + u) * TPI + sub);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) o[x] = mul_h2(o[x], f);
               }
               if (check) {
 #pragma unroll
@@ -471,48 +566,65 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
         return bad;
       };
       auto finish_v = [&](int i) {        // looked at where rows see the step in part
-        if (finish(smem + SM::V + (i & 1) * SM::TILE, !all_see(w.v_begin + i * PW_TOK, PW_TOK)))
-          odd[i & 1] = i + 1;
-        signal(&v_full[i & 1]);
+        char* tile = smem + SM::V + ((done + i) & 1) * SM::TILE;
+        if (Q8 && some_v) put_off(tile);
+        if (finish(tile, !all_see(w.v_begin + i * PW_TOK, PW_TOK), true))
+          odd[(done + i) & 1] = done + i + 1;
+        signal(&v_full[(done + i) & 1]);
       };
       bool ok = true;
       float sk, sv;
-      int page_next = page_of(w.v_begin);
 #pragma unroll 1
-      for (int i = 0; i < steps; ++i) {
-        const int st = i & 1;
-        const uint32_t at = locate(i, page_next, sk, sv);
-        page_next = page_of(w.v_begin + (i + 1) * PW_TOK);
-        if (i >= 2 && !group_wait<NL * 32>(&k_empty[st], ((i >> 1) - 1) & 1, abort_flag, 10, lw == 0)) {
-          ok = false;
-          break;
+      for (;;) {
+        int page_next = page_of(w.v_begin);
+#pragma unroll 1
+        for (int i = 0; i < steps; ++i) {
+          const int at_step = done + i, st = at_step & 1, before = ((at_step >> 1) - 1) & 1;
+          const uint32_t at = locate(i, page_next, sk, sv);
+          page_next = page_of(w.v_begin + (i + 1) * PW_TOK);
+          if (at_step >= 2 && !group_wait<NL * 32>(&k_empty[st], before, abort_flag, 10, lw == 0)) {
+            ok = false;
+            break;
+          }
+          copy(smem + SM::K + st * SM::TILE, at, 0);
+          if constexpr (Q8) {
+            mul_v = mul;
+            bit_v = bit;
+            some_v = some;
+            weigh(sv, at_step == 0);
+            // scales of 0 (blocks never written) stand for values of 0: any will do; a token that is
+            // not there gets an exponent of -inf
+            const float mu = __uint_as_float((__float_as_uint(fmaxf(sv, 9.0949470177e-13f)) & 0x7fffffu) | 0x3f800000u);
+            if (my)
+              tab[(at_step & 3) * PW_TOK + my_tok] =
+                  sv < 0.f ? make_float4(1.f, -INFINITY, 0.f, 0.f)
+                           : make_float4(fmaxf(sk, 1e-30f), log2f(mu), 1.f / mu, 0.f);
+          }
+          if (i > 0) {
+            cp_wait<1>();
+            finish_v(i - 1);
+          }
+          // K goes out before V's stage is waited for: that one comes free with the step before last
+          cp_wait<0>();
+          finish(smem + SM::K + st * SM::TILE, false, false);
+          signal(&k_full[st]);
+          if (at_step >= 2 && !group_wait<NL * 32>(&v_empty[st], before, abort_flag, 10, lw == 0)) {
+            ok = false;
+            break;
+          }
+          copy(smem + SM::V + st * SM::TILE, at, plane);
         }
-        copy(smem + SM::K + st * SM::TILE, at, 0);
-        if constexpr (Q8) {
-          // scales of 0 (blocks never written) stand for values of 0: any will do; a token that is
-          // not there gets an exponent of -inf
-          const float svc = fmaxf(sv, 9.0949470177e-13f);         // 2^-40
-          if (my)
-            tab[(i & 3) * PW_TOK + my_tok] =
-                sv < 0.f ? make_float4(1.f, -INFINITY, 0.f, 0.f)
-                         : make_float4(fmaxf(sk, 1e-30f), log2f(svc), 1.f / svc, 0.f);
-        }
-        if (i > 0) {
-          cp_wait<1>();
-          finish_v(i - 1);
-        }
-        // K goes out before V's stage is waited for: that one comes free with the step before last
         cp_wait<0>();
-        finish(smem + SM::K + st * SM::TILE, false);
-        signal(&k_full[st]);
-        if (i >= 2 && !group_wait<NL * 32>(&v_empty[st], ((i >> 1) - 1) & 1, abort_flag, 10, lw == 0)) {
-          ok = false;
-          break;
-        }
-        copy(smem + SM::V + st * SM::TILE, at, plane);
+        if (!ok) break;
+        mul_v = mul;
+        bit_v = bit;
+        some_v = some;
+        finish_v(steps - 1);
+        if (!Q8) break;
+        vote<NL * 32>(10, false);               // the other warps' windows
+        if (next_pass(win, anew) == 0) break;
+        done += steps;
       }
-      cp_wait<0>();
-      if (ok) finish_v(steps - 1);
       if (!ok) *abort_flag = 1;
     }
   } else {
@@ -590,184 +702,216 @@ __global__ void __launch_bounds__(PW_THREADS, 1) paged_wide_kernel(const PagedPa
       // what the row sees, in v: v <= vc and (v < sink_end or v >= vw)
       const int vc = last_of(pos), vw = first_of(pos);
       const int pair = 2 + tile * 4 + (warp & 3);     // barrier of the two warps with these rows
+      // 8-bit caches: the maximum is taken 2^6 lower, so that P uses fp16 from 2^-24 to 2^15
+      // (2^6 for the largest score, 2^8 while its maximum lags behind, 2 for mu)
+      constexpr float kHead = Q8 ? 6.f : 0.f;
       float m = kNoMax, l = 0.f;
       // A wait that ran out is told to the warp with the rows' other scores at the barrier of a half, so
       // that both leave their loop at the same place.
-      bool fail = false;
+      bool fail = false, anew = false;
+      int done = 0, ph = 0, win = 0;
+      float l_all = 0.f;                              // l of the first pass: the later ones have all of m and l
 #pragma unroll 1
-      for (int j = 0;; ++j) {
-        const int i = j >> 1, v0 = w.v_begin + j * 64 + part * 32;      // step; this thread's tokens
-        // this thread's columns: 32 scores, then its P in the first 16 of them
-        const uint32_t t_p = t_s + (j & 1) * 64 + part * 32;
-        uint32_t x[32];
-        if (j < halves) {
-          fail = fail || !warp_wait(&s_full[2 * tile + (j & 1)], i & 1, abort_flag);
-          tc_fence_after();
-          tmem_ld32_nw(t_p, x);
-        }
-        if (j > 0) {                       // P of the half before goes out while the scores come in
-          tmem_wait_st();
-          const int i = (j - 1) >> 1, v0 = w.v_begin + (j - 1) * 64 + part * 32;
-          if (!all_see(w.v_begin + i * PW_TOK, PW_TOK)) {
-            // values that are not finite, taken out of V: mark the dims of the rows that see them
-            // (before P is handed over: V's stage and its flag stay until P V of this half is done)
-            fail = fail || !warp_wait(&v_full[i & 1], (i >> 1) & 1, abort_flag);
-            if (odd[i & 1] == i + 1) {
-              uint32_t* mask = odd_mask + row * (2 * (D / 32));
+      for (;;) {
 #pragma unroll 1
-              for (int k = 0; row < rows && k < min(32, w.v_end - v0); ++k) {
+        for (int j = 0;; ++j) {
+          const int i = done + (j >> 1), v0 = w.v_begin + j * 64 + part * 32;    // step; this thread's tokens
+          // this thread's columns: 32 scores, then its P in the first 16 of them
+          const uint32_t t_p = t_s + (j & 1) * 64 + part * 32;
+          uint32_t x[32];
+          if (j < halves) {
+            fail = fail || !warp_wait(&s_full[2 * tile + (j & 1)], phase(ph, j), abort_flag);
+            tc_fence_after();
+            tmem_ld32_nw(t_p, x);
+          }
+          if (j > 0) {                       // P of the half before goes out while the scores come in
+            tmem_wait_st();
+            const int i = done + ((j - 1) >> 1), v0 = w.v_begin + (j - 1) * 64 + part * 32;
+            if (!all_see(w.v_begin + (i - done) * PW_TOK, PW_TOK)) {
+              // values that are not finite, taken out of V: mark the dims of the rows that see them
+              // (before P is handed over: V's stage and its flag stay until P V of this half is done)
+              fail = fail || !warp_wait(&v_full[i & 1], (i >> 1) & 1, abort_flag);
+              if (odd[i & 1] == i + 1) {
+                uint32_t* mask = odd_mask + row * (2 * (D / 32));
+#pragma unroll 1
+                for (int k = 0; row < rows && k < min(32, w.v_end - v0); ++k) {
+                  const int v = v0 + k, t = v + (v >= w.n0 ? w.shift : 0);
+                  const int page = kvlist[t / p.ps];
+                  if (page < 0 || page >= p.num_pages || (causal && t > pos) ||
+                      (window && t < pos - w.window && t >= w.sink_end))
+                    continue;
+                  const int64_t r = ((int64_t)page * 2 + 1) * p.ps + t % p.ps;
+                  const char* src = p.pool + (r * p.hkv + kvh) * ROWB;
+#pragma unroll 1
+                  for (int d = 0; d < D; ++d) {
+                    float val;
+                    if constexpr (Q8) {
+                      const uint32_t h2 = e4m3x2_to_h2(*reinterpret_cast<const uint8_t*>(src + d));
+                      val = __low2float(*reinterpret_cast<const __half2*>(&h2));
+                    } else {
+                      val = to_f(reinterpret_cast<const T*>(src)[d]);
+                    }
+                    if (!(val < INFINITY)) atomicOr(&mask[d >> 5], 1u << (d & 31));
+                    if (!(val > -INFINITY)) atomicOr(&mask[D / 32 + (d >> 5)], 1u << (d & 31));
+                  }
+                  *marked = 1;
+                }
+              }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[2 * tile + ((j - 1) & 1)]);
+          }
+          if (j == halves) break;
+          const float4* tb = tab + (i & 3) * PW_TOK + (j & 1) * 64 + part * 32;
+          const bool missing = !Q8 && gone[i & 3] == i + 1, cut = !all_see(v0, 32) || missing;
+          uint32_t see = ~0u;
+          if (cut) {
+            const int kc = min(vc >= v0 + 32 ? 32 : vc - v0 + 1, w.v_end - v0);
+            const int ks = min(w.sink_end - v0, 32), kw = vw <= v0 ? 0 : min(vw - v0, 32);
+            see = low_bits(kc) & (low_bits(ks) | ~low_bits(kw));
+            if (missing)                               // a page id out of range: its tokens drop out
+#pragma unroll 1
+              for (int k = 0; k < min(32, w.v_end - v0); ++k) {
                 const int v = v0 + k, t = v + (v >= w.n0 ? w.shift : 0);
                 const int page = kvlist[t / p.ps];
-                if (page < 0 || page >= p.num_pages || (causal && t > pos) ||
-                    (window && t < pos - w.window && t >= w.sink_end))
-                  continue;
-                const int64_t r = ((int64_t)page * 2 + 1) * p.ps + t % p.ps;
-                const char* src = p.pool + (r * p.hkv + kvh) * ROWB;
+                if (page < 0 || page >= p.num_pages) see &= ~(1u << k);
+              }
+          }
+          tmem_wait();
+          if (cut) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) x[k] = (see >> k) & 1 ? x[k] : 0xff800000u;             // -inf
+          }
+          float mx;
+          if (by_token) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              x[k] = __float_as_uint(fmaf(__uint_as_float(x[k]), fmaxf(tb[k].x * scale, kLeast), tb[k].y));
+          }
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          if (Q8 && !by_token) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 8) {
+              float y[8];
+#pragma unroll
+              for (int u = 0; u < 8; ++u) y[u] = __uint_as_float(x[k + u]);
+              const float gm = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])),
+                                     fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
+              m4[k >> 3] = fmaf(gm, fmaxf(tb[k].x * scale, kLeast), tb[k].y);
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 32; k += 8)
+#pragma unroll
+              for (int u = 0; u < 4; ++u)
+                m4[u] = fmaxf(fmaxf(m4[u], __uint_as_float(x[k + u])), __uint_as_float(x[k + 4 + u]));
+          }
+          mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+          if (!Q8) mx *= scale;
+          if (vote<64>(pair, mx > m + (kHead + kLazyMax) || fail)) {
+            meet[part * 256 + row] = mx;
+            if (vote<64>(pair, fail)) {
+              fail = true;
+              break;
+            }
+            const float to = fmaxf(m, fmaxf(mx, meet[(part ^ 1) * 256 + row]) - kHead), f = ex2(m - to);
+            m = to;
+            l *= f;
+            if (j > 0) {        // O of the halves before: complete, then rescaled, half the dims per thread
+              fail = !warp_wait(&o_done[2 * tile + ((j - 1) & 1)], phase(ph, j - 1), abort_flag);
+              tc_fence_after();
 #pragma unroll 1
-                for (int d = 0; d < D; ++d) {
-                  float val;
-                  if constexpr (Q8) {
-                    const uint32_t h2 = e4m3x2_to_h2(*reinterpret_cast<const uint8_t*>(src + d));
-                    val = __low2float(*reinterpret_cast<const __half2*>(&h2));
-                  } else {
-                    val = to_f(reinterpret_cast<const T*>(src)[d]);
-                  }
-                  if (!(val < INFINITY)) atomicOr(&mask[d >> 5], 1u << (d & 31));
-                  if (!(val > -INFINITY)) atomicOr(&mask[D / 32 + (d >> 5)], 1u << (d & 31));
-                }
-                *marked = 1;
+              for (int c0 = part * (D / 2); c0 < (part + 1) * (D / 2); c0 += 16) {
+                uint32_t y[16];
+                tmem_ld16_nw(t_o + c0, y);
+                tmem_wait();
+#pragma unroll
+                for (int k = 0; k < 16; ++k) y[k] = __float_as_uint(__uint_as_float(y[k]) * f);
+                tmem_st16(t_o + c0, y);
               }
             }
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[2 * tile + ((j - 1) & 1)]);
-        }
-        if (j == halves) break;
-        const float4* tb = tab + (i & 3) * PW_TOK + (j & 1) * 64 + part * 32;
-        const bool missing = !Q8 && gone[i & 3] == i + 1, cut = !all_see(v0, 32) || missing;
-        uint32_t see = ~0u;
-        if (cut) {
-          const int kc = min(vc >= v0 + 32 ? 32 : vc - v0 + 1, w.v_end - v0);
-          const int ks = min(w.sink_end - v0, 32), kw = vw <= v0 ? 0 : min(vw - v0, 32);
-          see = low_bits(kc) & (low_bits(ks) | ~low_bits(kw));
-          if (missing)                               // a page id out of range: its tokens drop out
-#pragma unroll 1
-            for (int k = 0; k < min(32, w.v_end - v0); ++k) {
-              const int v = v0 + k, t = v + (v >= w.n0 ? w.shift : 0);
-              const int page = kvlist[t / p.ps];
-              if (page < 0 || page >= p.num_pages) see &= ~(1u << k);
-            }
-        }
-        tmem_wait();
-        if (cut) {
+          // ---- P over S ----
+          uint32_t pk[16];
+          if (by_token) {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) x[k] = (see >> k) & 1 ? x[k] : 0xff800000u;             // -inf
-        }
-        float mx;
-        if (by_token) {
-#pragma unroll
-          for (int k = 0; k < 32; ++k)
-            x[k] = __float_as_uint(fmaf(__uint_as_float(x[k]), fmaxf(tb[k].x * scale, kLeast), tb[k].y));
-        }
-        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        if (Q8 && !by_token) {
-#pragma unroll
-          for (int k = 0; k < 32; k += 8) {
-            float y[8];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) y[u] = __uint_as_float(x[k + u]);
-            const float gm = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])),
-                                   fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
-            m4[k >> 3] = fmaf(gm, fmaxf(tb[k].x * scale, kLeast), tb[k].y);
-          }
-        } else {
-#pragma unroll
-          for (int k = 0; k < 32; k += 8)
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-              m4[u] = fmaxf(fmaxf(m4[u], __uint_as_float(x[k + u])), __uint_as_float(x[k + 4 + u]));
-        }
-        mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-        if (!Q8) mx *= scale;
-        if (vote<64>(pair, mx > m + kLazyMax || fail)) {
-          meet[part * 256 + row] = mx;
-          if (vote<64>(pair, fail)) {
-            fail = true;
-            break;
-          }
-          const float to = fmaxf(m, fmaxf(mx, meet[(part ^ 1) * 256 + row])), f = ex2(m - to);
-          m = to;
-          l *= f;
-          if (j > 0) {        // O of the halves before: complete, then rescaled, half the dims per thread
-            fail = !warp_wait(&o_done[2 * tile + ((j - 1) & 1)], ((j - 1) >> 1) & 1, abort_flag);
-            tc_fence_after();
-#pragma unroll 1
-            for (int c0 = part * (D / 2); c0 < (part + 1) * (D / 2); c0 += 16) {
-              uint32_t y[16];
-              tmem_ld16_nw(t_o + c0, y);
-              tmem_wait();
-#pragma unroll
-              for (int k = 0; k < 16; ++k) y[k] = __float_as_uint(__uint_as_float(y[k]) * f);
-              tmem_st16(t_o + c0, y);
-            }
-          }
-        }
-        // ---- P over S ----
-        uint32_t pk[16];
-        if (by_token) {
-#pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            const float a = ex2(__uint_as_float(x[k]) - m), b = ex2(__uint_as_float(x[k + 1]) - m);
-            l = fmaf(a, tb[k].z, fmaf(b, tb[k + 1].z, l));
-            pk[k >> 1] = pack2<MT>(a, b);
-          }
-        } else {
-          const uint64_t s2 = f2_pack(scale, scale), m2 = f2_pack(-m, -m);
-          uint64_t sum[2] = {0, 0};
-#pragma unroll
-          for (int k0 = 0; k0 < 32; k0 += 8) {
-            uint64_t gs = s2, gm = m2;
-            float inv = 1.f;
-            if constexpr (Q8) {
-              const float4 e = tb[k0];
-              const float both = fmaxf(e.x * scale, kLeast);
-              gs = f2_pack(both, both);
-              gm = f2_pack(e.y - m, e.y - m);
-              inv = e.z;
-              sum[0] = sum[1] = 0;
-            }
-#pragma unroll
-            for (int k = k0; k < k0 + 8; k += 2) {
-              const uint64_t y = f2_pack(__uint_as_float(x[k]), __uint_as_float(x[k + 1]));
-              float a, b;
-              f2_unpack(f2_fma(y, gs, gm), a, b);
-              a = ex2(a);
-              b = ex2(b);
-              sum[(k >> 1) & 1] = f2_add(sum[(k >> 1) & 1], f2_pack(a, b));
+            for (int k = 0; k < 32; k += 2) {
+              const float a = ex2(__uint_as_float(x[k]) - m), b = ex2(__uint_as_float(x[k + 1]) - m);
+              l = fmaf(a, tb[k].z, fmaf(b, tb[k + 1].z, l));
               pk[k >> 1] = pack2<MT>(a, b);
             }
-            if constexpr (Q8) {
+          } else {
+            const uint64_t s2 = f2_pack(scale, scale), m2 = f2_pack(-m, -m);
+            uint64_t sum[2] = {0, 0};
+#pragma unroll
+            for (int k0 = 0; k0 < 32; k0 += 8) {
+              uint64_t gs = s2, gm = m2;
+              float inv = 1.f;
+              if constexpr (Q8) {
+                const float4 e = tb[k0];
+                const float both = fmaxf(e.x * scale, kLeast);
+                gs = f2_pack(both, both);
+                gm = f2_pack(e.y - m, e.y - m);
+                inv = e.z;
+                sum[0] = sum[1] = 0;
+              }
+#pragma unroll
+              for (int k = k0; k < k0 + 8; k += 2) {
+                const uint64_t y = f2_pack(__uint_as_float(x[k]), __uint_as_float(x[k + 1]));
+                float a, b;
+                f2_unpack(f2_fma(y, gs, gm), a, b);
+                a = ex2(a);
+                b = ex2(b);
+                sum[(k >> 1) & 1] = f2_add(sum[(k >> 1) & 1], f2_pack(a, b));
+                pk[k >> 1] = pack2<MT>(a, b);
+              }
+              if constexpr (Q8) {
+                float a, b;
+                f2_unpack(f2_add(sum[0], sum[1]), a, b);
+                l = fmaf(a + b, inv, l);
+              }
+            }
+            if constexpr (!Q8) {
               float a, b;
               f2_unpack(f2_add(sum[0], sum[1]), a, b);
-              l = fmaf(a + b, inv, l);
+              l += a + b;
             }
           }
-          if constexpr (!Q8) {
-            float a, b;
-            f2_unpack(f2_add(sum[0], sum[1]), a, b);
-            l += a + b;
+          tmem_st16(t_p, pk);
+        }
+        fail = fail || !warp_wait(&o_done[2 * tile + ((halves - 1) & 1)], phase(ph, halves - 1), abort_flag);
+        if constexpr (!Q8) break;
+        if (vote<64>(pair, fail)) {                     // both warps of the rows go on, or neither
+          fail = true;
+          break;
+        }
+        if (done == 0) l_all = l;
+        const int was = win, next = next_pass(win, anew);
+        if (next == 0) break;
+        if (next == 1) {                                // O in the next window's unit
+          const float f = __uint_as_float((uint32_t)max(127 - (win - was) * PW_SPAN, 1) << 23);
+          tc_fence_after();
+#pragma unroll 1
+          for (int c0 = part * (D / 2); c0 < (part + 1) * (D / 2); c0 += 16) {
+            uint32_t y[16];
+            tmem_ld16_nw(t_o + c0, y);
+            tmem_wait();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) y[k] = __float_as_uint(__uint_as_float(y[k]) * f);
+            tmem_st16(t_o + c0, y);
           }
         }
-        tmem_st16(t_p, pk);
+        done += steps;
+        ph ^= ph_step;
       }
+      if constexpr (Q8) l = l_all;
       // ---- epilogue: half the dims per thread ----
-      fail = fail || !warp_wait(&o_done[2 * tile + ((halves - 1) & 1)], ((halves - 1) >> 1) & 1, abort_flag);
       meet[part * 256 + row] = l;
       if (!vote<64>(pair, fail)) {
         tc_fence_after();
         l += meet[(part ^ 1) * 256 + row];
-        const float inv = l != 0.f ? 1.f / l : 0.f;
+        const float inv = (l != 0.f ? 1.f / l : 0.f) * (Q8 ? exp2f((float)(first_unit() + win * PW_SPAN)) : 1.f);
         const bool partial = w.part_base >= 0;
         // through this tile's Q rows (its last product has read them) so that rows leave in whole lines:
         // D / 4 dims of fp32 partials or D / 2 of results at a time, in 4 D bytes per warp and row pair

@@ -441,7 +441,8 @@ int be_paged_plan(int num_levels, const int32_t* const* qo_indptr, const int32_t
  * (kv_scale required) or dtype; head_dim 64 or 128.  q [n][num_qo_heads][head_dim]
  * with q_row_stride elements between queries.  mid_o / mid_lse: float32 scratch of
  * max_parts * num_qo_heads * head_dim and max_parts * num_qo_heads (calls that share
- * them must not overlap on the GPU).                                          */
+ * them must not overlap on the GPU).  V scales may lie anywhere in [2^-40, 2^40], whatever the other
+ * pages' are (a smaller one, 0 included, counts as 2^-40).                    */
 typedef struct be_paged_attn_args {
   const int32_t* plan_dev;
   const void* q;
