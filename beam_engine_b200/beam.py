@@ -439,6 +439,7 @@ class StepGraph:
         n = self.n
         self.dev_buf[:used].copy_(self.host_buf[:used], non_blocking=True)
         self.gen.h2d_bytes += 4 * used
+        ran = False
         if self.graph is None:
             t0 = time.perf_counter()
             if not self.gen._graph_warm:   # first capture of the generator: warm libraries up
@@ -446,9 +447,13 @@ class StepGraph:
                 side = torch.cuda.Stream(self.gen.device)
                 side.wait_stream(cur)
                 with torch.cuda.stream(side):
-                    self._body()            # warm-up (writes the same K/V the replay will)
+                    # warm-up: writes the same K/V the replay will.  Over an 8-bit pool it is the
+                    # step itself: its appends may raise a block's scale and round the block's
+                    # tokens to it, which a replay would then fork into other beams' pages.
+                    self._body()
                 cur.wait_stream(side)
                 self.gen._graph_warm = True
+                ran = self.gen.page_table.kv_scale is not None
             g = torch.cuda.CUDAGraph()
             # thread-local capture: other threads (NCCL's watchdog polling its
             # events) may keep making CUDA calls while this one records
@@ -456,9 +461,10 @@ class StepGraph:
                 self._body()
             self.graph = g
             self.gen.graph_captures.append(time.perf_counter() - t0)
-        self.graph.replay()
+        if not ran:
+            self.graph.replay()
         torch.cuda.current_stream(self.gen.device).synchronize()
-        if self.timing and self.gen.attn_times is not None:
+        if self.timing and self.gen.attn_times is not None and not ran:
             self.gen.attn_times.extend(self.attention_ms())
         k = self.k
         if self.select is not None:
