@@ -158,11 +158,7 @@ extern "C" int be_paged_plan(int num_levels, const int32_t* const* qo_indptr,
     set_error("be_paged_plan: %d query heads per KV head (at most 128)", g);
     return BE_EINVAL;
   }
-  // tokens of every query over all levels, and the start of each level's part
-  std::vector<int64_t> total(num_queries, 0);
-  std::vector<int32_t> kvlist;
-  std::vector<int> base(num_levels);
-  std::vector<std::vector<int>> lens(num_levels);
+  // every extent before anything is indexed by one
   for (int l = 0; l < num_levels; ++l) {
     const int G = num_groups[l];
     if (G < 0 || (G > 0 && (qo_indptr[l][0] != 0 || kv_indptr[l][0] != 0 ||
@@ -171,15 +167,23 @@ extern "C" int be_paged_plan(int num_levels, const int32_t* const* qo_indptr,
                 num_queries);
       return BE_EINVAL;
     }
-    base[l] = (int)kvlist.size();
-    lens[l].resize(G);
-    for (int i = 0; i < G; ++i) {
-      const int qlen = qo_indptr[l][i + 1] - qo_indptr[l][i];
-      const int np = kv_indptr[l][i + 1] - kv_indptr[l][i];
-      if (qlen < 0 || np < 0) {
+    for (int i = 0; i < G; ++i)
+      if (qo_indptr[l][i + 1] < qo_indptr[l][i] || kv_indptr[l][i + 1] < kv_indptr[l][i]) {
         set_error("be_paged_plan: level %d group %d has negative extent", l, i);
         return BE_EINVAL;
       }
+  }
+  // tokens of every query over all levels, and the start of each level's part
+  std::vector<int64_t> total(num_queries, 0);
+  std::vector<int32_t> kvlist;
+  std::vector<int> base(num_levels);
+  std::vector<std::vector<int>> lens(num_levels);
+  for (int l = 0; l < num_levels; ++l) {
+    const int G = num_groups[l];
+    base[l] = (int)kvlist.size();
+    lens[l].resize(G);
+    for (int i = 0; i < G; ++i) {
+      const int np = kv_indptr[l][i + 1] - kv_indptr[l][i];
       const int last = last_page_len[l][i];
       if (np > 0 && (last < 0 || last > page_size)) {
         set_error("be_paged_plan: level %d group %d last_page_len %d outside [0, %d]", l, i, last,

@@ -169,6 +169,16 @@ def test_plan_refuses(bad):
     assert rc == _lib.BE_EINVAL
 
 
+@pytest.mark.parametrize("qo,kp", [([0, 5000, 2], [0, 1, 2]), ([0, 3, 2], [0, 1, 2]), ([0, -3, 2], [0, 1, 2]),
+                                   ([0, 1, 2], [0, 400, 2]), ([0, 2, 5000], [0, 1, 2]),
+                                   ([0, 1, 2], [0, 2, 1])])
+def test_indptrs_that_do_not_ascend(qo, kp):
+    """Refused before anything is indexed by them (a later end may be back in range)."""
+    assert plan([(qo, kp, [3, 4], [5, 5])], 2, 16, 8, 2)[0] == _lib.BE_EINVAL
+    two = [([0, 1, 2], [0, 1, 2], [3, 4], [5, 5]), (qo, kp, [3, 4], [5, 5])]
+    assert plan(two, 2, 16, 8, 2)[0] == _lib.BE_EINVAL
+
+
 def test_empty_plan():
     rc, info, buf = plan([([0], [0], [], [])], 0, 16, 8, 2)
     assert rc == 0 and info.n_work == 0 and info.n_merge == 0
