@@ -22,7 +22,9 @@ kernel); ``BE_ATTN_TILES=0`` keeps the work-item kernels.
 its scales as ``kv_scale``), ``plan(..., window_left=w, num_sinks=s)`` lets the query at position
 p see the tokens t >= p - w and the first s tokens only; a query's tokens are those of its
 groups in level order, and the queries of a last-level group are its last tokens.  Both go
-through ``be_paged_plan`` / ``be_paged_attn_run`` (bf16 / fp16 queries, head_dim 64 or 128).
+through ``be_paged_plan`` / ``be_paged_attn_run`` (bf16 / fp16 queries, head_dim 64 or 128).  A run over
+an 8-bit cache on a plan that named no ``kv_data_type`` plans for it beside that plan, in memory
+of the wrapper's own, so runs and captured graphs over 16-bit or fp32 caches go on as planned.
 """
 from __future__ import annotations
 
@@ -135,14 +137,19 @@ class _Plan:
             rc = fn(self.host.data_ptr(), self.host.numel(), C.byref(self.info))
         check(rc, "attention plan")
 
+    def bytes_needed(self, num_qo_heads, head_dim):
+        """Workspace that ``place`` takes for the plan built last."""
+        parts = self.info.n_parts
+        return ((self.info.total_ints * 4 + 255) // 256 * 256
+                + (parts * num_qo_heads * head_dim * 4 + 255) // 256 * 256
+                + parts * num_qo_heads * 4)
+
     def place(self, num_qo_heads, head_dim):
         """Copy the plan to the front of the workspace; carve mid_o / mid_lse."""
         n = self.info.total_ints
         plan_bytes = (n * 4 + 255) // 256 * 256
-        parts = self.info.n_parts
-        mo = parts * num_qo_heads * head_dim * 4
-        ml = parts * num_qo_heads * 4
-        need = plan_bytes + (mo + 255) // 256 * 256 + ml
+        mo = self.info.n_parts * num_qo_heads * head_dim * 4
+        need = self.bytes_needed(num_qo_heads, head_dim)
         if need > self.ws.numel():
             raise ValueError(f"workspace too small: plan needs {need} bytes, "
                              f"buffer has {self.ws.numel()}")
@@ -286,6 +293,9 @@ class MultiLevelCascadeAttentionWrapper:
             raise ValueError("only the NHD layout is supported")
         self.num_levels = num_levels
         self._plan = _Plan(float_workspace_buffer)
+        # the plan for 8-bit caches beside one that did not name them, and the memory that it and
+        # those before it were placed in (captured graphs may read it)
+        self._plan8, self._plan8_mem, self._plan8_made = None, [], False
 
     def plan(self, qo_indptr_arr: List[torch.Tensor], paged_kv_indptr_arr: List[torch.Tensor],
              paged_kv_indices_arr: List[torch.Tensor], paged_kv_last_page_len: List[torch.Tensor],
@@ -313,8 +323,10 @@ class MultiLevelCascadeAttentionWrapper:
         most = 2 ** 31 - 1                   # tokens are counted in int32
         self._window = (min(window_left, most) if window_left >= 0 else -1, min(num_sinks, most))
         self.paged = window_left >= 0 or (kv_data_type is not None and is_8bit(kv_data_type))
+        self._plan8_made = False
         if self.paged:
-            self._plan_paged()
+            self._plan_paged(ps)
+            self.tiles = False
         elif split_tokens == 0 and tiles_eligible(head_dim, page_size, num_qo_heads, num_kv_heads):
             g = num_qo_heads // num_kv_heads
             qo0 = arrs[0][0] if L else np.zeros(1, np.int32)
@@ -350,12 +362,12 @@ class MultiLevelCascadeAttentionWrapper:
         ps.tinfo = None
         self.tiles = False
 
-    def _plan_paged(self):
-        """The plan (be_paged_plan) of the last plan() call's levels for 8-bit caches and windows."""
+    def _plan_paged(self, ps, own_memory=False):
+        """The plan (be_paged_plan) of the last plan() call's levels for 8-bit caches and windows,
+        placed in the workspace or in memory of the wrapper's own."""
         (L, ptrs, ng, nq, page_size, hq, hkv, causal, _, head_dim, _) = self._levels_args
         if head_dim not in (64, 128):
             raise ValueError(f"head_dim {head_dim}: 8-bit caches and windows take 64 or 128")
-        ps = self._plan
         window, sinks = self._window
 
         def fn(buf, cap, info):
@@ -364,27 +376,31 @@ class MultiLevelCascadeAttentionWrapper:
                                        info)
         ps.info = PagedPlanInfo()
         ps.build(fn)
+        need = ps.bytes_needed(hq, head_dim) if own_memory else 0
+        if own_memory and (not self._plan8_mem or self._plan8_mem[-1].numel() < need):
+            self._plan8_mem.append(torch.empty(need + need // 4, dtype=torch.uint8,
+                                               device=ps.device))
+        if own_memory:
+            ps.ws = self._plan8_mem[-1]
         ps.place(hq, head_dim)
         ps.tinfo = None
-        self.tiles = False
-        self.paged = True
 
-    def _run_paged(self, q, kv, kv_scale, return_lse, out):
+    def _run_paged(self, ps, q, kv, kv_scale, return_lse, out):
         n, hq, d = shape = (self.num_queries, self.hq, self.d)
         dtype, dev, ks = q.dtype, q.device, kv.shape
         if q.shape != shape:
             raise ValueError(f"q must be {shape}, got {tuple(q.shape)}")
-        if ks[1:] != (2, self._plan.info.page_size, self.hkv, d) or not kv.is_contiguous():
+        if ks[1:] != (2, ps.info.page_size, self.hkv, d) or not kv.is_contiguous():
             raise ValueError(f"paged_kv_cache must be contiguous [pages, 2, "
-                             f"{self._plan.info.page_size}, {self.hkv}, {d}], got {tuple(ks)}")
+                             f"{ps.info.page_size}, {self.hkv}, {d}], got {tuple(ks)}")
         if is_8bit(kv.dtype):
             check_pool8(kv, kv_scale)
-            require_same_device(kv, q, kv_scale, self._plan.ws)
+            require_same_device(kv, q, kv_scale, ps.ws)
         elif kv_scale is not None or kv.dtype is not dtype:
             raise ValueError(f"a cache of {kv.dtype} takes queries of its type (got {dtype}) and "
                              "no kv_scale")
         else:
-            require_same_device(kv, q, self._plan.ws)
+            require_same_device(kv, q, ps.ws)
         if out is None:              # (new_empty takes 1 us less than torch.empty)
             out = q.new_empty(shape)
         elif (out.shape != shape or out.dtype is not dtype or out.device != dev
@@ -392,20 +408,25 @@ class MultiLevelCascadeAttentionWrapper:
             raise ValueError(f"out must be {dtype} {shape} on {dev} with contiguous heads")
         lse = q.new_empty((n, hq), dtype=torch.float32) if return_lse else None
         if n:
-            self._plan.run_paged(q, kv, kv_scale, hq, self.hkv, d, self.sm_scale, out, lse)
+            ps.run_paged(q, kv, kv_scale, hq, self.hkv, d, self.sm_scale, out, lse)
         return (out, lse) if return_lse else out
 
     def run(self, q: torch.Tensor, paged_kv_cache: torch.Tensor, return_lse: bool = False,
             out: Optional[torch.Tensor] = None, kv_scale: Optional[torch.Tensor] = None):
         if q.shape[0] != self.num_queries:
             raise ValueError(f"q has {q.shape[0]} rows, plan has {self.num_queries} queries")
-        if is_8bit(paged_kv_cache.dtype) and not self.paged:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("plan with kv_data_type=torch.float8_e4m3fn before capturing a "
-                                   "run over an 8-bit cache")
-            self._plan_paged()               # 8-bit caches run on their own plan
         if self.paged:
-            return self._run_paged(q, paged_kv_cache, kv_scale, return_lse, out)
+            return self._run_paged(self._plan, q, paged_kv_cache, kv_scale, return_lse, out)
+        if is_8bit(paged_kv_cache.dtype):    # on a plan of their own, the one in place stays
+            if not self._plan8_made:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("plan with kv_data_type=torch.float8_e4m3fn before "
+                                       "capturing a run over an 8-bit cache")
+                if self._plan8 is None:
+                    self._plan8 = _Plan(self._plan.ws)
+                self._plan_paged(self._plan8, own_memory=True)
+                self._plan8_made = True
+            return self._run_paged(self._plan8, q, paged_kv_cache, kv_scale, return_lse, out)
         if kv_scale is not None:
             raise ValueError("kv_scale belongs to a float8_e4m3fn cache")
         if out is None:
