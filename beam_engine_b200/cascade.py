@@ -303,6 +303,21 @@ class MultiLevelCascadeAttentionWrapper:
              causal: bool = False, pos_encoding_mode: str = "NONE", sm_scale: Optional[float] = None,
              q_data_type=None, split_tokens: int = 0, kv_data_type=None, window_left: int = -1,
              num_sinks: int = 0, **_):
+        """A call that raises leaves the wrapper with the plan that it had."""
+        mine, placed = dict(self.__dict__), dict(self._plan.__dict__)
+        try:
+            self._plan_levels(qo_indptr_arr, paged_kv_indptr_arr, paged_kv_indices_arr,
+                              paged_kv_last_page_len, num_qo_heads, num_kv_heads, head_dim,
+                              page_size, causal, pos_encoding_mode, sm_scale, split_tokens,
+                              kv_data_type, window_left, num_sinks)
+        except BaseException:
+            self.__dict__.update(mine)
+            self._plan.__dict__.update(placed)
+            raise
+
+    def _plan_levels(self, qo_indptr_arr, paged_kv_indptr_arr, paged_kv_indices_arr,
+                     paged_kv_last_page_len, num_qo_heads, num_kv_heads, head_dim, page_size, causal,
+                     pos_encoding_mode, sm_scale, split_tokens, kv_data_type, window_left, num_sinks):
         if num_sinks < 0:
             raise ValueError(f"num_sinks {num_sinks} is negative")
         if pos_encoding_mode != "NONE":

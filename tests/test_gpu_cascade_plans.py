@@ -104,3 +104,29 @@ def test_a_new_plan_is_made_again_for_8_bits():
     fresh.plan([0, 1, 2], [0, 2, 4], [7, 6, 5, 4], [16, 3], HQ, HKV, D, PS, causal=True, kv_data_type=F8)
     a, b = fresh.run(q, pool, return_lse=True, kv_scale=scale)
     assert torch.equal(out, a) and torch.equal(lse, b)
+
+
+GOOD = dict(qo=QO, ptr=PTR, pages=PAGES, last=LAST, hq=HQ, hkv=HKV, d=D, ps=PS)
+
+
+@pytest.mark.parametrize("kind", ["tiles", "items", "8 bits", "window"])
+@pytest.mark.parametrize("bad", [dict(qo=[0, 2, 1]), dict(last=[17, 2]), dict(hq=7), dict(d=80, window_left=3),
+                                 dict(num_sinks=-1), dict(big=True, window_left=5), dict(big=True),
+                                 dict(big=True, kv_data_type=F8)])
+def test_a_plan_that_is_refused_leaves_the_one_before(kind, bad):
+    from beam_engine_b200.cascade import BatchPrefillWithPagedKVCacheWrapper
+    sets = caches()
+    q, pool, scale = sets["8" if kind == "8 bits" else "32" if kind == "items" else "16"]
+    kw = {"8 bits": dict(kv_data_type=F8), "window": dict(window_left=20)}.get(kind, {})
+    w = BatchPrefillWithPagedKVCacheWrapper(torch.empty(1 << 16, dtype=torch.uint8, device="cuda"))
+    w.plan(QO, PTR, PAGES, LAST, HQ, HKV, D, PS, causal=True, split_tokens=int(kind == "items") * 4096, **kw)
+    want, lse = w.run(q, pool, return_lse=True, kv_scale=scale)
+    a = dict(GOOD, **bad)
+    if a.pop("big", False):                    # a plan that the workspace of 64 KB does not hold
+        n = 20000
+        a.update(qo=[0, 1], ptr=[0, n], pages=[0] * n, last=[16])
+    with pytest.raises((ValueError, RuntimeError)):
+        w.plan(*[a.pop(k) for k in ("qo", "ptr", "pages", "last", "hq", "hkv", "d", "ps")], causal=True, **a)
+    got, e = w.run(q, pool, return_lse=True, kv_scale=scale)
+    assert torch.equal(got, want) and torch.equal(e, lse)
+    assert status() == 0
