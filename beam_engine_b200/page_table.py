@@ -321,13 +321,20 @@ class PageTable:
 
     def read_pages(self, layer: int, pages, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """Pages of one layer as values [n, 2, page_size, heads, head_dim]: the codes of an 8-bit
-        pool times their scales, a copy of the pages otherwise."""
+        pool times their scales, a copy of the pages otherwise.  A page id out of range reads as
+        zeros."""
         from .page import read_paged_kv_cache
         if not isinstance(pages, torch.Tensor):
             pages = torch.as_tensor(np.asarray(pages, np.int32))
         pages = pages.to(self.kv_cache.device)
         if self.kv_scale is None:
-            return self.kv_cache_at_layer[layer][pages.long()].to(dtype)
+            if pages.dim() != 1:
+                raise ValueError("pages must be [n]")
+            # (an index past the pool would end the process's CUDA context)
+            there = (pages >= 0) & (pages < self.max_num_pages)
+            at = torch.where(there, pages, torch.zeros_like(pages)).long()
+            out = self.kv_cache_at_layer[layer][at].to(dtype)
+            return out.masked_fill_(~there[:, None, None, None, None], 0)
         return read_paged_kv_cache(self.kv_cache_at_layer[layer], pages, self.kv_scale[layer],
                                    dtype)
 
