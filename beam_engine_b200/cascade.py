@@ -77,6 +77,18 @@ def _level_arrays(levels):
     return L, arrs, ng, ptrs
 
 
+def check_level_sizes(arrs):
+    """The planners read each level's arrays as far as its indptrs say."""
+    for l, (qo, kp, ki, last) in enumerate(zip(*arrs)):
+        if len(qo) < 1:
+            raise ValueError(f"level {l}: qo_indptr is empty")
+        n = len(qo) - 1
+        if n and (len(kp) <= n or len(last) < n or len(ki) < kp[n]):
+            raise ValueError(f"level {l}: {n} groups need {n + 1} kv_indptr entries, {n} last page "
+                             f"lengths and kv_indptr[{n}] page ids; got {len(kp)}, {len(last)} and "
+                             f"{len(ki)}")
+
+
 def level0_rows(levels, group_size):
     """Largest level-0 group (query-head rows): the tile height a plan needs."""
     if not levels:
@@ -322,11 +334,13 @@ class MultiLevelCascadeAttentionWrapper:
             raise ValueError(f"num_sinks {num_sinks} is negative")
         if pos_encoding_mode != "NONE":
             raise ValueError("only pos_encoding_mode='NONE' is supported")
-        if len(qo_indptr_arr) != self.num_levels:
-            raise ValueError(f"expected {self.num_levels} levels, got {len(qo_indptr_arr)}")
+        for a in (qo_indptr_arr, paged_kv_indptr_arr, paged_kv_indices_arr, paged_kv_last_page_len):
+            if len(a) != self.num_levels:
+                raise ValueError(f"expected {self.num_levels} levels, got {len(a)}")
         levels = list(zip(qo_indptr_arr, paged_kv_indptr_arr, paged_kv_indices_arr,
                           paged_kv_last_page_len))
         arrs = [[_i32(lv[k]) for lv in levels] for k in range(4)]
+        check_level_sizes(arrs)
         nq = int(arrs[0][-1][-1]) if levels else 0
         ng = np.asarray([len(a) - 1 for a in arrs[0]], np.int32)
         L = len(levels)

@@ -253,3 +253,20 @@ def test_argument_blocks_match_the_header():
         assert plain == fmt
     assert lib().be_paged_attn_run(None) == _lib.BE_EINVAL
     assert lib().be_rope_append_paged_kv(None) == _lib.BE_EINVAL
+
+
+@pytest.mark.parametrize("qo,kp,ki,last,ok", [
+    ([0, 1, 2], [0, 2, 3], [4, 5, 6], [1, 1], True), ([0], [0], [], [], True), ([0], [], [], [], True),
+    ([0, 1, 2], [0, 2, 3], [4, 5, 6, 7], [1, 1, 1], True), ([], [], [], [], False),
+    ([0, 1, 2], [0, 2], [4, 5, 6], [1, 1], False), ([0, 1, 2], [0, 2, 3], [4, 5], [1, 1], False),
+    ([0, 1, 2], [0, 2, 3], [4, 5, 6], [1], False), ([0, 1], [], [], [], False)])
+def test_arrays_shorter_than_the_indptrs_say_are_refused(qo, kp, ki, last, ok):
+    from beam_engine_b200.cascade import check_level_sizes
+    good = ([0, 1], [0, 1], [3], [2])
+    for levels in ([(qo, kp, ki, last)], [good, (qo, kp, ki, last)]):
+        arrs = [[np.asarray(lv[k], np.int32) for lv in levels] for k in range(4)]
+        if ok:
+            check_level_sizes(arrs)
+        else:
+            with pytest.raises(ValueError, match="level"):
+                check_level_sizes(arrs)
