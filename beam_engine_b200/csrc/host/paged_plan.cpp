@@ -14,6 +14,7 @@
 #include <algorithm>
 #include <climits>
 #include <cstring>
+#include <exception>
 #include <vector>
 
 #include "beam_b200.h"
@@ -137,17 +138,11 @@ int narrow_chunk(const std::vector<Tile>& tiles, int64_t total, int sms, int hkv
   return best_chunk;
 }
 
-}  // namespace
-}  // namespace be
-
-using namespace be;
-
-extern "C" int be_paged_plan(int num_levels, const int32_t* const* qo_indptr,
-                             const int32_t* const* kv_indptr, const int32_t* const* kv_indices,
-                             const int32_t* const* last_page_len, const int32_t* num_groups,
-                             int num_queries, int page_size, int num_qo_heads, int num_kv_heads,
-                             int causal_last, int window_left, int num_sinks, int num_sms,
-                             int32_t* plan, int64_t plan_capacity, be_paged_plan_info* info) {
+int make_plan(int num_levels, const int32_t* const* qo_indptr, const int32_t* const* kv_indptr,
+              const int32_t* const* kv_indices, const int32_t* const* last_page_len,
+              const int32_t* num_groups, int num_queries, int page_size, int num_qo_heads,
+              int num_kv_heads, int causal_last, int window_left, int num_sinks, int num_sms,
+              int32_t* plan, int64_t plan_capacity, be_paged_plan_info* info) {
   if (num_levels < 1 || num_queries < 0 || page_size < 1 || num_kv_heads < 1 || num_qo_heads < 1 ||
       num_qo_heads % num_kv_heads || num_sinks < 0 || !info) {
     set_error("be_paged_plan: invalid arguments");
@@ -425,4 +420,23 @@ extern "C" int be_paged_plan(int num_levels, const int32_t* const* qo_indptr,
   put(mptr);
   put(mparts);
   return BE_OK;
+}
+
+}  // namespace
+}  // namespace be
+
+extern "C" int be_paged_plan(int num_levels, const int32_t* const* qo_indptr,
+                             const int32_t* const* kv_indptr, const int32_t* const* kv_indices,
+                             const int32_t* const* last_page_len, const int32_t* num_groups,
+                             int num_queries, int page_size, int num_qo_heads, int num_kv_heads,
+                             int causal_last, int window_left, int num_sinks, int num_sms,
+                             int32_t* plan, int64_t plan_capacity, be_paged_plan_info* info) {
+  try {
+    return be::make_plan(num_levels, qo_indptr, kv_indptr, kv_indices, last_page_len, num_groups,
+                         num_queries, page_size, num_qo_heads, num_kv_heads, causal_last,
+                         window_left, num_sinks, num_sms, plan, plan_capacity, info);
+  } catch (const std::exception& e) {       // no memory for the lists
+    be::set_error("be_paged_plan: %s", e.what());
+    return BE_ENOMEM;
+  }
 }

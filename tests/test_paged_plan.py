@@ -270,3 +270,25 @@ def test_arrays_shorter_than_the_indptrs_say_are_refused(qo, kp, ki, last, ok):
         else:
             with pytest.raises(ValueError, match="level"):
                 check_level_sizes(arrs)
+
+
+NO_MEMORY = """
+import resource, sys
+import numpy as np
+sys.path[:0] = {path}
+from test_paged_plan import plan
+vm = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (vm + (256 << 20), vm + (256 << 20)))
+n = 1 << 27                                       # lists of 2^27 queries: 1 GB each
+sys.exit(plan([([0, 0], [0, 1], [0], [1])], n, 16, 8, 2, cap=64)[0])
+"""
+
+
+def test_no_memory_is_a_status():
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    p = subprocess.run([sys.executable, "-c", NO_MEMORY.format(path=[here, os.path.dirname(here)])],
+                       capture_output=True, text=True, timeout=300)
+    assert p.returncode == _lib.BE_ENOMEM, p.stderr
