@@ -248,7 +248,8 @@ class _Plan:
         """A be_paged_plan plan (placed like a work-item plan)."""
         qs = q.stride()
         if qs[2] != 1 or qs[1] != head_dim or qs[0] % 8 or q.data_ptr() % 16:
-            q = q.contiguous()
+            # (a copy: contiguous() would hand back rows that only start off a 16-byte border)
+            q = q.clone(memory_format=torch.contiguous_format)
             qs = q.stride()
         i = self.info
         index = q.device.index
