@@ -7,6 +7,8 @@ import torch
 from test_gpu_paged8 import F8, clean_status, make_pool, reference, status  # noqa: F401
 from test_gpu_paged8_scales import check, run
 
+from beam_engine_b200 import _lib
+
 pytestmark = pytest.mark.gpu
 
 
@@ -73,3 +75,23 @@ def test_merge_of_many_rows(cache8, dt):
         assert ((out.double() - o).abs() <= tol).all()
         assert ((lse.double() - e).abs() <= 2e-5).all()
     assert status() == 0
+
+
+@pytest.mark.parametrize("qlen", [1, 40])
+@pytest.mark.parametrize("missing", [8, 9, 17])
+def test_no_page_in_the_first_steps(qlen, missing):
+    """The first pages are out of range: flagged, and the rest is attended as if it were all (its scales far
+    apart: nothing was there to set the unit by)."""
+    n, ps = 24, 16
+    pool, scale = make_pool(n, ps, 2, 128, torch.bfloat16, True, 8)
+    scale[:, 1] = torch.ldexp(torch.ones(n, device="cuda"), torch.arange(n, device="cuda") * 3 - 40)[:, None]
+    pages = [n + 5] * missing + list(range(missing, n))
+    from beam_engine_b200.cascade import BatchPrefillWithPagedKVCacheWrapper
+    q = torch.randn((qlen, 8, 128), device="cuda", generator=torch.Generator(device="cuda").manual_seed(5)).bfloat16()
+    w = BatchPrefillWithPagedKVCacheWrapper(torch.empty(64 << 20, dtype=torch.uint8, device="cuda"))
+    w.plan([0, qlen], [0, n], pages, [ps], 8, 2, 128, ps, causal=True, kv_data_type=F8)
+    out, lse = w.run(q, pool, return_lse=True, kv_scale=scale)
+    ref = reference(q, pool, scale, [0, n - missing], pages[missing:], [(n - missing) * ps],
+                    [0, qlen], True, -1, 0, 128 ** -0.5)
+    check(out, lse, ref, torch.bfloat16)
+    assert status() == _lib.BE_EDEVICE_RANGE
