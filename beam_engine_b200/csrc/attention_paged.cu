@@ -33,9 +33,10 @@
 // 8 bits, 16 warps per SM); loading straight into registers kept one and ran at a quarter of
 // HBM's rate (1 600 GB/s over 64 requests of up to 4 096 tokens).
 //
-// Bound: HBM.  64 requests, window 4096 + 4 of 16 000 tokens, bf16: 159 to 170 us, 6.3 to 6.75 TB/s; 64 requests of up to
-// 4 096 tokens in 8 bits: 86 us, 4.7 TB/s (half as many bytes per instruction: 412 for 16 tokens' K and
-// V, 64 of them conversions).  Four warps of a CTA split the item's tokens and fold their states
+// Bound: HBM for 16-bit caches.  64 requests, window 4096 + 4 of 16 000 tokens, bf16: 159 to 170 us, 6.3 to
+// 6.75 TB/s; 64 requests of up to 4 096 tokens in 8 bits: 90 us, 4.5 TB/s (468 instructions for 16
+// tokens' K and V, 64 of them conversions, for half the bytes; 412 and 86 us with log2 s_V whole in the
+// exponent and no unit, which lost tokens).  Four warps of a CTA split the item's tokens and fold their states
 // through shared memory; items that split a sequence leave partial rows for merge_kernel.
 #include <atomic>
 

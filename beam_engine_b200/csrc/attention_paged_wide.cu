@@ -38,8 +38,8 @@
 // 8 tokens of one page costs one shared-memory read and three operations per row.  The
 // planner aligns ranges to 8 tokens; pages that are no multiple of 8 take scales token by token.
 //
-// Measured: bf16, 8192 tokens, 32 heads on 8, window 1024 + 4: 229 us, 565 TFLOP/s; 8-bit cache, a
-// prompt of 4096 tokens, causal: 209 us, 657 TFLOP/s.  A half takes 2 500 clocks per CTA against
+// Measured: bf16, 8192 tokens, 32 heads on 8, window 1024 + 4: 227 us, 570 TFLOP/s; 8-bit cache, a
+// prompt of 4096 tokens, causal: 213 us, 646 TFLOP/s (209 before V's halves were scaled).  A half takes 2 500 clocks per CTA against
 // 1 280 of the tensor core and 1 024 of the exponentials: the rest is the latency of the softmax's steps
 // (scores out of TMEM 500, exponentials 1 100 while four warps share a scheduler's unit).
 //

@@ -94,8 +94,10 @@ int wide_chunk(const std::vector<Tile>& tiles, int64_t total_steps, int sms, int
   return best_chunk;
 }
 
-// Tokens per narrow item.  (item, KV head) pairs run up to 4 x SMs at a time (window 4096 over 64 requests,
-// bf16, when this came: 172 us planned for 4 per SM, 185 for 3 or 6);
+// Tokens per narrow item.  Items are cut as if 4 CTAs, (item, KV head) pairs, ran per SM at a time.  That is the
+// most that any variant of the kernel has: 8-bit rows of up to 8 query rows do, 16-bit rows of 128 dims have 2 and
+// up to 16 query rows 3, for which the cuts come out finer than one wave.  (Measured on the latter kind, window
+// 4096 over 64 requests, bf16, when this came: 172 us planned for 4 per SM, 185 for 3 or 6.)
 // whole tiles and cuts at fractions of the average share are tried longest first, with 192 tokens'
 // time for a CTA's start and end and 512 for the merge launch that a cut brings.
 int narrow_chunk(const std::vector<Tile>& tiles, int64_t total, int sms, int hkv) {
