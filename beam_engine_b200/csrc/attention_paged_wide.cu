@@ -29,9 +29,9 @@
 // 8-bit caches: as in the narrow kernel the codes become halves by one exact conversion.  s_K multiplies
 // the score.  s_V = 2^E mu with mu in [1, 2): the loaders multiply V's halves by 2^(E - u), u the largest E of
 // the first step's tokens, which is exact from 2^-15 (codes down to 2^-9, fp16 down to 2^-24) to 2^7
-// (448 * 2^7 = 57 344), and log2 mu joins the exponent.  P then has fp16's range to itself (2^-24 to 2^15), whatever the
-// scales of other pages are.  Values of tokens outside those 23 binary orders are 0 in that pass over the
-// item's tokens, and where one has a code that is not 0 the item is walked again for it: a pass
+// (448 * 2^7 = 57 344), and log2 mu joins the exponent.  P then has fp16's range to itself (2^-24 to
+// 2^15), whatever the scales of other pages are.  Values of tokens outside those 23 binary orders are 0
+// in that pass over the item's tokens, and where one has a code that is not 0 the item is walked again for it: a pass
 // per 23 orders, from the lowest up (O times 2^-23 per window in between), with the maximum and
 // sum of the first.  (log2 s_V as a whole in the exponent would need no pass, but a page whose scale is
 // 2^25 above the others' takes their factors below fp16's smallest.)  A group of
@@ -39,8 +39,8 @@
 // planner aligns ranges to 8 tokens; pages that are no multiple of 8 take scales token by token.
 //
 // Measured: bf16, 8192 tokens, 32 heads on 8, window 1024 + 4: 227 us, 570 TFLOP/s; 8-bit cache, a
-// prompt of 4096 tokens, causal: 213 us, 646 TFLOP/s (209 before V's halves were scaled).  A half takes 2 500 clocks per CTA against
-// 1 280 of the tensor core and 1 024 of the exponentials: the rest is the latency of the softmax's steps
+// prompt of 4096 tokens, causal: 213 us, 646 TFLOP/s (209 before V's halves were scaled).  A half
+// takes 2 500 clocks per CTA against 1 280 of the tensor core and 1 024 of the exponentials: the rest is the latency of the softmax's steps
 // (scores out of TMEM 500, exponentials 1 100 while four warps share a scheduler's unit).
 //
 // Values that are not finite: 0 * NaN is NaN in the product, so in steps that some row
